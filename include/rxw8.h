@@ -278,6 +278,56 @@ int rxw8_gqa_prefill_into(rxw8_runtime *rt, rxw8_buffer *q,
                           rxw8_buffer *k_cache, rxw8_buffer *v_cache,
                           rxw8_buffer *starts, float scale, rxw8_buffer *out);
 
+/* ---- paged key/value cache (no counterpart in the reference, whose cache is one
+ * plane per sequence, kv_cache.rs:7-111) --------------------------------------
+ * k_pages/v_pages [P,Hkv,ps,D] BF16|F32 (two buffers of one shape and type): a
+ * pool of P pages of ps positions. table I32 [B,M]: entry (b, i) is the page
+ * of positions ps i .. ps i + ps - 1 of sequence b; an entry outside [0, P)
+ * (-1 for instance) means that it has none. M * ps is at most INT32_MAX. */
+
+/* Writes new rows into their pages: row offsets[b] + i of k, v [T,Hkv,D]
+ * BF16|F32 goes to position starts[b] + i of sequence b, for the rows before
+ * offsets[b + 1]. offsets I32 [B+1] does not decrease; NULL: T = B, one row for
+ * each sequence (a decode step). starts I32 [B]. F32 rows are rounded to nearest
+ * even into BF16 pages, BF16 rows widened into F32 ones. Left out: rows outside
+ * every sequence, negative positions, positions behind the table and positions
+ * without a page. Sequences that share a page and write one position of it race. */
+int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages,
+                         rxw8_buffer *v_pages, rxw8_buffer *k, rxw8_buffer *v,
+                         rxw8_buffer *table, rxw8_buffer *starts,
+                         rxw8_buffer *offsets);
+
+/* rxw8_gqa_decode over a paged cache: q [B,Hq,D] F32|BF16, Hq % Hkv == 0,
+ * lens I32 [B]: sequence b sees positions 0 .. lens[b] - 1 (clamped into
+ * [0, M ps]) that have a page. Query head h reads kv head h / (Hq/Hkv);
+ * scale <= 0 selects 1/sqrt(D); D <= 512. out [B,Hq,D] F32|BF16; the rows of a
+ * sequence that sees no key are 0. What positions that are not seen hold (NaN
+ * included) does not matter. The forms allocate nothing but `out`. */
+int rxw8_gqa_decode_paged(rxw8_runtime *rt, rxw8_buffer *q,
+                          rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                          rxw8_buffer *table, rxw8_buffer *lens, float scale,
+                          int out_dtype, rxw8_buffer **out);
+int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q,
+                               rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                               rxw8_buffer *table, rxw8_buffer *lens,
+                               float scale, rxw8_buffer *out);
+
+/* rxw8_gqa_prefill for whole prompts of different lengths packed one after
+ * another, keys and values beside their queries: q [T,Hq,D] F32|BF16, k/v
+ * [T,Hkv,D] BF16, Hq % Hkv == 0, D <= 512. offsets I32 [B+1] (device, not
+ * decreasing; values are clamped into [0, T]): sequence b owns rows
+ * offsets[b] .. offsets[b+1] - 1, none if they are equal, and its row t sees
+ * rows offsets[b] .. t. scale <= 0 selects 1/sqrt(D). out [T,Hq,D] F32|BF16:
+ * rows outside every sequence are 0 in a new buffer and left as they were by
+ * _into. */
+int rxw8_gqa_prefill_packed(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k,
+                            rxw8_buffer *v, rxw8_buffer *offsets, float scale,
+                            int out_dtype, rxw8_buffer **out);
+int rxw8_gqa_prefill_packed_into(rxw8_runtime *rt, rxw8_buffer *q,
+                                 rxw8_buffer *k, rxw8_buffer *v,
+                                 rxw8_buffer *offsets, float scale,
+                                 rxw8_buffer *out);
+
 /* Tensor::argmax(axis, keep_dims) (crates/rxla-core/src/indexing.rs:350-374):
  * index of the first maximum along `axis` of an F32 tensor, as I32 with that
  * axis removed (keep_dims: kept with length 1). Ties choose the lowest index;
@@ -286,6 +336,31 @@ int rxw8_gqa_prefill_into(rxw8_runtime *rt, rxw8_buffer *q,
  * empty result. The same two kernels end every decoder step (greedy ids). */
 int rxw8_argmax(rxw8_runtime *rt, rxw8_buffer *x, int axis, int keep_dims,
                 rxw8_buffer **out);
+
+/* The next token of each row of logits [B,V] F32|BF16 (V <= 2^24) from a random
+ * number in [0, 1), uniform F32 [B] (clamped into [0, 1 - 2^-24]; NaN counts as
+ * 0); out I32 [B]. Per row, with settings of its own (a NULL buffer: off):
+ *   words in order of (logit descending, index ascending);
+ *   top_k I32 [B]: the first top_k of them (<= 0 or >= V: all);
+ *   weights w = exp((logit - maximum) / temperature), temperature F32 [B]
+ *   (NULL: 1);
+ *   top_p F32 [B]: of those the shortest run from the first whose mass is at
+ *   least top_p times theirs (>= 1 or NaN: all; the first word always stays);
+ *   min_p F32 [B]: of that the words with w >= min_p, that is with at least
+ *   min_p times the first word's probability (<= 0 or NaN: all);
+ *   the token is the first word in the order whose running mass exceeds uniform
+ *   times the mass of what is left.
+ * A temperature that is not above 0 (NaN included), a NaN among the row's logits
+ * and a row whose maximum is infinite give what rxw8_argmax gives. Words at -inf
+ * weigh nothing. The same inputs give the same tokens: masses are summed in
+ * whole units of 2^-s of the first word's, V 2^s < 2^62 (s <= 52). */
+int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform,
+                rxw8_buffer *temperature, rxw8_buffer *top_k,
+                rxw8_buffer *top_p, rxw8_buffer *min_p, rxw8_buffer **out);
+int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits,
+                     rxw8_buffer *uniform, rxw8_buffer *temperature,
+                     rxw8_buffer *top_k, rxw8_buffer *top_p,
+                     rxw8_buffer *min_p, rxw8_buffer *out);
 
 /* KvCache::update_at / update_at_checked (kv_cache.rs:53-111): paired
  * dynamic_update_slice of k_update/v_update (equal shapes, rank = cache rank,

@@ -418,6 +418,67 @@ def grouped_query_attention_prefill(rt: Runtime, q: Buffer, k_cache: Buffer, v_c
     return Buffer(h)
 
 
+def paged_kv_append(rt: Runtime, k_pages: Buffer, v_pages: Buffer, k: Buffer, v: Buffer,
+                    table: Buffer, starts: Buffer, offsets: Buffer | None = None):
+    """New rows k, v [T, Hkv, D] into the pages [P, Hkv, ps, D] that table [B, M]
+    gives their sequences: row offsets[b] + i to position starts[b] + i; without
+    offsets row b to position starts[b] (a decode step). Returns the pages."""
+    o = offsets.handle if offsets is not None else None
+    _check(_lib.rxw8_paged_kv_append(rt.handle, k_pages.handle, v_pages.handle, k.handle,
+                                     v.handle, table.handle, starts.handle, o))
+    return k_pages, v_pages
+
+
+def grouped_query_attention_paged(rt: Runtime, q: Buffer, k_pages: Buffer, v_pages: Buffer,
+                                  table: Buffer, lens: Buffer, scale: float | None = None,
+                                  out_dtype=DType.F32, out: Buffer | None = None) -> Buffer:
+    """``grouped_query_attention`` (one query row per sequence, q [B, Hq, D]) over a
+    paged cache: the first lens[b] positions of sequence b, in the pages that
+    table [B, M] names. A sequence that sees no key gives rows of 0."""
+    s = 0.0 if scale is None else float(scale)
+    if out is not None:
+        _check(_lib.rxw8_gqa_decode_paged_into(rt.handle, q.handle, k_pages.handle,
+                                               v_pages.handle, table.handle, lens.handle, s,
+                                               out.handle))
+        return out
+    h = c_void_p()
+    _check(_lib.rxw8_gqa_decode_paged(rt.handle, q.handle, k_pages.handle, v_pages.handle,
+                                      table.handle, lens.handle, s, int(out_dtype), byref(h)))
+    return Buffer(h)
+
+
+def grouped_query_attention_packed(rt: Runtime, q: Buffer, k: Buffer, v: Buffer, offsets: Buffer,
+                                   scale: float | None = None, out_dtype=DType.F32,
+                                   out: Buffer | None = None) -> Buffer:
+    """Causal attention of whole prompts packed one after another: sequence b owns
+    rows offsets[b] .. offsets[b + 1] - 1 of q [T, Hq, D] and of k, v [T, Hkv, D]
+    BF16. Rows outside every sequence are 0 in a new buffer, left alone in ``out``."""
+    s = 0.0 if scale is None else float(scale)
+    if out is not None:
+        _check(_lib.rxw8_gqa_prefill_packed_into(rt.handle, q.handle, k.handle, v.handle,
+                                                 offsets.handle, s, out.handle))
+        return out
+    h = c_void_p()
+    _check(_lib.rxw8_gqa_prefill_packed(rt.handle, q.handle, k.handle, v.handle, offsets.handle,
+                                        s, int(out_dtype), byref(h)))
+    return Buffer(h)
+
+
+def sample(rt: Runtime, logits: Buffer, uniform: Buffer, temperature: Buffer | None = None,
+           top_k: Buffer | None = None, top_p: Buffer | None = None, min_p: Buffer | None = None,
+           out: Buffer | None = None) -> Buffer:
+    """The next token of each row of logits [B, V] from uniform [B] in [0, 1), with
+    a temperature, top-k, top-p and min-p for each row (None: off; see
+    ``rxw8_sample``). I32 [B]; a temperature of 0 is ``argmax``."""
+    opt = [b.handle if b is not None else None for b in (temperature, top_k, top_p, min_p)]
+    if out is not None:
+        _check(_lib.rxw8_sample_into(rt.handle, logits.handle, uniform.handle, *opt, out.handle))
+        return out
+    h = c_void_p()
+    _check(_lib.rxw8_sample(rt.handle, logits.handle, uniform.handle, *opt, byref(h)))
+    return Buffer(h)
+
+
 class KvCache:
     """Paired fixed-capacity K/V state (crates/rxla-core/src/kv_cache.rs:7-111)."""
 
@@ -526,6 +587,7 @@ __all__ = ["Runtime", "Buffer", "DType", "Status", "Error", "quantize_w8", "dequ
            "linear_bf16", "QuantizedLinear", "grouped_query_attention",
            "grouped_query_attention_prefill", "grouped_query_attention_noalloc", "gqa_attention",
            "scaled_dot_product_attention", "causal_attention_mask", "causal_attention_mask_static",
-           "argmax", "KvCache",
+           "argmax", "KvCache", "paged_kv_append", "grouped_query_attention_paged",
+           "grouped_query_attention_packed", "sample",
            "SafeTensors",
            "DecoderConfig", "DecoderModel", "Qwen35Config", "Qwen35Model", "bf16_to_f32"]

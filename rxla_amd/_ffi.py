@@ -27,6 +27,8 @@ EXPORTS = [
     "rxw8_gqa_decode_noalloc", "rxw8_gqa_attention", "rxw8_gqa_attention_into",
     "rxw8_causal_attention_mask",
     "rxw8_gqa_prefill", "rxw8_gqa_prefill_into", "rxw8_kv_update_at", "rxw8_argmax",
+    "rxw8_paged_kv_append", "rxw8_gqa_decode_paged", "rxw8_gqa_decode_paged_into",
+    "rxw8_gqa_prefill_packed", "rxw8_gqa_prefill_packed_into", "rxw8_sample", "rxw8_sample_into",
     "rxw8_safetensors_open", "rxw8_safetensors_close", "rxw8_safetensors_num_tensors",
     "rxw8_safetensors_tensor_info", "rxw8_safetensors_find", "rxw8_safetensors_metadata",
     "rxw8_safetensors_upload",
@@ -101,6 +103,13 @@ def _declare(L):
         "rxw8_gqa_prefill_into": (c_int, [vp, vp, vp, vp, vp, c_float, vp]),
         "rxw8_kv_update_at": (c_int, [vp, vp, vp, vp, vp, vp, c_int, vp]),
         "rxw8_argmax": (c_int, [vp, vp, c_int, c_int, POINTER(vp)]),
+        "rxw8_paged_kv_append": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp]),
+        "rxw8_gqa_decode_paged": (c_int, [vp, vp, vp, vp, vp, vp, c_float, c_int, POINTER(vp)]),
+        "rxw8_gqa_decode_paged_into": (c_int, [vp, vp, vp, vp, vp, vp, c_float, vp]),
+        "rxw8_gqa_prefill_packed": (c_int, [vp, vp, vp, vp, vp, c_float, c_int, POINTER(vp)]),
+        "rxw8_gqa_prefill_packed_into": (c_int, [vp, vp, vp, vp, vp, c_float, vp]),
+        "rxw8_sample": (c_int, [vp, vp, vp, vp, vp, vp, vp, POINTER(vp)]),
+        "rxw8_sample_into": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp]),
         "rxw8_safetensors_open": (c_int, [c_char_p, POINTER(vp)]),
         "rxw8_safetensors_close": (c_int, [vp]),
         "rxw8_safetensors_num_tensors": (c_int, [vp, i64p]),

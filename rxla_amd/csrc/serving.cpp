@@ -1,0 +1,276 @@
+// The serving operators: the paged key/value cache (append, decode attention),
+// causal attention of packed prompts, and sampling of the next token.
+#include <cmath>
+#include <cstdint>
+
+#include "internal.h"
+
+namespace rxw8 {
+
+// (the kernels' argument structs: kernels/paged.hip, packed.hip, sample.hip)
+struct PagedAppendArgs {
+  const void *k, *v;
+  void *kp, *vp;
+  const int32_t *table, *starts, *offsets;
+  int64_t T, P;
+  int B, M, Hkv, D, ps;
+  int k_f32, p_f32;
+};
+struct PagedDecodeArgs {
+  const void *q, *kp, *vp;
+  const int32_t *table, *lens;
+  void *out;
+  int64_t P;
+  int B, M, Hq, Hkv, D, ps;
+  float c;
+  int q_f32, p_f32, out_f32;
+};
+struct PackedArgs {
+  const void *q;
+  const uint16_t *k, *v;
+  const int32_t *offsets;
+  void *out;
+  int64_t T;
+  int B, Hq, Hkv, D;
+  float c;
+  int q_f32, out_f32;
+  int fill;
+};
+struct SampleArgs {
+  const void *logits;
+  const float *uniform, *temperature;
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  int32_t *out;
+  int64_t V;
+  int shift;
+  int bf16;
+};
+
+static bool is_f(int dt) { return dt == RXW8_F32 || dt == RXW8_BF16; }
+static bool is_vec(const Buffer *b, int dtype, int64_t n) {
+  return b->dtype == dtype && b->rank == 1 && b->dims[0] == n;
+}
+static bool same_shape(const Buffer *a, const Buffer *b) {
+  bool same = a->dtype == b->dtype && a->rank == b->rank;
+  for (int i = 0; same && i < a->rank; ++i) same = a->dims[i] == b->dims[i];
+  return same;
+}
+constexpr int64_t kGridMax = ((int64_t)1 << 31) - 1;
+constexpr int64_t kAnyMaxD = 512;  // RXW8_ATTN_ANY_MAX_D
+
+// Pages [P, Hkv, ps, D] F32|BF16 and the table I32 [B, M]
+static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, const Buffer *table) {
+  if (kp->rank != 4 || !is_f(kp->dtype) || !same_shape(kp, vp))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: pages must be two F32/BF16 [P,Hkv,ps,D] of one shape and type", what);
+  if (kp->dims[1] <= 0 || kp->dims[2] <= 0 || kp->dims[3] <= 0)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: pages %s need positive heads, rows and width", what, dims_str(kp).c_str());
+  if (table->dtype != RXW8_I32 || table->rank != 2)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: the page table must be I32 [B,M]", what);
+  for (int i = 1; i < 4; ++i)
+    if (kp->dims[i] > INT32_MAX) return fail(RXW8_UNIMPLEMENTED, "%s: pages %s", what, dims_str(kp).c_str());
+  // positions are I32
+  if (table->dims[0] > INT32_MAX || (table->dims[1] > 0 && kp->dims[2] > INT32_MAX / table->dims[1]))
+    return fail(RXW8_UNIMPLEMENTED, "%s: %lld pages of %lld positions exceed 32-bit positions", what,
+                (long long)table->dims[1], (long long)kp->dims[2]);
+  return RXW8_OK;
+}
+
+static int check_paged_decode(const Buffer *q, const Buffer *kp, const Buffer *vp, const Buffer *table,
+                              const Buffer *lens, float scale) {
+  if (!q || !kp || !vp || !table || !lens) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: NULL buffer");
+  if (int rc = check_pages("paged GQA decode", kp, vp, table)) return rc;
+  if (q->rank != 3 || !is_f(q->dtype))
+    return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode requires F32/BF16 q [B,Hq,D]");
+  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (table->dims[0] != B || D != kp->dims[3])
+    return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: q, page table and pages differ in batch or head width");
+  if (Hq <= 0 || Hq % kp->dims[1] != 0)
+    return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
+  if (!is_vec(lens, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: lens must be I32 [B]");
+  if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
+  if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: head dim %lld > 512", (long long)D);
+  if (Hq > INT32_MAX || (Hq > 0 && B > kGridMax / Hq))
+    return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: %lld x %lld rows exceed the kernel's grid", (long long)B,
+                (long long)Hq);
+  return RXW8_OK;
+}
+
+static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets, float scale) {
+  if (!q || !k || !v || !offsets) return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill: NULL buffer");
+  if (q->rank != 3 || k->rank != 3 || !is_f(q->dtype) || k->dtype != RXW8_BF16 || !same_shape(k, v))
+    return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill requires F32/BF16 q [T,Hq,D] and BF16 k, v [T,Hkv,D]");
+  const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (k->dims[0] != T || k->dims[2] != D || D <= 0)
+    return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill: q and k, v differ in rows or head width");
+  if (Hq <= 0 || k->dims[1] <= 0 || Hq % k->dims[1] != 0)
+    return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
+  if (offsets->dtype != RXW8_I32 || offsets->rank != 1 || offsets->dims[0] < 1)
+    return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill: offsets must be I32 [sequences + 1]");
+  if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
+  if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: head dim %lld > 512", (long long)D);
+  if (T > INT32_MAX || Hq > INT32_MAX || T > kGridMax / Hq || offsets->dims[0] > INT32_MAX)
+    return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: %lld x %lld rows exceed the kernel's grid", (long long)T,
+                (long long)Hq);
+  return RXW8_OK;
+}
+
+static float softmax_scale(float scale, int64_t D) {
+  return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f;
+}
+
+static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets,
+                         float scale, const Buffer *out, bool fill) {
+  const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (T == 0) return RXW8_OK;
+  PackedArgs a{q->ptr, (const uint16_t *)k->ptr, (const uint16_t *)v->ptr, (const int32_t *)offsets->ptr, out->ptr, T,
+               (int)(offsets->dims[0] - 1), (int)Hq, (int)k->dims[1], (int)D, softmax_scale(scale, D),
+               q->dtype == RXW8_F32, out->dtype == RXW8_F32, fill};
+  return launch(rt, "rxw8_packed_prefill_any", dim3((unsigned)((T * Hq + 3) / 4)), dim3(256), a);
+}
+
+}  // namespace rxw8
+
+using namespace rxw8;
+
+extern "C" {
+
+int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pages, rxw8_buffer *k,
+                         rxw8_buffer *v, rxw8_buffer *table, rxw8_buffer *starts, rxw8_buffer *offsets) {
+  if (!rt || !k_pages || !v_pages || !k || !v || !table || !starts)
+    return fail(RXW8_INVALID_ARGUMENT, "paged KV append: NULL argument");
+  if (int rc = check_pages("paged KV append", k_pages, v_pages, table)) return rc;
+  if (k_pages == v_pages || (k_pages->ptr == v_pages->ptr && k_pages->bytes))
+    return fail(RXW8_INVALID_ARGUMENT, "K and V pages must be distinct buffers");
+  if (k->rank != 3 || !is_f(k->dtype) || !same_shape(k, v) || k->dims[1] != k_pages->dims[1] ||
+      k->dims[2] != k_pages->dims[3])
+    return fail(RXW8_INVALID_ARGUMENT, "paged KV append requires F32/BF16 k, v [T,Hkv,D] of the pages' heads and width");
+  const int64_t T = k->dims[0], B = table->dims[0];
+  if (!is_vec(starts, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged KV append: starts must be I32 [B]");
+  if (offsets ? !is_vec(offsets, RXW8_I32, B + 1) : T != B)
+    return fail(RXW8_INVALID_ARGUMENT, "paged KV append: offsets must be I32 [B+1] (without them k, v hold one row a sequence)");
+  if (T > kGridMax / k->dims[1])
+    return fail(RXW8_UNIMPLEMENTED, "paged KV append: %lld rows exceed the kernel's grid", (long long)T);
+  if (T == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  PagedAppendArgs a{k->ptr, v->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr,
+                    (const int32_t *)starts->ptr, offsets ? (const int32_t *)offsets->ptr : nullptr, T,
+                    k_pages->dims[0], (int)B, (int)table->dims[1], (int)k->dims[1], (int)k->dims[2],
+                    (int)k_pages->dims[2], k->dtype == RXW8_F32, k_pages->dtype == RXW8_F32};
+  return launch(rt, "rxw8_paged_append", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+}
+
+int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                               rxw8_buffer *table, rxw8_buffer *lens, float scale, rxw8_buffer *out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_paged_decode(q, k_pages, v_pages, table, lens, scale)) return rc;
+  bool ok = is_f(out->dtype) && out->rank == 3;
+  for (int i = 0; ok && i < 3; ++i) ok = out->dims[i] == q->dims[i];
+  if (!ok) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode output: shape or dtype mismatch");
+  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (B == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  PagedDecodeArgs a{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
+                    out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
+                    (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32,
+                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32};
+  return launch(rt, "rxw8_paged_decode_any", dim3((unsigned)(B * Hq)), dim3(256), a);
+}
+
+int rxw8_gqa_decode_paged(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                          rxw8_buffer *table, rxw8_buffer *lens, float scale, int out_dtype, rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_paged_decode(q, k_pages, v_pages, table, lens, scale)) return rc;
+  if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA: out dtype must be F32 or BF16");
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *o = nullptr;
+  int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
+  if (rc) return rc;
+  rc = rxw8_gqa_decode_paged_into(rt, q, k_pages, v_pages, table, lens, scale, static_cast<rxw8_buffer *>(o));
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(o));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+int rxw8_gqa_prefill_packed_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k, rxw8_buffer *v,
+                                 rxw8_buffer *offsets, float scale, rxw8_buffer *out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_packed(q, k, v, offsets, scale)) return rc;
+  bool ok = is_f(out->dtype) && out->rank == 3;
+  for (int i = 0; ok && i < 3; ++i) ok = out->dims[i] == q->dims[i];
+  if (!ok) return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill output: shape or dtype mismatch");
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  return packed_launch(rt, q, k, v, offsets, scale, out, false);
+}
+
+int rxw8_gqa_prefill_packed(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k, rxw8_buffer *v, rxw8_buffer *offsets,
+                            float scale, int out_dtype, rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_packed(q, k, v, offsets, scale)) return rc;
+  if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA prefill: out dtype must be F32 or BF16");
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *o = nullptr;
+  int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
+  if (rc) return rc;
+  rc = packed_launch(rt, q, k, v, offsets, scale, o, true);
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(o));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+static int check_sample(const Buffer *logits, const Buffer *uniform, const Buffer *temperature, const Buffer *top_k,
+                        const Buffer *top_p, const Buffer *min_p) {
+  if (!logits || !uniform) return fail(RXW8_INVALID_ARGUMENT, "sample: NULL buffer");
+  if (logits->rank != 2 || !is_f(logits->dtype) || logits->dims[1] <= 0)
+    return fail(RXW8_INVALID_ARGUMENT, "sample requires F32/BF16 logits [B,V] with V > 0");
+  const int64_t B = logits->dims[0], V = logits->dims[1];
+  if (!is_vec(uniform, RXW8_F32, B)) return fail(RXW8_INVALID_ARGUMENT, "sample: uniform must be F32 [B]");
+  if ((temperature && !is_vec(temperature, RXW8_F32, B)) || (top_k && !is_vec(top_k, RXW8_I32, B)) ||
+      (top_p && !is_vec(top_p, RXW8_F32, B)) || (min_p && !is_vec(min_p, RXW8_F32, B)))
+    return fail(RXW8_INVALID_ARGUMENT, "sample: temperature, top_p and min_p must be F32 [B], top_k I32 [B]");
+  if (V > ((int64_t)1 << 24)) return fail(RXW8_UNIMPLEMENTED, "sample: %lld words > 2^24", (long long)V);
+  if (B > kGridMax) return fail(RXW8_UNIMPLEMENTED, "sample: %lld rows exceed the kernel's grid", (long long)B);
+  return RXW8_OK;
+}
+
+int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform, rxw8_buffer *temperature,
+                     rxw8_buffer *top_k, rxw8_buffer *top_p, rxw8_buffer *min_p, rxw8_buffer *out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_sample(logits, uniform, temperature, top_k, top_p, min_p)) return rc;
+  const int64_t B = logits->dims[0], V = logits->dims[1];
+  if (!is_vec(out, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "sample output must be I32 [B]");
+  if (B == 0) return RXW8_OK;
+  int bits = 0;  // ceil(log2 V)
+  while (((int64_t)1 << bits) < V) ++bits;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  SampleArgs a{logits->ptr, (const float *)uniform->ptr, temperature ? (const float *)temperature->ptr : nullptr,
+               top_k ? (const int32_t *)top_k->ptr : nullptr, top_p ? (const float *)top_p->ptr : nullptr,
+               min_p ? (const float *)min_p->ptr : nullptr, (int32_t *)out->ptr, V, 62 - bits > 52 ? 52 : 62 - bits,
+               logits->dtype == RXW8_BF16};
+  return launch(rt, "rxw8_sample_any", dim3((unsigned)B), dim3(1024), a);
+}
+
+int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform, rxw8_buffer *temperature,
+                rxw8_buffer *top_k, rxw8_buffer *top_p, rxw8_buffer *min_p, rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_sample(logits, uniform, temperature, top_k, top_p, min_p)) return rc;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *o = nullptr;
+  int rc = new_buffer(rt, RXW8_I32, logits->dims, 1, false, &o);
+  if (rc) return rc;
+  rc = rxw8_sample_into(rt, logits, uniform, temperature, top_k, top_p, min_p, static_cast<rxw8_buffer *>(o));
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(o));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+}  // extern "C"
