@@ -1,7 +1,9 @@
 // The serving operators: the paged key/value cache (append, decode attention),
 // causal attention of packed prompts, and sampling of the next token.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <cstdio>
 
 #include "internal.h"
 
@@ -24,6 +26,9 @@ struct PagedDecodeArgs {
   int B, M, Hq, Hkv, D, ps;
   float c;
   int q_f32, p_f32, out_f32;
+  int units;
+  int *counters;
+  float *part;
 };
 struct PackedArgs {
   const void *q;
@@ -119,6 +124,35 @@ static float softmax_scale(float scale, int64_t D) {
   return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f;
 }
 
+// The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row
+// pieces, 16-byte aligned operands and tile counts within 32 bits; else the plain
+// kernel. One workgroup fills a CU: as many waves, up to 8, as rings of two tiles and
+// records of the group's heads fit in LDS. `units` workgroups for each kv head (and
+// 16 query heads): the number that leaves the fewest CUs idle in the last round.
+static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
+  const int64_t G = a.Hq / a.Hkv, heads = a.Hkv * ((G + 15) / 16), gcap = G < 16 ? G : 16;
+  const int es = a.p_f32 ? 4 : 2, row = a.D * es, tile = row < 256 ? 32 : 16;
+  if ((a.D != 64 && a.D != 128 && a.D != 256) || a.ps % 16 || a.P == 0 || heads > 4096 ||
+      ((uintptr_t)a.q | (uintptr_t)a.kp | (uintptr_t)a.vp | (uintptr_t)a.out) % 16 ||
+      (int64_t)a.B * (((int64_t)a.M * a.ps + tile - 1) / tile) >= ((int64_t)1 << 30))
+    return launch(rt, "rxw8_paged_decode_any", dim3((unsigned)a.B * (unsigned)a.Hq), dim3(256), a);
+  const size_t record = (size_t)gcap * (size_t)(a.D + 4) * sizeof(float), wave = (size_t)(4 * tile * row) + record;
+  const int waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>({256, (int64_t)(RXW8_NOALLOC_COUNTER_BYTES / sizeof(int)) / heads,
+                                                               (int64_t)(RXW8_NOALLOC_PARTIAL_BYTES / (2 * record)) / heads}));
+  a.units = 1;
+  for (int64_t u = 2; u <= most; ++u) {  // rounds of workgroups per unit of work
+    const int64_t r0 = (heads * a.units + rt->cus - 1) / rt->cus, r1 = (heads * u + rt->cus - 1) / rt->cus;
+    if (r1 * a.units < r0 * u) a.units = (int)u;
+  }
+  char *block = rt->f32_attn[stream_capturing(rt) ? 1 : 0];
+  a.counters = (int *)block;
+  a.part = (float *)(block + RXW8_NOALLOC_COUNTER_BYTES);
+  char kname[40];
+  std::snprintf(kname, sizeof kname, "rxw8_paged_decode_%s_d%d", a.p_f32 ? "f32" : "bf16", a.D);
+  return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(64 * waves), a, wave * (size_t)waves);
+}
+
 static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets,
                          float scale, const Buffer *out, bool fill) {
   const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2];
@@ -173,8 +207,8 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_
   PagedDecodeArgs a{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
                     out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
                     (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32,
-                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32};
-  return launch(rt, "rxw8_paged_decode_any", dim3((unsigned)(B * Hq)), dim3(256), a);
+                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32, 0, nullptr, nullptr};
+  return paged_decode_launch(rt, a);
 }
 
 int rxw8_gqa_decode_paged(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,

@@ -4,13 +4,14 @@ roundings can make: |out - y| <= bound for every element.
 A score s = c q.k formed with relative error e per product is off by at most
 e scale sum |q_i k_i|; weights then by the factor exp(+-2 err) together with their
 sum; what the weights and the output are rounded to comes on top (half a step:
-2^-24 f32, 2^-8 bf16, and 2^-17 for a value split into bf16 high and low parts,
-2^-9 2^-9 for the part that is left, doubled)."""
+2^-24 f32, 2^-8 bf16). A value v in [2^e, 2^(e+1)) split into two bf16 with the high
+one cut leaves at most 2^(e-7), half a step of which (2^-8 of the power of two below
+it, at most 2^(e-8)) is 2^(e-16): 2^-16."""
 import math
 
 import numpy as np
 
-F32, BF16, SPLIT = 2.0 ** -24, 2.0 ** -8, 2.0 ** -17
+F32, BF16, SPLIT = 2.0 ** -24, 2.0 ** -8, 2.0 ** -16
 
 
 def bf16_bits(x):
