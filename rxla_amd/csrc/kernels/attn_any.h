@@ -24,23 +24,25 @@ __device__ __forceinline__ float wave_max64(float v) {
   return v;
 }
 
-// v as the sum of two bf16, high bits first: |v - hi - lo| <= 2^-16 |v|. The high one
-// is cut, not rounded, and is one step less where that leaves nothing: both parts of
-// a v that is not 0 have its sign and are not 0, so that a product with an infinite
-// factor is the infinity that v's own would be.
-struct Bf16Pair {
-  uint32_t hi;  // f32 bits, low half zero
-  float lo;     // (to be rounded)
-};
-__device__ __forceinline__ Bf16Pair split_bf16(float v) {
+// v as a sum of bf16 parts, high bits first: two leave |v| 2^-16 at most (the second is
+// rounded), three are v exactly (8 bits of its 24 each). A part is cut, not rounded, and
+// is one step less where that would leave nothing: every part of a v that is not 0 has
+// its sign and is not 0, so that a product with an infinite factor is the infinity that
+// v's own would be.
+__device__ __forceinline__ uint32_t cut_bf16(float v) {  // f32 bits, low half zero
   const uint32_t b = __float_as_uint(v);
-  const uint32_t cut = b & 0xffffu || !(b & 0x7fffffffu) ? b & 0xffff0000u : b - 0x10000u;
-  return Bf16Pair{cut, v - __uint_as_float(cut)};
+  return b & 0xffffu || !(b & 0x7fffffffu) ? b & 0xffff0000u : b - 0x10000u;
 }
-__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t &hi, uint32_t &lo) {
-  const Bf16Pair x = split_bf16(a), y = split_bf16(b);
-  hi = (x.hi >> 16) | y.hi;
-  lo = pack_bf16x2(x.lo, y.lo);
+// Parts of two values, packed in pairs: N = 2 or 3
+template <int N>
+__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t (&part)[N]) {
+#pragma unroll
+  for (int n = 0; n + 1 < N; ++n) {
+    const uint32_t x = cut_bf16(a), y = cut_bf16(b);
+    part[n] = (x >> 16) | y;
+    a -= __uint_as_float(x), b -= __uint_as_float(y);
+  }
+  part[N - 1] = pack_bf16x2(a, b);
 }
 
 // One wave over keys first, first + 1, .. in chunks of 64 (lane = key), the next

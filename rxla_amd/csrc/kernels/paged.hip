@@ -3,6 +3,8 @@
 // head's ps rows of a page in one piece); table [B, M] I32 gives sequence b the
 // page of its positions ps i .. ps i + ps - 1 in entry i, anything outside [0, P)
 // where it has none. An entry is checked before its page is touched.
+#include <type_traits>
+
 #include "attn_any.h"
 
 struct PagedAppendArgs {
@@ -59,9 +61,9 @@ struct PagedDecodeArgs {
   float c;                // scale log2 e
   int q_f32, p_f32, out_f32;
   // the matrix-core kernels: `units` workgroups for each kv head and 16 of its
-  // query heads; counters [Hkv HT units], zero between launches, and partials
-  // [Hkv HT units][2][min(G, 16)][D + 4]
-  int units;
+  // query heads; counters [Hkv HT units], zero between launches, and two
+  // records of min(G, 16) (D + 4) floats each, padded to whole KiB
+  int units, waves;       // waves that walk keys (a workgroup has 8; the others help to join)
   int *counters;
   float *part;
 };
@@ -112,25 +114,30 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_paged_decode_any(PagedDec
 // of it an equal piece of that, whatever the sequences' lengths. A wave that meets
 // a sequence's end goes on with the next one.
 //
-// A wave copies its tiles by LDS DMA into a ring of its own, two tiles deep (the
-// next tile's 8 to 32 KiB in flight while one is worked on), so the loop has no
-// barrier and holds no registers for loads. Rows keep their order in LDS, their
-// 16-byte chunks XOR-swizzled by row. Per 16 keys and 16 heads:
-//   S^T = K q^T    A = K rows, B = q: 16x16x32 bf16 (an f32 q as high and low
-//                  parts: exact products of what two bf16 hold), 16x16x4 f32;
+// A wave copies its tiles by LDS DMA into memory of its own, K and V a tile each, and
+// the next K goes out when the products with this one are done, the next V likewise:
+// the loop has no barrier and holds no registers for loads, and a CU has some 64 KiB on
+// their way. (Twice that, with two tiles of each: 32.2 us against 30.7 for 8 sequences
+// of 4096 keys, 32 / 8 heads; what is more in flight than the memory takes only waits
+// longer, and the waves end further apart.) Rows keep their order in LDS, their 16-byte
+// chunks XOR-swizzled by row. Per 16 keys and 16 heads:
+//   S^T = K q^T    A = K rows, B = q: 16x16x32 bf16 (an f32 q as its three bf16 parts:
+//                  exact products), 16x16x4 f32;
 //   softmax        lane = head, its four lanes share the keys; O is rescaled only
 //                  where the running maximum moves;
 //   O^T += V^T P^T A = V by transposing reads (bf16), B = P straight from the score
-//                  registers as high and low parts (16x16x16); f32 caches take the
-//                  f32 products and the dims in the order of 16-byte pieces.
+//                  registers, as its three bf16 parts for an f32 output, as two (2^-16
+//                  of P, behind an output rounded to 2^-8) for a bf16 one (16x16x16);
+//                  f32 caches take f32 products, the dims in the order of 16-byte pieces.
 // V rows that a tile's last key or a missing page leaves unseen are cleared in LDS
 // (their weights are zero, what they hold may be NaN); K's scores there are -inf.
 //
 // A sequence inside one wave's piece is written at once. Pieces of a sequence are
 // joined in the order of its keys: the waves' in LDS, then, if it passes a
 // workgroup's piece, by the last of its workgroups to arrive, over (max, sum, acc)
-// records in device memory (at most two a workgroup). Stores and loads of those are
-// device-coherent around an arrival counter; the last one sets it back to zero.
+// records in device memory (at most two a workgroup). Those are stored and copied
+// past the dies' own caches, around an arrival counter that the last one sets back to
+// zero.
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -172,11 +179,67 @@ struct PagedTile {
   static constexpr int ES = F32 ? 4 : 2, ROW = D * ES, CH = ROW / 16;
   static constexpr int KT = ROW < 256 ? 32 : 16;  // keys of a tile
   static constexpr int SUB = KT / 16, HALF = KT * ROW, N = HALF / 1024, RPI = 1024 / ROW;
-  static constexpr int RING = 4 * HALF;           // two tiles of K and V
+  static constexpr int RING = 2 * HALF;           // a wave's K and V
   static constexpr int REC = D + 4;               // floats of a record: acc [D], max, sum
   static __device__ __forceinline__ int kx(int row) { return row & (CH < 16 ? CH - 1 : 15); }
   static __device__ __forceinline__ int vx(int row) { return F32 ? 0 : 2 * (row & (CH < 16 ? 3 : 7)); }
 };
+
+// (max, sum, acc) records joined in order: NB of them, number k0 + k with
+// get(k, min(k0 + k, count - 1), m, l, o); those from `count` on do not count. o is two
+// of a head's dims.
+struct Joined {
+  float M = kMinusInf, L = 0.f;
+  float2 O = float2{0.f, 0.f};
+};
+__device__ __forceinline__ float record_weight(float m, float l, float M) {
+  return m == kMinusInf ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M);  // (l NaN: scores were)
+}
+template <int NB, typename Get>
+__device__ __forceinline__ void join(Joined &j, int k0, int count, Get get) {
+  float m[NB], l[NB], M = j.M;
+  float2 o[NB];
+#pragma unroll
+  for (int k = 0; k < NB; ++k) get(k, min(k0 + k, count - 1), m[k], l[k], o[k]);
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    if (k0 + k >= count) m[k] = kMinusInf, l[k] = 0.f, o[k] = float2{0.f, 0.f};
+    M = fmaxf(M, m[k]);
+  }
+  const float f0 = record_weight(j.M, j.L, M);
+  j.M = M, j.L *= f0, j.O.x *= f0, j.O.y *= f0;
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const float f = record_weight(m[k], l[k], M);
+    j.L += f * l[k];
+    j.O.x += f * o[k].x;
+    j.O.y += f * o[k].y;
+  }
+}
+// Two floats of a record, written through to where every workgroup sees them
+__device__ __forceinline__ void store_pair(float *p, float x, float y) {
+  const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store((unsigned long long *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// dma16 (common.h) of what others wrote so: past this die's caches
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16_coherent(const void *base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, %2 sc1"
+               :: "v"(voff), "s"(lds), "s"(base) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Inclusive sum over the 64 lanes
+__device__ __forceinline__ int scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return v;
+}
 
 struct Piece {  // of a sequence, that one wave or workgroup went over
   int b, first, n;  // sequence; its first tile in the head's run; its tiles
@@ -191,7 +254,7 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
   __shared__ Piece piece[kPagedWaves][2];
   __shared__ int last_one[2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nw = blockDim.x >> 6, col = lane & 15, g4 = lane >> 4;
+  const int nw = a.waves, col = lane & 15, g4 = lane >> 4;
   const int G = a.Hq / a.Hkv, HT = (G + 15) / 16, heads = a.Hkv * HT, gcap = min(G, 16);
   const int hk = blockIdx.x % heads, unit = blockIdx.x / heads, h = hk / HT, ht = hk - h * HT;
   const int gt = min(16, G - 16 * ht), hq0 = h * G + 16 * ht;
@@ -202,11 +265,7 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
   int total = 0, incl = 0, mine = 0;
   auto scan = [&](int b0) {  // of 64 sequences: lane's tiles and their inclusive sum
     mine = b0 + lane < a.B ? tiles_of(a.lens[b0 + lane]) : 0;
-    incl = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(incl, o);
-      if (lane >= o) incl += y;
-    }
+    incl = scan64(mine);
     return __builtin_amdgcn_readlane(incl, 63);
   };
   for (int b0 = 0; b0 < a.B; b0 += 64) total += scan(b0);
@@ -214,12 +273,15 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
   const Deal deal(total, max(units, 1));
   const int u0 = unit < units ? deal.start(unit) : 0, u1 = unit < units ? deal.start(unit + 1) : 0;
   const Deal waves(u1 - u0, nw);
-  int at = u0 + waves.start(wave), left = u0 + waves.start(wave + 1) - at;
+  int at = u0 + waves.start(wave), left = u0 + waves.start(wave + 1) - at;  // (wave < nw)
   piece[wave][0].b = piece[wave][1].b = -1;
 
-  char *const mem = lds + wave * (T::RING + gcap * T::REC * 4);
-  float *const first_rec = (float *)(mem + T::RING), *const last_rec = (float *)mem;
-  if (left > 0) {
+  // a wave's memory: its tiles, over them its last record when they are done, and its
+  // first record behind both
+  const int rec_bytes = gcap * T::REC * 4, first_at = max(T::RING, rec_bytes);
+  char *const mem = lds + wave * (first_at + rec_bytes);
+  float *const first_rec = (float *)(mem + first_at), *const last_rec = (float *)mem;
+  if (wave < nw && left > 0) {
     // ---- the sequence of the wave's first tile
     int b, t;
     {
@@ -270,8 +332,8 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
       return x;
     };
     const int lrow = lane / T::CH, lch = lane % T::CH;
-    auto copy = [&](const void *pool, const Tile &x, int slot, int half) {
-      const uint32_t dst = lds_addr(mem) + (2 * slot + half) * T::HALF;
+    auto copy = [&](const void *pool, const Tile &x, int half) {
+      const uint32_t dst = lds_addr(mem) + half * T::HALF;
 #pragma unroll
       for (int i = 0; i < T::N; ++i) {
         const int row = i * T::RPI + lrow, sx = half ? T::vx(row) : T::kx(row);
@@ -280,10 +342,10 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
       }
     };
 
-    Tile cur, nx;  // the tile at hand, the one after it
+    Tile cur;  // that the copies out are of
     // ---- q, O and the softmax of the sequence at hand
     constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a head's q per lane
-    u32x4 q[NQ], ql[F32 ? 1 : NQ];
+    u32x4 q[NQ], ql[F32 ? 1 : NQ], qe[F32 ? 1 : NQ];  // (f32 q over bf16 caches: three parts)
     f32x4 o[D / 16];
     float m = kMinusInf, l = 0.f;
     auto start = [&](int seq) {
@@ -304,9 +366,9 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
             const f32x4 r[2] = {*(const f32x4 *)((const float *)a.q + at8), *(const f32x4 *)((const float *)a.q + at8 + 4)};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              uint32_t hi, lo;
-              split_bf16x2(r[e >> 1][2 * (e & 1)], r[e >> 1][2 * (e & 1) + 1], hi, lo);
-              q[i][e] = hi, ql[i][e] = lo;
+              uint32_t x[3];
+              split_bf16x2(r[e >> 1][2 * (e & 1)], r[e >> 1][2 * (e & 1) + 1], x);
+              q[i][e] = x[0], ql[i][e] = x[1], qe[i][e] = x[2];
             }
           } else {
             q[i] = *(const u32x4 *)((const uint16_t *)a.q + at8);
@@ -319,7 +381,7 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
       for (int i = 0; i < D / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
     // dims of o[i]: bf16 16 i + 4 g4 + r; f32 64 (i / 4) + 16 g4 + 4 r + i % 4
-    auto finish = [&](int seq, int first, bool whole, float *rec, Piece *p) {
+    auto finish = [&](int seq, int first, int n, bool whole, float *rec, Piece *p) {
       const float sum = sum4(l);
       if (whole) {
         if (col < gt) {
@@ -349,7 +411,7 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
         }
         if (g4 == 0) rec[col * T::REC + D] = m, rec[col * T::REC + D + 1] = sum;
       }
-      if (lane == 0) *p = Piece{seq, first, cur.n};
+      if (lane == 0) *p = Piece{seq, first, n};
     };
 
     // (q is on its way while the first pages are looked up, and in before the copies
@@ -358,48 +420,47 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
     cur = next(left > 1);
 #pragma unroll
     for (int i = 0; i < NQ; ++i) asm volatile("" : "+v"(q[i]));
-    copy(a.kp, cur, 0, 0);
-    copy(a.vp, cur, 0, 1);
-    if (left > 1) {
-      nx = next(left > 2);
-      copy(a.kp, nx, 1, 0);
-      copy(a.vp, nx, 1, 1);
-    }
+    copy(a.kp, cur, 0);
+    copy(a.vp, cur, 1);
 
     // LDS byte addresses of the fragments in tile 0 (the swizzles are XORs below)
     const uint32_t kf = lds_addr(mem) + col * T::ROW;
     const int tr_j = col >> 2, tr_q = col & 3;
     const uint32_t vf = lds_addr(mem) + T::HALF + (F32 ? 4 * g4 * T::ROW + 16 * col : (4 * g4 + tr_j) * T::ROW + 8 * (tr_q & 1));
     int begun = cur.t;  // the tile at which this wave began the sequence
-    for (int i = 0;; ++i) {
-      const int slot = i & 1;
-      if (left > 1) wait_vm<3 * T::N>();
-      else wait_vm<T::N>();
+    for (;;) {
+      wait_vm<T::N>();  // (copies complete in order: all but this tile's V)
       f32x4 s[T::SUB];
-      const uint32_t ka = kf + slot * 2 * T::HALF;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        constexpr int NA = F32 ? 4 : 2;  // sums in turn: no product waits for the one before
+        f32x4 acc[NA];
+#pragma unroll
+        for (int n = 0; n < NA; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           const u32x4 f = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(
-              ka + u * 16 * T::ROW + (((4 * n + g4) ^ T::kx(col)) << 4));
+              kf + u * 16 * T::ROW + (((4 * n + g4) ^ T::kx(col)) << 4));
           if constexpr (F32) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f[e]), __uint_as_float(q[n][e]), s[u], 0, 0, 0);
+              acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f[e]), __uint_as_float(q[n][e]), acc[e], 0, 0, 0);
           } else {
-            s[u] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[n]), s[u]);
-            if (a.q_f32) s[u] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[n]), s[u]);
+            acc[n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[n]), acc[n & 1]);
+            if (a.q_f32) {
+              acc[~n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[n]), acc[~n & 1]);
+              acc[n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[n]), acc[n & 1]);
+            }
           }
         }
+        s[u] = acc[0] + acc[1];
+        if constexpr (F32) s[u] += acc[2] + acc[3];
       }
       wait_lds();
       const Tile done = cur;
-      Tile nn;
-      if (left > 2) {
-        nn = next(left > 3);
-        copy(a.kp, nn, slot, 0);
+      if (left > 1) {
+        cur = next(left > 2);
+        copy(a.kp, cur, 0);
       }
       // ---- softmax
       const bool part = done.seen < T::KT || done.holes;
@@ -429,19 +490,17 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
           l += s[u][r];
         }
       // ---- O^T += V^T P^T
-      if (left > 2) wait_vm<3 * T::N>();
-      else if (left > 1) wait_vm<2 * T::N>();
+      if (left > 1) wait_vm<T::N>();
       else wait_vm<0>();
       if (part) {
 #pragma unroll
         for (int n = 0; n < T::N; ++n) {
           const int row = n * T::RPI + lrow;
           if (row >= done.seen || (done.holes >> (row >> 4) & 1))
-            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(lds_addr(mem) + (2 * slot + 1) * T::HALF + 1024 * n + 16 * lane) = u32x4{0, 0, 0, 0};
+            *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(lds_addr(mem) + T::HALF + 1024 * n + 16 * lane) = u32x4{0, 0, 0, 0};
         }
         wait_lds();
       }
-      const uint32_t va = vf + slot * 2 * T::HALF;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u) {
         if constexpr (F32) {
@@ -449,45 +508,58 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int n = 0; n < D / 64; ++n) {
-              const u32x4 f = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(va + r * T::ROW + 256 * n);
+              const u32x4 f = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(vf + r * T::ROW + 256 * n);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 o[4 * n + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f[e]), s[u][r], o[4 * n + e], 0, 0, 0);
             }
         } else {
-          uint2 hi, lo;
-          split_bf16x2(s[u][0], s[u][1], hi.x, lo.x);
-          split_bf16x2(s[u][2], s[u][3], hi.y, lo.y);
+          uint32_t p01[3], p23[3];
+          if (a.out_f32) {
+            split_bf16x2(s[u][0], s[u][1], p01);
+            split_bf16x2(s[u][2], s[u][3], p23);
+          } else {
+            uint32_t x[2], y[2];
+            split_bf16x2(s[u][0], s[u][1], x);
+            split_bf16x2(s[u][2], s[u][3], y);
+            p01[0] = x[0], p01[1] = x[1], p23[0] = y[0], p23[1] = y[1];
+          }
 #pragma unroll
           for (int n = 0; n < D / 16; ++n) {
             const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
-                va + u * 16 * T::ROW + (((2 * n + (tr_q >> 1)) ^ T::vx(4 * g4 + tr_j)) << 4)));
-            o[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, hi), o[n], 0, 0, 0);
-            o[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, lo), o[n], 0, 0, 0);
+                vf + u * 16 * T::ROW + (((2 * n + (tr_q >> 1)) ^ T::vx(4 * g4 + tr_j)) << 4)));
+            auto add = [&](int k) {
+              o[n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, (uint2{p01[k], p23[k]})), o[n], 0, 0, 0);
+            };
+            add(0);
+            add(1);
+            if (a.out_f32) add(2);
           }
         }
       }
       wait_lds();
-      if (left > 2) copy(a.vp, nn, slot, 1);
+      if (left > 1) copy(a.vp, cur, 1);
       // ---- the sequence's end, or the wave's
       const bool ends = done.t == done.n - 1;
       if (ends || left == 1) {
         const bool whole = ends && begun == 0;
-        finish(done.b, at - done.t, whole, left > 1 ? first_rec : last_rec, &piece[wave][left > 1 ? 0 : 1]);
+        finish(done.b, at - done.t, done.n, whole, left > 1 ? first_rec : last_rec, &piece[wave][left > 1 ? 0 : 1]);
       }
       ++at;
       if (--left == 0) break;
-      cur = nx;
-      nx = nn;
       if (ends) {
         start(cur.b);
+        // (waited for here, with the copies ahead of it: a wait at the loop's top
+        // would drain the ring at every tile)
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) asm volatile("" : "+v"(q[n]));
         begun = 0;
       }
     }
   }
 
   // ---- rows of sequences without keys
-  for (int b = unit * nw + wave; b < a.B; b += a.units * nw)
+  for (int b = unit * kPagedWaves + wave; b < a.B; b += a.units * kPagedWaves)
     if (tiles_of(uniform_load(a.lens, b)) == 0)
       for (int i = lane; i < gt * D; i += 64) {
         const int64_t to = ((int64_t)b * a.Hq + hq0) * D + i;
@@ -496,104 +568,110 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
       }
   if (unit >= units) return;
 
-  // ---- the waves' pieces, in order; a sequence's are next to each other
+  // ---- the waves' pieces, in order: lane 2 w + k has wave w's k-th
   __syncthreads();
-  auto write = [&](int b, int i, float y) {
-    const int64_t to = ((int64_t)b * a.Hq + hq0) * D + i;
-    if (a.out_f32) ((float *)a.out)[to] = y;
-    else ((uint16_t *)a.out)[to] = f32_to_bf16_bits(y);
+  Piece mine_p;
+  mine_p.b = -1, mine_p.first = mine_p.n = 0;
+  if (lane < 2 * nw) mine_p = piece[lane >> 1][lane & 1];
+  const int64_t rec_size = (gcap * T::REC + 255) & ~255;  // of a record in device memory: whole KiB
+  constexpr int DP = D / 2;  // a thread joins two dims of a head
+  auto write = [&](int b, int i, const Joined &j) {
+    const int64_t to = ((int64_t)b * a.Hq + hq0) * D + 2 * i;
+    const float inv = j.L == 0.f ? 0.f : 1.0f / j.L;
+    if (a.out_f32) *(float2 *)((float *)a.out + to) = float2{j.O.x * inv, j.O.y * inv};
+    else *(uint32_t *)((uint16_t *)a.out + to) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
   };
-  const int64_t rec_size = (int64_t)gcap * T::REC;
-  Piece out[2];  // sequences that other workgroups have keys of: from before, and onwards
-  out[0].b = out[1].b = -1;
-  for (int e = 0; e < 2 * nw;) {
-    const Piece p = piece[e >> 1][e & 1];
-    if (p.b < 0) {
-      ++e;
-      continue;
-    }
-    int e1 = e + 1;
-    while (e1 < 2 * nw && (piece[e1 >> 1][e1 & 1].b < 0 || piece[e1 >> 1][e1 & 1].b == p.b)) ++e1;
-    const bool whole = p.first >= u0 && p.first + p.n <= u1;
-    const int which = p.first >= u0;
-    float *to = a.part + (((int64_t)hk * a.units + unit) * 2 + which) * rec_size;
-    if (!whole) out[which] = p;
-    for (int i = threadIdx.x; i < gt * D; i += blockDim.x) {
-      const int r = i / D, d = i - r * D;
-      auto rec = [&](int x) {
-        return (const float *)(lds + (x >> 1) * (T::RING + gcap * T::REC * 4) + ((x & 1) ? 0 : T::RING)) + r * T::REC;
+  // sequences that other workgroups have keys of: from before, and onwards
+  Piece out0, out1;
+  out0.b = out1.b = -1;
+  for (uint32_t left_p = (uint32_t)__ballot(mine_p.b >= 0); left_p;) {
+    const int e = __builtin_ctz(left_p);
+    Piece p;
+    p.b = __builtin_amdgcn_readlane(mine_p.b, e);
+    p.first = __builtin_amdgcn_readlane(mine_p.first, e);
+    p.n = __builtin_amdgcn_readlane(mine_p.n, e);
+    const uint32_t same = (uint32_t)__ballot(mine_p.b == p.b) & left_p;
+    left_p &= ~same;
+    const bool onwards = p.first >= u0, whole = onwards && p.first + p.n <= u1;
+    if (!whole) (onwards ? out1 : out0) = p;
+    float *const to = a.part + (((int64_t)onwards * heads + hk) * a.units + unit) * rec_size;
+    for (int i = threadIdx.x; i < gt * DP; i += blockDim.x) {
+      const int r = i / DP, d = 2 * (i - r * DP);
+      Joined j;
+      uint32_t bits = same;
+      int x = e;
+      auto get = [&](int, int, float &m, float &l, float2 &o) {
+        if (bits) x = __builtin_ctz(bits), bits &= bits - 1;
+        const float *const rec = (const float *)(lds + (x >> 1) * (first_at + rec_bytes) + ((x & 1) ? 0 : first_at)) + r * T::REC;
+        const float2 ml = *(const float2 *)(rec + D);
+        m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
       };
-      float M = kMinusInf, L = 0.f, O = 0.f;
-      for (int x = e; x < e1; ++x)
-        if (piece[x >> 1][x & 1].b >= 0) M = fmaxf(M, rec(x)[D]);
-      for (int x = e; x < e1; ++x)
-        if (piece[x >> 1][x & 1].b >= 0) {
-          const float *const rx = rec(x);
-          const float f = rx[D] == kMinusInf ? (rx[D + 1] == 0.f ? 0.f : 1.f) : exp2f(rx[D] - M);
-          L += f * rx[D + 1];
-          O += f * rx[d];
-        }
+      const int n = __builtin_popcount(same);
+#pragma unroll 1
+      for (int k0 = 0; k0 < n; k0 += 4) join<4>(j, k0, n, get);
       if (whole) {
-        write(p.b, i, L == 0.f ? 0.f : O / L);
+        write(p.b, i, j);
       } else {
         float *const tr = to + r * T::REC;
-        __hip_atomic_store(tr + d, O, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (d == 0) {
-          __hip_atomic_store(tr + D, M, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-          __hip_atomic_store(tr + D + 1, L, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        store_pair(tr + d, j.O.x, j.O.y);
+        if (d == 0) store_pair(tr + D, j.M, j.L);
       }
     }
-    e = e1;
   }
-  if (out[0].b < 0 && out[1].b < 0) return;
+  if (out0.b < 0 && out1.b < 0) return;
   wait_vm<0>();  // this wave's record stores are done
   __syncthreads();
   int from[2], count[2];
   for (int w = 0; w < 2; ++w) {
-    if (out[w].b < 0) continue;
-    from[w] = deal.taker(out[w].first);
-    count[w] = deal.taker(out[w].first + out[w].n - 1) - from[w] + 1;
-    if (threadIdx.x == 0)
+    const Piece p = w ? out1 : out0;
+    from[w] = p.b < 0 ? 0 : deal.taker(p.first);
+    count[w] = p.b < 0 ? 0 : deal.taker(p.first + p.n - 1) - from[w] + 1;
+    if (p.b >= 0 && threadIdx.x == 64 * w)
       last_one[w] = __hip_atomic_fetch_add(a.counters + (int64_t)hk * a.units + from[w], 1, __ATOMIC_RELAXED,
                                            __HIP_MEMORY_SCOPE_AGENT) == count[w] - 1;
   }
   __syncthreads();
+#pragma unroll 1
   for (int w = 0; w < 2; ++w) {
-    if (out[w].b < 0 || !last_one[w]) continue;
-    // records of workgroups from .. from + count - 1: the first's is its second one
-    const float *const base = a.part + ((int64_t)hk * a.units + from[w]) * 2 * rec_size;
-    auto rec = [&](int c) { return base + (2 * c + (c == 0)) * rec_size; };
-    float *const ml = (float *)lds;  // [count][gt][2]
-    for (int i = threadIdx.x; i < count[w] * gt; i += blockDim.x) {
-      const float *const p = rec(i / gt) + (i % gt) * T::REC + D;
-      ml[2 * i] = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      ml[2 * i + 1] = __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < gt * D; i += blockDim.x) {
-      const int r = i / D, d = i - r * D;
-      float M = kMinusInf, L = 0.f, O = 0.f;
-      for (int c = 0; c < count[w]; ++c) M = fmaxf(M, ml[2 * (c * gt + r)]);
-      for (int c0 = 0; c0 < count[w]; c0 += 8) {
-        float x[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          x[c] = c0 + c < count[w] ? __hip_atomic_load(rec(c0 + c) + r * T::REC + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c0 + c < count[w]) {
-            const float mc = ml[2 * ((c0 + c) * gt + r)], lc = ml[2 * ((c0 + c) * gt + r) + 1];
-            const float f = mc == kMinusInf ? (lc == 0.f ? 0.f : 1.f) : exp2f(mc - M);
-            L += f * lc;
-            O += f * x[c];
+    const Piece p = w ? out1 : out0;
+    if (p.b < 0 || !last_one[w]) continue;
+    // The records: the first workgroup's among those that go onwards, the others' among
+    // those that come from before, one after another, brought into LDS as many at a time
+    // as fit. (This runs once a workgroup, and what it costs beside the round trip is the
+    // fetching of instructions that no cache holds yet: joining 19 records of 4 KiB took
+    // 9 us with the loop over them unrolled.)
+    const int pieces = (int)(rec_size >> 8), fit = T::RING * nw / (1024 * pieces), pairs = gt * DP;
+    const int64_t on = ((int64_t)heads + hk) * a.units + from[w], past = (int64_t)hk * a.units + from[w];
+#pragma unroll 1
+    for (int i0 = 0; i0 < pairs; i0 += blockDim.x) {
+      const int i = min(i0 + (int)threadIdx.x, pairs - 1), r = i / DP, d = 2 * (i - r * DP);
+      Joined j;
+#pragma unroll 1
+      for (int c0 = 0; c0 < count[w]; c0 += fit) {
+        const int n = min(fit, count[w] - c0);
+        if (i0 == 0 || count[w] > fit) {
+          __syncthreads();  // (what LDS holds has been read)
+#pragma unroll 1
+          for (int y = wave; y < n * pieces; y += kPagedWaves) {
+            const int c = y / pieces;
+            dma16_coherent(a.part + (c0 + c == 0 ? on : past + c0 + c) * rec_size + 256 * (y - c * pieces), 16 * lane,
+                           lds_addr(lds) + 1024 * y);
           }
+          wait_vm<0>();
+          __syncthreads();
+        }
+#pragma unroll 1
+        for (int k0 = 0; k0 < n; k0 += 4)
+          join<4>(j, k0, n, [&](int, int c, float &m, float &l, float2 &o) {
+            const float *const rec = (const float *)lds + c * rec_size + r * T::REC;
+            const float2 ml = *(const float2 *)(rec + D);
+            m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
+          });
       }
-      write(out[w].b, i, L == 0.f ? 0.f : O / L);
+      if (i0 + (int)threadIdx.x < pairs) write(p.b, i, j);
     }
     if (threadIdx.x == 0)
       __hip_atomic_store(a.counters + (int64_t)hk * a.units + from[w], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
   }
 }
 

@@ -26,7 +26,7 @@ struct PagedDecodeArgs {
   int B, M, Hq, Hkv, D, ps;
   float c;
   int q_f32, p_f32, out_f32;
-  int units;
+  int units, waves;
   int *counters;
   float *part;
 };
@@ -126,9 +126,9 @@ static float softmax_scale(float scale, int64_t D) {
 
 // The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row
 // pieces, 16-byte aligned operands and tile counts within 32 bits; else the plain
-// kernel. One workgroup fills a CU: as many waves, up to 8, as rings of two tiles and
-// records of the group's heads fit in LDS. `units` workgroups for each kv head (and
-// 16 query heads): the number that leaves the fewest CUs idle in the last round.
+// kernel. As many waves walk keys, up to 8, as tiles and records of the group's heads
+// fit in LDS. `units` workgroups for each kv head (and 16 query heads): the number that
+// leaves the fewest CUs idle in the last round.
 static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   const int64_t G = a.Hq / a.Hkv, heads = a.Hkv * ((G + 15) / 16), gcap = G < 16 ? G : 16;
   const int es = a.p_f32 ? 4 : 2, row = a.D * es, tile = row < 256 ? 32 : 16;
@@ -136,10 +136,10 @@ static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
       ((uintptr_t)a.q | (uintptr_t)a.kp | (uintptr_t)a.vp | (uintptr_t)a.out) % 16 ||
       (int64_t)a.B * (((int64_t)a.M * a.ps + tile - 1) / tile) >= ((int64_t)1 << 30))
     return launch(rt, "rxw8_paged_decode_any", dim3((unsigned)a.B * (unsigned)a.Hq), dim3(256), a);
-  const size_t record = (size_t)gcap * (size_t)(a.D + 4) * sizeof(float), wave = (size_t)(4 * tile * row) + record;
-  const int waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
+  const size_t record = (size_t)gcap * (size_t)(a.D + 4) * sizeof(float), wave = std::max((size_t)(2 * tile * row), record) + record;
+  a.waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>({256, (int64_t)(RXW8_NOALLOC_COUNTER_BYTES / sizeof(int)) / heads,
-                                                               (int64_t)(RXW8_NOALLOC_PARTIAL_BYTES / (2 * record)) / heads}));
+                                                               (int64_t)(RXW8_NOALLOC_PARTIAL_BYTES / (2 * ((record + 1023) & ~(size_t)1023))) / heads}));
   a.units = 1;
   for (int64_t u = 2; u <= most; ++u) {  // rounds of workgroups per unit of work
     const int64_t r0 = (heads * a.units + rt->cus - 1) / rt->cus, r1 = (heads * u + rt->cus - 1) / rt->cus;
@@ -150,7 +150,7 @@ static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   a.part = (float *)(block + RXW8_NOALLOC_COUNTER_BYTES);
   char kname[40];
   std::snprintf(kname, sizeof kname, "rxw8_paged_decode_%s_d%d", a.p_f32 ? "f32" : "bf16", a.D);
-  return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(64 * waves), a, wave * (size_t)waves);
+  return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(512), a, wave * (size_t)a.waves);
 }
 
 static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets,
@@ -207,7 +207,7 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_
   PagedDecodeArgs a{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
                     out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
                     (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32,
-                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32, 0, nullptr, nullptr};
+                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32, 0, 0, nullptr, nullptr};
   return paged_decode_launch(rt, a);
 }
 

@@ -40,10 +40,11 @@ def attend(q, k, v, scale, p_step, out_step):
 
 def paged_keys(pages, table, n, h):
     """Keys (or values) of a sequence's first n positions that have a page."""
-    ps = pages.shape[2]
-    rows = [pages[table[j // ps], h, j % ps] for j in range(min(n, len(table) * ps))
-            if 0 <= table[j // ps] < pages.shape[0]]
-    return np.array(rows, np.float64).reshape(-1, pages.shape[3])
+    ps, rows = pages.shape[2], []
+    for i, page in enumerate(table):
+        if i * ps < n and 0 <= page < pages.shape[0]:
+            rows.append(pages[page, h, :n - i * ps])
+    return np.concatenate(rows).astype(np.float64) if rows else np.zeros((0, pages.shape[3]))
 
 
 def paged_decode(q, kp, vp, table, lens, scale=None, p_step=SPLIT, out_step=F32):

@@ -166,6 +166,20 @@ def test_paged_decode_long_and_ragged(rt, pk, qk, d, hq, hkv):
     assert np.array_equal(y, decode(rt, q, qk, kp, vp, pk, table, lens))
 
 
+@pytest.mark.parametrize("pk,d,hq,hkv", [("bf16", 128, 16, 1), ("bf16", 256, 16, 1), ("f32", 64, 3, 1),
+                                         ("bf16", 64, 34, 2)])
+def test_paged_decode_pieces(rt, pk, d, hq, hkv):
+    """So many keys that waves take several tiles each, some of them the end of one sequence and
+    the beginning of another; up to 17 query heads to a kv head."""
+    rng = np.random.default_rng(d)
+    lens = rng.integers(1500, 2600, 64)
+    lens[10:20] = rng.integers(0, 40, 10)
+    q = floats(rng, (64, hq, d), "f32")
+    kp, vp, table = make_pages(rng, lens, hkv, 16, d, pk)
+    y = decode(rt, q, "f32", kp, vp, pk, table, lens)
+    check(y, *ref.paged_decode(q, kp, vp, table, lens))
+
+
 @pytest.mark.parametrize("batch", [63, 64, 65, 130, 700])
 def test_paged_decode_many_sequences(rt, batch):
     rng = np.random.default_rng(batch)
