@@ -1,6 +1,8 @@
 // Causal attention of packed prompts: sequence b owns rows offsets[b] ..
 // offsets[b + 1] - 1 of q [T, Hq, D] and of k, v [T, Hkv, D], and row t of it sees
 // rows offsets[b] .. t. Offsets are read on the device and clamped into [0, T].
+#include <type_traits>
+
 #include "attn_any.h"
 
 struct PackedArgs {
@@ -13,6 +15,7 @@ struct PackedArgs {
   float c;                     // scale log2 e
   int q_f32, out_f32;
   int fill;                    // rows outside every sequence: zeros (else left as they are)
+  int heads;                   // query heads of a workgroup (1, 2 or 4; divides Hq / Hkv)
 };
 
 // Any head width up to 512: one wave per (row, query head).
@@ -36,3 +39,442 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_prefill_any(Packed
            [&](int64_t j) { return (j * a.Hkv + h) * a.D; });
   any_store(st, a.out, unit * a.D, a.D, a.out_f32);
 }
+
+// Rows outside every sequence of a new output
+extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a) {
+  const int64_t first = min((int64_t)max(a.offsets[0], 0), a.T), end = min((int64_t)max(a.offsets[a.B], 0), a.T);
+  const int64_t row = (int64_t)a.Hq * a.D, n = a.T * row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t at = i < first * row ? i : end * row + (i - first * row);
+    if (at >= n) return;
+    if (a.out_f32) ((float *)a.out)[at] = 0.f;
+    else ((uint16_t *)a.out)[at] = 0;
+  }
+}
+
+// ---- head widths 64, 128, 256 on the matrix cores ------------------------------------
+//
+// A workgroup of 4 waves, one to a SIMD, takes 4 x 32 QT rows: HW query heads of one kv
+// head times 4 / HW groups of 32 QT rows of one sequence. It walks the sequence's keys
+// in steps of 32, whose K and V rows it copies by LDS DMA into rings of 4 (row-major,
+// 16-byte chunks XOR-swizzled by row), two to three steps ahead, a barrier a step.
+// Per wave and step, on 32x32x16 bf16 products:
+//   S^T = K q^T     lane (l % 32) = row, keys 8 (r / 4) + 4 (l / 32) + r % 4 in register r;
+//   p = exp2(c s - m), m the row's reference;
+//   O^T += V^T P^T  P straight from the score registers, V^T by transposing LDS reads
+//                   in the same order of keys.
+// In a step the products are those of S one step ahead and of O one step behind, so
+// none of them waits for the softmax between: every LDS read is followed by its
+// products, and these by a share of the softmax, in that order (a barrier to the
+// scheduler keeps it). One fragment of K or V serves 32 QT rows: at QT = 2 the LDS reads
+// take half the time of the products. bf16 q and outputs run QT = 2 (one at D = 256, by
+// registers: O alone is 32 QT D / 64 of them); f32 ones split q and P in their three bf16
+// parts (exact products, f32 sums) and run QT = 1.
+//
+// m is not every step's maximum: it stays while a lane's 16 weights sum to 2^8 at most
+// (p then keeps bf16's range; l and O carry the same factor), and most steps take no
+// maximum and rescale nothing. The steps on the diagonal run one after the other, with
+// the mask; V values there that are no numbers are left out of the products (a row that
+// does not see a key has 0 for it, and 0 times them is not 0) and given to the rows that
+// see them.
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float max_xor32(float v) {
+  const uint2 p = pair_xor32(v);
+  return fmaxf(__uint_as_float(p.x), __uint_as_float(p.y));
+}
+// Sum over the 64 lanes, in every lane
+__device__ __forceinline__ int sum64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+constexpr int kStep = 32;  // keys
+constexpr int kRing = 4;
+
+}  // namespace
+
+// P: bf16 parts of q and of the weights (1 or 3)
+template <int D, int QT, int P>
+__device__ void packed_prefill(const PackedArgs &a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [kRing][32][D] K, the same V
+  constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
+  constexpr int NK = D / 16, ND = D / 32, WR = 32 * QT;                            // WR: rows of a wave
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hf = lane >> 5;
+  const int G = a.Hq / a.Hkv, HW = a.heads, RG = 4 / HW, ROWS = WR * RG, HP = G / HW, per = a.Hkv * HP;
+  const int kvh = blockIdx.x % a.Hkv, hp = blockIdx.x / a.Hkv % HP;
+  int rank = blockIdx.x / per;
+
+  // ---- the row tile: those that see the most keys first
+  int64_t first = 0;
+  int len = 0, tile = -1;
+  auto bounds = [&](int b, int64_t &s) {
+    s = min((int64_t)max(a.offsets[b], 0), a.T);
+    const int64_t e = min((int64_t)max(a.offsets[b + 1], 0), a.T);
+    return (int)max(e - s, (int64_t)0);
+  };
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int64_t s = 0;
+    const int n = b0 + lane < a.B ? bounds(b0 + lane, s) : 0, tiles = (n + ROWS - 1) / ROWS;
+    const int all = sum64(tiles);
+    if (rank >= all) {  // (of another 64 sequences)
+      rank -= all;
+      continue;
+    }
+    // tiles of index x and above, over the sequences: more than rank for x = lo, not for hi
+    int lo = 0, hi = (int)min((a.T + ROWS - 1) / ROWS, (int64_t)all), above = 0;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1, c = sum64(max(tiles - mid, 0));
+      if (c > rank) lo = mid;
+      else hi = mid;
+    }
+    above = sum64(max(tiles - lo - 1, 0));
+    const unsigned long long have = __ballot(tiles > lo);
+    const bool me = tiles > lo && __popcll(have & ((1ull << lane) - 1)) == rank - above;
+    const int src = __builtin_ctzll(__ballot(me));
+    tile = lo;
+    len = __builtin_amdgcn_readlane(n, src);
+    first = (uint32_t)__builtin_amdgcn_readlane((int)s, src);  // (T is below 2^31)
+    break;
+  }
+  if (tile < 0) return;
+
+  const int head = wave % HW, r0 = tile * ROWS + wave / HW * WR;  // the wave's first row
+  const int hq = kvh * G + hp * HW + head;
+  const int last_row = min(tile * ROWS + ROWS, len);              // past the workgroup's rows
+  const int steps = (last_row + kStep - 1) / kStep;
+  const int full = r0 / kStep;                                     // steps without a mask
+  const int mine = r0 < len ? (min(r0 + WR, len) + kStep - 1) / kStep : 0;
+
+  // ---- copies: instruction i of a wave takes rows RPI (4 i + wave) .. of a step's 32
+  constexpr int RPI = 1024 / ROWB;
+  auto kx = [](int row) { return row & (CH < 16 ? CH - 1 : 15); };
+  auto vx = [](int row) { return 2 * (row & (CH < 16 ? 3 : 7)); };
+  const uint32_t stride = (uint32_t)a.Hkv * ROWB;
+  const char *const kbase = (const char *)a.k + (first * a.Hkv + kvh) * ROWB;
+  const char *const vbase = (const char *)a.v + (first * a.Hkv + kvh) * ROWB;
+  auto copy = [&](const char *base, int step, bool is_v) {
+    const uint32_t dst = lds_addr(lds) + ((is_v ? kRing : 0) + (step & (kRing - 1))) * TILE;
+    const char *const from = base + (int64_t)step * kStep * stride;
+    const int most = len - 1 - step * kStep;  // (rows past the sequence repeat its last)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = RPI * (4 * i + wave) + lane / CH, x = is_v ? vx(row) : kx(row);
+      dma16(from, (uint32_t)min(row, most) * stride + (((lane % CH) ^ x) << 4), dst + 1024 * (4 * i + wave));
+    }
+  };
+  copy(kbase, 0, false);
+  copy(vbase, 0, true);
+
+  // ---- q
+  u32x4 q[QT][NK][P];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int64_t at = ((first + min(r0 + 32 * t + col, len - 1)) * a.Hq + hq) * D + 8 * hf;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      if (P == 3 && a.q_f32) {
+        const f32x4 x = *(const f32x4 *)((const float *)a.q + at + 16 * n), y = *(const f32x4 *)((const float *)a.q + at + 16 * n + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t part[3];
+          split_bf16x2(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], part);
+#pragma unroll
+          for (int p = 0; p < P; ++p) q[t][n][p][e] = part[p];
+        }
+      } else {
+        q[t][n][0] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * n);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+#pragma unroll
+    for (int n = 0; n < NK; ++n) asm volatile("" : "+v"(q[t][n][0]));  // (in before more copies go out)
+  if (steps > 1) {
+    copy(kbase, 1, false);
+    copy(vbase, 1, true);
+  }
+  if (steps > 2) copy(kbase, 2, false);
+
+  // ---- state
+  f32x16 o[QT][ND], sa[QT], sb[QT];
+  u32x4 pa[QT][2][P], pb[QT][2][P];
+  float m[QT], l[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    m[t] = 0.f, l[t] = 0.f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[t][d][r] = 0.f;
+  }
+  const float c = a.c;
+  int h = 0;
+  // Before step h every wave's copies of K up to h + 1 and V up to h are in; the slots
+  // of K h - 1 and V h - 2 are free.
+  auto begin = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    if (h + 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (h + 2 < steps) copy(vbase, h + 2, true);
+    if (h + 3 < steps) copy(kbase, h + 3, false);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const uint32_t k0 = lds_addr(lds) + col * ROWB;
+  const int tr_j = (lane & 15) >> 2, tr_q = lane & 3;
+  const uint32_t v0 = lds_addr(lds) + kRing * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1);
+  const int v_chunk = 2 * ((lane >> 4) & 1) + (tr_q >> 1);
+  auto k_frag = [&](int step, int n) {
+    return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(
+        k0 + (step & (kRing - 1)) * TILE + (((2 * n + hf) ^ kx(col)) << 4));
+  };
+  auto v_frag = [&](int step, int ks, int d) {
+    u32x4 f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // keys 16 ks + 8 e + 4 hf + j; their swizzle: rows 8 apart share it
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
+          v0 + (step & (kRing - 1)) * TILE + (16 * ks + 8 * e) * ROWB + (((4 * d + v_chunk) ^ vx(4 * hf + tr_j)) << 4)));
+      const uint2 u = __builtin_bit_cast(uint2, x);
+      f[2 * e] = u.x, f[2 * e + 1] = u.y;
+    }
+    return f;
+  };
+  const int qparts = P == 3 && a.q_f32 ? 3 : 1;
+  auto qk = [&](f32x16 (&s)[QT], int n, u32x4 f) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      if (n == 0)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+      s[t] = mfma32(f, q[t][n][0], s[t]);
+      if (P == 3 && qparts == 3) {
+        s[t] = mfma32(f, q[t][n][1 % P], s[t]);
+        s[t] = mfma32(f, q[t][n][2 % P], s[t]);
+      }
+    }
+  };
+  auto pv = [&](u32x4 (&p)[QT][2][P], int ks, int d, u32x4 f) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int x = 0; x < P; ++x) o[t][d] = mfma32(f, p[t][ks][x], o[t][d]);
+  };
+  // weights 2 i and 2 i + 1 of a lane's 16 (of row tile t)
+  auto pair = [&](f32x16 (&s)[QT], u32x4 (&p)[QT][2][P], float (&ls)[QT], int t, int i) {
+    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i], c, -m[t]));
+    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i + 1], c, -m[t]));
+    ls[t] += e0 + e1;
+    if constexpr (P == 1) {
+      p[t][i >> 2][0][i & 3] = pack_bf16x2(e0, e1);
+    } else {
+      uint32_t part[3];
+      split_bf16x2(e0, e1, part);
+#pragma unroll
+      for (int x = 0; x < P; ++x) p[t][i >> 2][x][i & 3] = part[x];
+    }
+  };
+  // after a step's weights: l, or where they were too large, or at the first step, a new
+  // reference, O and l to it, and the weights again
+  auto settle = [&](f32x16 (&s)[QT], u32x4 (&p)[QT][2][P], float (&ls)[QT], bool first_step) {
+    bool moves = first_step;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) moves |= !(ls[t] <= 256.f);
+    if (__ballot(moves)) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float mx = kMinusInf;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
+        mx = max_xor32(mx) * c;
+        const float to = first_step ? (mx == kMinusInf ? 0.f : mx) : fmaxf(m[t], mx);
+        const float f = first_step ? 0.f : __builtin_amdgcn_exp2f(m[t] - to);
+        m[t] = to;
+        l[t] = first_step ? 0.f : l[t] * f;
+        if (!first_step)
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[t][d] *= f;
+        ls[t] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pair(s, p, ls, t, i);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) l[t] += ls[t];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // One step of the pipeline: K of step h + 1 (QK), V of step h - 1 (PV), softmax of h
+  constexpr int AHEAD = 4;
+  auto body = [&](auto with_pv, auto with_qk, f32x16 (&s)[QT], f32x16 (&sn)[QT], u32x4 (&p)[QT][2][P],
+                  u32x4 (&pn)[QT][2][P]) {
+    constexpr bool PV = decltype(with_pv)::value, QK = decltype(with_qk)::value;
+    constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NP = 8 * QT;  // fragments, pairs of weights
+    static_assert(NK == 2 * ND, "K and V take turns");
+    u32x4 fr[AHEAD + 1];
+    auto is_k = [](int n) { return QK && (!PV || n % 2 == 0); };
+    auto at = [](int n) { return QK && PV ? n / 2 : n; };
+    auto read = [&](int n) {
+      fr[n % (AHEAD + 1)] = is_k(n) ? k_frag(h + 1, at(n)) : v_frag(h - 1, at(n) / ND, at(n) % ND);
+    };
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) read(n);
+    float ls[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) ls[t] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (n + AHEAD < NF) read(n + AHEAD);
+      const u32x4 f = fr[n % (AHEAD + 1)];
+      if (is_k(n)) qk(sn, at(n), f);
+      else pv(p, at(n) / ND, at(n) % ND, f);
+#pragma unroll
+      for (int i = n * NP / NF; i < (n + 1) * NP / NF; ++i) pair(s, pn, ls, i / 8, i % 8);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    settle(s, pn, ls, !PV && h == 0);
+  };
+  // A step on its own: scores, mask, softmax, output
+  auto alone = [&](bool masked) {
+#pragma unroll
+    for (int n = 0; n < NK; ++n) qk(sa, n, k_frag(h, n));
+    if (masked) {
+      const int rel = r0 + col - h * kStep - 4 * hf;  // the last key a row of tile 0 sees, minus the lane's first
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (8 * (r >> 2) + (r & 3) > rel + 32 * t) sa[t][r] = kMinusInf;
+    }
+    float ls[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      ls[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) pair(sa, pa, ls, t, i);
+    }
+    settle(sa, pa, ls, h == 0);
+    bool odd = false;  // a value of V that is no number
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < 2 * ND; ++n) {
+        const u32x4 f = v_frag(h, n / ND, n % ND);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (f[e] & 0x7f80u) == 0x7f80u || (f[e] & 0x7f800000u) == 0x7f800000u;
+      }
+      odd = __ballot(odd) != 0;
+    }
+    if (!odd) {
+#pragma unroll
+      for (int n = 0; n < 2 * ND; ++n) pv(pa, n / ND, n % ND, v_frag(h, n / ND, n % ND));
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < 2 * ND; ++n) {
+      u32x4 f = v_frag(h, n / ND, n % ND);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((f[e] & 0x7f80u) == 0x7f80u) f[e] &= 0xffff0000u;
+        if ((f[e] & 0x7f800000u) == 0x7f800000u) f[e] &= 0xffffu;
+      }
+      pv(pa, n / ND, n % ND, f);
+    }
+#pragma unroll 1
+    for (int key = 0; key < kStep; ++key) {
+      const uint32_t row = lds_addr(lds) + (kRing + (h & (kRing - 1))) * TILE + key * ROWB;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int dim = 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3);
+          const uint32_t x = *(const __attribute__((address_space(3))) uint16_t *)(uintptr_t)(
+              row + (((dim >> 3) ^ vx(key)) << 4) + 2 * (dim & 7));
+          if ((x & 0x7f80u) == 0x7f80u)
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              if (h * kStep + key <= r0 + 32 * t + col) o[t][d][r] += bf16_bits_to_f32(x);
+        }
+    }
+  };
+
+  if (mine > 0) {
+    if (full & 1) {
+      begin();
+      alone(false);
+      ++h;
+    }
+    bool pending = false;
+    if (h < full) {
+      begin();
+#pragma unroll
+      for (int n = 0; n < NK; ++n) qk(sa, n, k_frag(h, n));
+      body(std::false_type{}, std::true_type{}, sa, sb, pb, pa);
+      ++h;
+      while (h + 1 < full) {
+        begin();
+        body(std::true_type{}, std::true_type{}, sb, sa, pa, pb);
+        ++h;
+        begin();
+        body(std::true_type{}, std::true_type{}, sa, sb, pb, pa);
+        ++h;
+      }
+      begin();
+      body(std::true_type{}, std::false_type{}, sb, sa, pa, pb);
+      ++h;
+      pending = true;
+    }
+    for (; h < mine; ++h) {
+      begin();
+      if (pending) {
+#pragma unroll
+        for (int n = 0; n < 2 * ND; ++n) pv(pb, n / ND, n % ND, v_frag(h - 1, n / ND, n % ND));
+        pending = false;
+      }
+      alone(true);
+    }
+  }
+  for (; h < steps; ++h) begin();  // the other waves' rows
+  if (mine == 0) return;
+
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float sum = sum_xor32(l[t]), inv = sum == 0.f ? 0.f : 1.0f / sum;
+    const int row = r0 + 32 * t + col;
+    if (row >= len) continue;
+    const int64_t to = ((first + row) * a.Hq + hq) * D + 4 * hf;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const f32x4 y = f32x4{o[t][d][4 * x], o[t][d][4 * x + 1], o[t][d][4 * x + 2], o[t][d][4 * x + 3]} * inv;
+        if (a.out_f32)
+          *(f32x4 *)((float *)a.out + to + 32 * d + 8 * x) = y;
+        else
+          *(uint2 *)((uint16_t *)a.out + to + 32 * d + 8 * x) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      }
+  }
+}
+
+#define RXW8_PACKED_PREFILL(D, QT, P, NAME)                                                          \
+  extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))       \
+      rxw8_packed_prefill_##NAME##_d##D(PackedArgs a) {                                              \
+    packed_prefill<D, QT, P>(a);                                                                     \
+  }
+RXW8_PACKED_PREFILL(64, 2, 1, bf16)
+RXW8_PACKED_PREFILL(128, 2, 1, bf16)
+RXW8_PACKED_PREFILL(256, 1, 1, bf16)
+RXW8_PACKED_PREFILL(64, 1, 3, f32)
+RXW8_PACKED_PREFILL(128, 1, 3, f32)
+RXW8_PACKED_PREFILL(256, 1, 3, f32)

@@ -40,6 +40,7 @@ struct PackedArgs {
   float c;
   int q_f32, out_f32;
   int fill;
+  int heads;
 };
 struct SampleArgs {
   const void *logits;
@@ -157,10 +158,25 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
                          float scale, const Buffer *out, bool fill) {
   const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2];
   if (T == 0) return RXW8_OK;
+  const int64_t B = offsets->dims[0] - 1, Hkv = k->dims[1], G = Hq / Hkv;
   PackedArgs a{q->ptr, (const uint16_t *)k->ptr, (const uint16_t *)v->ptr, (const int32_t *)offsets->ptr, out->ptr, T,
-               (int)(offsets->dims[0] - 1), (int)Hq, (int)k->dims[1], (int)D, softmax_scale(scale, D),
-               q->dtype == RXW8_F32, out->dtype == RXW8_F32, fill};
-  return launch(rt, "rxw8_packed_prefill_any", dim3((unsigned)((T * Hq + 3) / 4)), dim3(256), a);
+               (int)B, (int)Hq, (int)Hkv, (int)D, softmax_scale(scale, D), q->dtype == RXW8_F32,
+               out->dtype == RXW8_F32, fill, G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1};
+  // Row tiles of a workgroup: 4 waves of 32 or 64 rows (kernels/packed.hip) over its
+  // heads; at most one more than T's for each sequence
+  const bool f32 = a.q_f32 || a.out_f32;
+  const int64_t rows = (f32 || D == 256 ? 32 : 64) * (4 / a.heads);
+  const int64_t grid = ((T + rows - 1) / rows + B) * (Hq / a.heads);
+  if ((D != 64 && D != 128 && D != 256) || Hkv * D * 2 * 32 >= ((int64_t)1 << 31) || grid > kGridMax ||
+      ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16)
+    return launch(rt, "rxw8_packed_prefill_any", dim3((unsigned)((T * Hq + 3) / 4)), dim3(256), a);
+  if (fill) {
+    int rc = launch(rt, "rxw8_packed_fill", dim3((unsigned)std::min<int64_t>((T * Hq * D + 255) / 256, 2048)), dim3(256), a);
+    if (rc) return rc;
+  }
+  char kname[40];
+  std::snprintf(kname, sizeof kname, "rxw8_packed_prefill_%s_d%d", f32 ? "f32" : "bf16", (int)D);
+  return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, (size_t)(2 * 4 * 32 * 2) * (size_t)D);
 }
 
 }  // namespace rxw8
