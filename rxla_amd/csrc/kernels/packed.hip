@@ -71,16 +71,18 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a)
 // registers: O alone is 32 QT D / 64 of them); f32 ones split q and P in their three bf16
 // parts (exact products, f32 sums) and run QT = 1.
 //
-// m is not every step's maximum: it stays while a lane's 16 weights sum to 2^8 at most
-// (p then keeps bf16's range; l and O carry the same factor), and most steps take no
-// maximum and rescale nothing. The steps on the diagonal run one after the other, with
-// the mask; V values there that are no numbers are left out of the products (a row that
-// does not see a key has 0 for it, and 0 times them is not 0) and given to the rows that
-// see them.
+// m is the maximum of the row's first 32 keys and does not move: weights may grow past 1
+// as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l or O leaves that
+// range, or meets values that are no numbers (a key that a row does not see has weight 0,
+// and 0 times an infinity is none), are done again, key by key, by the wave alone.
+// (the lambdas below hold the wave's registers: they have to be part of the kernel)
+#define RXW8_INLINE __attribute__((always_inline))
+
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
@@ -100,13 +102,22 @@ __device__ __forceinline__ int sum64(int v) {
   return __builtin_amdgcn_readlane(v, 63);
 }
 
+// f(0), f(1), .., f(N - 1) with constants for arguments
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
+
 constexpr int kStep = 32;  // keys
 constexpr int kRing = 4;
 
 }  // namespace
 
-// P: bf16 parts of q and of the weights (1 or 3)
-template <int D, int QT, int P>
+// PQ, P: bf16 parts of q and of the weights (1 or 3)
+template <int D, int QT, int PQ, int P>
 __device__ void packed_prefill(const PackedArgs &a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [kRing][32][D] K, the same V
   constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
@@ -165,7 +176,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
   const uint32_t stride = (uint32_t)a.Hkv * ROWB;
   const char *const kbase = (const char *)a.k + (first * a.Hkv + kvh) * ROWB;
   const char *const vbase = (const char *)a.v + (first * a.Hkv + kvh) * ROWB;
-  auto copy = [&](const char *base, int step, bool is_v) {
+  auto copy = [&](const char *base, int step, bool is_v) RXW8_INLINE {
     const uint32_t dst = lds_addr(lds) + ((is_v ? kRing : 0) + (step & (kRing - 1))) * TILE;
     const char *const from = base + (int64_t)step * kStep * stride;
     const int most = len - 1 - step * kStep;  // (rows past the sequence repeat its last)
@@ -177,38 +188,33 @@ __device__ void packed_prefill(const PackedArgs &a) {
   };
   copy(kbase, 0, false);
   copy(vbase, 0, true);
-
-  // ---- q
-  u32x4 q[QT][NK][P];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int64_t at = ((first + min(r0 + 32 * t + col, len - 1)) * a.Hq + hq) * D + 8 * hf;
-#pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      if (P == 3 && a.q_f32) {
-        const f32x4 x = *(const f32x4 *)((const float *)a.q + at + 16 * n), y = *(const f32x4 *)((const float *)a.q + at + 16 * n + 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t part[3];
-          split_bf16x2(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], part);
-#pragma unroll
-          for (int p = 0; p < P; ++p) q[t][n][p][e] = part[p];
-        }
-      } else {
-        q[t][n][0] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * n);
-      }
-    }
-  }
-#pragma unroll
-  for (int t = 0; t < QT; ++t)
-#pragma unroll
-    for (int n = 0; n < NK; ++n) asm volatile("" : "+v"(q[t][n][0]));  // (in before more copies go out)
   if (steps > 1) {
     copy(kbase, 1, false);
     copy(vbase, 1, true);
   }
   if (steps > 2) copy(kbase, 2, false);
 
+  // ---- q
+  u32x4 q[QT][NK][PQ];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int64_t at = ((first + min(r0 + 32 * t + col, len - 1)) * a.Hq + hq) * D + 8 * hf;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      if constexpr (PQ == 3) {
+        const f32x4 x = *(const f32x4 *)((const float *)a.q + at + 16 * n), y = *(const f32x4 *)((const float *)a.q + at + 16 * n + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t part[3];
+          split_bf16x2(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], part);
+#pragma unroll
+          for (int p = 0; p < PQ; ++p) q[t][n][p][e] = part[p];
+        }
+      } else {
+        q[t][n][0] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * n);
+      }
+    }
+  }
   // ---- state
   f32x16 o[QT][ND], sa[QT], sb[QT];
   u32x4 pa[QT][2][P], pb[QT][2][P];
@@ -225,7 +231,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
   int h = 0;
   // Before step h every wave's copies of K up to h + 1 and V up to h are in; the slots
   // of K h - 1 and V h - 2 are free.
-  auto begin = [&] {
+  auto begin = [&]() RXW8_INLINE {
     __builtin_amdgcn_sched_barrier(0);
     if (h + 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -237,11 +243,11 @@ __device__ void packed_prefill(const PackedArgs &a) {
   const int tr_j = (lane & 15) >> 2, tr_q = lane & 3;
   const uint32_t v0 = lds_addr(lds) + kRing * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1);
   const int v_chunk = 2 * ((lane >> 4) & 1) + (tr_q >> 1);
-  auto k_frag = [&](int step, int n) {
+  auto k_frag = [&](int step, int n) RXW8_INLINE {
     return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(
         k0 + (step & (kRing - 1)) * TILE + (((2 * n + hf) ^ kx(col)) << 4));
   };
-  auto v_frag = [&](int step, int ks, int d) {
+  auto v_frag = [&](int step, int ks, int d) RXW8_INLINE {
     u32x4 f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {  // keys 16 ks + 8 e + 4 hf + j; their swizzle: rows 8 apart share it
@@ -252,229 +258,238 @@ __device__ void packed_prefill(const PackedArgs &a) {
     }
     return f;
   };
-  const int qparts = P == 3 && a.q_f32 ? 3 : 1;
-  auto qk = [&](f32x16 (&s)[QT], int n, u32x4 f) {
+  // The products of a fragment, after(i) behind the i-th (QT PQ of K's n-th, QT P of V's)
+  auto qk = [&](f32x16 (&s)[QT], auto n, u32x4 f, auto after) RXW8_INLINE {
+    unrolled<QT * PQ>([&](auto i) RXW8_INLINE {
+      constexpr int t = i % QT, x = i / QT;
+      if constexpr (n == 0 && x == 0) {
+        f32x16 zero;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if (n == 0)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
-      s[t] = mfma32(f, q[t][n][0], s[t]);
-      if (P == 3 && qparts == 3) {
-        s[t] = mfma32(f, q[t][n][1 % P], s[t]);
-        s[t] = mfma32(f, q[t][n][2 % P], s[t]);
+        for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+        s[t] = mfma32(f, q[t][n][x], zero);
+      } else {
+        s[t] = mfma32(f, q[t][n][x], s[t]);
       }
-    }
+      after(i);
+    });
   };
-  auto pv = [&](u32x4 (&p)[QT][2][P], int ks, int d, u32x4 f) {
+  auto pv = [&](u32x4 (&p)[QT][2][P], auto n, u32x4 f, auto after) RXW8_INLINE {
+    unrolled<QT * P>([&](auto i) RXW8_INLINE {
+      constexpr int t = i % QT, x = i / QT, ks = n / ND, d = n % ND;
+      o[t][d] = mfma32(f, p[t][ks][x], o[t][d]);
+      after(i);
+    });
+  };
+  const auto nothing = [](auto) {};
+  // keys that the rows do not see
+  auto mask = [&](f32x16 (&s)[QT]) RXW8_INLINE {
+    const int rel = r0 + col - h * kStep - 4 * hf;  // a row of tile 0's last key, counted from the lane's first
 #pragma unroll
     for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int x = 0; x < P; ++x) o[t][d] = mfma32(f, p[t][ks][x], o[t][d]);
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) > rel + 32 * t) s[t][r] = kMinusInf;
   };
-  // weights 2 i and 2 i + 1 of a lane's 16 (of row tile t)
-  auto pair = [&](f32x16 (&s)[QT], u32x4 (&p)[QT][2][P], float (&ls)[QT], int t, int i) {
-    const float e0 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i], c, -m[t]));
-    const float e1 = __builtin_amdgcn_exp2f(fmaf(s[t][2 * i + 1], c, -m[t]));
-    ls[t] += e0 + e1;
-    if constexpr (P == 1) {
-      p[t][i >> 2][0][i & 3] = pack_bf16x2(e0, e1);
-    } else {
-      uint32_t part[3];
-      split_bf16x2(e0, e1, part);
-#pragma unroll
-      for (int x = 0; x < P; ++x) p[t][i >> 2][x][i & 3] = part[x];
-    }
+  // weight e of a lane's 16 QT (of row tile e / 16), and what is done with it, behind the
+  // next one's exponential: into l, and with its neighbour into p
+  float w[4];
+  auto weigh = [&](f32x16 (&s)[QT], auto e) RXW8_INLINE {
+    constexpr int t = e >> 4, r = e & 15;
+    w[e & 3] = __builtin_amdgcn_exp2f(fmaf(s[t][r], c, -m[t]));
+    // (formed here: the compiler would sink the exponentials to their use, a step later)
+    asm volatile("" : "+v"(w[e & 3]));
   };
-  // after a step's weights: l, or where they were too large, or at the first step, a new
-  // reference, O and l to it, and the weights again
-  auto settle = [&](f32x16 (&s)[QT], u32x4 (&p)[QT][2][P], float (&ls)[QT], bool first_step) {
-    bool moves = first_step;
+  auto put = [&](u32x4 (&p)[QT][2][P], auto e) RXW8_INLINE {
+    constexpr int t = e >> 4, r = e & 15, ks = r >> 3, at = (r >> 1) & 3;
+    l[t] += w[e & 3];
+    if constexpr (r % 2 == 1) {
+      uint32_t part[P];
+      if constexpr (P == 1) part[0] = pack_bf16x2(w[(e - 1) & 3], w[e & 3]);
+      else split_bf16x2(w[(e - 1) & 3], w[e & 3], part);
 #pragma unroll
-    for (int t = 0; t < QT; ++t) moves |= !(ls[t] <= 256.f);
-    if (__ballot(moves)) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float mx = kMinusInf;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[t][r]);
-        mx = max_xor32(mx) * c;
-        const float to = first_step ? (mx == kMinusInf ? 0.f : mx) : fmaxf(m[t], mx);
-        const float f = first_step ? 0.f : __builtin_amdgcn_exp2f(m[t] - to);
-        m[t] = to;
-        l[t] = first_step ? 0.f : l[t] * f;
-        if (!first_step)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[t][d] *= f;
-        ls[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pair(s, p, ls, t, i);
+      for (int x = 0; x < P; ++x) {
+        asm volatile("" : "+v"(part[x]), "+v"(l[t]));
+        p[t][ks][x][at] = part[x];
       }
     }
-#pragma unroll
-    for (int t = 0; t < QT; ++t) l[t] += ls[t];
-    __builtin_amdgcn_sched_barrier(0);
   };
-  // One step of the pipeline: K of step h + 1 (QK), V of step h - 1 (PV), softmax of h
+  // Step h of the pipeline: S of step h + 1 into sn (with_qk), O of step h - 1 from p
+  // (with_pv), and between them the weights of step h, from s to pn
   constexpr int AHEAD = 4;
-  auto body = [&](auto with_pv, auto with_qk, f32x16 (&s)[QT], f32x16 (&sn)[QT], u32x4 (&p)[QT][2][P],
-                  u32x4 (&pn)[QT][2][P]) {
+  auto body = [&](auto with_pv, auto with_qk, f32x16 (&s)[QT], f32x16 (&sn)[QT], u32x4 (&p)[QT][2][P], u32x4 (&pn)[QT][2][P]) RXW8_INLINE {
     constexpr bool PV = decltype(with_pv)::value, QK = decltype(with_qk)::value;
-    constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NP = 8 * QT;  // fragments, pairs of weights
+    // fragments, products and weights of the step
+    constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NM = QT * ((QK ? PQ * NK : 0) + (PV ? P * 2 * ND : 0)), NE = 16 * QT;
     static_assert(NK == 2 * ND, "K and V take turns");
     u32x4 fr[AHEAD + 1];
-    auto is_k = [](int n) { return QK && (!PV || n % 2 == 0); };
-    auto at = [](int n) { return QK && PV ? n / 2 : n; };
-    auto read = [&](int n) {
-      fr[n % (AHEAD + 1)] = is_k(n) ? k_frag(h + 1, at(n)) : v_frag(h - 1, at(n) / ND, at(n) % ND);
+    auto read = [&](auto n) RXW8_INLINE {
+      constexpr bool k = QK && (!PV || n % 2 == 0);
+      constexpr int at = QK && PV ? n / 2 : n;
+      fr[n % (AHEAD + 1)] = k ? k_frag(h + 1, at) : v_frag(h - 1, at / ND, at % ND);
     };
-#pragma unroll
-    for (int n = 0; n < AHEAD; ++n) read(n);
-    float ls[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) ls[t] = 0.f;
-#pragma unroll
-    for (int n = 0; n < NF; ++n) {
+    unrolled<AHEAD>(read);
+    unrolled<NF>([&](auto n) RXW8_INLINE {
+      constexpr bool k = QK && (!PV || n % 2 == 0);
+      constexpr std::integral_constant<int, QK && PV ? n / 2 : n> at{};
+      constexpr int before = QT * (QK && PV ? (n + 1) / 2 * PQ + n / 2 * P : QK ? n * PQ : n * P);  // products
       __builtin_amdgcn_sched_barrier(0);
-      if (n + AHEAD < NF) read(n + AHEAD);
+      if constexpr (n + AHEAD < NF) read(std::integral_constant<int, n + AHEAD>{});
       const u32x4 f = fr[n % (AHEAD + 1)];
-      if (is_k(n)) qk(sn, at(n), f);
-      else pv(p, at(n) / ND, at(n) % ND, f);
-#pragma unroll
-      for (int i = n * NP / NF; i < (n + 1) * NP / NF; ++i) pair(s, pn, ls, i / 8, i % 8);
-    }
+      auto share = [&](auto i) RXW8_INLINE {
+        constexpr int e0 = (before + i) * NE / NM, e1 = (before + i + 1) * NE / NM;
+        unrolled<e1 - e0>([&](auto e) RXW8_INLINE {
+          weigh(s, std::integral_constant<int, e0 + e>{});
+          if constexpr (e0 + e > 0) put(pn, std::integral_constant<int, e0 + e - 1>{});
+        });
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      if constexpr (k) qk(sn, at, f, share);
+      else pv(p, at, f, share);
+    });
+    put(pn, std::integral_constant<int, NE - 1>{});
     __builtin_amdgcn_sched_barrier(0);
-    settle(s, pn, ls, !PV && h == 0);
   };
-  // A step on its own: scores, mask, softmax, output
-  auto alone = [&](bool masked) {
-#pragma unroll
-    for (int n = 0; n < NK; ++n) qk(sa, n, k_frag(h, n));
-    if (masked) {
-      const int rel = r0 + col - h * kStep - 4 * hf;  // the last key a row of tile 0 sees, minus the lane's first
-#pragma unroll
-      for (int t = 0; t < QT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (8 * (r >> 2) + (r & 3) > rel + 32 * t) sa[t][r] = kMinusInf;
-    }
-    float ls[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      ls[t] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pair(sa, pa, ls, t, i);
-    }
-    settle(sa, pa, ls, h == 0);
-    bool odd = false;  // a value of V that is no number
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < 2 * ND; ++n) {
-        const u32x4 f = v_frag(h, n / ND, n % ND);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= (f[e] & 0x7f80u) == 0x7f80u || (f[e] & 0x7f800000u) == 0x7f800000u;
-      }
-      odd = __ballot(odd) != 0;
-    }
-    if (!odd) {
-#pragma unroll
-      for (int n = 0; n < 2 * ND; ++n) pv(pa, n / ND, n % ND, v_frag(h, n / ND, n % ND));
-      return;
-    }
-#pragma unroll
-    for (int n = 0; n < 2 * ND; ++n) {
-      u32x4 f = v_frag(h, n / ND, n % ND);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if ((f[e] & 0x7f80u) == 0x7f80u) f[e] &= 0xffff0000u;
-        if ((f[e] & 0x7f800000u) == 0x7f800000u) f[e] &= 0xffffu;
-      }
-      pv(pa, n / ND, n % ND, f);
-    }
-#pragma unroll 1
-    for (int key = 0; key < kStep; ++key) {
-      const uint32_t row = lds_addr(lds) + (kRing + (h & (kRing - 1))) * TILE + key * ROWB;
-#pragma unroll
-      for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int dim = 32 * d + 8 * (r >> 2) + 4 * hf + (r & 3);
-          const uint32_t x = *(const __attribute__((address_space(3))) uint16_t *)(uintptr_t)(
-              row + (((dim >> 3) ^ vx(key)) << 4) + 2 * (dim & 7));
-          if ((x & 0x7f80u) == 0x7f80u)
-#pragma unroll
-            for (int t = 0; t < QT; ++t)
-              if (h * kStep + key <= r0 + 32 * t + col) o[t][d][r] += bf16_bits_to_f32(x);
-        }
-    }
+  auto finish = [&](u32x4 (&p)[QT][2][P]) RXW8_INLINE {  // O of the last step
+    begin();
+    unrolled<2 * ND>([&](auto n) RXW8_INLINE { pv(p, n, v_frag(h - 1, n / ND, n % ND), nothing); });
+    ++h;
   };
 
+  // Every wave goes through steps + 1 barriers. (The loop holds two steps, for the two
+  // sets of registers, and nothing else: with the mask's or the end's branches in it the
+  // allocator moves O about.)
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
   if (mine > 0) {
-    if (full & 1) {
+    begin();
+    unrolled<NK>([&](auto n) RXW8_INLINE { qk(sa, n, k_frag(0, n), nothing); });
+    if (full == 0) mask(sa);
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {  // the reference: step 0's maximum
+      float mx = kMinusInf;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sa[t][r]);
+      mx = max_xor32(mx) * c;
+      m[t] = mx == kMinusInf ? 0.f : mx;
+    }
+    body(no, yes, sa, sb, pb, pa);
+    for (h = 1; h + 1 < full;) {
       begin();
-      alone(false);
+      body(yes, yes, sb, sa, pa, pb);
+      ++h;
+      begin();
+      body(yes, yes, sa, sb, pb, pa);
       ++h;
     }
-    bool pending = false;
+    // S of step h in sb, P of the one before in pa
+    bool swapped = false;  // (sa and pb instead)
     if (h < full) {
       begin();
-#pragma unroll
-      for (int n = 0; n < NK; ++n) qk(sa, n, k_frag(h, n));
-      body(std::false_type{}, std::true_type{}, sa, sb, pb, pa);
+      body(yes, yes, sb, sa, pa, pb);
       ++h;
-      while (h + 1 < full) {
+      if constexpr (QT == 2) {  // (here always, where full > 0: it is even)
         begin();
-        body(std::true_type{}, std::true_type{}, sb, sa, pa, pb);
+        mask(sa);
+        body(yes, yes, sa, sb, pb, pa);
         ++h;
+      } else {
         begin();
-        body(std::true_type{}, std::true_type{}, sa, sb, pb, pa);
+        mask(sa);
+        body(yes, no, sa, sb, pb, pa);
         ++h;
+        finish(pa);
+        swapped = true;
       }
-      begin();
-      body(std::true_type{}, std::false_type{}, sb, sa, pa, pb);
-      ++h;
-      pending = true;
     }
-    for (; h < mine; ++h) {
-      begin();
-      if (pending) {
-#pragma unroll
-        for (int n = 0; n < 2 * ND; ++n) pv(pb, n / ND, n % ND, v_frag(h - 1, n / ND, n % ND));
-        pending = false;
+    if (!swapped) {
+      if (h < mine) {
+        begin();
+        mask(sb);
+        body(yes, no, sb, sa, pa, pb);
+        ++h;
+        finish(pb);
+      } else {
+        finish(pa);
       }
-      alone(true);
     }
   }
-  for (; h < steps; ++h) begin();  // the other waves' rows
+  for (; h <= steps; ++h) begin();
+  __syncthreads();  // (the rings are read)
   if (mine == 0) return;
 
+  // ---- rows that did not come out as numbers, one after the other
+  bool odd = false;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const float sum = sum_xor32(l[t]), inv = sum == 0.f ? 0.f : 1.0f / sum;
-    const int row = r0 + 32 * t + col;
-    if (row >= len) continue;
-    const int64_t to = ((first + row) * a.Hq + hq) * D + 4 * hf;
+    const float sum = sum_xor32(l[t]);
+    l[t] = sum;
+    odd |= !(sum < __builtin_huge_valf());
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const f32x4 y = f32x4{o[t][d][4 * x], o[t][d][4 * x + 1], o[t][d][4 * x + 2], o[t][d][4 * x + 3]} * inv;
-        if (a.out_f32)
-          *(f32x4 *)((float *)a.out + to + 32 * d + 8 * x) = y;
-        else
-          *(uint2 *)((uint16_t *)a.out + to + 32 * d + 8 * x) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-      }
+      for (int r = 0; r < 16; ++r) odd |= !(fabsf(o[t][d][r]) < __builtin_huge_valf());
   }
+  if (__ballot(odd)) {
+    float *const qs = (float *)((char *)lds + wave * 4 * D);
+#pragma unroll 1
+    for (int row = r0; row < min(r0 + WR, len); ++row) {
+      const int64_t at = ((first + row) * a.Hq + hq) * D;
+      for (int i = lane; i < D; i += 64) qs[i] = any_load(a.q, at + i, a.q_f32);
+      __builtin_amdgcn_wave_barrier();
+      AnyState st;
+      any_walk(st, qs, a.k, a.v, false, D, first, first + row + 1, 1, c,
+               [&](int64_t j) { return (j * a.Hkv + kvh) * D; });
+      any_store(st, a.out, at, D, a.out_f32);
+    }
+    return;
+  }
+
+  // ---- rows out, turned in LDS: 16 bytes of one row a lane
+  auto store = [&](auto f32_out) RXW8_INLINE {
+    constexpr bool F = decltype(f32_out)::value;
+    constexpr int OB = D * (F ? 4 : 2), OC = OB / 16, RPS = 1024 / OB;  // bytes and pieces of a row, rows a store
+    const uint32_t mem = lds_addr(lds) + wave * WR * OB;
+    auto ox = [](int row) { return row & (OC < 16 ? OC - 1 : 15); };
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const float inv = l[t] == 0.f ? 0.f : 1.0f / l[t];
+      const uint32_t row = mem + (32 * t + col) * OB;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const f32x4 y = f32x4{o[t][d][4 * x], o[t][d][4 * x + 1], o[t][d][4 * x + 2], o[t][d][4 * x + 3]} * inv;
+          if constexpr (F)
+            *(__attribute__((address_space(3))) f32x4 *)(uintptr_t)(row + (((8 * d + 2 * x + hf) ^ ox(col)) << 4)) = y;
+          else
+            *(__attribute__((address_space(3))) u32x2 *)(uintptr_t)(row + (((4 * d + x) ^ ox(col)) << 4) + 8 * hf) =
+                u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+        }
+    }
+    const int piece = lane % OC;
+#pragma unroll 4
+    for (int i = 0; i < WR / RPS; ++i) {
+      const int row = i * RPS + lane / OC;
+      const u32x4 y = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(mem + row * OB + ((piece ^ ox(row)) << 4));
+      if (r0 + row < len) *(u32x4 *)((char *)a.out + ((first + r0 + row) * a.Hq + hq) * OB + 16 * piece) = y;
+    }
+  };
+  if (P == 3 && a.out_f32) store(std::true_type{});
+  else store(std::false_type{});
 }
 
-#define RXW8_PACKED_PREFILL(D, QT, P, NAME)                                                          \
-  extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1)))       \
+#define RXW8_PACKED_PREFILL(D, QT, PQ, P, W, NAME)                                                   \
+  extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, W)))       \
       rxw8_packed_prefill_##NAME##_d##D(PackedArgs a) {                                              \
-    packed_prefill<D, QT, P>(a);                                                                     \
+    packed_prefill<D, QT, PQ, P>(a);                                                                 \
   }
-RXW8_PACKED_PREFILL(64, 2, 1, bf16)
-RXW8_PACKED_PREFILL(128, 2, 1, bf16)
-RXW8_PACKED_PREFILL(256, 1, 1, bf16)
-RXW8_PACKED_PREFILL(64, 1, 3, f32)
-RXW8_PACKED_PREFILL(128, 1, 3, f32)
-RXW8_PACKED_PREFILL(256, 1, 3, f32)
+// q and output bf16; q bf16, output f32; q f32
+RXW8_PACKED_PREFILL(64, 2, 1, 1, 1, bf16)
+RXW8_PACKED_PREFILL(128, 2, 1, 1, 1, bf16)
+RXW8_PACKED_PREFILL(256, 1, 1, 1, 1, bf16)
+RXW8_PACKED_PREFILL(64, 1, 1, 3, 2, bf16_f32)
+RXW8_PACKED_PREFILL(128, 1, 1, 3, 1, bf16_f32)
+RXW8_PACKED_PREFILL(256, 1, 1, 3, 1, bf16_f32)
+RXW8_PACKED_PREFILL(64, 1, 3, 3, 2, f32)
+RXW8_PACKED_PREFILL(128, 1, 3, 3, 1, f32)
+RXW8_PACKED_PREFILL(256, 1, 3, 3, 1, f32)

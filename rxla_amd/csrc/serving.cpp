@@ -122,7 +122,8 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
 }
 
 static float softmax_scale(float scale, int64_t D) {
-  return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f;
+  // (at least 1e-30, below which every key weighs the same: -inf times it stays -inf)
+  return std::max((scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f, 1e-30f);
 }
 
 // The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row
@@ -174,8 +175,8 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
     int rc = launch(rt, "rxw8_packed_fill", dim3((unsigned)std::min<int64_t>((T * Hq * D + 255) / 256, 2048)), dim3(256), a);
     if (rc) return rc;
   }
-  char kname[40];
-  std::snprintf(kname, sizeof kname, "rxw8_packed_prefill_%s_d%d", f32 ? "f32" : "bf16", (int)D);
+  char kname[48];
+  std::snprintf(kname, sizeof kname, "rxw8_packed_prefill_%s_d%d", a.q_f32 ? "f32" : a.out_f32 ? "bf16_f32" : "bf16", (int)D);
   return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, (size_t)(2 * 4 * 32 * 2) * (size_t)D);
 }
 
