@@ -29,16 +29,18 @@ __device__ __forceinline__ float wave_max64(float v) {
 // is one step less where that would leave nothing: every part of a v that is not 0 has
 // its sign and is not 0, so that a product with an infinite factor is the infinity that
 // v's own would be.
-__device__ __forceinline__ uint32_t cut_bf16(float v) {  // f32 bits, low half zero
-  const uint32_t b = __float_as_uint(v);
-  return b & 0xffffu || !(b & 0x7fffffffu) ? b & 0xffff0000u : b - 0x10000u;
+__device__ __forceinline__ uint32_t cut_weight(float v) {  // v >= 0: f32 bits, low half zero
+  return __builtin_elementwise_sub_sat(__float_as_uint(v), 1u) & 0xffff0000u;
 }
-// Parts of two values, packed in pairs: N = 2 or 3
-template <int N>
+__device__ __forceinline__ uint32_t cut_bf16(float v) {
+  return cut_weight(fabsf(v)) | (__float_as_uint(v) & 0x80000000u);
+}
+// Parts of two values (Weights: not below 0), packed in pairs: N = 2 or 3
+template <bool Weights = false, int N>
 __device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t (&part)[N]) {
 #pragma unroll
   for (int n = 0; n + 1 < N; ++n) {
-    const uint32_t x = cut_bf16(a), y = cut_bf16(b);
+    const uint32_t x = Weights ? cut_weight(a) : cut_bf16(a), y = Weights ? cut_weight(b) : cut_bf16(b);
     part[n] = (x >> 16) | y;
     a -= __uint_as_float(x), b -= __uint_as_float(y);
   }

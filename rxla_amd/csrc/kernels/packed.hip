@@ -239,20 +239,26 @@ __device__ void packed_prefill(const PackedArgs &a) {
     if (h + 3 < steps) copy(kbase, h + 3, false);
     __builtin_amdgcn_sched_barrier(0);
   };
-  const uint32_t k0 = lds_addr(lds) + col * ROWB;
+  // LDS byte addresses of the fragments: one XOR from a lane's base in the step's slot
+  // (chunk 2 n + hf of K row col; chunks 4 d + .. of V rows 4 hf + j, 8 rows apart two reads)
+  const uint32_t k0 = lds_addr(lds) + col * ROWB + ((hf ^ kx(col)) << 4);
   const int tr_j = (lane & 15) >> 2, tr_q = lane & 3;
-  const uint32_t v0 = lds_addr(lds) + kRing * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1);
-  const int v_chunk = 2 * ((lane >> 4) & 1) + (tr_q >> 1);
-  auto k_frag = [&](int step, int n) RXW8_INLINE {
-    return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(
-        k0 + (step & (kRing - 1)) * TILE + (((2 * n + hf) ^ kx(col)) << 4));
+  const uint32_t v0 = lds_addr(lds) + kRing * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1) +
+                      (((2 * ((lane >> 4) & 1) + (tr_q >> 1)) ^ vx(4 * hf + tr_j)) << 4);
+  auto slot = [&](uint32_t base, int step) RXW8_INLINE {
+    uint32_t at = base + (step & (kRing - 1)) * TILE;
+    asm("" : "+v"(at));  // (the XORs stay where they are used, not in registers)
+    return at;
   };
-  auto v_frag = [&](int step, int ks, int d) RXW8_INLINE {
+  auto k_frag = [&](uint32_t base, int n) RXW8_INLINE {
+    return *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(base ^ (n << 5));
+  };
+  auto v_frag = [&](uint32_t base, int n) RXW8_INLINE {
     u32x4 f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {  // keys 16 ks + 8 e + 4 hf + j; their swizzle: rows 8 apart share it
+    for (int e = 0; e < 2; ++e) {
       const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
-          v0 + (step & (kRing - 1)) * TILE + (16 * ks + 8 * e) * ROWB + (((4 * d + v_chunk) ^ vx(4 * hf + tr_j)) << 4)));
+          (base ^ (n % ND << 6)) + (16 * (n / ND) + 8 * e) * ROWB));
       const uint2 u = __builtin_bit_cast(uint2, x);
       f[2 * e] = u.x, f[2 * e + 1] = u.y;
     }
@@ -290,42 +296,75 @@ __device__ void packed_prefill(const PackedArgs &a) {
       for (int r = 0; r < 16; ++r)
         if (8 * (r >> 2) + (r & 3) > rel + 32 * t) s[t][r] = kMinusInf;
   };
-  // weight e of a lane's 16 QT (of row tile e / 16), and what is done with it, behind the
-  // next one's exponential: into l, and with its neighbour into p
-  float w[4];
-  auto weigh = [&](f32x16 (&s)[QT], auto e) RXW8_INLINE {
-    constexpr int t = e >> 4, r = e & 15;
-    w[e & 3] = __builtin_amdgcn_exp2f(fmaf(s[t][r], c, -m[t]));
+  // The softmax of a step in shares, some behind each product: two weights at a time, each
+  // of which waits for nothing that the one before it has just asked for. Pair g of a
+  // lane's 8 QT: exponentials, sum and bf16 parts.
+  constexpr int ITEMS = P == 1 ? 2 : 5;  // of a pair
+  float w0 = 0.f, w1 = 0.f, was0 = 0.f, was1 = 0.f;
+  uint32_t part = 0;
+  auto item = [&](f32x16 (&s)[QT], u32x4 (&p)[QT][2][P], auto i) RXW8_INLINE {
+    constexpr int g = i / ITEMS, k = i % ITEMS, t = g >> 3, r = 2 * (g & 7), ks = r >> 3, at = (r >> 1) & 3;
     // (formed here: the compiler would sink the exponentials to their use, a step later)
-    asm volatile("" : "+v"(w[e & 3]));
-  };
-  auto put = [&](u32x4 (&p)[QT][2][P], auto e) RXW8_INLINE {
-    constexpr int t = e >> 4, r = e & 15, ks = r >> 3, at = (r >> 1) & 3;
-    l[t] += w[e & 3];
-    if constexpr (r % 2 == 1) {
-      uint32_t part[P];
-      if constexpr (P == 1) part[0] = pack_bf16x2(w[(e - 1) & 3], w[e & 3]);
-      else split_bf16x2(w[(e - 1) & 3], w[e & 3], part);
-#pragma unroll
-      for (int x = 0; x < P; ++x) {
-        asm volatile("" : "+v"(part[x]), "+v"(l[t]));
-        p[t][ks][x][at] = part[x];
+    auto weigh = [&](int e) RXW8_INLINE {
+      float w = __builtin_amdgcn_exp2f(fmaf(s[t][r + e], c, -m[t]));
+      asm volatile("" : "+v"(w));
+      return w;
+    };
+    auto keep = [&](int tt, int kk, int aa, int x, uint32_t v) RXW8_INLINE {
+      asm volatile("" : "+v"(v));
+      p[tt][kk][x][aa] = v;
+    };
+    if constexpr (P == 1) {
+      constexpr int gp = g - 1, tp = gp >> 3, rp = 2 * (gp & 7);  // the pair before
+      if constexpr (k == 0) {
+        was0 = w0, was1 = w1;
+        w0 = weigh(0);
+        if constexpr (g > 0) l[tp] += was0;
+      } else {
+        w1 = weigh(1);
+        if constexpr (g > 0) {
+          l[tp] += was1;
+          asm volatile("" : "+v"(l[tp]));
+          keep(tp, rp >> 3, (rp >> 1) & 3, 0, pack_bf16x2(was0, was1));
+        }
       }
+    } else {
+      if constexpr (k == 0) w0 = weigh(0);
+      if constexpr (k == 1) w1 = weigh(1);
+      if constexpr (k == 2 || k == 3) {
+        if constexpr (k == 2) {
+          l[t] += w0 + w1;
+          asm volatile("" : "+v"(l[t]));
+        }
+        const uint32_t x = cut_weight(w0), y = cut_weight(w1);
+        keep(t, ks, at, k - 2, (x >> 16) | y);
+        w0 -= __uint_as_float(x), w1 -= __uint_as_float(y);
+      }
+      if constexpr (k == 4) keep(t, ks, at, 2 % P, pack_bf16x2(w0, w1));
+    }
+  };
+  auto last_item = [&](u32x4 (&p)[QT][2][P]) RXW8_INLINE {
+    if constexpr (P == 1) {
+      l[QT - 1] += w0 + w1;
+      uint32_t v = pack_bf16x2(w0, w1);
+      asm volatile("" : "+v"(v), "+v"(l[QT - 1]));
+      p[QT - 1][1][0][3] = v;
     }
   };
   // Step h of the pipeline: S of step h + 1 into sn (with_qk), O of step h - 1 from p
   // (with_pv), and between them the weights of step h, from s to pn
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = D == 256 && P == 3 ? 2 : 4;  // fragments asked for ahead, by registers
   auto body = [&](auto with_pv, auto with_qk, f32x16 (&s)[QT], f32x16 (&sn)[QT], u32x4 (&p)[QT][2][P], u32x4 (&pn)[QT][2][P]) RXW8_INLINE {
     constexpr bool PV = decltype(with_pv)::value, QK = decltype(with_qk)::value;
-    // fragments, products and weights of the step
-    constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NM = QT * ((QK ? PQ * NK : 0) + (PV ? P * 2 * ND : 0)), NE = 16 * QT;
+    // fragments, products and shares of the softmax
+    constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NM = QT * ((QK ? PQ * NK : 0) + (PV ? P * 2 * ND : 0)), NE = 8 * QT * ITEMS;
     static_assert(NK == 2 * ND, "K and V take turns");
+    const uint32_t ks = slot(k0, h + 1), vs = slot(v0, h - 1);
     u32x4 fr[AHEAD + 1];
     auto read = [&](auto n) RXW8_INLINE {
       constexpr bool k = QK && (!PV || n % 2 == 0);
       constexpr int at = QK && PV ? n / 2 : n;
-      fr[n % (AHEAD + 1)] = k ? k_frag(h + 1, at) : v_frag(h - 1, at / ND, at % ND);
+      fr[n % (AHEAD + 1)] = k ? k_frag(ks, at) : v_frag(vs, at);
     };
     unrolled<AHEAD>(read);
     unrolled<NF>([&](auto n) RXW8_INLINE {
@@ -337,21 +376,19 @@ __device__ void packed_prefill(const PackedArgs &a) {
       const u32x4 f = fr[n % (AHEAD + 1)];
       auto share = [&](auto i) RXW8_INLINE {
         constexpr int e0 = (before + i) * NE / NM, e1 = (before + i + 1) * NE / NM;
-        unrolled<e1 - e0>([&](auto e) RXW8_INLINE {
-          weigh(s, std::integral_constant<int, e0 + e>{});
-          if constexpr (e0 + e > 0) put(pn, std::integral_constant<int, e0 + e - 1>{});
-        });
+        unrolled<e1 - e0>([&](auto e) RXW8_INLINE { item(s, pn, std::integral_constant<int, e0 + e>{}); });
         __builtin_amdgcn_sched_barrier(0);
       };
       if constexpr (k) qk(sn, at, f, share);
       else pv(p, at, f, share);
     });
-    put(pn, std::integral_constant<int, NE - 1>{});
+    last_item(pn);
     __builtin_amdgcn_sched_barrier(0);
   };
   auto finish = [&](u32x4 (&p)[QT][2][P]) RXW8_INLINE {  // O of the last step
     begin();
-    unrolled<2 * ND>([&](auto n) RXW8_INLINE { pv(p, n, v_frag(h - 1, n / ND, n % ND), nothing); });
+    const uint32_t vs = slot(v0, h - 1);
+    unrolled<2 * ND>([&](auto n) RXW8_INLINE { pv(p, n, v_frag(vs, n), nothing); });
     ++h;
   };
 
@@ -362,7 +399,8 @@ __device__ void packed_prefill(const PackedArgs &a) {
   constexpr std::false_type no{};
   if (mine > 0) {
     begin();
-    unrolled<NK>([&](auto n) RXW8_INLINE { qk(sa, n, k_frag(0, n), nothing); });
+    const uint32_t ks = slot(k0, 0);
+    unrolled<NK>([&](auto n) RXW8_INLINE { qk(sa, n, k_frag(ks, n), nothing); });
     if (full == 0) mask(sa);
 #pragma unroll
     for (int t = 0; t < QT; ++t) {  // the reference: step 0's maximum
@@ -417,48 +455,29 @@ __device__ void packed_prefill(const PackedArgs &a) {
   __syncthreads();  // (the rings are read)
   if (mine == 0) return;
 
-  // ---- rows that did not come out as numbers, one after the other
-  bool odd = false;
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const float sum = sum_xor32(l[t]);
-    l[t] = sum;
-    odd |= !(sum < __builtin_huge_valf());
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) odd |= !(fabsf(o[t][d][r]) < __builtin_huge_valf());
-  }
-  if (__ballot(odd)) {
-    float *const qs = (float *)((char *)lds + wave * 4 * D);
-#pragma unroll 1
-    for (int row = r0; row < min(r0 + WR, len); ++row) {
-      const int64_t at = ((first + row) * a.Hq + hq) * D;
-      for (int i = lane; i < D; i += 64) qs[i] = any_load(a.q, at + i, a.q_f32);
-      __builtin_amdgcn_wave_barrier();
-      AnyState st;
-      any_walk(st, qs, a.k, a.v, false, D, first, first + row + 1, 1, c,
-               [&](int64_t j) { return (j * a.Hkv + kvh) * D; });
-      any_store(st, a.out, at, D, a.out_f32);
-    }
-    return;
-  }
-
   // ---- rows out, turned in LDS: 16 bytes of one row a lane
   auto store = [&](auto f32_out) RXW8_INLINE {
     constexpr bool F = decltype(f32_out)::value;
     constexpr int OB = D * (F ? 4 : 2), OC = OB / 16, RPS = 1024 / OB;  // bytes and pieces of a row, rows a store
     const uint32_t mem = lds_addr(lds) + wave * WR * OB;
     auto ox = [](int row) { return row & (OC < 16 ? OC - 1 : 15); };
+    float odd = 0.f;  // 0 times a number is 0
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const float inv = l[t] == 0.f ? 0.f : 1.0f / l[t];
+      const float sum = sum_xor32(l[t]), inv = sum == 0.f ? 0.f : 1.0f / sum;
+      odd = fmaf(sum, 0.f, odd);
       const uint32_t row = mem + (32 * t + col) * OB;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const f32x4 y = f32x4{o[t][d][4 * x], o[t][d][4 * x + 1], o[t][d][4 * x + 2], o[t][d][4 * x + 3]} * inv;
+          f32x4 y;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[e] = o[t][d][4 * x + e];
+            odd = fmaf(y[e], 0.f, odd);
+            y[e] *= inv;
+          }
           if constexpr (F)
             *(__attribute__((address_space(3))) f32x4 *)(uintptr_t)(row + (((8 * d + 2 * x + hf) ^ ox(col)) << 4)) = y;
           else
@@ -466,6 +485,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
                 u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
         }
     }
+    if (__ballot(odd != 0.f)) return false;
     const int piece = lane % OC;
 #pragma unroll 4
     for (int i = 0; i < WR / RPS; ++i) {
@@ -473,9 +493,23 @@ __device__ void packed_prefill(const PackedArgs &a) {
       const u32x4 y = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(mem + row * OB + ((piece ^ ox(row)) << 4));
       if (r0 + row < len) *(u32x4 *)((char *)a.out + ((first + r0 + row) * a.Hq + hq) * OB + 16 * piece) = y;
     }
+    return true;
   };
-  if (P == 3 && a.out_f32) store(std::true_type{});
-  else store(std::false_type{});
+  if (P == 3 && a.out_f32 ? store(yes) : store(no)) return;
+
+  // ---- rows that did not come out as numbers, one after the other
+  float *const qs = (float *)((char *)lds + wave * 4 * D);
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (int row = r0; row < min(r0 + WR, len); ++row) {
+    const int64_t at = ((first + row) * a.Hq + hq) * D;
+    for (int i = lane; i < D; i += 64) qs[i] = any_load(a.q, at + i, a.q_f32);
+    __builtin_amdgcn_wave_barrier();
+    AnyState st;
+    any_walk(st, qs, a.k, a.v, false, D, first, first + row + 1, 1, c,
+             [&](int64_t j) { return (j * a.Hkv + kvh) * D; });
+    any_store(st, a.out, at, D, a.out_f32);
+  }
 }
 
 #define RXW8_PACKED_PREFILL(D, QT, PQ, P, W, NAME)                                                   \
@@ -484,7 +518,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
     packed_prefill<D, QT, PQ, P>(a);                                                                 \
   }
 // q and output bf16; q bf16, output f32; q f32
-RXW8_PACKED_PREFILL(64, 2, 1, 1, 1, bf16)
+RXW8_PACKED_PREFILL(64, 2, 1, 1, 2, bf16)
 RXW8_PACKED_PREFILL(128, 2, 1, 1, 1, bf16)
 RXW8_PACKED_PREFILL(256, 1, 1, 1, 1, bf16)
 RXW8_PACKED_PREFILL(64, 1, 1, 3, 2, bf16_f32)

@@ -516,12 +516,12 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
         } else {
           uint32_t p01[3], p23[3];
           if (a.out_f32) {
-            split_bf16x2(s[u][0], s[u][1], p01);
-            split_bf16x2(s[u][2], s[u][3], p23);
+            split_bf16x2<true>(s[u][0], s[u][1], p01);
+            split_bf16x2<true>(s[u][2], s[u][3], p23);
           } else {
             uint32_t x[2], y[2];
-            split_bf16x2(s[u][0], s[u][1], x);
-            split_bf16x2(s[u][2], s[u][3], y);
+            split_bf16x2<true>(s[u][0], s[u][1], x);
+            split_bf16x2<true>(s[u][2], s[u][3], y);
             p01[0] = x[0], p01[1] = x[1], p23[0] = y[0], p23[1] = y[1];
           }
 #pragma unroll
