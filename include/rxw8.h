@@ -353,7 +353,7 @@ int rxw8_argmax(rxw8_runtime *rt, rxw8_buffer *x, int axis, int keep_dims,
  * A temperature that is not above 0 (NaN included), a NaN among the row's logits
  * and a row whose maximum is infinite give what rxw8_argmax gives. Words at -inf
  * weigh nothing. The same inputs give the same tokens: masses are summed in
- * whole units of 2^-s of the first word's, V 2^s < 2^62 (s <= 52). */
+ * whole units of 2^-s of the first word's, V 2^s <= 2^62 (s <= 51). */
 int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform,
                 rxw8_buffer *temperature, rxw8_buffer *top_k,
                 rxw8_buffer *top_p, rxw8_buffer *min_p, rxw8_buffer **out);

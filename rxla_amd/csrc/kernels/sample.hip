@@ -7,11 +7,23 @@
 // the mass of what is left. Every filter leaves a prefix of the order, so what the
 // filters leave is known by its mass alone: the least of the prefixes' masses.
 //
-// Masses are whole numbers, round(w 2^s) in 64 bits with V 2^s < 2^62, w in f64:
+// Masses are whole numbers, round(w 2^s) in 64 bits with V 2^s <= 2^62, w in f64:
 // their sums do not depend on the order of the additions (atomics included), and a
 // sum over V words is off by at most V / 2 units of 2^-s (2^-45 of the largest
-// weight each at V = 2^18). Equal logits have equal masses, so within a run of
-// ties a mass says how many of them it takes, and the lowest indices come first.
+// weight each at V = 2^18). Words lighter than half a unit weigh nothing and can
+// neither be drawn nor move a sum; they are passed over. Equal logits have equal
+// masses, so within a run of ties a mass says how many of them it takes, and the
+// lowest indices come first.
+//
+// Nothing is sorted. With z = (max - l) log2(e) / T the words go into bins of z, so
+// the bins are in the words' order; the running counts and masses of the bins tell the
+// bins that the borders of top_k, top_p and min_p and the token can lie in; and only the
+// words of those bins, one row's some dozens to hundreds, are looked at one by one.
+// Two launches where workgroups share a row (the maxima, then the bins, which the last
+// workgroup of a row to arrive joins and draws from), one where each has its own. What
+// bounds a batch is reading the logits: once from memory, then twice more from the
+// caches, the second time with an exponential in f64 and two LDS atomics for each
+// word; a single row is bound by the length of the chain.
 #include "common.h"
 
 struct SampleArgs {
@@ -24,149 +36,559 @@ struct SampleArgs {
   int64_t V;
   int shift;                   // s
   int bf16;
+  // S workgroups share a row, `chunk` words each (0 and V: one has it alone): extremes
+  // [B][S], arrivals [B] (zero between launches), and bins [B][S] of 24 KiB
+  int S;
+  int64_t chunk;
+  struct SampleExtremes *extremes;
+  int *arrivals;
+  char *bins;
 };
 
 typedef unsigned long long u64;
 
-// Ascending keys for ascending values, -0 and +0 alike
+namespace {
+
+constexpr int kThreads = 1024, kBins = 2048, kList = 8192, kPairwise = 1024;
+
+// Ascending keys for ascending values, -0 and +0 alike; above them all a NaN
 __device__ __forceinline__ uint32_t sample_key(float v) {
   const uint32_t b = __float_as_uint(v + 0.f);
-  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+  return v != v ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float sample_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+// A word, the larger the earlier in the order
+__device__ __forceinline__ u64 sample_word(uint32_t key, uint32_t index) { return (u64)key << 32 | (0xffffffffu - index); }
+
+// f(value, index) for the words lo <= index < hi of a row, by the workgroup's threads: 16
+// bytes a load where the row's alignment has them, four loads at a time
+template <typename F>
+__device__ void each_word(const void *row, bool bf16, int64_t lo, int64_t hi, F f) {
+  const int tid = threadIdx.x, es = bf16 ? 2 : 4, W = 16 / es;
+  const char *const p = (const char *)row;
+  auto one = [&](int64_t i) {
+    f(bf16 ? bf16_bits_to_f32(((const uint16_t *)row)[i]) : ((const float *)row)[i], (uint32_t)i);
+  };
+  const int64_t head = min(hi, lo + (int64_t)((16 - ((uintptr_t)(p + lo * es) & 15)) & 15) / es);
+  const int64_t body = head + (hi - head) / W * W;
+  if (lo + tid < head) one(lo + tid);
+  constexpr int N = 4;
+  for (int64_t i0 = head; i0 < body; i0 += (int64_t)N * W * kThreads) {
+    u32x4 x[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t i = i0 + (int64_t)W * (n * kThreads + tid);
+      if (i < body) x[n] = *(const u32x4 *)(p + i * es);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t i = i0 + (int64_t)W * (n * kThreads + tid);
+      if (i >= body) break;
+      if (bf16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f(__uint_as_float(x[n][e] << 16), (uint32_t)i + 2 * e);
+          f(__uint_as_float(x[n][e] & 0xffff0000u), (uint32_t)i + 2 * e + 1);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(__uint_as_float(x[n][e]), (uint32_t)i + e);
+      }
+    }
+  }
+  if (body + tid < hi) one(body + tid);
+}
+
+__device__ __forceinline__ u64 max_u64(u64 a, u64 b) { return a > b ? a : b; }
+
+}  // namespace
+
+// The first maximum of some words (a NaN above every number), and their least value
+// that is not -inf
+struct SampleExtremes {
+  u64 top;
+  float least;
+  int pad;
+};
+
+namespace {
 
 struct Found {
-  u64 mass, count;
+  u64 mass, count;  // of the words before those with `key`
   uint32_t key, ties;
 };
 
-// One workgroup per row. Radix descent over the keys, 8 bits a pass: a pass counts
-// the words and masses of 256 bins among those that share the bits found so far.
-extern "C" __global__ void __launch_bounds__(1024) rxw8_sample_any(SampleArgs a) {
-  __shared__ unsigned cnt[256];
-  __shared__ u64 mass[256];
-  __shared__ u64 red[16];
-  __shared__ Found found;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x, base = row * a.V;
-  auto value = [&](int64_t i) {
-    return a.bf16 ? bf16_bits_to_f32(((const uint16_t *)a.logits)[base + i]) : ((const float *)a.logits)[base + i];
-  };
-  // the first maximum, a NaN above every number: (key, lowest index) packed for a maximum
-  u64 best = 0;
-  for (int64_t i = tid; i < a.V; i += 1024) {
-    const float v = value(i);
-    const u64 c = ((u64)(v != v ? 0xffffffffu : sample_key(v)) << 32) | (0xffffffffu - (uint32_t)i);
-    best = c > best ? c : best;
-  }
+struct SampleShared {
+  u64 mass[kBins];      // (mass and count: 24 KiB in one piece)
+  uint32_t count[kBins];
+  u64 list[kList];      // words of the bins looked at
+  u64 unit[kPairwise];  // their masses and bins
+  uint16_t bin[kPairwise];
+  uint8_t marked[kBins];
+  double exp2_table[64];
+  u64 wave_mass[16];
+  uint32_t wave_count[16];
+  SampleExtremes wave_ext[16];
+  Found found;
+  u64 result;
+  int n, flag;
+};
+
+struct Row {
+  const void *words;
+  bool bf16;
+  int64_t V;
+  float top;         // the maximum
+  double inv;        // log2(e) / T
+  double per_bin;    // bins per unit of z
+  double unit;       // 2^s
+  double far;        // z from which on words weigh nothing
+
+  __device__ double z(float v) const { return ((double)top - (double)v) * inv; }
+  __device__ int bin(double zv) const { return min((int)(zv * per_bin), kBins - 1); }
+};
+
+// 2^-z for 0 <= z < 64: z = n / 64 + r, 2^(-n / 64) from a table of 64 and an exponent, and the
+// series of exp(-r ln 2) to the fifth power: the next term is below 2^-48
+__device__ __forceinline__ double exp2_minus(const SampleShared &sh, double z) {
+  const int n = (int)(z * 64.0);
+  const double x = (z - (double)n * 0.015625) * -0.69314718055994530942;
+  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(x, p, 1.0 / 6.0);
+  p = fma(x, p, 0.5);
+  p = fma(x, p, 1.0);
+  p = fma(x, p, 1.0);
+  return ldexp(p * sh.exp2_table[n & 63], -(n >> 6));
+}
+__device__ __forceinline__ u64 units_of(const Row &r, double w) {  // (w unit + 2^52 holds it in its low bits)
+  return __builtin_bit_cast(u64, fma(w, r.unit, 0x1p52)) & 0xfffffffffffffull;
+}
+// The mass of a word (0 from r.far on)
+__device__ __forceinline__ u64 units_at(const SampleShared &sh, const Row &r, float v) {
+  const double z = r.z(v);
+  return z < r.far ? units_of(r, exp2_minus(sh, z)) : 0;
+}
+
+// Extremes over the workgroup, in every thread
+__device__ SampleExtremes join_extremes(SampleShared &sh, SampleExtremes e) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int o = 32; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor(best, o);
-    best = c > best ? c : best;
+    e.top = max_u64(e.top, __shfl_xor(e.top, o));
+    e.least = fminf(e.least, __shfl_xor(e.least, o));
   }
-  if (lane == 0) red[wave] = best;
   __syncthreads();
-  for (int w = 0; w < 16; ++w) best = red[w] > best ? red[w] : best;
-  const uint32_t top = (uint32_t)(best >> 32);
-  const float vmax = sample_value(top);
+  if (lane == 0) sh.wave_ext[wave] = e;
+  __syncthreads();
+  for (int w = 0; w < kThreads / 64; ++w) {
+    e.top = max_u64(e.top, sh.wave_ext[w].top);
+    e.least = fminf(e.least, sh.wave_ext[w].least);
+  }
+  return e;
+}
+__device__ SampleExtremes extremes_of(const void *row, bool bf16, int64_t lo, int64_t hi) {
+  SampleExtremes e{0, __builtin_huge_valf(), 0};
+  each_word(row, bf16, lo, hi, [&](float v, uint32_t i) {
+    e.top = max_u64(e.top, sample_word(sample_key(v), i));
+    if (v > -__builtin_huge_valf()) e.least = fminf(e.least, v);
+  });
+  return e;
+}
+
+// Radix descent, 8 bits a pass, over the i < n that get(i, key, units) admits: the key at which
+// the running count reaches `count` (if above 0), else the running mass m satisfies m >= want
+// (m > want where `over`), as some key's does; counts and masses begin with `before`'s.
+template <typename Get>
+__device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64 count, bool over, double want) {
+  const int tid = threadIdx.x;
+  Found f = before;
+  f.key = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    if (tid < 256) sh.count[tid] = 0, sh.mass[tid] = 0;
+    __syncthreads();
+    for (int64_t i = tid; i < n; i += kThreads) {
+      uint32_t k;
+      u64 u;
+      if (!get(i, k, u) || (shift < 24 && (k >> (shift + 8)) != f.key)) continue;
+      atomicAdd(&sh.count[(k >> shift) & 255], 1u);
+      atomicAdd(&sh.mass[(k >> shift) & 255], u);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int b = 255;
+      for (; b > 0; --b) {
+        const u64 m = f.mass + sh.mass[b], c = f.count + sh.count[b];
+        if (sh.count[b] && (count ? c >= count : over ? (double)m > want : (double)m >= want)) break;
+        f.mass = m, f.count = c;
+      }
+      f.key = (f.key << 8) | (uint32_t)b;
+      f.ties = sh.count[b];
+      sh.found = f;
+    }
+    __syncthreads();
+    f = sh.found;
+  }
+  __syncthreads();
+  return f;
+}
+
+struct Settings {
+  float u, p, m;
+  int64_t k;
+};
+
+// The mass of a prefix that ends within ties: `before` and as many of them as reach `want`
+__device__ u64 mass_reaching(const Found &f, u64 one, double want) {
+  const double n = one ? ceil((want - (double)f.mass) / (double)one) : 1.0;
+  return f.mass + (n > 1.0 ? min((u64)n, (u64)f.ties) : 1) * one;
+}
+// Which of the ties (from 0) the running mass passes `want` at
+__device__ u64 tie_passing(const Found &f, u64 one, double want) {
+  const u64 n = one && want > (double)f.mass ? (u64)((want - (double)f.mass) / (double)one) : 0;
+  return n < f.ties ? n : f.ties - 1;
+}
+
+// The token by descents over all words of the row (where a bin holds more of them than the list:
+// long runs of ties): some milliseconds, as every descent reads the row four times
+__device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings &s) {
+  auto value = [&](int64_t i) {
+    return r.bf16 ? bf16_bits_to_f32(((const uint16_t *)r.words)[i]) : ((const float *)r.words)[i];
+  };
+  auto word = [&](int64_t i, uint32_t &k, u64 &u) {
+    const float v = value(i);
+    k = sample_key(v), u = units_at(sh, r, v);
+    return true;
+  };
+  auto sum = [&](double least) {  // of the words with w >= least
+    u64 m = 0;
+    each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t) {
+      const double z = r.z(v), w = z < r.far ? exp2_minus(sh, z) : 0.0;
+      if (w >= least) m += units_of(r, w);
+    });
+    for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0;
+    for (int w = 0; w < kThreads / 64; ++w) m += sh.wave_mass[w];
+    return m;
+  };
+  const Found none{};
+  u64 kept = sum(0.0);
+  if (s.k > 0 && s.k < r.V) {
+    const Found f = descend(sh, r.V, word, none, (u64)s.k, false, 0.0);
+    kept = f.mass + ((u64)s.k - f.count) * units_at(sh, r, sample_value(f.key));
+  }
+  const double all = (double)kept;
+  if (s.p < 1.f) {
+    const Found f = descend(sh, r.V, word, none, 0, false, (double)s.p * all);
+    kept = min(kept, mass_reaching(f, units_at(sh, r, sample_value(f.key)), (double)s.p * all));
+  }
+  if (s.m > 0.f) kept = min(kept, sum((double)s.m));
+  kept = max_u64(kept, (u64)r.unit);
+  const double want = (double)s.u * (double)kept;
+  const Found f = descend(sh, r.V, word, none, 0, true, want);
+  const u64 nth = tie_passing(f, units_at(sh, r, sample_value(f.key)), want);
+  const Found at = descend(sh, r.V, [&](int64_t i, uint32_t &k, u64 &u) {
+    k = 0xffffffffu - (uint32_t)i, u = 0;
+    return sample_key(value(i)) == f.key;
+  }, none, nth + 1, false, 0.0);
+  return (int32_t)(0xffffffffu - at.key);
+}
+
+// The token, from the counts and masses of the row's bins (in sh)
+__device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  // ---- running masses and counts before each bin, in place: thread t has bins 2 t and 2 t + 1
+  u64 m0 = sh.mass[2 * tid], m1 = sh.mass[2 * tid + 1], m = m0 + m1;
+  uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], c = c0 + c1;
+  const u64 mine = m;
+  const uint32_t mine_c = c;
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 x = __shfl_up(m, o);
+    const uint32_t y = __shfl_up(c, o);
+    if (lane >= o) m += x, c += y;
+  }
+  if (lane == 63) sh.wave_mass[wave] = m, sh.wave_count[wave] = c;
+  for (int b = tid; b < kBins; b += kThreads) sh.marked[b] = 0;
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  u64 total = 0;
+  uint32_t counted = 0;
+  m -= mine, c -= mine_c;
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) m += sh.wave_mass[w], c += sh.wave_count[w];
+    total += sh.wave_mass[w], counted += sh.wave_count[w];
+  }
+  sh.mass[2 * tid] = m, sh.mass[2 * tid + 1] = m + m0;
+  sh.count[2 * tid] = c, sh.count[2 * tid + 1] = c + c0;
+  __syncthreads();
+  auto mass_end = [&](int b) { return b + 1 < kBins ? sh.mass[b + 1] : total; };
+  // first bin at whose end the running mass satisfies the condition
+  auto bin_of_mass = [&](bool over, double want) {
+    int lo = 0, hi = kBins - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      const double e = (double)mass_end(mid);
+      if (over ? e > want : e >= want) hi = mid;
+      else lo = mid + 1;
+    }
+    return lo;
+  };
+  // ---- the bins in which borders and token can lie (uniform over the workgroup)
+  u64 kept_lo = total, kept_hi = total;  // bounds of what is left
+  int kb = -1, pb0 = 1, pb1 = 0, mb = -1;
+  if (s.k > 0 && s.k < counted) {
+    int lo = 0, hi = kBins - 1;  // last bin that begins before rank k
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sh.count[mid] < s.k) lo = mid;
+      else hi = mid - 1;
+    }
+    kb = lo;
+    kept_lo = sh.mass[kb], kept_hi = mass_end(kb);
+  }
+  if (s.p < 1.f) {
+    pb0 = bin_of_mass(false, (double)s.p * (double)kept_lo);
+    pb1 = bin_of_mass(false, (double)s.p * (double)kept_hi);
+    kept_lo = min(kept_lo, sh.mass[pb0]);
+    kept_hi = min(kept_hi, mass_end(pb1));
+  }
+  if (s.m > 0.f) {
+    mb = s.m >= 1.f ? 0 : r.bin(fmin(-log2((double)s.m), 63.0));
+    kept_lo = min(kept_lo, sh.mass[max(mb - 1, 0)]);
+    kept_hi = min(kept_hi, mass_end(min(mb + 1, kBins - 1)));
+  }
+  const u64 first = (u64)r.unit;  // the first word stays
+  kept_lo = max_u64(kept_lo, first), kept_hi = max_u64(kept_hi, first);
+  const int db0 = bin_of_mass(true, (double)s.u * (double)kept_lo), db1 = bin_of_mass(true, (double)s.u * (double)kept_hi);
+  for (int b = tid; b < kBins; b += kThreads)
+    sh.marked[b] = b == kb || (b >= pb0 && b <= pb1) || (mb >= 0 && abs(b - mb) <= 1) || (b >= db0 && b <= db1);
+  __syncthreads();
+
+  // ---- their words
+  each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t i) {
+    const double z = r.z(v);
+    if (z < r.far && sh.marked[r.bin(z)]) {
+      const int at = atomicAdd(&sh.n, 1);
+      if (at < kList) sh.list[at] = sample_word(sample_key(v), i);
+    }
+  });
+  __syncthreads();
+  const int n = sh.n;
+  if (n > kList) return draw_from_row(sh, r, s);
+
+  u64 kept = total;
+  if (n <= kPairwise) {
+    // each thread a word, and the words before it in its bin
+    u64 word = 0, one = 0, before = 0;
+    uint32_t rank = 0;
+    double w = 0.0;
+    int b = -1;
+    if (tid < n) {
+      word = sh.list[tid];
+      const double z = r.z(sample_value((uint32_t)(word >> 32)));
+      b = r.bin(z), w = exp2_minus(sh, z), one = units_of(r, w);
+      sh.bin[tid] = (uint16_t)b, sh.unit[tid] = one;
+    }
+    __syncthreads();
+    if (tid < n) {
+      before = sh.mass[b], rank = sh.count[b];
+      for (int j = 0; j < n; ++j)
+        if (sh.list[j] > word && sh.bin[j] == b) before += sh.unit[j], ++rank;
+    }
+    auto ask = [&](bool here, u64 answer) {  // from the one thread that has it
+      if (here) sh.result = answer;
+      __syncthreads();
+      const u64 a = sh.result;
+      __syncthreads();
+      return a;
+    };
+    const u64 end = before + one;
+    if (kb >= 0) kept = ask(tid < n && b == kb && rank + 1 == s.k, end);
+    if (s.p < 1.f) {
+      const double want = (double)s.p * (double)kept;
+      if (tid == 0) sh.result = first;  // (want not above 0: the first word)
+      __syncthreads();
+      const u64 at = ask(tid < n && (double)before < want && (double)end >= want, end);
+      kept = min(kept, at);
+    }
+    if (mb >= 0) {
+      u64 sum = tid < n && abs(b - mb) <= 1 && w >= (double)s.m ? one : 0;
+      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+      if (lane == 0) sh.wave_mass[wave] = sum;
+      __syncthreads();
+      sum = sh.mass[max(mb - 1, 0)];
+      for (int x = 0; x < kThreads / 64; ++x) sum += sh.wave_mass[x];
+      kept = min(kept, sum);
+    }
+    kept = max_u64(kept, first);
+    const double want = (double)s.u * (double)kept;
+    return (int32_t)ask(tid < n && (double)before <= want && (double)end > want, 0xffffffffu - (uint32_t)word);
+  }
+
+  // many words: descents over the list, bin by bin (sh.mass and sh.count are the descents' own:
+  // what begins before a bin is read first)
+  auto begin_of = [&](int b) { return Found{sh.mass[b], sh.count[b], 0, 0}; };
+  const Found kf = begin_of(max(kb, 0)), mf = begin_of(max(mb - 1, 0));
+  // (running masses at the ends of the bins from pb0 and db0 on, at most kPairwise of them)
+  __syncthreads();
+  const int np = s.p < 1.f ? pb1 - pb0 + 1 : 0, nd = db1 - db0 + 1;
+  if (np + nd + 2 > kPairwise) return draw_from_row(sh, r, s);
+  for (int i = tid; i < np + nd; i += kThreads) sh.unit[i] = sh.mass[i < np ? pb0 + i : db0 + i - np];
+  __syncthreads();
+  auto in_bin = [&](int bin) {
+    return [&, bin](int64_t i, uint32_t &k, u64 &u) {
+      k = (uint32_t)(sh.list[i] >> 32);
+      const double z = r.z(sample_value(k));
+      if (r.bin(z) != bin) return false;
+      u = units_of(r, exp2_minus(sh, z));
+      return true;
+    };
+  };
+  auto last_before = [&](int at, int count, bool over, double want) {  // the bin the mass `want` lies in
+    int i = 0;
+    while (i + 1 < count && (over ? (double)sh.unit[at + i + 1] <= want : (double)sh.unit[at + i + 1] < want)) ++i;
+    return i;
+  };
+  if (kb >= 0) {
+    const Found f = descend(sh, n, in_bin(kb), kf, (u64)s.k, false, 0.0);
+    kept = f.mass + ((u64)s.k - f.count) * units_at(sh, r, sample_value(f.key));
+  }
+  if (s.p < 1.f) {
+    const double want = (double)s.p * (double)kept;
+    const int i = last_before(0, np, false, want);
+    const Found f = descend(sh, n, in_bin(pb0 + i), Found{sh.unit[i], 0, 0, 0}, 0, false, want);
+    kept = min(kept, want > 0.0 ? mass_reaching(f, units_at(sh, r, sample_value(f.key)), want) : first);
+  }
+  if (mb >= 0) {
+    u64 sum = 0;
+    for (int i = tid; i < n; i += kThreads) {
+      const double z = r.z(sample_value((uint32_t)(sh.list[i] >> 32))), w = exp2_minus(sh, z);
+      if (abs(r.bin(z) - mb) <= 1 && w >= (double)s.m) sum += units_of(r, w);
+    }
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    __syncthreads();
+    if (lane == 0) sh.wave_mass[wave] = sum;
+    __syncthreads();
+    sum = mf.mass;
+    for (int x = 0; x < kThreads / 64; ++x) sum += sh.wave_mass[x];
+    kept = min(kept, sum);
+  }
+  kept = max_u64(kept, first);
+  const double want = (double)s.u * (double)kept;
+  const int i = last_before(np, nd, true, want);
+  const Found f = descend(sh, n, in_bin(db0 + i), Found{sh.unit[np + i], 0, 0, 0}, 0, true, want);
+  const u64 nth = tie_passing(f, units_at(sh, r, sample_value(f.key)), want);
+  const Found at = descend(sh, n, [&](int64_t x, uint32_t &k, u64 &u) {
+    k = (uint32_t)sh.list[x], u = 0;
+    return (uint32_t)(sh.list[x] >> 32) == f.key;
+  }, Found{}, nth + 1, false, 0.0);
+  return (int32_t)(0xffffffffu - at.key);
+}
+
+}  // namespace
+
+static_assert(sizeof(SampleShared) <= 106 << 10 && sizeof(SampleExtremes) == 16, "what the host lays out");
+
+extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_extremes(SampleArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  SampleShared &sh = *(SampleShared *)lds;
+  const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S, lo = part * a.chunk;
+  const void *const words = (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4);
+  const SampleExtremes e = join_extremes(sh, extremes_of(words, a.bf16, lo, min(lo + a.chunk, a.V)));
+  if (threadIdx.x == 0) a.extremes[blockIdx.x] = e;
+}
+
+extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  SampleShared &sh = *(SampleShared *)lds;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S;
+  Row r;
+  r.words = (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4);
+  r.bf16 = a.bf16, r.V = a.V;
+  SampleExtremes e;
+  if (a.S == 1) {
+    e = join_extremes(sh, extremes_of(r.words, r.bf16, 0, a.V));
+  } else {
+    e = a.extremes[row * a.S];
+    for (int i = 1; i < a.S; ++i) {
+      const SampleExtremes x = a.extremes[row * a.S + i];
+      e.top = max_u64(e.top, x.top), e.least = fminf(e.least, x.least);
+    }
+  }
+  const uint32_t top = (uint32_t)(e.top >> 32);
   const float T = a.temperature ? a.temperature[row] : 1.f;
-  if (!(T > 0.f) || top == 0xffffffffu || !(fabsf(vmax) < __builtin_huge_valf())) {
-    if (tid == 0) a.out[row] = (int32_t)(0xffffffffu - (uint32_t)best);
+  r.top = sample_value(top);
+  // the first maximum: no temperature, a NaN, or an infinite maximum (uniform over the row)
+  if (!(T > 0.f) || top == 0xffffffffu || !(fabsf(r.top) < __builtin_huge_valf())) {
+    if (part == 0 && tid == 0) a.out[row] = (int32_t)(0xffffffffu - (uint32_t)e.top);
     return;
   }
-  const double inv = 1.0 / (double)T, unit = (double)(1ull << a.shift);
-  auto weight = [&](float v) { return v == -__builtin_huge_valf() ? 0.0 : exp(((double)v - (double)vmax) * inv); };
-  auto units = [&](float v) { return (u64)(weight(v) * unit + 0.5); };
+  r.inv = 1.44269504088896340736 / (double)T;
+  r.unit = (double)(1ull << a.shift);
+  r.far = (double)a.shift + 1.0;
+  // bins over what weighs something, and no further than the row goes
+  const double span = fmin(r.z(e.least), r.far);
+  r.per_bin = span > 0.0 ? (double)kBins / span : 0.0;
 
-  // The word at which the running count reaches `count` (if above 0), else the running
-  // mass m satisfies m >= want (m > want where `over`), which some word does: its key,
-  // how many words have it, and the count and mass of the words of larger keys.
-  auto descend = [&](u64 count, bool over, double want) {
-    Found f{};
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += 1024) cnt[i] = 0, mass[i] = 0;
-      __syncthreads();
-      for (int64_t i = tid; i < a.V; i += 1024) {
-        const float v = value(i);
-        const uint32_t k = sample_key(v);
-        if (shift < 24 && (k >> (shift + 8)) != f.key) continue;
-        atomicAdd(&cnt[(k >> shift) & 255], 1u);
-        atomicAdd(&mass[(k >> shift) & 255], units(v));
-      }
-      __syncthreads();
-      if (tid == 0) {
-        int bin = 255;
-        for (; bin > 0; --bin) {
-          const u64 m = f.mass + mass[bin], c = f.count + cnt[bin];
-          if (cnt[bin] && (count ? c >= count : over ? (double)m > want : (double)m >= want)) break;
-          f.mass = m, f.count = c;
-        }
-        f.key = (f.key << 8) | (uint32_t)bin;
-        f.ties = cnt[bin];
-        found = f;
-      }
-      __syncthreads();
-      f = found;
-      __syncthreads();
+  for (int b = tid; b < kBins; b += kThreads) sh.mass[b] = 0, sh.count[b] = 0;
+  if (tid < 64) sh.exp2_table[tid] = exp2(-0.015625 * (double)tid);
+  __syncthreads();
+  const int64_t lo = part * a.chunk;
+  each_word(r.words, r.bf16, lo, min(lo + a.chunk, a.V), [&](float v, uint32_t) {
+    const double z = r.z(v);
+    if (z < r.far) {
+      const int b = r.bin(z);
+      atomicAdd(&sh.mass[b], units_of(r, exp2_minus(sh, z)));
+      atomicAdd(&sh.count[b], 1u);
     }
-    return f;
-  };
-  auto sum_units = [&](auto keep) {
-    u64 s = 0;
-    for (int64_t i = tid; i < a.V; i += 1024) {
-      const float v = value(i);
-      if (keep(v)) s += units(v);
+  });
+  __syncthreads();
+  if (a.S > 1) {
+    // the row's last workgroup joins the bins of all: written through and read past the dies'
+    // caches around the arrival counter, which goes back to zero
+    constexpr int words = 24 * 1024 / 8;
+    static_assert(sizeof sh.mass + sizeof sh.count == 8 * words, "mass and count in one piece");
+    u64 *const own = (u64 *)a.bins + blockIdx.x * (int64_t)words, *const here = sh.mass;
+    for (int i = tid; i < words; i += kThreads) __hip_atomic_store(own + i, here[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0)
+      sh.flag = __hip_atomic_fetch_add(a.arrivals + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
+    __syncthreads();
+    if (!sh.flag) return;
+    // (counts two to a word, none above 2^24: their sums do not meet)
+    const u64 *const all = (const u64 *)a.bins + row * a.S * (int64_t)words;
+    u64 sum[words / kThreads];
+#pragma unroll
+    for (int k = 0; k < words / kThreads; ++k) sum[k] = here[tid + k * kThreads];
+    for (int p0 = 0; p0 < a.S; p0 += 4) {
+      u64 x[4][words / kThreads];
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int k = 0; k < words / kThreads; ++k)
+          x[p][k] = p0 + p < a.S && p0 + p != part ? __hip_atomic_load(all + (p0 + p) * words + tid + k * kThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int k = 0; k < words / kThreads; ++k) sum[k] += x[p][k];
     }
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+#pragma unroll
+    for (int k = 0; k < words / kThreads; ++k) here[tid + k * kThreads] = sum[k];
+    if (tid == 0) __hip_atomic_store(a.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (lane == 0) red[wave] = s;
-    __syncthreads();
-    s = 0;
-    for (int w = 0; w < 16; ++w) s += red[w];
-    return s;
-  };
-
-  u64 kept = sum_units([](float) { return true; });
-  const int64_t k = a.top_k ? a.top_k[row] : 0;
-  if (k > 0 && k < a.V) {
-    const Found f = descend((u64)k, false, 0.0);
-    kept = f.mass + ((u64)k - f.count) * units(sample_value(f.key));
   }
-  const float p = a.top_p ? a.top_p[row] : 1.f;
-  const float mp = a.min_p ? a.min_p[row] : 0.f;
-  const double all = (double)kept;
-  if (p < 1.f) {
-    const double want = (double)p * all;
-    const Found f = descend(0, false, want);
-    const u64 one = units(sample_value(f.key));
-    const double n = ceil((want - (double)f.mass) / (double)one);  // (want lies in these ties: one > 0)
-    const u64 m = f.mass + (n > 1.0 ? (u64)n : 1) * one;
-    kept = m < kept ? m : kept;
-  }
-  if (mp > 0.f) {
-    const u64 m = sum_units([&](float v) { return weight(v) >= (double)mp; });
-    kept = m < kept ? m : kept;
-  }
-  if (kept < (1ull << a.shift)) kept = 1ull << a.shift;  // the first word stays
-  const float r = a.uniform[row], u = r > 0.f ? fminf(r, 0x1.fffffep-1f) : 0.f;
-  const double want = (double)u * (double)kept;
-  const Found f = descend(0, true, want);
-  u64 nth = (u64)((want - (double)f.mass) / (double)units(sample_value(f.key)));
-  if (nth >= f.ties) nth = f.ties - 1;
-  // the nth (from 0) of the words with this key, by index
-  u64 seen = 0;
-  for (int64_t i0 = 0; seen <= nth; i0 += 1024) {
-    __syncthreads();
-    const bool hit = i0 + tid < a.V && sample_key(value(i0 + tid)) == f.key;
-    const unsigned long long bal = __ballot(hit);
-    if (lane == 0) red[wave] = __popcll(bal);
-    __syncthreads();
-    u64 before = seen + __popcll(bal & ((1ull << lane) - 1));
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) before += red[w];
-      seen += red[w];
-    }
-    if (hit && before == nth) a.out[row] = (int32_t)(i0 + tid);
-  }
+  Settings s;
+  const float u = a.uniform[row];
+  s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  s.k = a.top_k ? a.top_k[row] : 0;
+  s.p = a.top_p ? a.top_p[row] : 1.f;
+  s.m = a.min_p ? a.min_p[row] : 0.f;
+  const int32_t token = draw(sh, r, s);
+  if (tid == 0) a.out[row] = token;
 }

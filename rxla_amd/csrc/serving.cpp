@@ -51,7 +51,14 @@ struct SampleArgs {
   int64_t V;
   int shift;
   int bf16;
+  int S;
+  int64_t chunk;
+  char *extremes;
+  int *arrivals;
+  char *bins;
 };
+constexpr int64_t kSampleExtremes = 16, kSampleBins = 24 << 10;  // bytes of a workgroup's records
+constexpr size_t kSampleLds = 106 << 10;                         // SampleShared
 
 static bool is_f(int dt) { return dt == RXW8_F32 || dt == RXW8_BF16; }
 static bool is_vec(const Buffer *b, int dtype, int64_t n) {
@@ -302,9 +309,25 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   SampleArgs a{logits->ptr, (const float *)uniform->ptr, temperature ? (const float *)temperature->ptr : nullptr,
                top_k ? (const int32_t *)top_k->ptr : nullptr, top_p ? (const float *)top_p->ptr : nullptr,
-               min_p ? (const float *)min_p->ptr : nullptr, (int32_t *)out->ptr, V, 62 - bits > 52 ? 52 : 62 - bits,
-               logits->dtype == RXW8_BF16};
-  return launch(rt, "rxw8_sample_any", dim3((unsigned)B), dim3(1024), a);
+               min_p ? (const float *)min_p->ptr : nullptr, (int32_t *)out->ptr, V, 62 - bits > 51 ? 51 : 62 - bits,
+               logits->dtype == RXW8_BF16, 1, V, nullptr, nullptr, nullptr};
+  // Workgroups to a row: as many as leave one to a CU, but no more than 16, whose bins the
+  // last one reads, and none with fewer than 4096 words
+  a.S = (int)std::max<int64_t>(1, std::min<int64_t>({16, rt->cus / B, (V + 4095) / 4096}));
+  a.chunk = (V + a.S - 1) / a.S;
+  if (a.S > 1) {
+    char *block = rt->f32_attn[stream_capturing(rt) ? 1 : 0];
+    a.arrivals = (int *)block;
+    a.extremes = block + RXW8_NOALLOC_COUNTER_BYTES;
+    a.bins = a.extremes + (64 << 10);
+    if (a.S * B * kSampleExtremes > (64 << 10) || a.S * B * kSampleBins > (int64_t)RXW8_NOALLOC_PARTIAL_BYTES - (64 << 10))
+      a.S = 1, a.chunk = V;
+  }
+  if (a.S > 1) {
+    int rc = launch(rt, "rxw8_sample_extremes", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
+    if (rc) return rc;
+  }
+  return launch(rt, "rxw8_sample_draw", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
 }
 
 int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform, rxw8_buffer *temperature,
