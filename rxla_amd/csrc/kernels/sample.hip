@@ -36,8 +36,8 @@ struct SampleArgs {
   int64_t V;
   int shift;                   // s
   int bf16;
-  // S workgroups share a row, `chunk` words each (0 and V: one has it alone): extremes
-  // [B][S], arrivals [B] (zero between launches), and bins [B][S] of 24 KiB
+  // S workgroups share a row, `chunk` words each (1 and V: one has it alone): extremes
+  // [B][S], arrivals [B] (zero between launches), and bins [B][S] of 12 KiB
   int S;
   int64_t chunk;
   struct SampleExtremes *extremes;
@@ -49,7 +49,7 @@ typedef unsigned long long u64;
 
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048, kList = 8192, kPairwise = 1024;
+constexpr int kThreads = 1024, kBins = 1024, kList = 8192, kPairwise = 1024;
 
 // Ascending keys for ascending values, -0 and +0 alike; above them all a NaN
 __device__ __forceinline__ uint32_t sample_key(float v) {
@@ -121,7 +121,7 @@ struct Found {
 };
 
 struct SampleShared {
-  u64 mass[kBins];      // (mass and count: 24 KiB in one piece)
+  u64 mass[kBins];      // (mass and count: 12 KiB in one piece)
   uint32_t count[kBins];
   u64 list[kList];      // words of the bins looked at
   u64 unit[kPairwise];  // their masses and bins
@@ -133,7 +133,7 @@ struct SampleShared {
   SampleExtremes wave_ext[16];
   Found found;
   u64 result;
-  int n, flag;
+  int n, flag, at[2];
 };
 
 struct Row {
@@ -147,22 +147,28 @@ struct Row {
   double far;        // z from which on words weigh nothing
 
   __device__ double z(float v) const { return ((double)top - (double)v) * inv; }
-  __device__ int bin(double zv) const { return min((int)(zv * per_bin), kBins - 1); }
+  // (the nearest whole number, in the low bits of a sum with 1.5 2^52)
+  __device__ int bin(double zv) const {
+    return min((int)(uint32_t)__builtin_bit_cast(u64, fma(zv, per_bin, 0x1.8p52)), kBins - 1);
+  }
 };
 
-// 2^-z for 0 <= z < 64: z = n / 64 + r, 2^(-n / 64) from a table of 64 and an exponent, and the
-// series of exp(-r ln 2) to the fifth power: the next term is below 2^-48
+// The mass of z, 0 <= z < 54: round(2^(s - z)). z = n / 64 + r with |r| <= 1 / 128 (the addition
+// rounds to 64ths and leaves n in its low bits), 2^(-n / 64) from a table of 64 and the
+// exponent, 2^-r from the series of exp(-r ln 2) to the fifth power, the next term of which is
+// below 2^-54; and the sum with 2^52 holds the whole number in its low bits.
 __device__ __forceinline__ double exp2_minus(const SampleShared &sh, double z) {
-  const int n = (int)(z * 64.0);
-  const double x = (z - (double)n * 0.015625) * -0.69314718055994530942;
+  const double t = z + 0x1.8p46;
+  const int n = (int)(uint32_t)__builtin_bit_cast(u64, t);
+  const double x = (z - (t - 0x1.8p46)) * -0.69314718055994530942;
   double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
   p = fma(x, p, 1.0 / 6.0);
   p = fma(x, p, 0.5);
   p = fma(x, p, 1.0);
   p = fma(x, p, 1.0);
-  return ldexp(p * sh.exp2_table[n & 63], -(n >> 6));
+  return __builtin_bit_cast(double, __builtin_bit_cast(u64, p * sh.exp2_table[n & 63]) - ((u64)(n >> 6) << 52));
 }
-__device__ __forceinline__ u64 units_of(const Row &r, double w) {  // (w unit + 2^52 holds it in its low bits)
+__device__ __forceinline__ u64 units_of(const Row &r, double w) {
   return __builtin_bit_cast(u64, fma(w, r.unit, 0x1p52)) & 0xfffffffffffffull;
 }
 // The mass of a word (0 from r.far on)
@@ -188,12 +194,15 @@ __device__ SampleExtremes join_extremes(SampleShared &sh, SampleExtremes e) {
   return e;
 }
 __device__ SampleExtremes extremes_of(const void *row, bool bf16, int64_t lo, int64_t hi) {
-  SampleExtremes e{0, __builtin_huge_valf(), 0};
-  each_word(row, bf16, lo, hi, [&](float v, uint32_t i) {
-    e.top = max_u64(e.top, sample_word(sample_key(v), i));
-    if (v > -__builtin_huge_valf()) e.least = fminf(e.least, v);
+  uint32_t key = 0, index = 0xffffffffu;
+  float least = __builtin_huge_valf();
+  each_word(row, bf16, lo, hi, [&](float v, uint32_t i) {  // (a thread's words come in order but for its first and last)
+    const uint32_t k = sample_key(v);
+    const bool better = k > key || (k == key && i < index);
+    key = better ? k : key, index = better ? i : index;
+    least = fminf(least, v > -__builtin_huge_valf() ? v : __builtin_huge_valf());
   });
-  return e;
+  return SampleExtremes{sample_word(key, index), least, 0};
 }
 
 // Radix descent, 8 bits a pass, over the i < n that get(i, key, units) admits: the key at which
@@ -301,75 +310,80 @@ __device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings 
 // The token, from the counts and masses of the row's bins (in sh)
 __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // ---- running masses and counts before each bin, in place: thread t has bins 2 t and 2 t + 1
-  u64 m0 = sh.mass[2 * tid], m1 = sh.mass[2 * tid + 1], m = m0 + m1;
-  uint32_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], c = c0 + c1;
-  const u64 mine = m;
-  const uint32_t mine_c = c;
+  // ---- running masses and counts before each bin, in place: a bin a thread
+  const u64 mine = sh.mass[tid];
+  const uint32_t mine_c = sh.count[tid];
+  u64 m = mine;
+  uint32_t c = mine_c;
   for (int o = 1; o < 64; o <<= 1) {
     const u64 x = __shfl_up(m, o);
     const uint32_t y = __shfl_up(c, o);
     if (lane >= o) m += x, c += y;
   }
   if (lane == 63) sh.wave_mass[wave] = m, sh.wave_count[wave] = c;
-  for (int b = tid; b < kBins; b += kThreads) sh.marked[b] = 0;
   if (tid == 0) sh.n = 0;
   __syncthreads();
   u64 total = 0;
   uint32_t counted = 0;
-  m -= mine, c -= mine_c;
   for (int w = 0; w < kThreads / 64; ++w) {
     if (w < wave) m += sh.wave_mass[w], c += sh.wave_count[w];
     total += sh.wave_mass[w], counted += sh.wave_count[w];
   }
-  sh.mass[2 * tid] = m, sh.mass[2 * tid + 1] = m + m0;
-  sh.count[2 * tid] = c, sh.count[2 * tid + 1] = c + c0;
-  __syncthreads();
+  const double end = (double)m;  // of this thread's bin
+  m -= mine, c -= mine_c;
+  const double begin = (double)m;
+  sh.mass[tid] = m, sh.count[tid] = c;
   auto mass_end = [&](int b) { return b + 1 < kBins ? sh.mass[b + 1] : total; };
-  // first bin at whose end the running mass satisfies the condition
-  auto bin_of_mass = [&](bool over, double want) {
-    int lo = 0, hi = kBins - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      const double e = (double)mass_end(mid);
-      if (over ? e > want : e >= want) hi = mid;
-      else lo = mid + 1;
-    }
-    return lo;
+  // The bins in which masses want[0] and want[1] are reached (`over`: passed): the thread whose bin it is says so
+  auto bins_of = [&](bool over, double want0, double want1, int &b0, int &b1) {
+    if (tid < 2) sh.at[tid] = over ? kBins - 1 : 0;
+    __syncthreads();
+    if (over ? begin <= want0 && end > want0 : begin < want0 && end >= want0) sh.at[0] = tid;
+    if (over ? begin <= want1 && end > want1 : begin < want1 && end >= want1) sh.at[1] = tid;
+    __syncthreads();
+    b0 = sh.at[0], b1 = sh.at[1];
+    __syncthreads();
   };
   // ---- the bins in which borders and token can lie (uniform over the workgroup)
   u64 kept_lo = total, kept_hi = total;  // bounds of what is left
-  int kb = -1, pb0 = 1, pb1 = 0, mb = -1;
+  int kb = -1, pb0 = 1, pb1 = 0, mb = -1, db0, db1;
+  __syncthreads();
   if (s.k > 0 && s.k < counted) {
-    int lo = 0, hi = kBins - 1;  // last bin that begins before rank k
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (sh.count[mid] < s.k) lo = mid;
-      else hi = mid - 1;
-    }
-    kb = lo;
+    if (c < s.k && c + mine_c >= s.k) sh.at[0] = tid;
+    __syncthreads();
+    kb = sh.at[0];
+    __syncthreads();
     kept_lo = sh.mass[kb], kept_hi = mass_end(kb);
   }
   if (s.p < 1.f) {
-    pb0 = bin_of_mass(false, (double)s.p * (double)kept_lo);
-    pb1 = bin_of_mass(false, (double)s.p * (double)kept_hi);
+    bins_of(false, (double)s.p * (double)kept_lo, (double)s.p * (double)kept_hi, pb0, pb1);
     kept_lo = min(kept_lo, sh.mass[pb0]);
     kept_hi = min(kept_hi, mass_end(pb1));
   }
   if (s.m > 0.f) {
-    mb = s.m >= 1.f ? 0 : r.bin(fmin(-log2((double)s.m), 63.0));
+    mb = s.m >= 1.f ? 0 : r.bin(fmin(-log2((double)s.m), r.far));
     kept_lo = min(kept_lo, sh.mass[max(mb - 1, 0)]);
     kept_hi = min(kept_hi, mass_end(min(mb + 1, kBins - 1)));
   }
   const u64 first = (u64)r.unit;  // the first word stays
   kept_lo = max_u64(kept_lo, first), kept_hi = max_u64(kept_hi, first);
-  const int db0 = bin_of_mass(true, (double)s.u * (double)kept_lo), db1 = bin_of_mass(true, (double)s.u * (double)kept_hi);
-  for (int b = tid; b < kBins; b += kThreads)
-    sh.marked[b] = b == kb || (b >= pb0 && b <= pb1) || (mb >= 0 && abs(b - mb) <= 1) || (b >= db0 && b <= db1);
+  bins_of(true, (double)s.u * (double)kept_lo, (double)s.u * (double)kept_hi, db0, db1);
+  const bool look = tid == kb || (tid >= pb0 && tid <= pb1) || (mb >= 0 && abs(tid - mb) <= 1) || (tid >= db0 && tid <= db1);
+  sh.marked[tid] = look;
+  // ... and the values these bins lie between, a bin and two steps wider
+  int b_lo = min(db0, kBins - 1), b_hi = db1;
+  if (kb >= 0) b_lo = min(b_lo, kb), b_hi = max(b_hi, kb);
+  if (pb0 <= pb1) b_lo = min(b_lo, pb0), b_hi = max(b_hi, pb1);
+  if (mb >= 0) b_lo = min(b_lo, mb - 1), b_hi = max(b_hi, mb + 1);
+  auto key_at = [&](int b) { return sample_key((float)((double)r.top - (double)b / (r.per_bin * r.inv))); };
+  const float v_lo = sample_value(max(key_at(b_hi + 1) - 2, sample_key(-__builtin_huge_valf())));
+  const float v_hi = b_lo <= 1 ? r.top : sample_value(min(key_at(b_lo - 1) + 2, sample_key(r.top)));
+  const float least = b_hi + 1 < kBins ? v_lo : -__builtin_huge_valf();
   __syncthreads();
 
   // ---- their words
   each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t i) {
+    if (!(v >= least && v <= v_hi)) return;
     const double z = r.z(v);
     if (z < r.far && sh.marked[r.bin(z)]) {
       const int at = atomicAdd(&sh.n, 1);
@@ -406,13 +420,13 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
       __syncthreads();
       return a;
     };
-    const u64 end = before + one;
-    if (kb >= 0) kept = ask(tid < n && b == kb && rank + 1 == s.k, end);
+    const u64 end_of = before + one;
+    if (kb >= 0) kept = ask(tid < n && b == kb && rank + 1 == s.k, end_of);
     if (s.p < 1.f) {
       const double want = (double)s.p * (double)kept;
       if (tid == 0) sh.result = first;  // (want not above 0: the first word)
       __syncthreads();
-      const u64 at = ask(tid < n && (double)before < want && (double)end >= want, end);
+      const u64 at = ask(tid < n && (double)before < want && (double)end_of >= want, end_of);
       kept = min(kept, at);
     }
     if (mb >= 0) {
@@ -426,7 +440,7 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
     }
     kept = max_u64(kept, first);
     const double want = (double)s.u * (double)kept;
-    return (int32_t)ask(tid < n && (double)before <= want && (double)end > want, 0xffffffffu - (uint32_t)word);
+    return (int32_t)ask(tid < n && (double)before <= want && (double)end_of > want, 0xffffffffu - (uint32_t)word);
   }
 
   // many words: descents over the list, bin by bin (sh.mass and sh.count are the descents' own:
@@ -491,7 +505,7 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
 
 }  // namespace
 
-static_assert(sizeof(SampleShared) <= 106 << 10 && sizeof(SampleExtremes) == 16, "what the host lays out");
+static_assert(sizeof(SampleShared) <= 92 << 10 && sizeof(SampleExtremes) == 16, "what the host lays out");
 
 extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_extremes(SampleArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -514,10 +528,10 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   if (a.S == 1) {
     e = join_extremes(sh, extremes_of(r.words, r.bf16, 0, a.V));
   } else {
-    e = a.extremes[row * a.S];
-    for (int i = 1; i < a.S; ++i) {
-      const SampleExtremes x = a.extremes[row * a.S + i];
-      e.top = max_u64(e.top, x.top), e.least = fminf(e.least, x.least);
+    e = a.extremes[row * a.S + min(tid & 63, a.S - 1)];
+    for (int o = 32; o > 0; o >>= 1) {
+      e.top = max_u64(e.top, __shfl_xor(e.top, o));
+      e.least = fminf(e.least, __shfl_xor(e.least, o));
     }
   }
   const uint32_t top = (uint32_t)(e.top >> 32);
@@ -533,10 +547,27 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   r.far = (double)a.shift + 1.0;
   // bins over what weighs something, and no further than the row goes
   const double span = fmin(r.z(e.least), r.far);
-  r.per_bin = span > 0.0 ? (double)kBins / span : 0.0;
+  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
+  Settings s;
+  const float u = a.uniform[row];
+  s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  s.k = a.top_k ? a.top_k[row] : 0;
+  s.p = a.top_p ? a.top_p[row] : 1.f;
+  s.m = a.min_p ? a.min_p[row] : 0.f;
+  if (s.k >= a.V) s.k = 0;
 
-  for (int b = tid; b < kBins; b += kThreads) sh.mass[b] = 0, sh.count[b] = 0;
-  if (tid < 64) sh.exp2_table[tid] = exp2(-0.015625 * (double)tid);
+  static_assert(kBins == kThreads, "a bin a thread");
+  sh.mass[tid] = 0, sh.count[tid] = 0;
+  if (tid < 64) {  // 2^(-tid / 64), bit by bit
+    double t = 1.0;
+    if (tid & 1) t *= 0x1.fa7c1819e90d8p-1;
+    if (tid & 2) t *= 0x1.f50765b6e4540p-1;
+    if (tid & 4) t *= 0x1.ea4afa2a490dap-1;
+    if (tid & 8) t *= 0x1.d5818dcfba487p-1;
+    if (tid & 16) t *= 0x1.ae89f995ad3adp-1;
+    if (tid & 32) t *= 0x1.6a09e667f3bcdp-1;
+    sh.exp2_table[tid] = t;
+  }
   __syncthreads();
   const int64_t lo = part * a.chunk;
   each_word(r.words, r.bf16, lo, min(lo + a.chunk, a.V), [&](float v, uint32_t) {
@@ -544,51 +575,37 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
     if (z < r.far) {
       const int b = r.bin(z);
       atomicAdd(&sh.mass[b], units_of(r, exp2_minus(sh, z)));
-      atomicAdd(&sh.count[b], 1u);
+      if (s.k > 0) atomicAdd(&sh.count[b], 1u);
     }
   });
   __syncthreads();
   if (a.S > 1) {
     // the row's last workgroup joins the bins of all: written through and read past the dies'
     // caches around the arrival counter, which goes back to zero
-    constexpr int words = 24 * 1024 / 8;
+    constexpr int words = 12 * 1024 / 8;  // masses, then counts two to a word, none above 2^24
     static_assert(sizeof sh.mass + sizeof sh.count == 8 * words, "mass and count in one piece");
-    u64 *const own = (u64 *)a.bins + blockIdx.x * (int64_t)words, *const here = sh.mass;
-    for (int i = tid; i < words; i += kThreads) __hip_atomic_store(own + i, here[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    u64 *const here = sh.mass, *const all = (u64 *)a.bins + row * a.S * (int64_t)words;
+    const int used = s.k > 0 ? words : kBins;
+    for (int i = tid; i < used; i += kThreads)
+      __hip_atomic_store(all + part * words + i, here[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0)
       sh.flag = __hip_atomic_fetch_add(a.arrivals + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
     __syncthreads();
     if (!sh.flag) return;
-    // (counts two to a word, none above 2^24: their sums do not meet)
-    const u64 *const all = (const u64 *)a.bins + row * a.S * (int64_t)words;
-    u64 sum[words / kThreads];
+    for (int i = tid; i < used; i += kThreads) {
+      u64 x[8], sum = 0;
 #pragma unroll
-    for (int k = 0; k < words / kThreads; ++k) sum[k] = here[tid + k * kThreads];
-    for (int p0 = 0; p0 < a.S; p0 += 4) {
-      u64 x[4][words / kThreads];
+      for (int p = 0; p < 8; ++p)
+        x[p] = p < a.S ? __hip_atomic_load(all + p * words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int k = 0; k < words / kThreads; ++k)
-          x[p][k] = p0 + p < a.S && p0 + p != part ? __hip_atomic_load(all + (p0 + p) * words + tid + k * kThreads, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int k = 0; k < words / kThreads; ++k) sum[k] += x[p][k];
+      for (int p = 0; p < 8; ++p) sum += x[p];
+      here[i] = sum;
     }
-#pragma unroll
-    for (int k = 0; k < words / kThreads; ++k) here[tid + k * kThreads] = sum[k];
     if (tid == 0) __hip_atomic_store(a.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
   }
-  Settings s;
-  const float u = a.uniform[row];
-  s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  s.k = a.top_k ? a.top_k[row] : 0;
-  s.p = a.top_p ? a.top_p[row] : 1.f;
-  s.m = a.min_p ? a.min_p[row] : 0.f;
   const int32_t token = draw(sh, r, s);
   if (tid == 0) a.out[row] = token;
 }

@@ -57,8 +57,8 @@ struct SampleArgs {
   int *arrivals;
   char *bins;
 };
-constexpr int64_t kSampleExtremes = 16, kSampleBins = 24 << 10;  // bytes of a workgroup's records
-constexpr size_t kSampleLds = 106 << 10;                         // SampleShared
+constexpr int64_t kSampleExtremes = 16, kSampleBins = 12 << 10;  // bytes of a workgroup's records
+constexpr size_t kSampleLds = 92 << 10;                          // SampleShared
 
 static bool is_f(int dt) { return dt == RXW8_F32 || dt == RXW8_BF16; }
 static bool is_vec(const Buffer *b, int dtype, int64_t n) {
@@ -311,9 +311,9 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
                top_k ? (const int32_t *)top_k->ptr : nullptr, top_p ? (const float *)top_p->ptr : nullptr,
                min_p ? (const float *)min_p->ptr : nullptr, (int32_t *)out->ptr, V, 62 - bits > 51 ? 51 : 62 - bits,
                logits->dtype == RXW8_BF16, 1, V, nullptr, nullptr, nullptr};
-  // Workgroups to a row: as many as leave one to a CU, but no more than 16, whose bins the
+  // Workgroups to a row: as many as leave one to a CU, but no more than 8, whose bins the
   // last one reads, and none with fewer than 4096 words
-  a.S = (int)std::max<int64_t>(1, std::min<int64_t>({16, rt->cus / B, (V + 4095) / 4096}));
+  a.S = (int)std::max<int64_t>(1, std::min<int64_t>({8, rt->cus / B, (V + 4095) / 4096}));
   a.chunk = (V + a.S - 1) / a.S;
   if (a.S > 1) {
     char *block = rt->f32_attn[stream_capturing(rt) ? 1 : 0];
