@@ -19,11 +19,13 @@
 // the bins are in the words' order; the running counts and masses of the bins tell the
 // bins that the borders of top_k, top_p and min_p and the token can lie in; and only the
 // words of those bins, one row's some dozens to hundreds, are looked at one by one.
-// Two launches where workgroups share a row (the maxima, then the bins, which the last
-// workgroup of a row to arrive joins and draws from), one where each has its own. What
-// bounds a batch is reading the logits: once from memory, then twice more from the
+// Three launches where workgroups share a row (the maxima; the bins, which the last
+// workgroup of a row to arrive joins; the words, from which the last one draws), one where
+// each has its own. What bounds a batch is reading the logits: once from memory, then twice more from the
 // caches, the second time with an exponential in f64 and two LDS atomics for each
 // word; a single row is bound by the length of the chain.
+#include <stddef.h>
+
 #include "common.h"
 
 struct SampleArgs {
@@ -37,11 +39,14 @@ struct SampleArgs {
   int shift;                   // s
   int bf16;
   // S workgroups share a row, `chunk` words each (1 and V: one has it alone): extremes
-  // [B][S], arrivals [B] (zero between launches), and bins [B][S] of 12 KiB
+  // [B][S], arrivals [B] and listed words [B] (zero between launches), and bins [B][S] of
+  // 12 KiB; the row's joined bins take the place of the first's, its words and Borders
+  // that of the second's
   int S;
   int64_t chunk;
   struct SampleExtremes *extremes;
   int *arrivals;
+  int *listed;
   char *bins;
 };
 
@@ -152,6 +157,21 @@ struct Row {
     return min((int)(uint32_t)__builtin_bit_cast(u64, fma(zv, per_bin, 0x1.8p52)), kBins - 1);
   }
 };
+
+// 2^(-i / 64), i < 64, bit by bit
+__device__ __forceinline__ void fill_table(SampleShared &sh) {
+  const int tid = threadIdx.x;
+  if (tid < 64) {
+    double t = 1.0;
+    if (tid & 1) t *= 0x1.fa7c1819e90d8p-1;
+    if (tid & 2) t *= 0x1.f50765b6e4540p-1;
+    if (tid & 4) t *= 0x1.ea4afa2a490dap-1;
+    if (tid & 8) t *= 0x1.d5818dcfba487p-1;
+    if (tid & 16) t *= 0x1.ae89f995ad3adp-1;
+    if (tid & 32) t *= 0x1.6a09e667f3bcdp-1;
+    sh.exp2_table[tid] = t;
+  }
+}
 
 // The mass of z, 0 <= z < 54: round(2^(s - z)). z = n / 64 + r with |r| <= 1 / 128 (the addition
 // rounds to 64ths and leaves n in its low bits), 2^(-n / 64) from a table of 64 and the
@@ -307,8 +327,17 @@ __device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings 
   return (int32_t)(0xffffffffu - at.key);
 }
 
-// The token, from the counts and masses of the row's bins (in sh)
-__device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
+// The bins that a row's borders and token can lie in
+struct Borders {
+  u64 total;          // the row's mass
+  float least, most;  // what the values of these bins lie between
+  int kb, mb;         // the bins of top_k's border, and of min_p's, give or take one (-1: none)
+  int pb0, pb1;       // ... of top_p's (pb0 > pb1: none)
+  int db0, db1;       // ... of the token
+};
+
+// ... from the counts and masses of the row's bins, which become running ones (in sh)
+__device__ Borders borders_of(SampleShared &sh, const Row &r, const Settings &s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // ---- running masses and counts before each bin, in place: a bin a thread
   const u64 mine = sh.mass[tid];
@@ -321,7 +350,6 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
     if (lane >= o) m += x, c += y;
   }
   if (lane == 63) sh.wave_mass[wave] = m, sh.wave_count[wave] = c;
-  if (tid == 0) sh.n = 0;
   __syncthreads();
   u64 total = 0;
   uint32_t counted = 0;
@@ -368,8 +396,6 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
   const u64 first = (u64)r.unit;  // the first word stays
   kept_lo = max_u64(kept_lo, first), kept_hi = max_u64(kept_hi, first);
   bins_of(true, (double)s.u * (double)kept_lo, (double)s.u * (double)kept_hi, db0, db1);
-  const bool look = tid == kb || (tid >= pb0 && tid <= pb1) || (mb >= 0 && abs(tid - mb) <= 1) || (tid >= db0 && tid <= db1);
-  sh.marked[tid] = look;
   // ... and the values these bins lie between, a bin and two steps wider
   int b_lo = min(db0, kBins - 1), b_hi = db1;
   if (kb >= 0) b_lo = min(b_lo, kb), b_hi = max(b_hi, kb);
@@ -378,12 +404,19 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
   auto key_at = [&](int b) { return sample_key((float)((double)r.top - (double)b / (r.per_bin * r.inv))); };
   const float v_lo = sample_value(max(key_at(b_hi + 1) - 2, sample_key(-__builtin_huge_valf())));
   const float v_hi = b_lo <= 1 ? r.top : sample_value(min(key_at(b_lo - 1) + 2, sample_key(r.top)));
-  const float least = b_hi + 1 < kBins ? v_lo : -__builtin_huge_valf();
-  __syncthreads();
+  return Borders{total, b_hi + 1 < kBins ? v_lo : -__builtin_huge_valf(), v_hi, kb, mb, pb0, pb1, db0, db1};
+}
 
-  // ---- their words
-  each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t i) {
-    if (!(v >= least && v <= v_hi)) return;
+// The words lo <= index < hi in these bins, the first kList of them in sh.list; sh.n of them
+__device__ void words_of(SampleShared &sh, const Row &r, const Borders &b, int64_t lo, int64_t hi) {
+  const int tid = threadIdx.x;
+  __syncthreads();
+  sh.marked[tid] = tid == b.kb || (tid >= b.pb0 && tid <= b.pb1) || (b.mb >= 0 && abs(tid - b.mb) <= 1) ||
+                   (tid >= b.db0 && tid <= b.db1);
+  if (tid == 0) sh.n = 0;
+  __syncthreads();
+  each_word(r.words, r.bf16, lo, hi, [&](float v, uint32_t i) {
+    if (!(v >= b.least && v <= b.most)) return;
     const double z = r.z(v);
     if (z < r.far && sh.marked[r.bin(z)]) {
       const int at = atomicAdd(&sh.n, 1);
@@ -391,6 +424,13 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
     }
   });
   __syncthreads();
+}
+
+// The token, from these words and the running masses and counts (in sh)
+__device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const Borders &borders) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const u64 total = borders.total, first = (u64)r.unit;
+  const int kb = borders.kb, mb = borders.mb, pb0 = borders.pb0, pb1 = borders.pb1, db0 = borders.db0, db1 = borders.db1;
   const int n = sh.n;
   if (n > kList) return draw_from_row(sh, r, s);
 
@@ -503,6 +543,60 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s) {
   return (int32_t)(0xffffffffu - at.key);
 }
 
+constexpr int kBinWords = 12 * 1024 / 8;  // masses, then counts two to a word, none above 2^24
+static_assert(sizeof SampleShared::mass + sizeof SampleShared::count == 8 * kBinWords &&
+                  offsetof(SampleShared, count) == sizeof SampleShared::mass && 8 * kPairwise + sizeof(Borders) <= 8 * kBinWords,
+              "mass and count in one piece; words and borders in the second's place");
+
+__device__ const void *words_at(const SampleArgs &a, int64_t row) { return (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4); }
+__device__ u64 *bins_at(const SampleArgs &a, int64_t row, int part) { return (u64 *)a.bins + (row * a.S + part) * kBinWords; }
+__device__ u64 *list_at(const SampleArgs &a, int64_t row) { return bins_at(a, row, 1); }
+__device__ Borders *borders_at(const SampleArgs &a, int64_t row) { return (Borders *)(bins_at(a, row, 1) + kPairwise); }
+
+__device__ SampleExtremes row_extremes(const SampleArgs &a, int64_t row) {
+  SampleExtremes e = a.extremes[row * a.S + min((int)(threadIdx.x & 63), a.S - 1)];
+  for (int o = 32; o > 0; o >>= 1) {
+    e.top = max_u64(e.top, __shfl_xor(e.top, o));
+    e.least = fminf(e.least, __shfl_xor(e.least, o));
+  }
+  return e;
+}
+
+// False where the token is the first maximum: no temperature, a NaN, or an infinite maximum
+// (uniform over the row)
+__device__ bool set_row(const SampleArgs &a, int64_t row, const SampleExtremes &e, Row &r, Settings &s) {
+  r.words = words_at(a, row), r.bf16 = a.bf16, r.V = a.V;
+  const uint32_t top = (uint32_t)(e.top >> 32);
+  const float T = a.temperature ? a.temperature[row] : 1.f;
+  r.top = sample_value(top);
+  if (!(T > 0.f) || top == 0xffffffffu || !(fabsf(r.top) < __builtin_huge_valf())) return false;
+  r.inv = 1.44269504088896340736 / (double)T;
+  r.unit = (double)(1ull << a.shift);
+  r.far = (double)a.shift + 1.0;
+  // bins over what weighs something, and no further than the row goes
+  const double span = fmin(r.z(e.least), r.far);
+  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
+  const float u = a.uniform[row];
+  s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
+  s.k = a.top_k ? a.top_k[row] : 0;
+  s.p = a.top_p ? a.top_p[row] : 1.f;
+  s.m = a.min_p ? a.min_p[row] : 0.f;
+  if (s.k >= a.V) s.k = 0;
+  return true;
+}
+// Whether this workgroup is the row's last to arrive; what all have stored past the dies' caches
+// (agent scope) before is then there to read, and the counter is back at zero
+__device__ bool last_of_row(const SampleArgs &a, SampleShared &sh, int64_t row) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sh.flag = __hip_atomic_fetch_add(a.arrivals + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
+    if (sh.flag) __hip_atomic_store(a.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  return sh.flag;
+}
+
 }  // namespace
 
 static_assert(sizeof(SampleShared) <= 92 << 10 && sizeof(SampleExtremes) == 16, "what the host lays out");
@@ -522,52 +616,20 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S;
   Row r;
-  r.words = (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4);
-  r.bf16 = a.bf16, r.V = a.V;
   SampleExtremes e;
   if (a.S == 1) {
-    e = join_extremes(sh, extremes_of(r.words, r.bf16, 0, a.V));
+    e = join_extremes(sh, extremes_of(words_at(a, row), a.bf16, 0, a.V));
   } else {
-    e = a.extremes[row * a.S + min(tid & 63, a.S - 1)];
-    for (int o = 32; o > 0; o >>= 1) {
-      e.top = max_u64(e.top, __shfl_xor(e.top, o));
-      e.least = fminf(e.least, __shfl_xor(e.least, o));
-    }
+    e = row_extremes(a, row);
   }
-  const uint32_t top = (uint32_t)(e.top >> 32);
-  const float T = a.temperature ? a.temperature[row] : 1.f;
-  r.top = sample_value(top);
-  // the first maximum: no temperature, a NaN, or an infinite maximum (uniform over the row)
-  if (!(T > 0.f) || top == 0xffffffffu || !(fabsf(r.top) < __builtin_huge_valf())) {
+  Settings s;
+  if (!set_row(a, row, e, r, s)) {
     if (part == 0 && tid == 0) a.out[row] = (int32_t)(0xffffffffu - (uint32_t)e.top);
     return;
   }
-  r.inv = 1.44269504088896340736 / (double)T;
-  r.unit = (double)(1ull << a.shift);
-  r.far = (double)a.shift + 1.0;
-  // bins over what weighs something, and no further than the row goes
-  const double span = fmin(r.z(e.least), r.far);
-  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
-  Settings s;
-  const float u = a.uniform[row];
-  s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
-  s.k = a.top_k ? a.top_k[row] : 0;
-  s.p = a.top_p ? a.top_p[row] : 1.f;
-  s.m = a.min_p ? a.min_p[row] : 0.f;
-  if (s.k >= a.V) s.k = 0;
-
   static_assert(kBins == kThreads, "a bin a thread");
   sh.mass[tid] = 0, sh.count[tid] = 0;
-  if (tid < 64) {  // 2^(-tid / 64), bit by bit
-    double t = 1.0;
-    if (tid & 1) t *= 0x1.fa7c1819e90d8p-1;
-    if (tid & 2) t *= 0x1.f50765b6e4540p-1;
-    if (tid & 4) t *= 0x1.ea4afa2a490dap-1;
-    if (tid & 8) t *= 0x1.d5818dcfba487p-1;
-    if (tid & 16) t *= 0x1.ae89f995ad3adp-1;
-    if (tid & 32) t *= 0x1.6a09e667f3bcdp-1;
-    sh.exp2_table[tid] = t;
-  }
+  fill_table(sh);
   __syncthreads();
   const int64_t lo = part * a.chunk;
   each_word(r.words, r.bf16, lo, min(lo + a.chunk, a.V), [&](float v, uint32_t) {
@@ -580,32 +642,68 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   });
   __syncthreads();
   if (a.S > 1) {
-    // the row's last workgroup joins the bins of all: written through and read past the dies'
-    // caches around the arrival counter, which goes back to zero
-    constexpr int words = 12 * 1024 / 8;  // masses, then counts two to a word, none above 2^24
-    static_assert(sizeof sh.mass + sizeof sh.count == 8 * words, "mass and count in one piece");
-    u64 *const here = sh.mass, *const all = (u64 *)a.bins + row * a.S * (int64_t)words;
-    const int used = s.k > 0 ? words : kBins;
+    // the row's last workgroup joins the bins of all
+    u64 *const here = sh.mass;
+    const int used = s.k > 0 ? kBinWords : kBins;
     for (int i = tid; i < used; i += kThreads)
-      __hip_atomic_store(all + part * words + i, here[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0)
-      sh.flag = __hip_atomic_fetch_add(a.arrivals + row, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
-    __syncthreads();
-    if (!sh.flag) return;
+      __hip_atomic_store(bins_at(a, row, part) + i, here[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!last_of_row(a, sh, row)) return;
     for (int i = tid; i < used; i += kThreads) {
       u64 x[8], sum = 0;
 #pragma unroll
       for (int p = 0; p < 8; ++p)
-        x[p] = p < a.S ? __hip_atomic_load(all + p * words + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        x[p] = p < a.S ? __hip_atomic_load(bins_at(a, row, p) + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
 #pragma unroll
       for (int p = 0; p < 8; ++p) sum += x[p];
       here[i] = sum;
     }
-    if (tid == 0) __hip_atomic_store(a.arrivals + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
   }
-  const int32_t token = draw(sh, r, s);
+  const Borders b = borders_of(sh, r, s);
+  if (a.S > 1) {
+    for (int i = tid; i < kBinWords; i += kThreads) bins_at(a, row, 0)[i] = sh.mass[i];
+    if (tid == 0) *borders_at(a, row) = b;
+    return;
+  }
+  words_of(sh, r, b, 0, a.V);
+  const int32_t token = draw(sh, r, s, b);
+  if (tid == 0) a.out[row] = token;
+}
+
+// The words of a shared row that are looked at, and its token
+extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_words(SampleArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  SampleShared &sh = *(SampleShared *)lds;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S;
+  const SampleExtremes e = row_extremes(a, row);
+  const Borders b = *borders_at(a, row);
+  Row r;
+  Settings s;
+  if (!set_row(a, row, e, r, s)) return;
+  fill_table(sh);
+  const int64_t lo = part * a.chunk;
+  words_of(sh, r, b, lo, min(lo + a.chunk, a.V));
+  u64 *const list = list_at(a, row);
+  const int n = sh.n;
+  if (tid == 0) sh.flag = __hip_atomic_fetch_add(a.listed + row, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int at = sh.flag;
+  for (int i = tid; i < n && at + i < kPairwise; i += kThreads)
+    __hip_atomic_store(list + at + i, sh.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of_row(a, sh, row)) return;
+  if (tid == 0) {
+    sh.n = __hip_atomic_load(a.listed + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(a.listed + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (sh.n <= kPairwise) {
+    if (tid < sh.n) sh.list[tid] = __hip_atomic_load(list + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  } else {  // more than the list takes: all of them by this one
+    words_of(sh, r, b, 0, a.V);
+  }
+  for (int i = tid; i < kBinWords; i += kThreads) sh.mass[i] = bins_at(a, row, 0)[i];
+  __syncthreads();
+  const int32_t token = draw(sh, r, s, b);
   if (tid == 0) a.out[row] = token;
 }

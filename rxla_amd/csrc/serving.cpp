@@ -54,7 +54,7 @@ struct SampleArgs {
   int S;
   int64_t chunk;
   char *extremes;
-  int *arrivals;
+  int *arrivals, *listed;
   char *bins;
 };
 constexpr int64_t kSampleExtremes = 16, kSampleBins = 12 << 10;  // bytes of a workgroup's records
@@ -310,7 +310,7 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
   SampleArgs a{logits->ptr, (const float *)uniform->ptr, temperature ? (const float *)temperature->ptr : nullptr,
                top_k ? (const int32_t *)top_k->ptr : nullptr, top_p ? (const float *)top_p->ptr : nullptr,
                min_p ? (const float *)min_p->ptr : nullptr, (int32_t *)out->ptr, V, 62 - bits > 51 ? 51 : 62 - bits,
-               logits->dtype == RXW8_BF16, 1, V, nullptr, nullptr, nullptr};
+               logits->dtype == RXW8_BF16, 1, V, nullptr, nullptr, nullptr, nullptr};
   // Workgroups to a row: as many as leave one to a CU, but no more than 8, whose bins the
   // last one reads, and none with fewer than 4096 words
   a.S = (int)std::max<int64_t>(1, std::min<int64_t>({8, rt->cus / B, (V + 4095) / 4096}));
@@ -318,6 +318,7 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
   if (a.S > 1) {
     char *block = rt->f32_attn[stream_capturing(rt) ? 1 : 0];
     a.arrivals = (int *)block;
+    a.listed = a.arrivals + B;
     a.extremes = block + RXW8_NOALLOC_COUNTER_BYTES;
     a.bins = a.extremes + (64 << 10);
     if (a.S * B * kSampleExtremes > (64 << 10) || a.S * B * kSampleBins > (int64_t)RXW8_NOALLOC_PARTIAL_BYTES - (64 << 10))
@@ -327,7 +328,9 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
     int rc = launch(rt, "rxw8_sample_extremes", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
     if (rc) return rc;
   }
-  return launch(rt, "rxw8_sample_draw", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
+  int rc = launch(rt, "rxw8_sample_draw", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
+  if (rc || a.S == 1) return rc;
+  return launch(rt, "rxw8_sample_words", dim3((unsigned)(B * a.S)), dim3(1024), a, kSampleLds);
 }
 
 int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform, rxw8_buffer *temperature,
