@@ -18,12 +18,16 @@
 // Nothing is sorted. With z = (max - l) log2(e) / T the words go into bins of z, so
 // the bins are in the words' order; the running counts and masses of the bins tell the
 // bins that the borders of top_k, top_p and min_p and the token can lie in; and only the
-// words of those bins, one row's some dozens to hundreds, are looked at one by one.
+// words of those bins, one row's some dozens to hundreds, are looked at one by one. Words
+// that top_k cannot reach are passed over from the start (SampleExtremes::floor).
 // Three launches where workgroups share a row (the maxima; the bins, which the last
 // workgroup of a row to arrive joins; the words, from which the last one draws), one where
-// each has its own. What bounds a batch is reading the logits: once from memory, then twice more from the
-// caches, the second time with an exponential in f64 and two LDS atomics for each
-// word; a single row is bound by the length of the chain.
+// each has its own. What bounds a batch is reading the logits: once from memory, then twice
+// more from the caches, the second time with an exponential in f64 and an LDS atomic or two
+// for each word that counts. 64 rows of 248320 f32 words: 68 us, 0.94 TB/s of logits read
+// once, 2.8 as read (22 us the maxima, 21 the bins, 14 the words, 11 the joins and launches).
+// A single row is bound by the length of the chain: 33.6 us for 151936 words, a third of
+// it the words.
 #include <stddef.h>
 
 #include "common.h"
@@ -67,8 +71,9 @@ __device__ __forceinline__ float sample_value(uint32_t key) {
 // A word, the larger the earlier in the order
 __device__ __forceinline__ u64 sample_word(uint32_t key, uint32_t index) { return (u64)key << 32 | (0xffffffffu - index); }
 
-// f(value, index) for the words lo <= index < hi of a row, by the workgroup's threads: 16
-// bytes a load where the row's alignment has them, four loads at a time
+// f(value, index) for the words lo <= index < hi of a row, by the workgroup's threads, 16
+// bytes a load but for the ends. (One load at a time: 16 waves to a CU are 16 KiB under way; two or
+// four at a time took 3 to 8% longer for 64 rows of 248320, all loads of a step then being waited for.)
 template <typename F>
 __device__ void each_word(const void *row, bool bf16, int64_t lo, int64_t hi, F f) {
   const int tid = threadIdx.x, es = bf16 ? 2 : 4, W = 16 / es;
@@ -79,28 +84,17 @@ __device__ void each_word(const void *row, bool bf16, int64_t lo, int64_t hi, F 
   const int64_t head = min(hi, lo + (int64_t)((16 - ((uintptr_t)(p + lo * es) & 15)) & 15) / es);
   const int64_t body = head + (hi - head) / W * W;
   if (lo + tid < head) one(lo + tid);
-  constexpr int N = 4;
-  for (int64_t i0 = head; i0 < body; i0 += (int64_t)N * W * kThreads) {
-    u32x4 x[N];
+  for (int64_t i = head + (int64_t)W * tid; i < body; i += (int64_t)W * kThreads) {
+    const u32x4 x = *(const u32x4 *)(p + i * es);
+    if (bf16) {
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int64_t i = i0 + (int64_t)W * (n * kThreads + tid);
-      if (i < body) x[n] = *(const u32x4 *)(p + i * es);
-    }
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int64_t i = i0 + (int64_t)W * (n * kThreads + tid);
-      if (i >= body) break;
-      if (bf16) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          f(__uint_as_float(x[n][e] << 16), (uint32_t)i + 2 * e);
-          f(__uint_as_float(x[n][e] & 0xffff0000u), (uint32_t)i + 2 * e + 1);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(__uint_as_float(x[n][e]), (uint32_t)i + e);
+      for (int e = 0; e < 4; ++e) {
+        f(__uint_as_float(x[e] << 16), (uint32_t)i + 2 * e);
+        f(__uint_as_float(x[e] & 0xffff0000u), (uint32_t)i + 2 * e + 1);
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(__uint_as_float(x[e]), (uint32_t)i + e);
     }
   }
   if (body + tid < hi) one(body + tid);
@@ -110,12 +104,13 @@ __device__ __forceinline__ u64 max_u64(u64 a, u64 b) { return a > b ? a : b; }
 
 }  // namespace
 
-// The first maximum of some words (a NaN above every number), and their least value
-// that is not -inf
+// The first maximum of some words (a NaN above every number), their least value that is
+// not -inf, and a key that at least top_k words of the row reach once all its parts' are
+// joined by their minimum (0: no such key)
 struct SampleExtremes {
   u64 top;
   float least;
-  int pad;
+  uint32_t floor;
 };
 
 namespace {
@@ -150,6 +145,7 @@ struct Row {
   double per_bin;    // bins per unit of z
   double unit;       // 2^s
   double far;        // z from which on words weigh nothing
+  float floor;       // words below it are not asked for: they come after top_k, or min_p, alone
 
   __device__ double z(float v) const { return ((double)top - (double)v) * inv; }
   // (the nearest whole number, in the low bits of a sum with 1.5 2^52)
@@ -176,7 +172,8 @@ __device__ __forceinline__ void fill_table(SampleShared &sh) {
 // The mass of z, 0 <= z < 54: round(2^(s - z)). z = n / 64 + r with |r| <= 1 / 128 (the addition
 // rounds to 64ths and leaves n in its low bits), 2^(-n / 64) from a table of 64 and the
 // exponent, 2^-r from the series of exp(-r ln 2) to the fifth power, the next term of which is
-// below 2^-54; and the sum with 2^52 holds the whole number in its low bits.
+// below 2^-54; and the sum with 2^52 holds the whole number in its low bits. (Another z: no
+// matter what, but nothing is read out of range.)
 __device__ __forceinline__ double exp2_minus(const SampleShared &sh, double z) {
   const double t = z + 0x1.8p46;
   const int n = (int)(uint32_t)__builtin_bit_cast(u64, t);
@@ -203,6 +200,7 @@ __device__ SampleExtremes join_extremes(SampleShared &sh, SampleExtremes e) {
   for (int o = 32; o > 0; o >>= 1) {
     e.top = max_u64(e.top, __shfl_xor(e.top, o));
     e.least = fminf(e.least, __shfl_xor(e.least, o));
+    e.floor = min(e.floor, __shfl_xor(e.floor, o));
   }
   __syncthreads();
   if (lane == 0) sh.wave_ext[wave] = e;
@@ -210,19 +208,29 @@ __device__ SampleExtremes join_extremes(SampleShared &sh, SampleExtremes e) {
   for (int w = 0; w < kThreads / 64; ++w) {
     e.top = max_u64(e.top, sh.wave_ext[w].top);
     e.least = fminf(e.least, sh.wave_ext[w].least);
+    e.floor = min(e.floor, sh.wave_ext[w].floor);
   }
   return e;
 }
-__device__ SampleExtremes extremes_of(const void *row, bool bf16, int64_t lo, int64_t hi) {
+// ... of the words lo <= index < hi of a row. The floor: among `groups` groups of threads each
+// one's maximum, and the least of these, which `groups` words reach. (Of 150000 words it leaves
+// about 130 for 20 groups and 1600 for 200, so that the bins' f64 and atomics are few.)
+__device__ SampleExtremes extremes_of(SampleShared &sh, const SampleArgs &a, int64_t row, const void *words, int64_t lo, int64_t hi) {
   uint32_t key = 0, index = 0xffffffffu;
   float least = __builtin_huge_valf();
-  each_word(row, bf16, lo, hi, [&](float v, uint32_t i) {  // (a thread's words come in order but for its first and last)
+  each_word(words, a.bf16, lo, hi, [&](float v, uint32_t i) {  // (a thread's words come in order)
     const uint32_t k = sample_key(v);
-    const bool better = k > key || (k == key && i < index);
+    const bool better = k > key;
     key = better ? k : key, index = better ? i : index;
     least = fminf(least, v > -__builtin_huge_valf() ? v : __builtin_huge_valf());
   });
-  return SampleExtremes{sample_word(key, index), least, 0};
+  const int64_t k = a.top_k ? a.top_k[row] : 0, groups = (k + a.S - 1) / a.S;
+  uint32_t floor = 0;
+  if (k > 0 && k < a.V && groups <= kThreads) {
+    floor = key;
+    for (int o = 1; o < 64 && kThreads / (2 * o) >= groups; o <<= 1) floor = max(floor, __shfl_xor(floor, o));
+  }
+  return join_extremes(sh, SampleExtremes{sample_word(key, index), least, floor});
 }
 
 // Radix descent, 8 bits a pass, over the i < n that get(i, key, units) admits: the key at which
@@ -404,7 +412,7 @@ __device__ Borders borders_of(SampleShared &sh, const Row &r, const Settings &s)
   auto key_at = [&](int b) { return sample_key((float)((double)r.top - (double)b / (r.per_bin * r.inv))); };
   const float v_lo = sample_value(max(key_at(b_hi + 1) - 2, sample_key(-__builtin_huge_valf())));
   const float v_hi = b_lo <= 1 ? r.top : sample_value(min(key_at(b_lo - 1) + 2, sample_key(r.top)));
-  return Borders{total, b_hi + 1 < kBins ? v_lo : -__builtin_huge_valf(), v_hi, kb, mb, pb0, pb1, db0, db1};
+  return Borders{total, b_hi + 1 < kBins ? fmaxf(v_lo, r.floor) : r.floor, v_hi, kb, mb, pb0, pb1, db0, db1};
 }
 
 // The words lo <= index < hi in these bins, the first kList of them in sh.list; sh.n of them
@@ -558,6 +566,7 @@ __device__ SampleExtremes row_extremes(const SampleArgs &a, int64_t row) {
   for (int o = 32; o > 0; o >>= 1) {
     e.top = max_u64(e.top, __shfl_xor(e.top, o));
     e.least = fminf(e.least, __shfl_xor(e.least, o));
+    e.floor = min(e.floor, __shfl_xor(e.floor, o));
   }
   return e;
 }
@@ -573,15 +582,21 @@ __device__ bool set_row(const SampleArgs &a, int64_t row, const SampleExtremes &
   r.inv = 1.44269504088896340736 / (double)T;
   r.unit = (double)(1ull << a.shift);
   r.far = (double)a.shift + 1.0;
-  // bins over what weighs something, and no further than the row goes
-  const double span = fmin(r.z(e.least), r.far);
-  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
   const float u = a.uniform[row];
   s.u = u > 0.f ? fminf(u, 0x1.fffffep-1f) : 0.f;
   s.k = a.top_k ? a.top_k[row] : 0;
   s.p = a.top_p ? a.top_p[row] : 1.f;
   s.m = a.min_p ? a.min_p[row] : 0.f;
   if (s.k >= a.V) s.k = 0;
+  const float lowest = -__builtin_huge_valf();
+  r.floor = e.floor > sample_key(lowest) ? sample_value(e.floor) : lowest;
+  if (s.m > 0.f && !(s.p < 1.f)) {  // (min_p leaves nothing below two steps under this)
+    const double z = fmin(fmax(-log2((double)s.m), 0.0) + 0x1p-20, r.far);
+    r.floor = fmaxf(r.floor, sample_value(max(sample_key((float)((double)r.top - z / r.inv)) - 2, sample_key(lowest))));
+  }
+  // bins over what weighs something, and no further than the row goes
+  const double span = fmin(r.z(fmaxf(e.least, r.floor)), r.far);
+  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
   return true;
 }
 // Whether this workgroup is the row's last to arrive; what all have stored past the dies' caches
@@ -605,8 +620,7 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_extremes(Samp
   extern __shared__ __attribute__((aligned(16))) char lds[];
   SampleShared &sh = *(SampleShared *)lds;
   const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S, lo = part * a.chunk;
-  const void *const words = (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4);
-  const SampleExtremes e = join_extremes(sh, extremes_of(words, a.bf16, lo, min(lo + a.chunk, a.V)));
+  const SampleExtremes e = extremes_of(sh, a, row, words_at(a, row), lo, min(lo + a.chunk, a.V));
   if (threadIdx.x == 0) a.extremes[blockIdx.x] = e;
 }
 
@@ -618,7 +632,7 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   Row r;
   SampleExtremes e;
   if (a.S == 1) {
-    e = join_extremes(sh, extremes_of(words_at(a, row), a.bf16, 0, a.V));
+    e = extremes_of(sh, a, row, words_at(a, row), 0, a.V);
   } else {
     e = row_extremes(a, row);
   }
@@ -632,11 +646,14 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   fill_table(sh);
   __syncthreads();
   const int64_t lo = part * a.chunk;
+  // (the arithmetic for every word, wanted or not: branches around it, which keep the words'
+  // chains from running side by side, took 40 us longer for 64 rows of 248320)
   each_word(r.words, r.bf16, lo, min(lo + a.chunk, a.V), [&](float v, uint32_t) {
     const double z = r.z(v);
-    if (z < r.far) {
-      const int b = r.bin(z);
-      atomicAdd(&sh.mass[b], units_of(r, exp2_minus(sh, z)));
+    const int b = r.bin(z);
+    const u64 units = units_of(r, exp2_minus(sh, z));
+    if (v >= r.floor && z < r.far) {
+      atomicAdd(&sh.mass[b], units);
       if (s.k > 0) atomicAdd(&sh.count[b], 1u);
     }
   });
