@@ -18,26 +18,37 @@ struct PagedAppendArgs {
   int k_f32, p_f32;
 };
 
-// Row i of sequence b goes to position starts[b] + i. One wave per (row, kv head);
-// rows outside every sequence and positions without a page are passed over. An f32
-// row is rounded once (RNE) on its way into bf16 pages, a bf16 row widened exactly.
-extern "C" __global__ void __launch_bounds__(256) rxw8_paged_append(PagedAppendArgs a) {
+// Row t of k and v: the page and the place in it (below 0: none) of the position
+// starts[b] + i, for row i of sequence b; rows outside every sequence and positions
+// without a page have none. By a whole wave, t uniform.
+struct PagedPlace {
+  int64_t page;
+  int at;
+};
+__device__ __forceinline__ PagedPlace paged_place(const PagedAppendArgs &a, int64_t t) {
+  int64_t b = t, i = 0;
+  if (a.offsets) {
+    b = any_sequence(a.offsets, a.B, t);
+    if (b < 0 || t >= a.offsets[b + 1]) return PagedPlace{-1, 0};
+    i = t - a.offsets[b];
+  }
+  const int64_t pos = a.starts[b] + i;
+  if (pos < 0 || pos >= (int64_t)a.M * a.ps) return PagedPlace{-1, 0};
+  const int slot = (int)(pos / a.ps);
+  const int64_t page = a.table[b * a.M + slot];
+  return PagedPlace{page < a.P ? page : -1, (int)(pos - (int64_t)slot * a.ps)};
+}
+
+// Any width and alignment: a wave for each (row, kv head), an element a lane.
+extern "C" __global__ void __launch_bounds__(256) rxw8_paged_append_any(PagedAppendArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (unit >= a.T * a.Hkv) return;
   const int64_t t = unit / a.Hkv;
   const int h = (int)(unit - t * a.Hkv);
-  int64_t b = t, i = 0;
-  if (a.offsets) {
-    b = any_sequence(a.offsets, a.B, t);
-    if (b < 0 || t >= a.offsets[b + 1]) return;
-    i = t - a.offsets[b];
-  }
-  const int64_t pos = a.starts[b] + i;
-  if (pos < 0 || pos >= (int64_t)a.M * a.ps) return;
-  const int64_t page = a.table[b * a.M + pos / a.ps];
-  if (page < 0 || page >= a.P) return;
-  const int64_t src = unit * a.D, dst = ((page * a.Hkv + h) * a.ps + pos % a.ps) * a.D;
+  const PagedPlace to = paged_place(a, t);
+  if (to.page < 0) return;
+  const int64_t src = unit * a.D, dst = ((to.page * a.Hkv + h) * a.ps + to.at) * a.D;
   for (int e = lane; e < a.D; e += 64) {
     const float x = any_load(a.k, src + e, a.k_f32), y = any_load(a.v, src + e, a.k_f32);
     if (a.p_f32) {
@@ -48,6 +59,69 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_paged_append(PagedAppendA
       ((uint16_t *)a.vp)[dst + e] = f32_to_bf16_bits(y);
     }
   }
+}
+
+// Widths of whole 8 elements at 16-byte boundaries: a wave for each row and `kAppend` x 64
+// of its pieces of 8 elements, all heads' in a row, with K's and V's pieces under way before
+// the wave looks for its sequence and page. An f32 row is rounded once (RNE) on its way into
+// bf16 pages, a bf16 row widened exactly. Bound by memory for prompts, by the chain of
+// dependent loads (offsets, start, table) for a step's single rows.
+constexpr int kAppend = 2;
+
+template <typename S, typename P>
+__device__ __forceinline__ void paged_append(const PagedAppendArgs &a) {
+  constexpr int NS = sizeof(S) / 2, NP = sizeof(P) / 2;  // 16-byte words of 8 elements
+  const int lane = threadIdx.x & 63, per_head = a.D / 8, pieces = a.Hkv * per_head;
+  const int parts = (pieces + 64 * kAppend - 1) / (64 * kAppend);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = unit / parts;
+  const int p0 = (int)(unit - t * parts) * 64 * kAppend + lane;
+  if (t >= a.T) return;
+  u32x4 k[kAppend][NS], v[kAppend][NS];
+#pragma unroll
+  for (int n = 0; n < kAppend; ++n)
+    if (p0 + 64 * n < pieces) {
+      const int64_t at = (t * pieces + p0 + 64 * n) * NS;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) k[n][i] = ((const u32x4 *)a.k)[at + i], v[n][i] = ((const u32x4 *)a.v)[at + i];
+    }
+  const PagedPlace to = paged_place(a, t);
+  if (to.page < 0) return;
+  auto put = [&](void *pages, int64_t at, const u32x4 *x) {
+    u32x4 y[NP];
+    if constexpr (NS == NP) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) y[i] = x[i];
+    } else if constexpr (NS == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[0][i] = pack_bf16x2(__uint_as_float(x[i / 2][2 * i % 4]), __uint_as_float(x[i / 2][2 * i % 4 + 1]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i / 2][2 * i % 4] = x[0][i] << 16, y[i / 2][2 * i % 4 + 1] = x[0][i] & 0xffff0000u;
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) ((u32x4 *)pages)[at + i] = y[i];
+  };
+#pragma unroll
+  for (int n = 0; n < kAppend; ++n) {
+    const int p = p0 + 64 * n;
+    if (p < pieces) {
+      const int h = p / per_head;
+      const int64_t at = (((to.page * a.Hkv + h) * a.ps + to.at) * per_head + (p - h * per_head)) * NP;
+      put(a.kp, at, k[n]);
+      put(a.vp, at, v[n]);
+    }
+  }
+}
+extern "C" __global__ void __launch_bounds__(256) rxw8_paged_append(PagedAppendArgs a) {
+  if (a.k_f32 && a.p_f32)
+    paged_append<float, float>(a);
+  else if (a.k_f32)
+    paged_append<float, uint16_t>(a);
+  else if (a.p_f32)
+    paged_append<uint16_t, float>(a);
+  else
+    paged_append<uint16_t, uint16_t>(a);
 }
 
 struct PagedDecodeArgs {

@@ -215,7 +215,11 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
                     (const int32_t *)starts->ptr, offsets ? (const int32_t *)offsets->ptr : nullptr, T,
                     k_pages->dims[0], (int)B, (int)table->dims[1], (int)k->dims[1], (int)k->dims[2],
                     (int)k_pages->dims[2], k->dtype == RXW8_F32, k_pages->dtype == RXW8_F32};
-  return launch(rt, "rxw8_paged_append", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  if (a.D % 8 || ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
+    return launch(rt, "rxw8_paged_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  // a wave takes 128 pieces of 8 elements of a row
+  const int64_t parts = (a.Hkv * a.D / 8 + 127) / 128;
+  return launch(rt, "rxw8_paged_append", dim3((unsigned)((T * parts + 3) / 4)), dim3(256), a);
 }
 
 int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
