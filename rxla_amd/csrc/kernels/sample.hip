@@ -44,8 +44,8 @@ struct SampleArgs {
   int bf16;
   // S workgroups share a row, `chunk` words each (1 and V: one has it alone): extremes
   // [B][S], arrivals [B] and listed words [B] (zero between launches), and bins [B][S] of
-  // 12 KiB; the row's joined bins take the place of the first's, its words and Borders
-  // that of the second's
+  // 12 KiB; the row's joined bins take the place of the first's, its Borders and words that
+  // of the others'
   int S;
   int64_t chunk;
   struct SampleExtremes *extremes;
@@ -253,16 +253,33 @@ __device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64
       atomicAdd(&sh.mass[(k >> shift) & 255], u);
     }
     __syncthreads();
-    if (tid == 0) {
-      int b = 255;
-      for (; b > 0; --b) {
-        const u64 m = f.mass + sh.mass[b], c = f.count + sh.count[b];
-        if (sh.count[b] && (count ? c >= count : over ? (double)m > want : (double)m >= want)) break;
-        f.mass = m, f.count = c;
+    if (tid < 64) {  // the bins from the last down, four to a lane
+      uint32_t cnt[4];
+      u64 m[4], own_m = 0, own_c = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        cnt[j] = sh.count[255 - 4 * tid - j], m[j] = sh.mass[255 - 4 * tid - j];
+        own_m += m[j], own_c += cnt[j];
       }
-      f.key = (f.key << 8) | (uint32_t)b;
-      f.ties = sh.count[b];
-      sh.found = f;
+      u64 all_m = own_m, all_c = own_c;
+      for (int o = 1; o < 64; o <<= 1) {
+        const u64 x = __shfl_up(all_m, o), y = __shfl_up(all_c, o);
+        if (tid >= o) all_m += x, all_c += y;
+      }
+      Found g{f.mass + all_m - own_m, f.count + all_c - own_c, 0, 0};
+      bool hit = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!hit) {
+          const int b = 255 - 4 * tid - j;
+          const u64 mass = g.mass + m[j], n = g.count + cnt[j];
+          hit = b == 0 || (cnt[j] && (count ? n >= count : over ? (double)mass > want : (double)mass >= want));
+          if (hit)
+            g.key = (f.key << 8) | (uint32_t)b, g.ties = cnt[j];
+          else
+            g.mass = mass, g.count = n;
+        }
+      if (tid == __builtin_ctzll(__ballot(hit))) sh.found = g;  // (the last lane's is one at least)
     }
     __syncthreads();
     f = sh.found;
@@ -553,13 +570,14 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
 
 constexpr int kBinWords = 12 * 1024 / 8;  // masses, then counts two to a word, none above 2^24
 static_assert(sizeof SampleShared::mass + sizeof SampleShared::count == 8 * kBinWords &&
-                  offsetof(SampleShared, count) == sizeof SampleShared::mass && 8 * kPairwise + sizeof(Borders) <= 8 * kBinWords,
-              "mass and count in one piece; words and borders in the second's place");
+                  offsetof(SampleShared, count) == sizeof SampleShared::mass && sizeof(Borders) <= 64,
+              "mass and count in one piece");
 
 __device__ const void *words_at(const SampleArgs &a, int64_t row) { return (const char *)a.logits + row * a.V * (a.bf16 ? 2 : 4); }
 __device__ u64 *bins_at(const SampleArgs &a, int64_t row, int part) { return (u64 *)a.bins + (row * a.S + part) * kBinWords; }
-__device__ u64 *list_at(const SampleArgs &a, int64_t row) { return bins_at(a, row, 1); }
-__device__ Borders *borders_at(const SampleArgs &a, int64_t row) { return (Borders *)(bins_at(a, row, 1) + kPairwise); }
+__device__ Borders *borders_at(const SampleArgs &a, int64_t row) { return (Borders *)bins_at(a, row, 1); }
+__device__ u64 *list_at(const SampleArgs &a, int64_t row) { return bins_at(a, row, 1) + 8; }
+__device__ int list_size(const SampleArgs &a) { return min((a.S - 1) * kBinWords - 8, kList); }
 
 __device__ SampleExtremes row_extremes(const SampleArgs &a, int64_t row) {
   SampleExtremes e = a.extremes[row * a.S + min((int)(threadIdx.x & 63), a.S - 1)];
@@ -706,7 +724,8 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_words(SampleA
   if (tid == 0) sh.flag = __hip_atomic_fetch_add(a.listed + row, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   const int at = sh.flag;
-  for (int i = tid; i < n && at + i < kPairwise; i += kThreads)
+  const int most = list_size(a);
+  for (int i = tid; i < n && at + i < most; i += kThreads)
     __hip_atomic_store(list + at + i, sh.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (!last_of_row(a, sh, row)) return;
   if (tid == 0) {
@@ -714,8 +733,9 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_words(SampleA
     __hip_atomic_store(a.listed + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (sh.n <= kPairwise) {
-    if (tid < sh.n) sh.list[tid] = __hip_atomic_load(list + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (sh.n <= most) {
+    for (int i = tid; i < sh.n; i += kThreads)
+      sh.list[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   } else {  // more than the list takes: all of them by this one
     words_of(sh, r, b, 0, a.V);
   }

@@ -444,6 +444,27 @@ def test_sample_ties_and_special_values(rt, v):
         check_sample(rt, z, us, p=[0.5] * n, m=[0.5] * n, t=[0.7] * n)
 
 
+@pytest.mark.parametrize("v,b", [(1 << 20, 3), (1 << 20, 130), (200000, 100), (40000, 3)])
+def test_sample_crowded_borders(rt, v, b):
+    """Borders and tokens among words of nearly the same weight, thousands of them at a time, and
+    far down the row; rows that one, two and more workgroups share."""
+    rng = np.random.default_rng(v + b)
+    crowd = (0.01 * rng.standard_normal(v)).astype(np.float32)
+    crowd[v // 5] = 12
+    even = rng.standard_normal(v).astype(np.float32)
+    kinds = [crowd, even, ref.bf16_value(ref.bf16_bits(even)), (3 * even).astype(np.float32)]
+    z = np.stack([kinds[i % 4] for i in range(min(b, 12))])
+    sets = [dict(k=[0]), dict(k=[0], p=[.99]), dict(k=[1000]), dict(k=[9000]), dict(k=[v - 1]), dict(k=[200], p=[.95]),
+            dict(m=[.2]), dict(m=[.02], p=[.999]), dict(k=[5000], p=[.9], m=[.05])]
+    u = rng.random(b).astype(np.float32)
+    for f in sets:
+        n = min(b, 12)
+        want = [ref.sample(z[i], u[i], *(pick(f.get(x), 0) for x in "tkpm")) for i in range(n)]
+        rows = np.arange(b) % n
+        got = sample(rt, z[rows], u[rows], **{x: np.repeat(np.asarray(y), b) for x, y in f.items()})
+        assert got.tolist() == [want[i] for i in rows], f
+
+
 @pytest.mark.parametrize("b", [1, 3, 64, 300])
 def test_sample_batches(rt, b):
     """Rows of a batch are independent; the same inputs give the same tokens, into a buffer too."""
