@@ -278,6 +278,12 @@ int rxw8_gqa_prefill_into(rxw8_runtime *rt, rxw8_buffer *q,
                           rxw8_buffer *k_cache, rxw8_buffer *v_cache,
                           rxw8_buffer *starts, float scale, rxw8_buffer *out);
 
+/* The serving calls (paged cache, packed prompts, rxw8_sample) take buffers of their
+ * runtime only, and what they write must share no memory with another argument. Paged
+ * decode and rxw8_sample work in the f32 attention's fixed blocks of their runtime, one
+ * for the calls that run and one for those that a capture records: a graph may replay
+ * beside the runtime's other calls, two graphs at the same time need a runtime each. */
+
 /* ---- paged key/value cache (no counterpart in the reference, whose cache is one
  * plane per sequence, kv_cache.rs:7-111) --------------------------------------
  * k_pages/v_pages [P,Hkv,ps,D] BF16|F32 (two buffers of one shape and type): a

@@ -69,8 +69,26 @@ static bool same_shape(const Buffer *a, const Buffer *b) {
   for (int i = 0; same && i < a->rank; ++i) same = a->dims[i] == b->dims[i];
   return same;
 }
-constexpr int64_t kGridMax = ((int64_t)1 << 31) - 1;
+// Workgroups of `threads` that one launch takes: 2^32 - 1 threads
+constexpr int64_t grid_max(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 constexpr int64_t kAnyMaxD = 512;  // RXW8_ATTN_ANY_MAX_D
+
+// Whether the buffers (NULL ones aside) are the runtime's, and none of the first `written`
+// shares memory with another
+static int check_buffers(const char *what, const Runtime *rt, std::initializer_list<const Buffer *> bufs, int written) {
+  for (const Buffer *b : bufs)
+    if (b && b->rt != rt) return fail(RXW8_INVALID_ARGUMENT, "%s: buffers of another runtime", what);
+  int i = 0;
+  for (const Buffer *w : bufs) {
+    if (i++ == written) break;
+    int j = 0;
+    for (const Buffer *b : bufs)
+      if (j++ != i - 1 && w && b && w->bytes && b->bytes && (char *)w->ptr < (char *)b->ptr + b->bytes &&
+          (char *)b->ptr < (char *)w->ptr + w->bytes)
+        return fail(RXW8_INVALID_ARGUMENT, "%s: what is written must not share memory with another argument", what);
+  }
+  return RXW8_OK;
+}
 
 // Pages [P, Hkv, ps, D] F32|BF16 and the table I32 [B, M]
 static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, const Buffer *table) {
@@ -103,7 +121,7 @@ static int check_paged_decode(const Buffer *q, const Buffer *kp, const Buffer *v
   if (!is_vec(lens, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: lens must be I32 [B]");
   if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
   if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: head dim %lld > 512", (long long)D);
-  if (Hq > INT32_MAX || (Hq > 0 && B > kGridMax / Hq))
+  if (Hq > INT32_MAX || B > grid_max(256) / Hq)
     return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: %lld x %lld rows exceed the kernel's grid", (long long)B,
                 (long long)Hq);
   return RXW8_OK;
@@ -122,7 +140,7 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
     return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill: offsets must be I32 [sequences + 1]");
   if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
   if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: head dim %lld > 512", (long long)D);
-  if (T > INT32_MAX || Hq > INT32_MAX || T > kGridMax / Hq || offsets->dims[0] > INT32_MAX)
+  if (T > INT32_MAX || Hq > INT32_MAX || T > 4 * grid_max(256) / Hq || offsets->dims[0] > INT32_MAX)
     return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: %lld x %lld rows exceed the kernel's grid", (long long)T,
                 (long long)Hq);
   return RXW8_OK;
@@ -175,7 +193,7 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
   const bool f32 = a.q_f32 || a.out_f32;
   const int64_t rows = (f32 || D == 256 ? 32 : 64) * (4 / a.heads);
   const int64_t grid = ((T + rows - 1) / rows + B) * (Hq / a.heads);
-  if ((D != 64 && D != 128 && D != 256) || Hkv * D * 2 * 32 >= ((int64_t)1 << 31) || grid > kGridMax ||
+  if ((D != 64 && D != 128 && D != 256) || Hkv * D * 2 * 32 >= ((int64_t)1 << 31) || grid > grid_max(256) ||
       ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16)
     return launch(rt, "rxw8_packed_prefill_any", dim3((unsigned)((T * Hq + 3) / 4)), dim3(256), a);
   if (fill) {
@@ -198,8 +216,7 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
   if (!rt || !k_pages || !v_pages || !k || !v || !table || !starts)
     return fail(RXW8_INVALID_ARGUMENT, "paged KV append: NULL argument");
   if (int rc = check_pages("paged KV append", k_pages, v_pages, table)) return rc;
-  if (k_pages == v_pages || (k_pages->ptr == v_pages->ptr && k_pages->bytes))
-    return fail(RXW8_INVALID_ARGUMENT, "K and V pages must be distinct buffers");
+  if (k_pages == v_pages) return fail(RXW8_INVALID_ARGUMENT, "K and V pages must be distinct buffers");
   if (k->rank != 3 || !is_f(k->dtype) || !same_shape(k, v) || k->dims[1] != k_pages->dims[1] ||
       k->dims[2] != k_pages->dims[3])
     return fail(RXW8_INVALID_ARGUMENT, "paged KV append requires F32/BF16 k, v [T,Hkv,D] of the pages' heads and width");
@@ -207,8 +224,11 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
   if (!is_vec(starts, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged KV append: starts must be I32 [B]");
   if (offsets ? !is_vec(offsets, RXW8_I32, B + 1) : T != B)
     return fail(RXW8_INVALID_ARGUMENT, "paged KV append: offsets must be I32 [B+1] (without them k, v hold one row a sequence)");
-  if (T > kGridMax / k->dims[1])
+  // a wave takes 128 pieces of 8 elements of a row, or a row of one head
+  const int64_t parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
+  if (T > 4 * grid_max(256) / std::max(k->dims[1], parts))
     return fail(RXW8_UNIMPLEMENTED, "paged KV append: %lld rows exceed the kernel's grid", (long long)T);
+  if (int rc = check_buffers("paged KV append", rt, {k_pages, v_pages, k, v, table, starts, offsets}, 2)) return rc;
   if (T == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   PagedAppendArgs a{k->ptr, v->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr,
@@ -217,8 +237,6 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
                     (int)k_pages->dims[2], k->dtype == RXW8_F32, k_pages->dtype == RXW8_F32};
   if (a.D % 8 || ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
     return launch(rt, "rxw8_paged_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
-  // a wave takes 128 pieces of 8 elements of a row
-  const int64_t parts = (a.Hkv * a.D / 8 + 127) / 128;
   return launch(rt, "rxw8_paged_append", dim3((unsigned)((T * parts + 3) / 4)), dim3(256), a);
 }
 
@@ -229,6 +247,7 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_
   bool ok = is_f(out->dtype) && out->rank == 3;
   for (int i = 0; ok && i < 3; ++i) ok = out->dims[i] == q->dims[i];
   if (!ok) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode output: shape or dtype mismatch");
+  if (int rc = check_buffers("paged GQA decode", rt, {out, q, k_pages, v_pages, table, lens}, 1)) return rc;
   const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
   if (B == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
@@ -244,6 +263,7 @@ int rxw8_gqa_decode_paged(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages
   if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
   if (int rc = check_paged_decode(q, k_pages, v_pages, table, lens, scale)) return rc;
   if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA: out dtype must be F32 or BF16");
+  if (int rc = check_buffers("paged GQA decode", rt, {q, k_pages, v_pages, table, lens}, 0)) return rc;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   Buffer *o = nullptr;
   int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
@@ -264,6 +284,7 @@ int rxw8_gqa_prefill_packed_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *
   bool ok = is_f(out->dtype) && out->rank == 3;
   for (int i = 0; ok && i < 3; ++i) ok = out->dims[i] == q->dims[i];
   if (!ok) return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill output: shape or dtype mismatch");
+  if (int rc = check_buffers("packed GQA prefill", rt, {out, q, k, v, offsets}, 1)) return rc;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   return packed_launch(rt, q, k, v, offsets, scale, out, false);
 }
@@ -273,6 +294,7 @@ int rxw8_gqa_prefill_packed(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k, rx
   if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
   if (int rc = check_packed(q, k, v, offsets, scale)) return rc;
   if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA prefill: out dtype must be F32 or BF16");
+  if (int rc = check_buffers("packed GQA prefill", rt, {q, k, v, offsets}, 0)) return rc;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   Buffer *o = nullptr;
   int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
@@ -297,7 +319,7 @@ static int check_sample(const Buffer *logits, const Buffer *uniform, const Buffe
       (top_p && !is_vec(top_p, RXW8_F32, B)) || (min_p && !is_vec(min_p, RXW8_F32, B)))
     return fail(RXW8_INVALID_ARGUMENT, "sample: temperature, top_p and min_p must be F32 [B], top_k I32 [B]");
   if (V > ((int64_t)1 << 24)) return fail(RXW8_UNIMPLEMENTED, "sample: %lld words > 2^24", (long long)V);
-  if (B > kGridMax) return fail(RXW8_UNIMPLEMENTED, "sample: %lld rows exceed the kernel's grid", (long long)B);
+  if (B > grid_max(1024)) return fail(RXW8_UNIMPLEMENTED, "sample: %lld rows exceed the kernel's grid", (long long)B);
   return RXW8_OK;
 }
 
@@ -307,6 +329,7 @@ int rxw8_sample_into(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform
   if (int rc = check_sample(logits, uniform, temperature, top_k, top_p, min_p)) return rc;
   const int64_t B = logits->dims[0], V = logits->dims[1];
   if (!is_vec(out, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "sample output must be I32 [B]");
+  if (int rc = check_buffers("sample", rt, {out, logits, uniform, temperature, top_k, top_p, min_p}, 1)) return rc;
   if (B == 0) return RXW8_OK;
   int bits = 0;  // ceil(log2 V)
   while (((int64_t)1 << bits) < V) ++bits;
@@ -344,6 +367,7 @@ int rxw8_sample(rxw8_runtime *rt, rxw8_buffer *logits, rxw8_buffer *uniform, rxw
                 rxw8_buffer *top_k, rxw8_buffer *top_p, rxw8_buffer *min_p, rxw8_buffer **out) {
   if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
   if (int rc = check_sample(logits, uniform, temperature, top_k, top_p, min_p)) return rc;
+  if (int rc = check_buffers("sample", rt, {logits, uniform, temperature, top_k, top_p, min_p}, 0)) return rc;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
   Buffer *o = nullptr;
   int rc = new_buffer(rt, RXW8_I32, logits->dims, 1, false, &o);
