@@ -114,23 +114,10 @@ __device__ __forceinline__ void unrolled(F f) {
 constexpr int kStep = 32;  // keys
 constexpr int kRing = 4;
 
-}  // namespace
-
-// PQ, P: bf16 parts of q and of the weights (1 or 3)
-template <int D, int QT, int PQ, int P>
-__device__ void packed_prefill(const PackedArgs &a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [kRing][32][D] K, the same V
-  constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
-  constexpr int NK = D / 16, ND = D / 32, WR = 32 * QT;                            // WR: rows of a wave
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, hf = lane >> 5;
-  const int G = a.Hq / a.Hkv, HW = a.heads, RG = 4 / HW, ROWS = WR * RG, HP = G / HW, per = a.Hkv * HP;
-  const int kvh = blockIdx.x % a.Hkv, hp = blockIdx.x / a.Hkv % HP;
-  int rank = blockIdx.x / per;
-
-  // ---- the row tile: those that see the most keys first
-  int64_t first = 0;
-  int len = 0, tile = -1;
+// The row tile of the given rank, those that see the most keys first: its index in its
+// sequence, whose first row and length these are (-1: there are not that many)
+__device__ __forceinline__ int row_tile(const PackedArgs &a, int ROWS, int rank, int64_t &first, int &len) {
+  const int lane = threadIdx.x & 63;
   auto bounds = [&](int b, int64_t &s) {
     s = min((int64_t)max(a.offsets[b], 0), a.T);
     const int64_t e = min((int64_t)max(a.offsets[b + 1], 0), a.T);
@@ -155,11 +142,47 @@ __device__ void packed_prefill(const PackedArgs &a) {
     const unsigned long long have = __ballot(tiles > lo);
     const bool me = tiles > lo && __popcll(have & ((1ull << lane) - 1)) == rank - above;
     const int src = __builtin_ctzll(__ballot(me));
-    tile = lo;
     len = __builtin_amdgcn_readlane(n, src);
     first = (uint32_t)__builtin_amdgcn_readlane((int)s, src);  // (T is below 2^31)
-    break;
+    return lo;
   }
+  return -1;
+}
+
+}  // namespace
+
+// Rows row, row + step, .. below end of a sequence again, key by key, where some did not
+// come out as numbers
+__device__ __forceinline__ void rows_again(const PackedArgs &a, int D, float *qs, int64_t first, int row, int end, int step, int hq) {
+  const int lane = threadIdx.x & 63, kvh = hq / (a.Hq / a.Hkv);
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+  for (; row < end; row += step) {
+    const int64_t at = ((first + row) * a.Hq + hq) * D;
+    for (int i = lane; i < D; i += 64) qs[i] = any_load(a.q, at + i, a.q_f32);
+    __builtin_amdgcn_wave_barrier();
+    AnyState st;
+    any_walk(st, qs, a.k, a.v, false, D, first, first + row + 1, 1, a.c,
+             [&](int64_t j) { return (j * a.Hkv + kvh) * D; });
+    any_store(st, a.out, at, D, a.out_f32);
+  }
+}
+
+// PQ, P: bf16 parts of q and of the weights (1 or 3)
+template <int D, int QT, int PQ, int P>
+__device__ void packed_prefill(const PackedArgs &a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [kRing][32][D] K, the same V
+  constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
+  constexpr int NK = D / 16, ND = D / 32, WR = 32 * QT;                            // WR: rows of a wave
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hf = lane >> 5;
+  const int G = a.Hq / a.Hkv, HW = a.heads, RG = 4 / HW, ROWS = WR * RG, HP = G / HW, per = a.Hkv * HP;
+  const int kvh = blockIdx.x % a.Hkv, hp = blockIdx.x / a.Hkv % HP;
+  const int rank = blockIdx.x / per;
+
+  int64_t first = 0;
+  int len = 0;
+  const int tile = row_tile(a, ROWS, rank, first, len);
   if (tile < 0) return;
 
   const int head = wave % HW, r0 = tile * ROWS + wave / HW * WR;  // the wave's first row
@@ -497,19 +520,8 @@ __device__ void packed_prefill(const PackedArgs &a) {
   };
   if (P == 3 && a.out_f32 ? store(yes) : store(no)) return;
 
-  // ---- rows that did not come out as numbers, one after the other
   float *const qs = (float *)((char *)lds + wave * 4 * D);
-  __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-  for (int row = r0; row < min(r0 + WR, len); ++row) {
-    const int64_t at = ((first + row) * a.Hq + hq) * D;
-    for (int i = lane; i < D; i += 64) qs[i] = any_load(a.q, at + i, a.q_f32);
-    __builtin_amdgcn_wave_barrier();
-    AnyState st;
-    any_walk(st, qs, a.k, a.v, false, D, first, first + row + 1, 1, c,
-             [&](int64_t j) { return (j * a.Hkv + kvh) * D; });
-    any_store(st, a.out, at, D, a.out_f32);
-  }
+  rows_again(a, D, qs, first, r0, min(r0 + WR, len), 1, hq);
 }
 
 #define RXW8_PACKED_PREFILL(D, QT, PQ, P, W, NAME)                                                   \
@@ -527,3 +539,233 @@ RXW8_PACKED_PREFILL(256, 1, 1, 3, 1, bf16_f32)
 RXW8_PACKED_PREFILL(64, 1, 3, 3, 2, f32)
 RXW8_PACKED_PREFILL(128, 1, 3, 3, 1, f32)
 RXW8_PACKED_PREFILL(256, 1, 3, 3, 1, f32)
+
+// ---- few rows: the waves share the keys -----------------------------------------------
+//
+// Where the tiles above would leave CUs idle, a workgroup takes 32 rows of one query head
+// and each of its 4 waves every fourth step of 32 keys: up to 8 times as many workgroups,
+// each a quarter as long (a half of that again in rows). A wave goes alone, without a
+// barrier: its K and V tiles in LDS are its own, one each, copied by LDS DMA as soon as the
+// products with the one before are done; S, its softmax with a running maximum, and O
+// follow one another. At the end the four (m, l, O) are joined in LDS, in the order of the
+// waves. (16 heads of 128 over 8, one prompt of 500 rows: 10.8 us, 21.2 on the tiles above; of
+// 1000: 16.6 and 33.6.) Rows that do not come out as numbers are done again as above. QL: the third parts of
+// an f32 q stay in LDS, where the registers do not hold them (at D = 256 O takes 128, two
+// parts of q as many).
+template <int D, int PQ, int P, bool QL = PQ == 3 && D == 256>
+__device__ void packed_quarters(const PackedArgs &a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [4][K, V of 32 rows], then [4][32] (m, l), a flag, q's third parts
+  constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 1024, NK = D / 16, ND = D / 32;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, hf = lane >> 5;
+  const int hq = blockIdx.x % a.Hq, kvh = hq / (a.Hq / a.Hkv);
+  int64_t first = 0;
+  int len = 0;
+  const int tile = row_tile(a, 32, blockIdx.x / a.Hq, first, len);
+  if (tile < 0) return;
+  const int r0 = tile * 32, steps = tile + 1;  // (the last one holds the tile's diagonal)
+
+  const uint32_t own = lds_addr(lds) + wave * 2 * TILE;
+  float2 *const ml = (float2 *)((char *)lds + 8 * TILE);
+  int &again = *(int *)(ml + 128);
+  u32x4 *const q_low = (u32x4 *)((char *)lds + 8 * TILE + 2048) + lane;  // [NK][64]
+  constexpr int QR = QL ? PQ - 1 : PQ;                                    // parts in registers
+  if (threadIdx.x == 0) again = 0;
+  auto kx = [](int row) { return row & (CH < 16 ? CH - 1 : 15); };
+  auto vx = [](int row) { return 2 * (row & (CH < 16 ? 3 : 7)); };
+  const uint32_t stride = (uint32_t)a.Hkv * ROWB;
+  const char *const kbase = (const char *)a.k + (first * a.Hkv + kvh) * ROWB;
+  const char *const vbase = (const char *)a.v + (first * a.Hkv + kvh) * ROWB;
+  auto copy = [&](const char *base, int step, bool is_v) RXW8_INLINE {
+    const char *const from = base + (int64_t)step * kStep * stride;
+    const int most = len - 1 - step * kStep;  // (rows past the sequence repeat its last)
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = 1024 / ROWB * i + lane / CH, x = is_v ? vx(row) : kx(row);
+      dma16(from, (uint32_t)min(row, most) * stride + (((lane % CH) ^ x) << 4), __builtin_amdgcn_readfirstlane(own + is_v * TILE + 1024 * i));
+    }
+  };
+  if (wave < steps) {
+    copy(kbase, wave, false);
+    copy(vbase, wave, true);
+  }
+
+  // ---- q
+  u32x4 q[NK][QR];
+  const int64_t q_at = ((first + min(r0 + col, len - 1)) * a.Hq + hq) * D + 8 * hf;
+  constexpr int NL = 8;  // fragments asked for at a time
+  unrolled<NK / (NK < NL ? NK : NL)>([&](auto g) RXW8_INLINE {
+    constexpr int n0 = g * NL, N = NK < NL ? NK : NL;
+    if constexpr (PQ == 3) {
+      f32x4 x[N][2];
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[n][i] = *(const f32x4 *)((const float *)a.q + q_at + 16 * (n0 + n) + 4 * i);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        u32x4 low;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t part[3];
+          split_bf16x2(x[n][e / 2][2 * e % 4], x[n][e / 2][2 * e % 4 + 1], part);
+#pragma unroll
+          for (int p = 0; p < QR; ++p) q[n0 + n][p][e] = part[p];
+          low[e] = part[2];
+        }
+        if constexpr (QL) q_low[64 * (n0 + n)] = low;  // (the same from each wave)
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) q[n0 + n][0] = *(const u32x4 *)((const uint16_t *)a.q + q_at + 16 * (n0 + n));
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int p = 0; p < QR; ++p) asm volatile("" : "+v"(q[n0 + n][p]));  // (here, before the loop)
+  });
+  if constexpr (QL) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  f32x16 o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m = kMinusInf, l = 0.f;
+  const uint32_t k0 = own + col * ROWB + ((hf ^ kx(col)) << 4);
+  const int tr_j = (lane & 15) >> 2, tr_q = lane & 3;
+  const uint32_t v0 = own + TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1) +
+                      (((2 * ((lane >> 4) & 1) + (tr_q >> 1)) ^ vx(4 * hf + tr_j)) << 4);
+#pragma unroll 1
+  for (int h = wave; h < steps; h += 4) {
+    const bool more = h + 4 < steps;
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");  // K is in (V, behind it, may not be)
+    f32x16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      const u32x4 f = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)(k0 ^ (n << 5));
+#pragma unroll
+      for (int p = 0; p < QR; ++p) s = mfma32(f, q[n][p], s);
+      if constexpr (QL) s = mfma32(f, q_low[64 * n], s);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) copy(kbase, h + 4, false);
+    if (h == tile) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (8 * (r >> 2) + (r & 3) + 4 * hf > col) s[r] = kMinusInf;
+    }
+    // ---- softmax
+    float mx = kMinusInf;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    mx = fmaxf(m, max_xor32(mx) * a.c);
+    const float ref = mx == kMinusInf ? 0.f : mx;
+    if (__ballot(mx != m)) {
+      const float f = __builtin_amdgcn_exp2f(m - ref);
+      m = mx, l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= f;
+    }
+    u32x4 w[2][P];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const int r = 2 * g;
+      const float x = __builtin_amdgcn_exp2f(fmaf(s[r], a.c, -ref)), y = __builtin_amdgcn_exp2f(fmaf(s[r + 1], a.c, -ref));
+      l += x + y;
+      if constexpr (P == 3) {
+        uint32_t part[3];
+        split_bf16x2<true>(x, y, part);
+#pragma unroll
+        for (int p = 0; p < P; ++p) w[r >> 3][p][(r >> 1) & 3] = part[p];
+      } else {
+        w[r >> 3][0][(r >> 1) & 3] = pack_bf16x2(x, y);
+      }
+    }
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");  // V is in
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int n = 0; n < 2 * ND; ++n) {
+      u32x4 f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
+            (v0 ^ (n % ND << 6)) + (16 * (n / ND) + 8 * e) * ROWB));
+        const uint2 u = __builtin_bit_cast(uint2, x);
+        f[2 * e] = u.x, f[2 * e + 1] = u.y;
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p) o[n % ND] = mfma32(f, w[n / ND][p], o[n % ND]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) copy(vbase, h + 4, true);
+  }
+
+  // ---- the waves' (m, l, O), in their own tiles' place: row by row, pieces of 4 swizzled
+  auto ox = [](int row) { return row & 15; };
+  if (wave < steps) {
+    l = sum_xor32(l);
+    if (hf == 0) ml[32 * wave + col] = float2{m, l};
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        *(__attribute__((address_space(3))) f32x4 *)(uintptr_t)(own + col * 4 * D + (((8 * d + 2 * x + hf) ^ ox(col)) << 4)) =
+            f32x4{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+  }
+  __syncthreads();
+  const int waves = min(steps, 4);
+  constexpr int OC = D / 4;  // pieces of a row
+  float odd = 0.f;
+#pragma unroll 1
+  for (int i = wave * 64; i < 32 * OC; i += 256) {
+    const int row = (i + lane) / OC, piece = (i + lane) % OC;
+    float M = kMinusInf, L = 0.f;
+    for (int j = 0; j < waves; ++j) M = fmaxf(M, ml[32 * j + row].x);
+    const float ref = M == kMinusInf ? 0.f : M;
+    f32x4 y{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < waves; ++j) {
+      const float2 x = ml[32 * j + row];
+      const float f = __builtin_amdgcn_exp2f(x.x - ref);
+      const f32x4 z = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(
+          lds_addr(lds) + j * 2 * TILE + row * 4 * D + ((piece ^ ox(row)) << 4));
+      L = fmaf(f, x.y, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(f, z[e], y[e]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    odd = fmaf(L, 0.f, odd);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd = fmaf(y[e], 0.f, odd), y[e] *= inv;
+    if (r0 + row < len) {
+      const int64_t to = ((first + r0 + row) * a.Hq + hq) * D + 4 * piece;
+      if (P == 3 && a.out_f32) *(f32x4 *)((float *)a.out + to) = y;
+      else *(u32x2 *)((uint16_t *)a.out + to) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+    }
+  }
+  if (odd != 0.f) again = 1;
+  __syncthreads();
+  if (!again) return;
+  float *const qs = (float *)((char *)lds + wave * 4 * D);
+  rows_again(a, D, qs, first, r0 + wave, min(r0 + 32, len), 4, hq);
+}
+
+#define RXW8_PACKED_QUARTERS(D, PQ, P, W, NAME)                                                      \
+  extern "C" __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(W, W)))       \
+      rxw8_packed_quarters_##NAME##_d##D(PackedArgs a) {                                             \
+    packed_quarters<D, PQ, P>(a);                                                                    \
+  }
+RXW8_PACKED_QUARTERS(64, 1, 1, 2, bf16)
+RXW8_PACKED_QUARTERS(128, 1, 1, 2, bf16)
+RXW8_PACKED_QUARTERS(256, 1, 1, 1, bf16)
+RXW8_PACKED_QUARTERS(64, 1, 3, 2, bf16_f32)
+RXW8_PACKED_QUARTERS(128, 1, 3, 2, bf16_f32)
+RXW8_PACKED_QUARTERS(256, 1, 3, 1, bf16_f32)
+RXW8_PACKED_QUARTERS(64, 3, 3, 2, f32)
+RXW8_PACKED_QUARTERS(128, 3, 3, 2, f32)
+RXW8_PACKED_QUARTERS(256, 3, 3, 1, f32)

@@ -200,9 +200,20 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
     int rc = launch(rt, "rxw8_packed_fill", dim3((unsigned)std::min<int64_t>((T * Hq * D + 255) / 256, 2048)), dim3(256), a);
     if (rc) return rc;
   }
+  // Up to five workgroups for eight CUs: the kernel whose waves share a row's keys, 32 rows of
+  // one head to a workgroup. One prompt, the tiles above and that one: 500 rows of 16 heads of
+  // 128 21.2 and 10.8 us (40 workgroups), 1000 rows of 32 34.1 and 27.7 (136), 2000 rows of 32
+  // 59.9 and 68.4 (264); 16 of 30 rows 8.2 and 6.5 (160); f32 rows, 16 heads of 256, 1000 of
+  // them 125 and 61 (132), 4000 of them 499 and 508 (504).
+  const int64_t quarters = ((T + 31) / 32 + B) * Hq;
+  const bool few = 8 * grid <= 5 * (int64_t)rt->cus && quarters <= grid_max(256);
+  const size_t tiles = (size_t)(2 * 4 * 32 * 2) * (size_t)D;  // K and V of 128 keys
   char kname[48];
-  std::snprintf(kname, sizeof kname, "rxw8_packed_prefill_%s_d%d", a.q_f32 ? "f32" : a.out_f32 ? "bf16_f32" : "bf16", (int)D);
-  return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, (size_t)(2 * 4 * 32 * 2) * (size_t)D);
+  std::snprintf(kname, sizeof kname, "rxw8_packed_%s_%s_d%d", few ? "quarters" : "prefill",
+                a.q_f32 ? "f32" : a.out_f32 ? "bf16_f32" : "bf16", (int)D);
+  if (few)  // and the records' maxima and sums, and the third parts of an f32 q of 256
+    return launch(rt, kname, dim3((unsigned)quarters), dim3(256), a, tiles + (2 << 10) + (a.q_f32 && D == 256 ? 16 << 10 : 0));
+  return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, tiles);
 }
 
 }  // namespace rxw8

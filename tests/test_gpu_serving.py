@@ -258,7 +258,15 @@ def test_paged_append_of_many_sequences(rt, batch):
 
 # ---- packed prompts ---------------------------------------------------------------
 
-def packed(rt, q, qk, k, v, offsets, out="f32", scale=None, into=None):
+def packed(rt, q, qk, k, v, offsets, out="f32", scale=None, into=None, copies=1):
+    """copies: of all heads beside each other, which have to come out alike (with many of them there are
+    workgroups enough without sharing a row's keys among waves)."""
+    if copies > 1:
+        wide = [np.tile(x, (1, copies, 1)) for x in (q, k, v)] + [None if into is None else np.tile(into, (1, copies, 1))]
+        y = packed(rt, wide[0], qk, wide[1], wide[2], offsets, out, scale, wide[3])
+        y = y.reshape(q.shape[0], copies, q.shape[1], q.shape[2])
+        assert all(np.array_equal(y[:, 0], y[:, i], equal_nan=True) for i in range(copies))
+        return y[:, 0]
     r = rx()
     bufs = [up(rt, q, qk), up(rt, k, "bf16"), up(rt, v, "bf16"),
             rt.buffer(np.asarray(offsets, np.int32))]
@@ -293,6 +301,24 @@ def test_packed_prefill(rt, d, qk, out):
     check(y[~outside], want[~outside], bound[~outside])
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("qk,out", [("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("hq,hkv", [(64, 16), (96, 48), (60, 60), (168, 14)])
+def test_packed_prefill_of_many_heads(rt, d, qk, out, hq, hkv):
+    """The same where there are workgroups enough without sharing a row's keys among waves."""
+    rng = np.random.default_rng(d + hq)
+    q, k, v, offsets = prompts(rng, [1, 0, 16, 17, 33, 64, 65, 0, 130, 200], hq, hkv, d, qk, first=3, tail=5)
+    y = packed(rt, q, qk, k, v, offsets, out)
+    g = hq // hkv
+    for h in (0, hkv // 2, hkv - 1):
+        mine = slice(h * g, (h + 1) * g)
+        want, bound = ref.packed_prefill(q[:, mine], k[:, h:h + 1], v[:, h:h + 1], offsets, p_step=P_STEP[out],
+                                         out_step=STEP[out])
+        outside = np.isnan(want).all(axis=(1, 2))
+        assert outside.sum() == 8 and not y[outside].any()
+        check(y[~outside][:, mine], want[~outside], bound[~outside])
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 3), (6, 2), (8, 1), (16, 1), (20, 2), (12, 4)])
 def test_packed_prefill_heads(rt, hq, hkv):
     rng = np.random.default_rng(hq)
@@ -301,9 +327,10 @@ def test_packed_prefill_heads(rt, hq, hkv):
     check(y, *ref.packed_prefill(q, k, v, offsets, scale=0.11, p_step=ref.BF16, out_step=ref.BF16))
 
 
+@pytest.mark.parametrize("copies", [1, 90])
 @pytest.mark.parametrize("d,qk,out", [(128, "bf16", "bf16"), (128, "f32", "f32"), (64, "bf16", "bf16"),
                                       (256, "f32", "f32"), (72, "f32", "f32")])
-def test_packed_prefill_into_leaves_other_rows(rt, d, qk, out):
+def test_packed_prefill_into_leaves_other_rows(rt, d, qk, out, copies):
     """_into writes its sequences' rows and no other; NaN in rows of other sequences stay there."""
     rng = np.random.default_rng(9)
     q, k, v, offsets = prompts(rng, [33, 90], 4, 2, d, qk, first=4, tail=70)
@@ -311,30 +338,31 @@ def test_packed_prefill_into_leaves_other_rows(rt, d, qk, out):
     q[offsets[-1]:], k[offsets[-1]:], v[offsets[-1]:] = np.nan, np.inf, np.nan
     k[4:37], v[4:37] = np.nan, np.inf  # the first sequence must not reach the second
     old = floats(rng, q.shape, out)
-    y = packed(rt, q, qk, k, v, offsets, out, into=old)
+    y = packed(rt, q, qk, k, v, offsets, out, into=old, copies=copies)
     assert np.array_equal(y[:4], old[:4]) and np.array_equal(y[offsets[-1]:], old[offsets[-1]:])
     want, bound = ref.packed_prefill(q, k, v, [37, 127], p_step=P_STEP[out], out_step=STEP[out])
     check(y[37:127], want[37:127], bound[37:127])
     # a value that is infinite in a sequence's last row reaches that row alone
     v[offsets[-1] - 1, :, 5] = np.inf
-    y = packed(rt, q, qk, k, v, offsets, out)
+    y = packed(rt, q, qk, k, v, offsets, out, copies=copies)
     assert np.isfinite(y[37:126]).all() and np.isposinf(y[126, :, 5]).all()
     assert np.isfinite(np.delete(y[126], 5, axis=1)).all()
 
 
+@pytest.mark.parametrize("copies", [1, 40])
 @pytest.mark.parametrize("hq,hkv,d,qk,out,counts", [
     (8, 2, 128, "bf16", "bf16", [1500, 3, 777, 128]), (2, 2, 128, "f32", "f32", [1000, 129]),
     (8, 1, 64, "bf16", "bf16", [1025]), (4, 1, 256, "f32", "f32", [700, 1])])
-def test_packed_prefill_long(rt, hq, hkv, d, qk, out, counts):
+def test_packed_prefill_long(rt, hq, hkv, d, qk, out, counts, copies):
     rng = np.random.default_rng(len(counts))
     q, k, v, offsets = prompts(rng, counts, hq, hkv, d, qk)
-    y = packed(rt, q, qk, k, v, offsets, out)
+    y = packed(rt, q, qk, k, v, offsets, out, copies=copies)
     rows = set(rng.integers(0, offsets[-1], 60).tolist()) | {0, int(offsets[-1]) - 1, counts[0] - 1}
     want, bound = ref.packed_prefill(q, k, v, offsets, p_step=P_STEP[out], out_step=STEP[out], rows=rows)
     at = sorted(rows)
     check(y[at], want[at], bound[at])
     assert np.isfinite(y).all()
-    assert np.array_equal(y, packed(rt, q, qk, k, v, offsets, out))
+    assert np.array_equal(y, packed(rt, q, qk, k, v, offsets, out, copies=copies))
 
 
 @pytest.mark.parametrize("batch", [63, 64, 65, 500])
@@ -360,15 +388,16 @@ def test_packed_prefill_offsets_out_of_range(rt):
     assert packed(rt, q[:0], "f32", k[:0], v[:0], [0, 0]).size == 0
 
 
+@pytest.mark.parametrize("copies", [1, 60])
 @pytest.mark.parametrize("d,qk,out", [(128, "bf16", "bf16"), (128, "f32", "f32"), (64, "f32", "f32"),
                                       (256, "f32", "f32")])
-def test_packed_prefill_large_scores(rt, d, qk, out):
+def test_packed_prefill_large_scores(rt, d, qk, out, copies):
     rng = np.random.default_rng(6)
     q, k, v, offsets = prompts(rng, [300, 200], 2, 1, d, qk)
     k[:300] *= (1 + np.arange(300, dtype=np.float32) / 40)[:, None, None]
     k[400] *= 30
     k = ref.bf16_value(ref.bf16_bits(k))
-    y = packed(rt, q, qk, k, v, offsets, out)
+    y = packed(rt, q, qk, k, v, offsets, out, copies=copies)
     check(y, *ref.packed_prefill(q, k, v, offsets, p_step=P_STEP[out], out_step=STEP[out]))
 
 

@@ -283,8 +283,13 @@ def test_prefill_plans(lib):
             assert name == "rxw8_packed_prefill_any" and got[-1][1] == (t * hkv * g + 3) // 4
             continue
         kind = "f32" if qt == F32 else "bf16_f32" if ot == F32 else "bf16"
-        assert name == "rxw8_packed_prefill_%s_d%d" % (kind, d)
-    assert len(seen) == 10
+        heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
+        rows = (64 if kind == "bf16" and d < 256 else 32) * (4 // heads)
+        grid = (-(-t // rows) + b) * hkv * g // heads
+        few = 8 * grid <= 5 * 256
+        assert name == "rxw8_packed_%s_%s_d%d" % ("quarters" if few else "prefill", kind, d)
+        assert got[-1][1] == ((-(-t // 32) + b) * hkv * g if few else grid)
+    assert len(seen) == 19
 
 
 def test_append_plans(lib):
