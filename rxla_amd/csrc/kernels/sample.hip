@@ -19,15 +19,16 @@
 // the bins are in the words' order; the running counts and masses of the bins tell the
 // bins that the borders of top_k, top_p and min_p and the token can lie in; and only the
 // words of those bins, one row's some dozens to hundreds, are looked at one by one. Words
-// that top_k cannot reach are passed over from the start (SampleExtremes::floor).
+// that top_k cannot reach are passed over from the start (SampleExtremes::floor); where
+// it is small, the others come as a list and the row is read twice.
 // Three launches where workgroups share a row (the maxima; the bins, which the last
-// workgroup of a row to arrive joins; the words, from which the last one draws), one where
-// each has its own. What bounds a batch is reading the logits: once from memory, then twice
-// more from the caches, the second time with an exponential in f64 and an LDS atomic or two
-// for each word that counts. 64 rows of 248320 f32 words: 68 us, 0.94 TB/s of logits read
-// once, 2.8 as read (22 us the maxima, 21 the bins, 14 the words, 11 the joins and launches).
-// A single row is bound by the length of the chain: 33.6 us for 151936 words, a third of
-// it the words.
+// workgroup of a row to arrive joins, or the list, from which it draws; the words, where
+// there is no list), one where each has its own. What bounds a batch is reading the
+// logits, once from memory and once or twice more from the caches; a row without a list
+// takes an exponential in f64 and an LDS atomic or two for each word besides. 64 rows of
+// 248320 f32 words: 49 us with top_k 200 (1.3 TB/s of logits read once: 22 us the maxima,
+// 14 the list, 13 the joins and launches), 74 without. A single row of 151936 is bound by
+// the length of the chain: 27.5 us, a third of it the words.
 #include <stddef.h>
 
 #include "common.h"
@@ -212,10 +213,11 @@ __device__ SampleExtremes join_extremes(SampleShared &sh, SampleExtremes e) {
   }
   return e;
 }
-// ... of the words lo <= index < hi of a row. The floor: among `groups` groups of threads each
-// one's maximum, and the least of these, which `groups` words reach. (Of 150000 words it leaves
-// about 130 for 20 groups and 1600 for 200, so that the bins' f64 and atomics are few.)
+// ... of the words lo <= index < hi of a row. The floor: of the threads' maxima (not -inf) the
+// top_k / S-th from above or one a little below it, found in a histogram over their range.
+// (As many words reach it and not many more: each thread has its words from all over the row.)
 __device__ SampleExtremes extremes_of(SampleShared &sh, const SampleArgs &a, int64_t row, const void *words, int64_t lo, int64_t hi) {
+  const int tid = threadIdx.x;
   uint32_t key = 0, index = 0xffffffffu;
   float least = __builtin_huge_valf();
   each_word(words, a.bf16, lo, hi, [&](float v, uint32_t i) {  // (a thread's words come in order)
@@ -224,13 +226,46 @@ __device__ SampleExtremes extremes_of(SampleShared &sh, const SampleArgs &a, int
     key = better ? k : key, index = better ? i : index;
     least = fminf(least, v > -__builtin_huge_valf() ? v : __builtin_huge_valf());
   });
-  const int64_t k = a.top_k ? a.top_k[row] : 0, groups = (k + a.S - 1) / a.S;
-  uint32_t floor = 0;
-  if (k > 0 && k < a.V && groups <= kThreads) {
-    floor = key;
-    for (int o = 1; o < 64 && kThreads / (2 * o) >= groups; o <<= 1) floor = max(floor, __shfl_xor(floor, o));
+  const uint32_t none = sample_key(-__builtin_huge_valf());
+  const bool has = key > none && key != 0xffffffffu;
+  SampleExtremes e = join_extremes(sh, SampleExtremes{sample_word(key, index), least, has ? key : 0xffffffffu});
+  const int64_t k = a.top_k ? a.top_k[row] : 0, wanted = (k + a.S - 1) / a.S;
+  const float from = sample_value(e.floor), to = sample_value((uint32_t)(e.top >> 32));
+  e.floor = 0;
+  if (k <= 0 || k >= a.V || wanted > kThreads / 2 || !(to < __builtin_huge_valf()) || !(from <= to)) return e;
+  const float per = to - from, scale = per > 0.f ? (float)(kBins - 1) / per : 0.f;
+  const int bin = has ? min((int)((sample_value(key) - from) * scale), kBins - 1) : -1;
+  sh.count[tid] = 0;
+  if (tid == 0) sh.at[0] = -1, sh.at[1] = -1;
+  __syncthreads();
+  if (has) atomicAdd(&sh.count[bin], 1u);
+  __syncthreads();
+  if (tid < 64) {  // 16 bins a lane, from the last down
+    const uint32_t *const mine = sh.count + kBins - 16 * (tid + 1);
+    uint32_t sum = 0;
+    for (int i = 0; i < 16; ++i) sum += mine[i];
+    uint32_t all = sum;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = __shfl_up(all, o);
+      if (tid >= o) all += x;
+    }
+    uint32_t before = all - sum;
+    if (before < wanted && all >= wanted) {
+      int i = 15;
+      while ((before += mine[i]) < wanted) --i;
+      sh.at[0] = kBins - 16 * (tid + 1) + i;
+    }
   }
-  return join_extremes(sh, SampleExtremes{sample_word(key, index), least, floor});
+  __syncthreads();
+  const int border = sh.at[0];
+  if (border >= 0) {  // (below 0: not as many threads have words)
+    uint32_t floor = bin >= border ? key : 0xffffffffu;
+    for (int o = 32; o > 0; o >>= 1) floor = min(floor, __shfl_xor(floor, o));
+    if ((tid & 63) == 0) atomicMin((uint32_t *)&sh.at[1], floor);
+    __syncthreads();
+    e.floor = (uint32_t)sh.at[1];
+  }
+  return e;
 }
 
 // Radix descent, 8 bits a pass, over the i < n that get(i, key, units) admits: the key at which
@@ -359,6 +394,7 @@ struct Borders {
   int kb, mb;         // the bins of top_k's border, and of min_p's, give or take one (-1: none)
   int pb0, pb1;       // ... of top_p's (pb0 > pb1: none)
   int db0, db1;       // ... of the token
+  int done;           // the token is out already
 };
 
 // ... from the counts and masses of the row's bins, which become running ones (in sh)
@@ -429,24 +465,38 @@ __device__ Borders borders_of(SampleShared &sh, const Row &r, const Settings &s)
   auto key_at = [&](int b) { return sample_key((float)((double)r.top - (double)b / (r.per_bin * r.inv))); };
   const float v_lo = sample_value(max(key_at(b_hi + 1) - 2, sample_key(-__builtin_huge_valf())));
   const float v_hi = b_lo <= 1 ? r.top : sample_value(min(key_at(b_lo - 1) + 2, sample_key(r.top)));
-  return Borders{total, b_hi + 1 < kBins ? fmaxf(v_lo, r.floor) : r.floor, v_hi, kb, mb, pb0, pb1, db0, db1};
+  return Borders{total, b_hi + 1 < kBins ? fmaxf(v_lo, r.floor) : r.floor, v_hi, kb, mb, pb0, pb1, db0, db1, 0};
 }
 
+__device__ __forceinline__ bool looked_at(const Borders &b, int bin) {
+  return bin == b.kb || (bin >= b.pb0 && bin <= b.pb1) || (b.mb >= 0 && abs(bin - b.mb) <= 1) ||
+         (bin >= b.db0 && bin <= b.db1);
+}
+__device__ __forceinline__ void list_word(SampleShared &sh, u64 word) {
+  const int at = atomicAdd(&sh.n, 1);
+  if (at < kList) sh.list[at] = word;
+}
 // The words lo <= index < hi in these bins, the first kList of them in sh.list; sh.n of them
 __device__ void words_of(SampleShared &sh, const Row &r, const Borders &b, int64_t lo, int64_t hi) {
   const int tid = threadIdx.x;
   __syncthreads();
-  sh.marked[tid] = tid == b.kb || (tid >= b.pb0 && tid <= b.pb1) || (b.mb >= 0 && abs(tid - b.mb) <= 1) ||
-                   (tid >= b.db0 && tid <= b.db1);
+  sh.marked[tid] = looked_at(b, tid);
   if (tid == 0) sh.n = 0;
   __syncthreads();
   each_word(r.words, r.bf16, lo, hi, [&](float v, uint32_t i) {
     if (!(v >= b.least && v <= b.most)) return;
     const double z = r.z(v);
-    if (z < r.far && sh.marked[r.bin(z)]) {
-      const int at = atomicAdd(&sh.n, 1);
-      if (at < kList) sh.list[at] = sample_word(sample_key(v), i);
-    }
+    if (z < r.far && sh.marked[r.bin(z)]) list_word(sh, sample_word(sample_key(v), i));
+  });
+  __syncthreads();
+}
+// ... not below the row's floor
+__device__ void words_from_floor(SampleShared &sh, const Row &r, int64_t lo, int64_t hi) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  each_word(r.words, r.bf16, lo, hi, [&](float v, uint32_t i) {
+    if (v >= r.floor) list_word(sh, sample_word(sample_key(v), i));
   });
   __syncthreads();
 }
@@ -630,6 +680,30 @@ __device__ bool last_of_row(const SampleArgs &a, SampleShared &sh, int64_t row) 
   return sh.flag;
 }
 
+// The words that a row's workgroups have each in its sh.list, sh.n of them, in the last one's:
+// whether this is it. (sh.n above kList: they are not there, the row's list being too small.)
+__device__ bool list_of_row(const SampleArgs &a, SampleShared &sh, int64_t row) {
+  const int tid = threadIdx.x, n = sh.n, most = list_size(a);
+  u64 *const list = list_at(a, row);
+  if (tid == 0) sh.flag = __hip_atomic_fetch_add(a.listed + row, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int at = sh.flag;
+  for (int i = tid; i < n && at + i < most; i += kThreads)
+    __hip_atomic_store(list + at + i, sh.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (!last_of_row(a, sh, row)) return false;
+  if (tid == 0) {
+    const int all = __hip_atomic_load(a.listed + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sh.n = all <= most ? all : kList + 1;
+    __hip_atomic_store(a.listed + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (sh.n <= kList)
+    for (int i = tid; i < sh.n; i += kThreads)
+      sh.list[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return true;
+}
+
 }  // namespace
 
 static_assert(sizeof(SampleShared) <= 92 << 10 && sizeof(SampleExtremes) == 16, "what the host lays out");
@@ -663,10 +737,10 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
   sh.mass[tid] = 0, sh.count[tid] = 0;
   fill_table(sh);
   __syncthreads();
-  const int64_t lo = part * a.chunk;
+  const int64_t lo = part * a.chunk, hi = min(lo + a.chunk, a.V);
   // (the arithmetic for every word, wanted or not: branches around it, which keep the words'
-  // chains from running side by side, took 40 us longer for 64 rows of 248320)
-  each_word(r.words, r.bf16, lo, min(lo + a.chunk, a.V), [&](float v, uint32_t) {
+  // chains from running side by side, took 40 us longer for 64 rows of 248320 without top_k)
+  auto weigh = [&](float v) {
     const double z = r.z(v);
     const int b = r.bin(z);
     const u64 units = units_of(r, exp2_minus(sh, z));
@@ -674,9 +748,25 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
       atomicAdd(&sh.mass[b], units);
       if (s.k > 0) atomicAdd(&sh.count[b], 1u);
     }
-  });
-  __syncthreads();
-  if (a.S > 1) {
+  };
+  const bool listed_path = s.k > 0 && 2 * s.k + 64 <= (a.S > 1 ? list_size(a) : kList) && e.floor > sample_key(-__builtin_huge_valf());
+  bool listed = false;  // (too many for the list: this workgroup takes the row's bins alone)
+  if (listed_path) {
+    // top_k leaves few words that it can reach, as a rule not twice as many: these go into a
+    // list, and from there into the bins
+    words_from_floor(sh, r, lo, hi);
+    if (a.S > 1 && !list_of_row(a, sh, row)) return;
+    listed = sh.n <= kList;
+    if (listed)
+      for (int i = tid; i < sh.n; i += kThreads) weigh(sample_value((uint32_t)(sh.list[i] >> 32)));
+    else
+      each_word(r.words, r.bf16, 0, a.V, [&](float v, uint32_t) { weigh(v); });
+    __syncthreads();
+  } else {
+    each_word(r.words, r.bf16, lo, hi, [&](float v, uint32_t) { weigh(v); });
+    __syncthreads();
+  }
+  if (a.S > 1 && !listed_path) {
     // the row's last workgroup joins the bins of all
     u64 *const here = sh.mass;
     const int used = s.k > 0 ? kBinWords : kBins;
@@ -694,13 +784,33 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_draw(SampleAr
     }
     __syncthreads();
   }
-  const Borders b = borders_of(sh, r, s);
-  if (a.S > 1) {
-    for (int i = tid; i < kBinWords; i += kThreads) bins_at(a, row, 0)[i] = sh.mass[i];
-    if (tid == 0) *borders_at(a, row) = b;
-    return;
+  Borders b = borders_of(sh, r, s);
+  if (listed) {
+    // of the list the words in the bins looked at
+    u64 word[kList / kThreads];
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      const int i = j * kThreads + tid;
+      word[j] = i < sh.n ? sh.list[i] : 0;  // (no word is 0)
+    }
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kList / kThreads; ++j) {
+      const double z = r.z(sample_value((uint32_t)(word[j] >> 32)));
+      if (word[j] && z < r.far && looked_at(b, r.bin(z))) list_word(sh, word[j]);
+    }
+    __syncthreads();
+    b.done = 1;
   }
-  words_of(sh, r, b, 0, a.V);
+  if (a.S > 1) {
+    if (!b.done)
+      for (int i = tid; i < kBinWords; i += kThreads) bins_at(a, row, 0)[i] = sh.mass[i];
+    if (tid == 0) *borders_at(a, row) = b;
+    if (!b.done) return;
+  }
+  if (!b.done) words_of(sh, r, b, 0, a.V);
   const int32_t token = draw(sh, r, s, b);
   if (tid == 0) a.out[row] = token;
 }
@@ -715,30 +825,12 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_words(SampleA
   const Borders b = *borders_at(a, row);
   Row r;
   Settings s;
-  if (!set_row(a, row, e, r, s)) return;
+  if (b.done || !set_row(a, row, e, r, s)) return;
   fill_table(sh);
   const int64_t lo = part * a.chunk;
   words_of(sh, r, b, lo, min(lo + a.chunk, a.V));
-  u64 *const list = list_at(a, row);
-  const int n = sh.n;
-  if (tid == 0) sh.flag = __hip_atomic_fetch_add(a.listed + row, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  const int at = sh.flag;
-  const int most = list_size(a);
-  for (int i = tid; i < n && at + i < most; i += kThreads)
-    __hip_atomic_store(list + at + i, sh.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!last_of_row(a, sh, row)) return;
-  if (tid == 0) {
-    sh.n = __hip_atomic_load(a.listed + row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(a.listed + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (sh.n <= most) {
-    for (int i = tid; i < sh.n; i += kThreads)
-      sh.list[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  } else {  // more than the list takes: all of them by this one
-    words_of(sh, r, b, 0, a.V);
-  }
+  if (!list_of_row(a, sh, row)) return;
+  if (sh.n > kList) words_of(sh, r, b, 0, a.V);  // more than the list takes: all of them by this one
   for (int i = tid; i < kBinWords; i += kThreads) sh.mass[i] = bins_at(a, row, 0)[i];
   __syncthreads();
   const int32_t token = draw(sh, r, s, b);
