@@ -8,6 +8,9 @@ names follow the reference's operator surface:
 * ``grouped_query_attention(q, k_cache, v_cache, lens, mask, scale)`` --
   ``Tensor::grouped_query_attention`` (crates/rxla-core/src/attention.rs:83-135)
   in its decode form over a contiguous per-sequence cache
+* ``paged_kv_append``, ``grouped_query_attention_paged``,
+  ``grouped_query_attention_packed``, ``sample`` -- serving over many sequences: a
+  paged cache, packed prompts, the next token (no counterpart in the reference)
 * ``KvCache.update_at / update_at_checked`` -- crates/rxla-core/src/kv_cache.rs:53-111
 * ``DecoderModel.compile().bind_parameters(...).run(...)`` --
   ``AppliedModel::compile`` / ``CompiledModel::bind_parameters`` / ``BoundModel::run``

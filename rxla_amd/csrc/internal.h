@@ -122,9 +122,9 @@ struct Runtime {
   Workspace xcast;     // bf16 copy of f32 activations ahead of the GEMM
   Workspace wdeq;      // bf16 dequantised weights ahead of the large-M GEMM
   Workspace attn_counters;  // i32 split arrival counters of decode attention (zeroed once)
-  // Split counters and partials of the f32 attention kernels, fixed blocks of
-  // kF32AttnBlock bytes (kernels/attention_f32.hip): of calls that run, and of
-  // calls that a capture records
+  // Split counters and partials of the f32 attention kernels, of paged decode
+  // attention and of sampling, fixed blocks of kF32AttnBlock bytes
+  // (kernels/attention_f32.hip): of calls that run, and of calls that a capture records
   char *f32_attn[2] = {nullptr, nullptr};
 
   std::vector<void *> retired;  // replaced workspace blocks that a caller's graph may hold
