@@ -520,7 +520,8 @@ __device__ void packed_prefill(const PackedArgs &a) {
   };
   if (P == 3 && a.out_f32 ? store(yes) : store(no)) return;
 
-  float *const qs = (float *)((char *)lds + wave * 4 * D);
+  // (q in this wave's own rows' place: the others may still be turning theirs)
+  float *const qs = (float *)((char *)lds + wave * WR * D * (P == 3 && a.out_f32 ? 4 : 2));
   rows_again(a, D, qs, first, r0, min(r0 + WR, len), 1, hq);
 }
 
