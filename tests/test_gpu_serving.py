@@ -389,6 +389,28 @@ def test_packed_prefill_offsets_out_of_range(rt):
 
 
 @pytest.mark.parametrize("copies", [1, 60])
+@pytest.mark.parametrize("d,qk,out", [(64, "bf16", "bf16"), (128, "bf16", "bf16"), (256, "bf16", "bf16"), (64, "f32", "f32"),
+                                      (128, "f32", "f32"), (256, "f32", "f32"), (128, "f32", "bf16"), (256, "bf16", "f32")])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (4, 2), (4, 1)])
+def test_packed_prefill_infinite_values(rt, d, qk, out, hq, hkv, copies):
+    """Infinite values of a key: in the rows that see it, and in no row of the same workgroup, wave or
+    step that does not."""
+    rng = np.random.default_rng(d)
+    q, k, v, offsets = prompts(rng, [300, 40], hq, hkv, d, qk)
+    v[133, :, 7], v[250, 0, 9] = np.inf, -np.inf
+    y = packed(rt, q, qk, k, v, offsets, out, copies=copies)
+    rows = {0, 31, 32, 100, 127, 128, 130, 132, 133, 140, 249, 250, 299, 300, 339}
+    want, bound = ref.packed_prefill(q, k, v, offsets, p_step=P_STEP[out], out_step=STEP[out], rows=rows)
+    at = sorted(rows)
+    far = np.isinf(want[at])
+    assert np.array_equal(y[at][far], want[at][far])
+    check(np.where(far, 0, y[at]), np.where(far, 0, want[at]), np.where(far, 0, bound[at]))
+    seen = np.zeros(y.shape, bool)
+    seen[133:300, :, 7], seen[250:300, :hq // hkv, 9] = True, True
+    assert np.isinf(y[seen]).all() and np.isfinite(y[~seen]).all()
+
+
+@pytest.mark.parametrize("copies", [1, 60])
 @pytest.mark.parametrize("d,qk,out", [(128, "bf16", "bf16"), (128, "f32", "f32"), (64, "f32", "f32"),
                                       (256, "f32", "f32")])
 def test_packed_prefill_large_scores(rt, d, qk, out, copies):
