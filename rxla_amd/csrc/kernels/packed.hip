@@ -112,7 +112,6 @@ __device__ __forceinline__ void unrolled(F f) {
 }
 
 constexpr int kStep = 32;  // keys
-constexpr int kRing = 4;
 
 // The row tile of the given rank, those that see the most keys first: its index in its
 // sequence, whose first row and length these are (-1: there are not that many)
@@ -168,11 +167,14 @@ __device__ __forceinline__ void rows_again(const PackedArgs &a, int D, float *qs
   }
 }
 
-// PQ, P: bf16 parts of q and of the weights (1 or 3)
-template <int D, int QT, int PQ, int P>
+// PQ, P: bf16 parts of q and of the weights (1 or 3). QL: the third parts of q stay in LDS,
+// where the registers do not hold them (D = 256: O takes 128, two parts of q as many), and
+// the rings have three places: V is then copied a step later.
+template <int D, int QT, int PQ, int P, bool QL = PQ == 3 && D == 256>
 __device__ void packed_prefill(const PackedArgs &a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [kRing][32][D] K, the same V
+  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [RING][32][D] K, the same V; q's third parts
   constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
+  constexpr int RING = QL ? 3 : 4, QR = QL ? PQ - 1 : PQ;                         // parts of q in registers
   constexpr int NK = D / 16, ND = D / 32, WR = 32 * QT;                            // WR: rows of a wave
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hf = lane >> 5;
@@ -199,8 +201,9 @@ __device__ void packed_prefill(const PackedArgs &a) {
   const uint32_t stride = (uint32_t)a.Hkv * ROWB;
   const char *const kbase = (const char *)a.k + (first * a.Hkv + kvh) * ROWB;
   const char *const vbase = (const char *)a.v + (first * a.Hkv + kvh) * ROWB;
+  auto place = [](int step) RXW8_INLINE { return RING == 4 ? step & 3 : (int)((unsigned)step % RING); };
   auto copy = [&](const char *base, int step, bool is_v) RXW8_INLINE {
-    const uint32_t dst = lds_addr(lds) + ((is_v ? kRing : 0) + (step & (kRing - 1))) * TILE;
+    const uint32_t dst = lds_addr(lds) + ((is_v ? RING : 0) + place(step)) * TILE;
     const char *const from = base + (int64_t)step * kStep * stride;
     const int most = len - 1 - step * kStep;  // (rows past the sequence repeat its last)
 #pragma unroll
@@ -210,33 +213,47 @@ __device__ void packed_prefill(const PackedArgs &a) {
     }
   };
   copy(kbase, 0, false);
+  if (QL && steps > 1) copy(kbase, 1, false);
   copy(vbase, 0, true);
-  if (steps > 1) {
+  if (!QL && steps > 1) {
     copy(kbase, 1, false);
     copy(vbase, 1, true);
   }
   if (steps > 2) copy(kbase, 2, false);
 
   // ---- q
-  u32x4 q[QT][NK][PQ];
+  u32x4 q[QT][NK][QR];
+  u32x4 *const q_low = (u32x4 *)((char *)lds + 2 * RING * TILE) + wave * NK * 64 + lane;  // [NK][64] (QL)
+  constexpr int NL = QL ? 8 : NK;  // fragments asked for at a time
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int64_t at = ((first + min(r0 + 32 * t + col, len - 1)) * a.Hq + hq) * D + 8 * hf;
+    unrolled<NK / NL>([&](auto g) RXW8_INLINE {
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      if constexpr (PQ == 3) {
-        const f32x4 x = *(const f32x4 *)((const float *)a.q + at + 16 * n), y = *(const f32x4 *)((const float *)a.q + at + 16 * n + 4);
+      for (int n = g * NL; n < (g + 1) * NL; ++n) {
+        if constexpr (PQ == 3) {
+          const f32x4 x = *(const f32x4 *)((const float *)a.q + at + 16 * n), y = *(const f32x4 *)((const float *)a.q + at + 16 * n + 4);
+          u32x4 low;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t part[3];
-          split_bf16x2(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], part);
+          for (int e = 0; e < 4; ++e) {
+            uint32_t part[3];
+            split_bf16x2(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], part);
 #pragma unroll
-          for (int p = 0; p < PQ; ++p) q[t][n][p][e] = part[p];
+            for (int p = 0; p < QR; ++p) q[t][n][p][e] = part[p];
+            low[e] = part[2];
+          }
+          if constexpr (QL) q_low[64 * n] = low;
+        } else {
+          q[t][n][0] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * n);
         }
-      } else {
-        q[t][n][0] = *(const u32x4 *)((const uint16_t *)a.q + at + 16 * n);
       }
-    }
+      if constexpr (QL) {
+#pragma unroll
+        for (int n = g * NL; n < (g + 1) * NL; ++n)
+#pragma unroll
+          for (int p = 0; p < QR; ++p) asm volatile("" : "+v"(q[t][n][p]));  // (here: one group's rows at a time)
+      }
+    });
   }
   // ---- state
   f32x16 o[QT][ND], sa[QT], sb[QT];
@@ -252,24 +269,30 @@ __device__ void packed_prefill(const PackedArgs &a) {
   }
   const float c = a.c;
   int h = 0;
-  // Before step h every wave's copies of K up to h + 1 and V up to h are in; the slots
-  // of K h - 1 and V h - 2 are free.
-  auto begin = [&]() RXW8_INLINE {
+  // Before step h every wave's copies of K up to h + 1 and V up to h (QL: h - 1) are in; the
+  // slots of K h - 1 (QL: h) and V h - 2 are free.
+  auto begin = [&](bool k = true) RXW8_INLINE {
     __builtin_amdgcn_sched_barrier(0);
     if (h + 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (h + 2 < steps) copy(vbase, h + 2, true);
-    if (h + 3 < steps) copy(kbase, h + 3, false);
+    if (h + (QL ? 1 : 2) < steps) copy(vbase, h + (QL ? 1 : 2), true);
+    if (k && h + 3 < steps) copy(kbase, h + 3, false);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto third = [&]() RXW8_INLINE {  // K of step 3, into the place of step 0's, which every wave has read
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (steps > 3) copy(kbase, 3, false);
     __builtin_amdgcn_sched_barrier(0);
   };
   // LDS byte addresses of the fragments: one XOR from a lane's base in the step's slot
   // (chunk 2 n + hf of K row col; chunks 4 d + .. of V rows 4 hf + j, 8 rows apart two reads)
   const uint32_t k0 = lds_addr(lds) + col * ROWB + ((hf ^ kx(col)) << 4);
   const int tr_j = (lane & 15) >> 2, tr_q = lane & 3;
-  const uint32_t v0 = lds_addr(lds) + kRing * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1) +
+  const uint32_t v0 = lds_addr(lds) + RING * TILE + (4 * hf + tr_j) * ROWB + 8 * (tr_q & 1) +
                       (((2 * ((lane >> 4) & 1) + (tr_q >> 1)) ^ vx(4 * hf + tr_j)) << 4);
   auto slot = [&](uint32_t base, int step) RXW8_INLINE {
-    uint32_t at = base + (step & (kRing - 1)) * TILE;
+    uint32_t at = base + place(step) * TILE;
     asm("" : "+v"(at));  // (the XORs stay where they are used, not in registers)
     return at;
   };
@@ -288,7 +311,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
     return f;
   };
   // The products of a fragment, after(i) behind the i-th (QT PQ of K's n-th, QT P of V's)
-  auto qk = [&](f32x16 (&s)[QT], auto n, u32x4 f, auto after) RXW8_INLINE {
+  auto qk = [&](f32x16 (&s)[QT], auto n, u32x4 f, u32x4 low, auto after) RXW8_INLINE {
     unrolled<QT * PQ>([&](auto i) RXW8_INLINE {
       constexpr int t = i % QT, x = i / QT;
       if constexpr (n == 0 && x == 0) {
@@ -297,7 +320,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
         for (int r = 0; r < 16; ++r) zero[r] = 0.f;
         s[t] = mfma32(f, q[t][n][x], zero);
       } else {
-        s[t] = mfma32(f, q[t][n][x], s[t]);
+        s[t] = mfma32(f, QL && x == PQ - 1 ? low : q[t][n][x < QR ? x : 0], s[t]);
       }
       after(i);
     });
@@ -383,11 +406,12 @@ __device__ void packed_prefill(const PackedArgs &a) {
     constexpr int NF = (QK ? NK : 0) + (PV ? 2 * ND : 0), NM = QT * ((QK ? PQ * NK : 0) + (PV ? P * 2 * ND : 0)), NE = 8 * QT * ITEMS;
     static_assert(NK == 2 * ND, "K and V take turns");
     const uint32_t ks = slot(k0, h + 1), vs = slot(v0, h - 1);
-    u32x4 fr[AHEAD + 1];
+    u32x4 fr[AHEAD + 1], lows[QL ? AHEAD + 1 : 1];
     auto read = [&](auto n) RXW8_INLINE {
       constexpr bool k = QK && (!PV || n % 2 == 0);
       constexpr int at = QK && PV ? n / 2 : n;
       fr[n % (AHEAD + 1)] = k ? k_frag(ks, at) : v_frag(vs, at);
+      if constexpr (QL && k) lows[n % (AHEAD + 1)] = q_low[64 * at];
     };
     unrolled<AHEAD>(read);
     unrolled<NF>([&](auto n) RXW8_INLINE {
@@ -402,7 +426,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
         unrolled<e1 - e0>([&](auto e) RXW8_INLINE { item(s, pn, std::integral_constant<int, e0 + e>{}); });
         __builtin_amdgcn_sched_barrier(0);
       };
-      if constexpr (k) qk(sn, at, f, share);
+      if constexpr (k) qk(sn, at, f, lows[QL ? n % (AHEAD + 1) : 0], share);
       else pv(p, at, f, share);
     });
     last_item(pn);
@@ -415,15 +439,16 @@ __device__ void packed_prefill(const PackedArgs &a) {
     ++h;
   };
 
-  // Every wave goes through steps + 1 barriers. (The loop holds two steps, for the two
+  // Every wave goes through steps + 1 barriers (QL: one more behind the first). (The loop holds two steps, for the two
   // sets of registers, and nothing else: with the mask's or the end's branches in it the
   // allocator moves O about.)
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
   if (mine > 0) {
-    begin();
+    begin(!QL);
     const uint32_t ks = slot(k0, 0);
-    unrolled<NK>([&](auto n) RXW8_INLINE { qk(sa, n, k_frag(ks, n), nothing); });
+    unrolled<NK>([&](auto n) RXW8_INLINE { qk(sa, n, k_frag(ks, n), QL ? q_low[64 * n] : u32x4{}, nothing); });
+    if constexpr (QL) third();
     if (full == 0) mask(sa);
 #pragma unroll
     for (int t = 0; t < QT; ++t) {  // the reference: step 0's maximum
@@ -473,6 +498,11 @@ __device__ void packed_prefill(const PackedArgs &a) {
         finish(pa);
       }
     }
+  }
+  if (QL && h == 0) {
+    begin(false);
+    third();
+    ++h;
   }
   for (; h <= steps; ++h) begin();
   __syncthreads();  // (the rings are read)

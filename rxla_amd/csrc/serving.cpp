@@ -203,8 +203,8 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
   // Up to five workgroups for eight CUs: the kernel whose waves share a row's keys, 32 rows of
   // one head to a workgroup. One prompt, the tiles above and that one: 500 rows of 16 heads of
   // 128 21.2 and 10.8 us (40 workgroups), 1000 rows of 32 34.1 and 27.7 (136), 2000 rows of 32
-  // 59.9 and 68.4 (264); 16 of 30 rows 8.2 and 6.5 (160); f32 rows, 16 heads of 256, 1000 of
-  // them 125 and 61 (132), 4000 of them 499 and 508 (504).
+  // 59.9 and 68.4 (264); 16 of 30 rows 8.2 and 6.5 (160); 4000 f32 rows of 16 heads of 256 310
+  // and 508 (504).
   const int64_t quarters = ((T + 31) / 32 + B) * Hq;
   const bool few = 8 * grid <= 5 * (int64_t)rt->cus && quarters <= grid_max(256);
   const size_t tiles = (size_t)(2 * 4 * 32 * 2) * (size_t)D;  // K and V of 128 keys
@@ -213,7 +213,7 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
                 a.q_f32 ? "f32" : a.out_f32 ? "bf16_f32" : "bf16", (int)D);
   if (few)  // and the records' maxima and sums, and the third parts of an f32 q of 256
     return launch(rt, kname, dim3((unsigned)quarters), dim3(256), a, tiles + (2 << 10) + (a.q_f32 && D == 256 ? 16 << 10 : 0));
-  return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, tiles);
+  return launch(rt, kname, dim3((unsigned)grid), dim3(256), a, a.q_f32 && D == 256 ? (size_t)160 << 10 : tiles);
 }
 
 }  // namespace rxw8
