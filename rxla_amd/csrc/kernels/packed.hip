@@ -69,7 +69,9 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a)
 // scheduler keeps it). One fragment of K or V serves 32 QT rows: at QT = 2 the LDS reads
 // take half the time of the products. bf16 q and outputs run QT = 2 (one at D = 256, by
 // registers: O alone is 32 QT D / 64 of them); f32 ones split q and P in their three bf16
-// parts (exact products, f32 sums) and run QT = 1.
+// parts (exact products, f32 sums) and run QT = 1. Prompts of 5000 and 7000 rows, 64 / 8
+// heads of 128, bf16: 1.10 PFLOP/s; 4 of 2048 f32 rows, 32 / 8 heads of 128: 0.36, each
+// product counted once.
 //
 // m is the maximum of the row's first 32 keys and does not move: weights may grow past 1
 // as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l or O leaves that
