@@ -280,12 +280,29 @@ __device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64
     __syncthreads();
     if (tid < 256) sh.count[tid] = 0, sh.mass[tid] = 0;
     __syncthreads();
-    for (int64_t i = tid; i < n; i += kThreads) {
-      uint32_t k;
-      u64 u;
-      if (!get(i, k, u) || (shift < 24 && (k >> (shift + 8)) != f.key)) continue;
-      atomicAdd(&sh.count[(k >> shift) & 255], 1u);
-      atomicAdd(&sh.mass[(k >> shift) & 255], u);
+    for (int64_t i0 = 0; i0 < n; i0 += kThreads) {  // (whole waves)
+      uint32_t k = 0;
+      u64 u = 0;
+      const bool here = i0 + tid < n && get(i0 + tid, k, u) && (shift == 24 || (k >> (shift + 8)) == f.key);
+      const u64 all = __ballot(here);
+      if (!all) continue;
+      // words of one digit, as ties are, in one addition: 64 of them to one address take turns
+      const uint32_t digit = (k >> shift) & 255;
+      const int lead = __builtin_ctzll(all);
+      const bool same = here && digit == (uint32_t)__builtin_amdgcn_readlane((int)digit, lead);
+      const int together = __popcll(__ballot(same));
+      if (together > 8) {
+        u64 sum = same ? u : 0;
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if ((tid & 63) == lead) {
+          atomicAdd(&sh.count[digit], (uint32_t)together);
+          atomicAdd(&sh.mass[digit], sum);
+        }
+      }
+      if (here && !(same && together > 8)) {
+        atomicAdd(&sh.count[digit], 1u);
+        atomicAdd(&sh.mass[digit], u);
+      }
     }
     __syncthreads();
     if (tid < 64) {  // the bins from the last down, four to a lane
