@@ -26,9 +26,9 @@
 // there is no list), one where each has its own. What bounds a batch is reading the
 // logits, once from memory and once or twice more from the caches; a row without a list
 // takes an exponential in f64 and an LDS atomic or two for each word besides. 64 rows of
-// 248320 f32 words: 49 us with top_k 200 (1.3 TB/s of logits read once: 22 us the maxima,
-// 14 the list, 13 the joins and launches), 74 without. A single row of 151936 is bound by
-// the length of the chain: 27.5 us, a third of it the words.
+// 248320 f32 words: 47 us with top_k 200 (1.35 TB/s of logits read once: 22 us the maxima,
+// 14 the list, 11 the joins and launches), 74 without. A single row of 151936 is bound by
+// the length of the chain: 27 us, a third of it the words.
 #include <stddef.h>
 
 #include "common.h"
@@ -59,7 +59,7 @@ typedef unsigned long long u64;
 
 namespace {
 
-constexpr int kThreads = 1024, kBins = 1024, kList = 8192, kPairwise = 1024;
+constexpr int kThreads = 1024, kBins = 1024, kList = 8192, kPairwise = 512;
 
 // Ascending keys for ascending values, -0 and +0 alike; above them all a NaN
 __device__ __forceinline__ uint32_t sample_key(float v) {
@@ -125,7 +125,7 @@ struct SampleShared {
   u64 mass[kBins];      // (mass and count: 12 KiB in one piece)
   uint32_t count[kBins];
   u64 list[kList];      // words of the bins looked at
-  u64 unit[kPairwise];  // their masses and bins
+  u64 unit[kPairwise];  // their masses and bins, where they are few
   uint16_t bin[kPairwise];
   uint8_t marked[kBins];
   double exp2_table[64];
@@ -528,7 +528,12 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
 
   u64 kept = total;
   if (n <= kPairwise) {
-    // each thread a word, and the words before it in its bin
+    // of each word those before it in its bin, by as many threads as there are. (A thread each,
+    // for up to 1024 words: 123 us for 4 rows of 248320 bf16 words cut in a crowd of ties, 58 so.)
+    u64 *const ahead = sh.list + kPairwise;
+    uint32_t *const ranks = (uint32_t *)(sh.list + 2 * kPairwise);
+    int wide = 64;
+    while (wide < n) wide <<= 1;
     u64 word = 0, one = 0, before = 0;
     uint32_t rank = 0;
     double w = 0.0;
@@ -538,13 +543,23 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
       const double z = r.z(sample_value((uint32_t)(word >> 32)));
       b = r.bin(z), w = exp2_minus(sh, z), one = units_of(r, w);
       sh.bin[tid] = (uint16_t)b, sh.unit[tid] = one;
+      ahead[tid] = sh.mass[b], ranks[tid] = sh.count[b];
     }
     __syncthreads();
-    if (tid < n) {
-      before = sh.mass[b], rank = sh.count[b];
-      for (int j = 0; j < n; ++j)
-        if (sh.list[j] > word && sh.bin[j] == b) before += sh.unit[j], ++rank;
+    if (const int at = tid & (wide - 1); at < n) {
+      const u64 its = sh.list[at];
+      const int its_bin = sh.bin[at];
+      u64 sum = 0;
+      uint32_t some = 0;
+      for (int j = tid / wide; j < n; j += kThreads / wide)
+        if (sh.list[j] > its && sh.bin[j] == its_bin) sum += sh.unit[j], ++some;
+      if (some) {
+        atomicAdd(&ahead[at], sum);
+        atomicAdd(&ranks[at], some);
+      }
     }
+    __syncthreads();
+    if (tid < n) before = ahead[tid], rank = ranks[tid];
     auto ask = [&](bool here, u64 answer) {  // from the one thread that has it
       if (here) sh.result = answer;
       __syncthreads();
