@@ -853,11 +853,12 @@ extern "C" __global__ void __launch_bounds__(kThreads) rxw8_sample_words(SampleA
   SampleShared &sh = *(SampleShared *)lds;
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x / a.S, part = blockIdx.x - row * a.S;
-  const SampleExtremes e = row_extremes(a, row);
   const Borders b = *borders_at(a, row);
+  if (b.done) return;  // (where the token is the first maximum, whatever this is: set_row says so)
+  const SampleExtremes e = row_extremes(a, row);
   Row r;
   Settings s;
-  if (b.done || !set_row(a, row, e, r, s)) return;
+  if (!set_row(a, row, e, r, s)) return;
   fill_table(sh);
   const int64_t lo = part * a.chunk;
   words_of(sh, r, b, lo, min(lo + a.chunk, a.V));
