@@ -27,7 +27,7 @@
 // logits, once from memory and once or twice more from the caches; a row without a list
 // takes an exponential in f64 and an LDS atomic or two for each word besides. 64 rows of
 // 248320 f32 words: 47 us with top_k 200 (1.35 TB/s of logits read once: 22 us the maxima,
-// 14 the list, 11 the joins and launches), 74 without. A single row of 151936 is bound by
+// 14 the list, 11 the joins and launches), 70 without. A single row of 151936 is bound by
 // the length of the chain: 27 us, a third of it the words.
 #include <stddef.h>
 
