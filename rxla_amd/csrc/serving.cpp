@@ -200,13 +200,17 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
     int rc = launch(rt, "rxw8_packed_fill", dim3((unsigned)std::min<int64_t>((T * Hq * D + 255) / 256, 2048)), dim3(256), a);
     if (rc) return rc;
   }
-  // Up to five workgroups for eight CUs: the kernel whose waves share a row's keys, 32 rows of
-  // one head to a workgroup. One prompt, the tiles above and that one: 500 rows of 16 heads of
-  // 128 21.2 and 10.8 us (40 workgroups), 1000 rows of 32 34.1 and 27.7 (136), 2000 rows of 32
-  // 59.9 and 68.4 (264); 16 of 30 rows 8.2 and 6.5 (160); 4000 f32 rows of 16 heads of 256 310
-  // and 508 (504).
+  // Few rows: the kernel whose waves share a row's keys, 32 rows of one head to a workgroup, two
+  // of them on a CU (one at D = 256). It needs no more rounds of workgroups than pay for steps
+  // done a quarter at a time: 3/4 and one more for each 512 rows of a sequence, at most 2, or
+  // 5/4 for bf16 rows of 256. In us, the tiles above and that one. 16 heads of 128, bf16: 1 x 500
+  // rows 21.2, 10.8; 1 x 2000 57.3, 38.8; 8 x 100 12.2, 8.5; 6 x 200 14.6, 15.6; of 32 heads
+  // 1 x 1000 34.1, 27.7; 1 x 2000 59.9, 68.4; 2 x 800 29.3, 38.5. f32: 1 x 2000 78.3, 69.5;
+  // 4 x 500 27.9, 32.5. 16 heads of 256, f32: 1 x 1000 68.3, 59.9; 1 x 1100 73.7, 78.3;
+  // 3 x 100 18.1, 16.7; 4 x 150 21.6, 29.3; bf16: 1 x 500 21.8, 19.1; 1 x 850 31.4, 35.2.
   const int64_t quarters = ((T + 31) / 32 + B) * Hq;
-  const bool few = 8 * grid <= 5 * (int64_t)rt->cus && quarters <= grid_max(256);
+  const double likely = (T / 32.0 + B / 2.0) * (double)Hq, rounds = 0.75 + (double)T / std::max<int64_t>(B, 1) / 512;
+  const bool few = likely <= std::min(rounds, !f32 && D == 256 ? 1.25 : 2.0) * (D == 256 ? 1 : 2) * rt->cus && quarters <= grid_max(256);
   const size_t tiles = (size_t)(2 * 4 * 32 * 2) * (size_t)D;  // K and V of 128 keys
   char kname[48];
   std::snprintf(kname, sizeof kname, "rxw8_packed_%s_%s_d%d", few ? "quarters" : "prefill",

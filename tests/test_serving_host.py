@@ -286,7 +286,8 @@ def test_prefill_plans(lib):
         heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
         rows = (64 if kind == "bf16" and d < 256 else 32) * (4 // heads)
         grid = (-(-t // rows) + b) * hkv * g // heads
-        few = 8 * grid <= 5 * 256
+        rounds = min(0.75 + t / max(b, 1) / 512, 1.25 if kind == "bf16" and d == 256 else 2)
+        few = (t / 32 + b / 2) * hkv * g <= rounds * (1 if d == 256 else 2) * 256
         assert name == "rxw8_packed_%s_%s_d%d" % ("quarters" if few else "prefill", kind, d)
         assert got[-1][1] == ((-(-t // 32) + b) * hkv * g if few else grid)
     assert len(seen) == 19
