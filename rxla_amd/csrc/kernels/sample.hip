@@ -268,11 +268,12 @@ __device__ SampleExtremes extremes_of(SampleShared &sh, const SampleArgs &a, int
   return e;
 }
 
-// Radix descent, 8 bits a pass, over the i < n that get(i, key, units) admits: the key at which
-// the running count reaches `count` (if above 0), else the running mass m satisfies m >= want
-// (m > want where `over`), as some key's does; counts and masses begin with `before`'s.
-template <typename Get>
-__device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64 count, bool over, double want) {
+// Radix descent, 8 bits a pass, over the words that each(f) hands to f(here, key, units), whole
+// waves at a time: the key at which the running count reaches `count` (if above 0), else the
+// running mass m satisfies m >= want (m > want where `over`), as some key's does; counts and
+// masses begin with `before`'s.
+template <typename Each>
+__device__ Found descend(SampleShared &sh, Each each, Found before, u64 count, bool over, double want) {
   const int tid = threadIdx.x;
   Found f = before;
   f.key = 0;
@@ -280,12 +281,10 @@ __device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64
     __syncthreads();
     if (tid < 256) sh.count[tid] = 0, sh.mass[tid] = 0;
     __syncthreads();
-    for (int64_t i0 = 0; i0 < n; i0 += kThreads) {  // (whole waves)
-      uint32_t k = 0;
-      u64 u = 0;
-      const bool here = i0 + tid < n && get(i0 + tid, k, u) && (shift == 24 || (k >> (shift + 8)) == f.key);
+    each([&](bool word, uint32_t k, u64 u) {
+      const bool here = word && (shift == 24 || (k >> (shift + 8)) == f.key);
       const u64 all = __ballot(here);
-      if (!all) continue;
+      if (!all) return;
       // words of one digit, as ties are, in one addition: 64 of them to one address take turns
       const uint32_t digit = (k >> shift) & 255;
       const int lead = __builtin_ctzll(all);
@@ -303,7 +302,7 @@ __device__ Found descend(SampleShared &sh, int64_t n, Get get, Found before, u64
         atomicAdd(&sh.count[digit], 1u);
         atomicAdd(&sh.mass[digit], u);
       }
-    }
+    });
     __syncthreads();
     if (tid < 64) {  // the bins from the last down, four to a lane
       uint32_t cnt[4];
@@ -357,16 +356,21 @@ __device__ u64 tie_passing(const Found &f, u64 one, double want) {
 }
 
 // The token by descents over all words of the row (where a bin holds more of them than the list:
-// long runs of ties): some milliseconds, as every descent reads the row four times
+// long runs of ties): up to a millisecond, as every descent reads the row four times
 __device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings &s) {
-  auto value = [&](int64_t i) {
-    return r.bf16 ? bf16_bits_to_f32(((const uint16_t *)r.words)[i]) : ((const float *)r.words)[i];
+  auto each_of_row = [&](auto f) {  // f(here, value, index), four loads at a time
+    for (int64_t i0 = threadIdx.x; i0 - threadIdx.x < r.V; i0 += 4 * kThreads) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t i = min(i0 + e * kThreads, r.V - 1);
+        v[e] = r.bf16 ? bf16_bits_to_f32(((const uint16_t *)r.words)[i]) : ((const float *)r.words)[i];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f(i0 + e * kThreads < r.V, v[e], (uint32_t)(i0 + e * kThreads));
+    }
   };
-  auto word = [&](int64_t i, uint32_t &k, u64 &u) {
-    const float v = value(i);
-    k = sample_key(v), u = units_at(sh, r, v);
-    return true;
-  };
+  auto word = [&](auto f) { each_of_row([&](bool here, float v, uint32_t) { f(here, sample_key(v), units_at(sh, r, v)); }); };
   auto sum = [&](double least) {  // of the words with w >= least
     u64 m = 0;
     each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t) {
@@ -384,22 +388,21 @@ __device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings 
   const Found none{};
   u64 kept = sum(0.0);
   if (s.k > 0 && s.k < r.V) {
-    const Found f = descend(sh, r.V, word, none, (u64)s.k, false, 0.0);
+    const Found f = descend(sh, word, none, (u64)s.k, false, 0.0);
     kept = f.mass + ((u64)s.k - f.count) * units_at(sh, r, sample_value(f.key));
   }
   const double all = (double)kept;
   if (s.p < 1.f) {
-    const Found f = descend(sh, r.V, word, none, 0, false, (double)s.p * all);
+    const Found f = descend(sh, word, none, 0, false, (double)s.p * all);
     kept = min(kept, mass_reaching(f, units_at(sh, r, sample_value(f.key)), (double)s.p * all));
   }
   if (s.m > 0.f) kept = min(kept, sum((double)s.m));
   kept = max_u64(kept, (u64)r.unit);
   const double want = (double)s.u * (double)kept;
-  const Found f = descend(sh, r.V, word, none, 0, true, want);
+  const Found f = descend(sh, word, none, 0, true, want);
   const u64 nth = tie_passing(f, units_at(sh, r, sample_value(f.key)), want);
-  const Found at = descend(sh, r.V, [&](int64_t i, uint32_t &k, u64 &u) {
-    k = 0xffffffffu - (uint32_t)i, u = 0;
-    return sample_key(value(i)) == f.key;
+  const Found at = descend(sh, [&](auto g) {
+    each_of_row([&](bool here, float v, uint32_t i) { g(here && sample_key(v) == f.key, 0xffffffffu - i, 0); });
   }, none, nth + 1, false, 0.0);
   return (int32_t)(0xffffffffu - at.key);
 }
@@ -600,13 +603,16 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
   if (np + nd + 2 > kPairwise) return draw_from_row(sh, r, s);
   for (int i = tid; i < np + nd; i += kThreads) sh.unit[i] = sh.mass[i < np ? pb0 + i : db0 + i - np];
   __syncthreads();
+  auto each_of_list = [&](auto f) {  // f(here, word)
+    for (int i0 = 0; i0 < n; i0 += kThreads) f(i0 + tid < n, i0 + tid < n ? sh.list[i0 + tid] : 0);
+  };
   auto in_bin = [&](int bin) {
-    return [&, bin](int64_t i, uint32_t &k, u64 &u) {
-      k = (uint32_t)(sh.list[i] >> 32);
-      const double z = r.z(sample_value(k));
-      if (r.bin(z) != bin) return false;
-      u = units_of(r, exp2_minus(sh, z));
-      return true;
+    return [&, bin](auto f) {
+      each_of_list([&](bool here, u64 word) {
+        const uint32_t k = (uint32_t)(word >> 32);
+        const double z = r.z(sample_value(k));
+        f(here && r.bin(z) == bin, k, units_of(r, exp2_minus(sh, z)));
+      });
     };
   };
   auto last_before = [&](int at, int count, bool over, double want) {  // the bin the mass `want` lies in
@@ -615,13 +621,13 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
     return i;
   };
   if (kb >= 0) {
-    const Found f = descend(sh, n, in_bin(kb), kf, (u64)s.k, false, 0.0);
+    const Found f = descend(sh, in_bin(kb), kf, (u64)s.k, false, 0.0);
     kept = f.mass + ((u64)s.k - f.count) * units_at(sh, r, sample_value(f.key));
   }
   if (s.p < 1.f) {
     const double want = (double)s.p * (double)kept;
     const int i = last_before(0, np, false, want);
-    const Found f = descend(sh, n, in_bin(pb0 + i), Found{sh.unit[i], 0, 0, 0}, 0, false, want);
+    const Found f = descend(sh, in_bin(pb0 + i), Found{sh.unit[i], 0, 0, 0}, 0, false, want);
     kept = min(kept, want > 0.0 ? mass_reaching(f, units_at(sh, r, sample_value(f.key)), want) : first);
   }
   if (mb >= 0) {
@@ -641,11 +647,10 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
   kept = max_u64(kept, first);
   const double want = (double)s.u * (double)kept;
   const int i = last_before(np, nd, true, want);
-  const Found f = descend(sh, n, in_bin(db0 + i), Found{sh.unit[np + i], 0, 0, 0}, 0, true, want);
+  const Found f = descend(sh, in_bin(db0 + i), Found{sh.unit[np + i], 0, 0, 0}, 0, true, want);
   const u64 nth = tie_passing(f, units_at(sh, r, sample_value(f.key)), want);
-  const Found at = descend(sh, n, [&](int64_t x, uint32_t &k, u64 &u) {
-    k = (uint32_t)sh.list[x], u = 0;
-    return (uint32_t)(sh.list[x] >> 32) == f.key;
+  const Found at = descend(sh, [&](auto g) {
+    each_of_list([&](bool here, u64 word) { g(here && (uint32_t)(word >> 32) == f.key, (uint32_t)word, 0); });
   }, Found{}, nth + 1, false, 0.0);
   return (int32_t)(0xffffffffu - at.key);
 }
