@@ -361,3 +361,39 @@ def test_sample_words_past_32_bits(rt, b, v):
     # of n equal words the first whose running mass exceeds n / 2
     want = [at[i] if one[i] else 500 if k[i] else v // 2 for i in range(b)]
     assert got.tolist() == want
+
+
+# ---- nothing there -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("pages,entries", [(0, 3), (4, 0), (0, 0)])
+def test_no_pages(rt, pages, entries):
+    """A pool without pages, a table without entries: rows see no key, and new rows have no place."""
+    r = rx()
+    kp, vp = (rt.zeros((pages, 2, 16, 64), r.DType.BF16) for _ in range(2))
+    table = rt.zeros((3, entries), r.DType.I32)
+    q = rt.buffer(np.ones((3, 4, 64), np.float32))
+    y = r.grouped_query_attention_paged(rt, q, kp, vp, table, i32(rt, [5, 0, 70]))
+    assert not down(y).any()
+    new = rt.buffer(np.ones((3, 2, 64), np.float32))
+    r.paged_kv_append(rt, kp, vp, new, new, table, i32(rt, [0, 5, 47]))
+    assert not kp.to_numpy().any() and not vp.to_numpy().any()
+
+
+def test_extreme_positions_and_lengths(rt):
+    """Lengths, starts and offsets at the ends of their type."""
+    r, rng = rx(), np.random.default_rng(12)
+    top = 2 ** 31 - 1
+    kp, vp, table = make_pages(rng, [48, 48, 48], 2, 16, 128, "bf16")
+    q = floats(rng, (3, 4, 128), "f32")
+    pools = [up(rt, kp, "bf16"), up(rt, vp, "bf16")]
+    y = down(r.grouped_query_attention_paged(rt, up(rt, q, "f32"), *pools, i32(rt, table), i32(rt, [top, -2 ** 31, 48]),
+                                             out_dtype=r.DType.F32))
+    check(y, *ref.paged_decode(q, kp, vp, table, [48, 0, 48]))
+    new = [floats(rng, (3, 2, 128), "bf16") for _ in range(2)]
+    r.paged_kv_append(rt, *pools, *(up(rt, x, "bf16") for x in new), i32(rt, table), i32(rt, [top, -2 ** 31, 47]))
+    for pool, old, x in zip(pools, (kp, vp), new):
+        assert np.array_equal(down(pool), ref.append(old, x, table, [top, -5, 47], [0, 1, 2, 3]))
+    q, k, v, _ = prompts(rng, [30], 4, 2, 128, "f32")
+    y = down(r.grouped_query_attention_packed(rt, up(rt, q, "f32"), up(rt, k, "bf16"), up(rt, v, "bf16"),
+                                              i32(rt, [-2 ** 31, 9, top]), out_dtype=r.DType.F32))
+    check(y, *ref.packed_prefill(q, k, v, [0, 9, 30]))
