@@ -66,12 +66,15 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a)
 // In a step the products are those of S one step ahead and of O one step behind, so
 // none of them waits for the softmax between: every LDS read is followed by its
 // products, and these by a share of the softmax, in that order (a barrier to the
-// scheduler keeps it). One fragment of K or V serves 32 QT rows: at QT = 2 the LDS reads
-// take half the time of the products. bf16 q and outputs run QT = 2 (one at D = 256, by
-// registers: O alone is 32 QT D / 64 of them); f32 ones split q and P in their three bf16
-// parts (exact products, f32 sums) and run QT = 1. Prompts of 5000 and 7000 rows, 64 / 8
-// heads of 128, bf16: 1.10 PFLOP/s; 4 of 2048 f32 rows, 32 / 8 heads of 128: 0.36, each
-// product counted once.
+// scheduler keeps it). bf16 q and outputs of 128 run QT = 1 with two workgroups to a CU,
+// whose prologues and stores pass under the other's products: 12 prompts of 64 to 2000 rows, 32 / 8
+// heads, take 124 us so and 136 with QT = 2 on a CU alone, though there the LDS reads take half
+// the time of the products (one fragment of K or V serves 32 QT rows); of 5000 and 7000 rows, 64 /
+// 8 heads, 1113 (1.09 PFLOP/s) and 1129. At 64 QT = 2 leaves registers for two workgroups all the
+// same (78 us for 4 of 2048 rows, 82 with QT = 1 and four). At 256 O alone is 128 registers: QT = 1
+// and one workgroup. f32 ones split q and P in their three bf16 parts (exact products, f32 sums)
+// and run QT = 1, from 128 on a CU alone (two spill: 480 us for 4 of 2048 rows, 32 / 8 heads of
+// 128, 382 so: 0.36 PFLOP/s, each product counted once).
 //
 // m is the maximum of the row's first 32 keys and does not move: weights may grow past 1
 // as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l or O leaves that
@@ -564,7 +567,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
   }
 // q and output bf16; q bf16, output f32; q f32
 RXW8_PACKED_PREFILL(64, 2, 1, 1, 2, bf16)
-RXW8_PACKED_PREFILL(128, 2, 1, 1, 1, bf16)
+RXW8_PACKED_PREFILL(128, 1, 1, 1, 2, bf16)
 RXW8_PACKED_PREFILL(256, 1, 1, 1, 1, bf16)
 RXW8_PACKED_PREFILL(64, 1, 1, 3, 2, bf16_f32)
 RXW8_PACKED_PREFILL(128, 1, 1, 3, 1, bf16_f32)
@@ -581,8 +584,8 @@ RXW8_PACKED_PREFILL(256, 1, 3, 3, 1, f32)
 // barrier: its K and V tiles in LDS are its own, one each, copied by LDS DMA as soon as the
 // products with the one before are done; S, its softmax with a running maximum, and O
 // follow one another. At the end the four (m, l, O) are joined in LDS, in the order of the
-// waves. (16 heads of 128 over 8, one prompt of 500 rows: 10.8 us, 21.2 on the tiles above; of
-// 1000: 16.6 and 33.6.) Rows that do not come out as numbers are done again as above. QL: the third parts of
+// waves. (16 heads of 128 over 8, one prompt of 500 rows: 10.5 us, 13.7 on the tiles above; of
+// 1000: 16.2 and 21.9.) Rows that do not come out as numbers are done again as above. QL: the third parts of
 // an f32 q stay in LDS, where the registers do not hold them (at D = 256 O takes 128, two
 // parts of q as many).
 template <int D, int PQ, int P, bool QL = PQ == 3 && D == 256>

@@ -191,7 +191,7 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
   // Row tiles of a workgroup: 4 waves of 32 or 64 rows (kernels/packed.hip) over its
   // heads; at most one more than T's for each sequence
   const bool f32 = a.q_f32 || a.out_f32;
-  const int64_t rows = (f32 || D == 256 ? 32 : 64) * (4 / a.heads);
+  const int64_t rows = (f32 || D > 64 ? 32 : 64) * (4 / a.heads);
   const int64_t grid = ((T + rows - 1) / rows + B) * (Hq / a.heads);
   if ((D != 64 && D != 128 && D != 256) || Hkv * D * 2 * 32 >= ((int64_t)1 << 31) || grid > grid_max(256) ||
       ((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) % 16)
@@ -202,15 +202,17 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
   }
   // Few rows: the kernel whose waves share a row's keys, 32 rows of one head to a workgroup, two
   // of them on a CU (one at D = 256). It needs no more rounds of workgroups than pay for steps
-  // done a quarter at a time: 3/4 and one more for each 512 rows of a sequence, at most 2, or
-  // 5/4 for bf16 rows of 256. In us, the tiles above and that one. 16 heads of 128, bf16: 1 x 500
-  // rows 21.2, 10.8; 1 x 2000 57.3, 38.8; 8 x 100 12.2, 8.5; 6 x 200 14.6, 15.6; of 32 heads
-  // 1 x 1000 34.1, 27.7; 1 x 2000 59.9, 68.4; 2 x 800 29.3, 38.5. f32: 1 x 2000 78.3, 69.5;
-  // 4 x 500 27.9, 32.5. 16 heads of 256, f32: 1 x 1000 68.3, 59.9; 1 x 1100 73.7, 78.3;
-  // 3 x 100 18.1, 16.7; 4 x 150 21.6, 29.3; bf16: 1 x 500 21.8, 19.1; 1 x 850 31.4, 35.2.
+  // done a quarter at a time, by the sequences' mean length: 3/4 and one more for each 512 rows,
+  // at most 2; or, where bf16 tiles run two workgroups to a CU or D = 256, 2/5 and one more for
+  // each 800, at most 1.05. In us, the tiles above and that one. 16 heads of 128, bf16: 8 x 100
+  // rows 8.1, 8.6; 1 x 300 10.6, 9.4; 4 x 300 11.4, 16.6; 1 x 1000 21.9, 16.2; 2 x 1000 23.7, 27.8;
+  // f32: 1 x 2000 78.3, 69.5; 4 x 500 27.9, 32.5. 16 of 256, f32: 1 x 1000 68.3, 59.9;
+  // 1 x 1100 73.7, 78.3; 3 x 100 18.1, 16.7; 4 x 150 21.6, 29.3; bf16: 1 x 500 21.8, 19.1;
+  // 1 x 850 31.4, 35.2. 32 of 64, bf16: 1 x 1000 23.1, 17.3; 1 x 2000 40.5, 43.2.
   const int64_t quarters = ((T + 31) / 32 + B) * Hq;
-  const double likely = (T / 32.0 + B / 2.0) * (double)Hq, rounds = 0.75 + (double)T / std::max<int64_t>(B, 1) / 512;
-  const bool few = likely <= std::min(rounds, !f32 && D == 256 ? 1.25 : 2.0) * (D == 256 ? 1 : 2) * rt->cus && quarters <= grid_max(256);
+  const double likely = (T / 32.0 + B / 2.0) * (double)Hq, mean = (double)T / std::max<int64_t>(B, 1);
+  const double rounds = !f32 && D > 64 ? std::min(0.4 + mean / 800, 1.05) : std::min(0.75 + mean / 512, 2.0);
+  const bool few = likely <= rounds * (D == 256 ? 1 : 2) * rt->cus && quarters <= grid_max(256);
   const size_t tiles = (size_t)(2 * 4 * 32 * 2) * (size_t)D;  // K and V of 128 keys
   char kname[48];
   std::snprintf(kname, sizeof kname, "rxw8_packed_%s_%s_d%d", few ? "quarters" : "prefill",

@@ -284,9 +284,10 @@ def test_prefill_plans(lib):
             continue
         kind = "f32" if qt == F32 else "bf16_f32" if ot == F32 else "bf16"
         heads = 4 if g % 4 == 0 else 2 if g % 2 == 0 else 1
-        rows = (64 if kind == "bf16" and d < 256 else 32) * (4 // heads)
+        rows = (64 if kind == "bf16" and d == 64 else 32) * (4 // heads)
         grid = (-(-t // rows) + b) * hkv * g // heads
-        rounds = min(0.75 + t / max(b, 1) / 512, 1.25 if kind == "bf16" and d == 256 else 2)
+        mean = t / max(b, 1)
+        rounds = min(0.4 + mean / 800, 1.05) if kind == "bf16" and d > 64 else min(0.75 + mean / 512, 2)
         few = (t / 32 + b / 2) * hkv * g <= rounds * (1 if d == 256 else 2) * 256
         assert name == "rxw8_packed_%s_%s_d%d" % ("quarters" if few else "prefill", kind, d)
         assert got[-1][1] == ((-(-t // 32) + b) * hkv * g if few else grid)
