@@ -143,13 +143,15 @@ struct Row {
   int64_t V;
   float top;         // the maximum
   double inv;        // log2(e) / T
+  double span;       // the largest z of the words in bins
   double per_bin;    // bins per unit of z
   double unit;       // 2^s
   double far;        // z from which on words weigh nothing
   float floor;       // words below it are not asked for: they come after top_k, or min_p, alone
 
   __device__ double z(float v) const { return ((double)top - (double)v) * inv; }
-  // (the nearest whole number, in the low bits of a sum with 1.5 2^52)
+  // (zv at most span, else what this gives means nothing and indexes nothing: the nearest whole
+  // number, in the low bits of a sum with 1.5 2^52)
   __device__ int bin(double zv) const {
     return min((int)(uint32_t)__builtin_bit_cast(u64, fma(zv, per_bin, 0x1.8p52)), kBins - 1);
   }
@@ -470,7 +472,8 @@ __device__ Borders borders_of(SampleShared &sh, const Row &r, const Settings &s)
     kept_hi = min(kept_hi, mass_end(pb1));
   }
   if (s.m > 0.f) {
-    mb = s.m >= 1.f ? 0 : r.bin(fmin(-log2((double)s.m), r.far));
+    // (min_p's border may lie far behind the last word: bins are as fine as the row's span is short)
+    mb = s.m >= 1.f ? 0 : r.bin(fmin(-log2((double)s.m), r.span));
     kept_lo = min(kept_lo, sh.mass[max(mb - 1, 0)]);
     kept_hi = min(kept_hi, mass_end(min(mb + 1, kBins - 1)));
   }
@@ -700,8 +703,8 @@ __device__ bool set_row(const SampleArgs &a, int64_t row, const SampleExtremes &
     r.floor = fmaxf(r.floor, sample_value(max(sample_key((float)((double)r.top - z / r.inv)) - 2, sample_key(lowest))));
   }
   // bins over what weighs something, and no further than the row goes
-  const double span = fmin(r.z(fmaxf(e.least, r.floor)), r.far);
-  r.per_bin = span > 0.0 ? (double)(kBins - 1) / span : 0.0;
+  r.span = fmin(r.z(fmaxf(e.least, r.floor)), r.far);
+  r.per_bin = r.span > 0.0 ? (double)(kBins - 1) / r.span : 0.0;
   return true;
 }
 // Whether this workgroup is the row's last to arrive; what all have stored past the dies' caches

@@ -1,0 +1,69 @@
+"""The serving operators at the ends of their inputs' range, against the 64-bit forms."""
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from test_gpu_serving import check_sample, sample
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- sampling ---------------------------------------------------------------------
+
+def check_min_p(rt, z, u, k, m, p=None):
+    """check_sample at temperature 1, with min_p's words told by their logits: exp(-d) >= m where d <= -log m.
+    (exp(-d) is below 1 for every d > 0, but 1 in 64 bits from d = 2^-54 down, so that ref.sample takes
+    such words for ties of the first at m = 1.)"""
+    want = []
+    for row, top_k in zip(z, k):
+        order = np.lexsort((np.arange(row.size), -row))
+        order = order[:top_k] if 0 < top_k < row.size else order
+        d = np.float64(row[order[0]]) - row[order].astype(np.float64)
+        mass = np.cumsum(np.exp(-d))
+        n = order.size if p is None else int(np.searchsorted(mass, np.float64(np.float32(p)) * mass[-1])) + 1
+        n = max(1, min(n, int((d <= -np.log(np.float64(np.float32(m)))).sum())))
+        want.append(int(order[np.searchsorted(mass[:n], min(np.float32(u), 1 - 2.0 ** -24) * mass[n - 1], side="right")]))
+        if m < 1:  # (the two forms are one)
+            assert want[-1] == ref.sample(row, np.float32(u), None, top_k, None if p is None else np.float32(p), np.float32(m))
+    n = len(z)
+    got = sample(rt, z, np.full(n, u, np.float32), k=k, m=[m] * n, p=None if p is None else [p] * n)
+    assert got.tolist() == want, (u, m, p)
+
+def short_spans(v):
+    """Rows whose words to choose from are two that lie close together: the others are at -inf, or out of
+    top_k's reach."""
+    rng = np.random.default_rng(v)
+    step = lambda x: np.nextafter(np.float32(x), np.float32(-np.inf))  # noqa: E731
+    pairs = [(1.0, step(1.0)), (10.0, step(10.0)), (-7.5, step(-7.5)), (1e-30, 0.0), (0.0, -1e-30), (1e-42, 0.0),
+             (1e30, step(1e30)), (3.0, 3.0 - 1e-5), (0.0, -1e-3)]
+    rows, ks = [], []
+    for a, b in pairs:
+        near = np.full(v, -np.inf, np.float32)
+        near[rng.permutation(v)[:2]] = a, b
+        deep = np.where(near > -np.inf, near, np.float32(min(a, b) - abs(a) - 20))
+        rows += [near, deep.astype(np.float32)]
+        ks += [0, 2]
+    return np.array(rows, np.float32), ks
+
+
+@pytest.mark.parametrize("v", [2, 5, 1030, 151936])
+def test_sample_min_p_over_a_short_span(rt, v):
+    """min_p's border far behind the last word that weighs anything; rows that one and several
+    workgroups share."""
+    z, ks = short_spans(v)
+    for u in (0.0, 0.3, 0.9, 1.0):
+        for m in (0.02, 0.05, 0.1, 0.5, 0.9999999):
+            check_min_p(rt, z, u, ks, m)
+            check_min_p(rt, z, u, ks, m, p=0.7)
+
+
+@pytest.mark.parametrize("v", [3, 1030, 151936])
+@pytest.mark.parametrize("t", [1e4, 1e7, 1e30, 3e38])
+def test_sample_min_p_at_high_temperatures(rt, v, t):
+    rng = np.random.default_rng(v)
+    z = (2 * rng.standard_normal((6, v))).astype(np.float32)
+    z[3:, 0] = -np.inf
+    for u in (0.3, 0.9):
+        for m in (0.05, 0.5, 0.999):
+            for k in (0, 2, 7):
+                check_sample(rt, z, np.full(6, u, np.float32), t=[t] * 6, k=[k] * 6, m=[m] * 6)
