@@ -191,6 +191,9 @@ __device__ __forceinline__ double exp2_minus(const SampleShared &sh, double z) {
 __device__ __forceinline__ u64 units_of(const Row &r, double w) {
   return __builtin_bit_cast(u64, fma(w, r.unit, 0x1p52)) & 0xfffffffffffffull;
 }
+// Whether min_p = m > 0 leaves a word of weight w at z. (m = 1 leaves the first's ties alone, though w
+// rounds to 1 from z = 2^-53 down; the m below it is 1 - 2^-24.)
+__device__ __forceinline__ bool min_p_leaves(double m, double z, double w) { return m < 1.0 ? w >= m : m == 1.0 && z == 0.0; }
 // The mass of a word (0 from r.far on)
 __device__ __forceinline__ u64 units_at(const SampleShared &sh, const Row &r, float v) {
   const double z = r.z(v);
@@ -373,11 +376,11 @@ __device__ int32_t draw_from_row(SampleShared &sh, const Row &r, const Settings 
     }
   };
   auto word = [&](auto f) { each_of_row([&](bool here, float v, uint32_t) { f(here, sample_key(v), units_at(sh, r, v)); }); };
-  auto sum = [&](double least) {  // of the words with w >= least
+  auto sum = [&](double min_p) {  // of the words that min_p leaves (0: all)
     u64 m = 0;
     each_word(r.words, r.bf16, 0, r.V, [&](float v, uint32_t) {
       const double z = r.z(v), w = z < r.far ? exp2_minus(sh, z) : 0.0;
-      if (w >= least) m += units_of(r, w);
+      if (!(min_p > 0.0) || min_p_leaves(min_p, z, w)) m += units_of(r, w);
     });
     for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o);
     __syncthreads();
@@ -542,11 +545,11 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
     while (wide < n) wide <<= 1;
     u64 word = 0, one = 0, before = 0;
     uint32_t rank = 0;
-    double w = 0.0;
+    double z = 0.0, w = 0.0;
     int b = -1;
     if (tid < n) {
       word = sh.list[tid];
-      const double z = r.z(sample_value((uint32_t)(word >> 32)));
+      z = r.z(sample_value((uint32_t)(word >> 32)));
       b = r.bin(z), w = exp2_minus(sh, z), one = units_of(r, w);
       sh.bin[tid] = (uint16_t)b, sh.unit[tid] = one;
       ahead[tid] = sh.mass[b], ranks[tid] = sh.count[b];
@@ -583,7 +586,7 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
       kept = min(kept, at);
     }
     if (mb >= 0) {
-      u64 sum = tid < n && abs(b - mb) <= 1 && w >= (double)s.m ? one : 0;
+      u64 sum = tid < n && abs(b - mb) <= 1 && min_p_leaves((double)s.m, z, w) ? one : 0;
       for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
       if (lane == 0) sh.wave_mass[wave] = sum;
       __syncthreads();
@@ -637,7 +640,7 @@ __device__ int32_t draw(SampleShared &sh, const Row &r, const Settings &s, const
     u64 sum = 0;
     for (int i = tid; i < n; i += kThreads) {
       const double z = r.z(sample_value((uint32_t)(sh.list[i] >> 32))), w = exp2_minus(sh, z);
-      if (abs(r.bin(z) - mb) <= 1 && w >= (double)s.m) sum += units_of(r, w);
+      if (abs(r.bin(z) - mb) <= 1 && min_p_leaves((double)s.m, z, w)) sum += units_of(r, w);
     }
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     __syncthreads();

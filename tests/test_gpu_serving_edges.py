@@ -57,6 +57,27 @@ def test_sample_min_p_over_a_short_span(rt, v):
             check_min_p(rt, z, u, ks, m, p=0.7)
 
 
+@pytest.mark.parametrize("v", [2, 5, 1030, 151936])
+def test_sample_min_p_of_one(rt, v):
+    """min_p = 1 leaves the first word and its ties, however near the next ones come; above 1 the first alone."""
+    z, ks = short_spans(v)
+    for u in (0.0, 0.3, 0.9, 1.0):
+        for m in (1.0, 1.0000001, 7.0):
+            check_min_p(rt, z, u, ks, m)
+            check_min_p(rt, z, u, ks, m, p=0.7)
+
+
+@pytest.mark.parametrize("v", [60, 3000, 30000, 151936])
+def test_sample_min_p_of_one_among_many(rt, v):
+    """The same with hundreds and thousands of words a hair below the first's ties."""
+    rng = np.random.default_rng(v)
+    near = np.where(rng.random(v) < 0.3, 1e-30, rng.uniform(0, 1e-30, v))
+    z = np.stack([near, -near, np.where(rng.random(v) < 0.9, near, -5.0)]).astype(np.float32)
+    for u in (0.0, 0.4, 0.9):
+        for k in (0, 50, v - 1):
+            check_min_p(rt, z, u, [k] * 3, 1.0)
+
+
 @pytest.mark.parametrize("v", [3, 1030, 151936])
 @pytest.mark.parametrize("t", [1e4, 1e7, 1e30, 3e38])
 def test_sample_min_p_at_high_temperatures(rt, v, t):
