@@ -76,10 +76,11 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a)
 // and run QT = 1, from 128 on a CU alone (two spill: 480 us for 4 of 2048 rows, 32 / 8 heads of
 // 128, 382 so: 0.36 PFLOP/s, each product counted once).
 //
-// m is the maximum of the row's first 32 keys and does not move: weights may grow past 1
-// as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l or O leaves that
-// range, or meets values that are no numbers (a key that a row does not see has weight 0,
-// and 0 times an infinity is none), are done again, key by key, by the wave alone.
+// m is the maximum of the row's first 32 keys (0 where these are at -inf) and does not move:
+// weights may grow past 1 as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l
+// or O leaves that range, whose l shows that weights were lost below it, or that meet values that
+// are no numbers (a key that a row does not see has weight 0, and 0 times an infinity is none),
+// are done again, key by key, by the wave alone.
 // (the lambdas below hold the wave's registers: they have to be part of the kernel)
 #define RXW8_INLINE __attribute__((always_inline))
 
@@ -117,6 +118,9 @@ __device__ __forceinline__ void unrolled(F f) {
 }
 
 constexpr int kStep = 32;  // keys
+// A row's least sum of weights: those 2^-42 of its largest and the three bf16 parts of these
+// are normal numbers
+constexpr float kLeastSum = 0x1p-60f;
 
 // The row tile of the given rank, those that see the most keys first: its index in its
 // sequence, whose first row and length these are (-1: there are not that many)
@@ -523,7 +527,7 @@ __device__ void packed_prefill(const PackedArgs &a) {
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       const float sum = sum_xor32(l[t]), inv = sum == 0.f ? 0.f : 1.0f / sum;
-      odd = fmaf(sum, 0.f, odd);
+      odd = sum < kLeastSum ? 1.f : fmaf(sum, 0.f, odd);
       const uint32_t row = mem + (32 * t + col) * OB;
 #pragma unroll
       for (int d = 0; d < ND; ++d)

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import serving_ref as ref
-from test_gpu_serving import check_sample, sample
+from test_gpu_serving import P_STEP, STEP, check, check_sample, packed, prompts, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,32 @@ def test_sample_min_p_at_high_temperatures(rt, v, t):
         for m in (0.05, 0.5, 0.999):
             for k in (0, 2, 7):
                 check_sample(rt, z, np.full(6, u, np.float32), t=[t] * 6, k=[k] * 6, m=[m] * 6)
+
+
+# ---- packed prompts ---------------------------------------------------------------
+
+TYPES = [(64, "bf16", "bf16"), (128, "bf16", "bf16"), (256, "bf16", "bf16"), (64, "f32", "f32"), (128, "f32", "f32"),
+         (256, "f32", "f32"), (128, "f32", "bf16"), (256, "bf16", "f32"), (80, "f32", "f32")]
+
+
+@pytest.mark.parametrize("copies", [1, 60])
+@pytest.mark.parametrize("d,qk,out", TYPES)
+def test_packed_prefill_first_keys_that_weigh_nothing(rt, d, qk, out, copies):
+    """Scores of -inf over a sequence's first 32 (and 64) keys and far below 0 after them: the others' softmax
+    all the same, whichever kernel takes the rows. A row with nothing but -inf is 0."""
+    rng = np.random.default_rng(d)
+    q, k, v, offsets = prompts(rng, [130, 40, 100], 2, 1, d, qk)
+    q[..., :2] = 1.0
+    k[..., 1] = -256.0  # (times the scale and log2 e: some -133, -185 and -259)
+    dead = {0: 32, 130: 32, 170: 64}
+    for a, n in dead.items():
+        k[a:a + n, :, 0] = -np.inf
+    for scale in (0.36, 0.5, 0.7):
+        y = packed(rt, q, qk, k, v, offsets, out, scale=scale, copies=copies)
+        for a, e in zip(offsets, offsets[1:]):
+            first = a + dead[int(a)]
+            assert not y[a:first].any()
+            for row in range(first, e):
+                for h in range(2):
+                    want, bound = ref.attend(q[row, h], k[first:row + 1, 0], v[first:row + 1, 0], scale, P_STEP[out], STEP[out])
+                    check(y[row, h], want, bound)
