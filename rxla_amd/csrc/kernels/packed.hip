@@ -589,9 +589,10 @@ RXW8_PACKED_PREFILL(256, 1, 3, 3, 1, f32)
 // products with the one before are done; S, its softmax with a running maximum, and O
 // follow one another. At the end the four (m, l, O) are joined in LDS, in the order of the
 // waves. (16 heads of 128 over 8, one prompt of 500 rows: 10.5 us, 13.7 on the tiles above; of
-// 1000: 16.2 and 21.9.) Rows that do not come out as numbers are done again as above. QL: the third parts of
-// an f32 q stay in LDS, where the registers do not hold them (at D = 256 O takes 128, two
-// parts of q as many).
+// 1000: 16.2 and 21.9.) Rows that do not come out as numbers are done again as above, and so are
+// those whose weights were lost (c s is rounded for the maximum and not for the weights, from
+// 2^31 on by more than their exponents hold). QL: the third parts of an f32 q stay in LDS, where
+// the registers do not hold them (at D = 256 O takes 128, two parts of q as many).
 template <int D, int PQ, int P, bool QL = PQ == 3 && D == 256>
 __device__ void packed_quarters(const PackedArgs &a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [4][K, V of 32 rows], then [4][32] (m, l), a flag, q's third parts
@@ -779,7 +780,7 @@ __device__ void packed_quarters(const PackedArgs &a) {
       for (int e = 0; e < 4; ++e) y[e] = fmaf(f, z[e], y[e]);
     }
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    odd = fmaf(L, 0.f, odd);
+    odd = L < kLeastSum ? 1.f : fmaf(L, 0.f, odd);
 #pragma unroll
     for (int e = 0; e < 4; ++e) odd = fmaf(y[e], 0.f, odd), y[e] *= inv;
     if (r0 + row < len) {

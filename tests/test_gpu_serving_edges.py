@@ -117,3 +117,28 @@ def test_packed_prefill_first_keys_that_weigh_nothing(rt, d, qk, out, copies):
                 for h in range(2):
                     want, bound = ref.attend(q[row, h], k[first:row + 1, 0], v[first:row + 1, 0], scale, P_STEP[out], STEP[out])
                     check(y[row, h], want, bound)
+
+
+@pytest.mark.parametrize("copies", [1, 60])
+@pytest.mark.parametrize("d,qk,out", TYPES)
+def test_packed_prefill_scores_past_the_exponent(rt, d, qk, out, copies):
+    """Scores of 10^10, where half a step of f32 is past the exponents of a weight: each row's largest takes
+    it all (the next is thousands below; a score is off by (d + 4) 2^-24 of its products)."""
+    rng = np.random.default_rng(d)
+    q, k, v, offsets = prompts(rng, [1, 1, 1, 1, 30, 40, 100], 2, 1, d, qk)
+    q, k = q * np.float32(2 ** 17), k * np.float32(2 ** 17)
+    y = packed(rt, q, qk, k, v, offsets, out, copies=copies)
+    step = P_STEP[out] + STEP[out] + 8 * ref.F32
+    seen = 0
+    for a, e in zip(offsets, offsets[1:]):
+        for row in range(a, e):
+            for h in range(2):
+                s = k[a:row + 1, 0].astype(np.float64) @ q[row, h].astype(np.float64) / np.sqrt(d)
+                size = (np.abs(k[a:row + 1, 0].astype(np.float64)) @ np.abs(q[row, h].astype(np.float64))).max() / np.sqrt(d)
+                top = np.sort(s)[::-1]
+                if s.size > 1 and top[0] - top[1] < 1000 + 4 * (d + 4) * ref.F32 * size:
+                    continue
+                seen += 1
+                want = v[a + int(np.argmax(s)), 0].astype(np.float64)
+                check(y[row, h], want, step * np.abs(want))
+    assert seen > 300
