@@ -335,7 +335,8 @@ __device__ void paged_decode(const PagedDecodeArgs &a) {
   const int hk = blockIdx.x % heads, unit = blockIdx.x / heads, h = hk / HT, ht = hk - h * HT;
   const int gt = min(16, G - 16 * ht), hq0 = h * G + 16 * ht;
   const int most = a.M * a.ps;
-  auto tiles_of = [&](int len) { return (min(max(len, 0), most) + T::KT - 1) / T::KT; };
+  // (unsigned: a length may be near 2^31)
+  auto tiles_of = [&](int len) { return (int)(((unsigned)min(max(len, 0), most) + T::KT - 1) / T::KT); };
 
   // the head's run: total tiles, and (up to 64 sequences) where each begins
   int total = 0, incl = 0, mine = 0;

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import serving_ref as ref
-from test_gpu_serving import P_STEP, STEP, check, check_sample, packed, prompts, sample
+from test_gpu_serving import P_STEP, STEP, check, check_sample, decode, floats, packed, prompts, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +142,20 @@ def test_packed_prefill_scores_past_the_exponent(rt, d, qk, out, copies):
                 want = v[a + int(np.argmax(s)), 0].astype(np.float64)
                 check(y[row, h], want, step * np.abs(want))
     assert seen > 300
+
+
+# ---- paged decode -----------------------------------------------------------------
+
+def test_paged_decode_lengths_up_to_the_last_position(rt):
+    """A table of 2^31 - 16 positions, most of them without a page, and lengths in its last tile."""
+    rng, ps = np.random.default_rng(0), 8176
+    entries = (2 ** 31 - 16) // ps
+    assert entries * ps == 2 ** 31 - 16
+    lens = [2 ** 31 - 1, 2 ** 31 - 31, 100, 0, 2 ** 31 - 32]
+    table = np.full((5, entries), -1, np.int32)
+    table[0, [0, 1000, entries - 1]] = 2, 0, 1
+    table[1, entries - 1], table[2, 0], table[4, entries - 1] = 0, 1, 2
+    q = floats(rng, (5, 4, 64), "f32")
+    kp, vp = (floats(rng, (3, 1, ps, 64), "bf16") for _ in range(2))
+    y = decode(rt, q, "f32", kp, vp, "bf16", table, lens)
+    check(y, *ref.paged_decode(q, kp, vp, table, lens))
