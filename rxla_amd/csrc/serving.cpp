@@ -147,8 +147,8 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
 }
 
 static float softmax_scale(float scale, int64_t D) {
-  // (at least 1e-30, below which every key weighs the same: -inf times it stays -inf)
-  return std::max((scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f, 1e-30f);
+  // (above 0 for every scale, so that -inf times it stays -inf)
+  return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f;
 }
 
 // The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import serving_ref as ref
-from test_gpu_serving import P_STEP, STEP, check, check_sample, decode, floats, packed, prompts, sample
+from test_gpu_serving import P_STEP, STEP, check, check_sample, decode, floats, make_pages, packed, prompts, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,37 @@ def test_paged_decode_lengths_up_to_the_last_position(rt):
     kp, vp = (floats(rng, (3, 1, ps, 64), "bf16") for _ in range(2))
     y = decode(rt, q, "f32", kp, vp, "bf16", table, lens)
     check(y, *ref.paged_decode(q, kp, vp, table, lens))
+
+
+# ---- scales -------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d,pk", [(64, "bf16"), (128, "f32"), (256, "bf16"), (80, "f32")])
+def test_small_scales(rt, d, pk):
+    """A scale of 2^-120 d^-1/2 over scores that are 2^120 times as large is an ordinary softmax."""
+    rng = np.random.default_rng(d)
+    big, scale = np.float32(2.0 ** 60), float(np.float32(d ** -0.5)) * 2.0 ** -120
+    lens = [70, 1, 200]
+    q = floats(rng, (3, 4, d), "f32") * big
+    kp, vp, table = make_pages(rng, lens, 2, 16, d, pk)
+    y = decode(rt, q, "f32", kp * big, vp, pk, table, lens, scale=scale)
+    check(y, *ref.paged_decode(q, kp * big, vp, table, lens, scale=scale))
+    for copies in (1, 60):
+        q, k, v, offsets = prompts(rng, [40, 100], 2, 1, d, "f32")
+        y = packed(rt, q * big, "f32", k * big, v, offsets, scale=scale, copies=copies)
+        check(y, *ref.packed_prefill(q * big, k * big, v, offsets, scale=scale))
+
+
+@pytest.mark.parametrize("d,pk", [(64, "bf16"), (128, "f32"), (256, "bf16"), (80, "f32")])
+def test_the_least_scale(rt, d, pk):
+    """Under the least f32 above 0 every key that a row sees weighs the same, and no other any."""
+    rng, scale = np.random.default_rng(d), float(np.finfo(np.float32).smallest_subnormal)
+    lens = [70, 1, 200, 0]
+    q = floats(rng, (4, 4, d), "f32")
+    kp, vp, table = make_pages(rng, lens, 2, 16, d, pk)
+    table[0, 1] = -1
+    y = decode(rt, q, "f32", kp, vp, pk, table, lens, scale=scale)
+    check(y, *ref.paged_decode(q, kp, vp, table, lens, scale=scale))
+    for copies in (1, 60):
+        q, k, v, offsets = prompts(rng, [40, 100], 2, 1, d, "f32")
+        y = packed(rt, q, "f32", k, v, offsets, scale=scale, copies=copies)
+        check(y, *ref.packed_prefill(q, k, v, offsets, scale=scale))
