@@ -306,9 +306,10 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages,
 /* rxw8_gqa_decode over a paged cache: q [B,Hq,D] F32|BF16, Hq % Hkv == 0,
  * lens I32 [B]: sequence b sees positions 0 .. lens[b] - 1 (clamped into
  * [0, M ps]) that have a page. Query head h reads kv head h / (Hq/Hkv);
- * scale <= 0 selects 1/sqrt(D); D <= 512. out [B,Hq,D] F32|BF16; the rows of a
- * sequence that sees no key are 0. What positions that are not seen hold (NaN
- * included) does not matter. The forms allocate nothing but `out`. */
+ * scale <= 0 selects 1/sqrt(D), another one is at most 2^127; D <= 512.
+ * out [B,Hq,D] F32|BF16; the rows of a sequence that sees no key are 0. What
+ * positions that are not seen hold (NaN included) does not matter. The forms
+ * allocate nothing but `out`. */
 int rxw8_gqa_decode_paged(rxw8_runtime *rt, rxw8_buffer *q,
                           rxw8_buffer *k_pages, rxw8_buffer *v_pages,
                           rxw8_buffer *table, rxw8_buffer *lens, float scale,
@@ -323,9 +324,8 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q,
  * [T,Hkv,D] BF16, Hq % Hkv == 0, D <= 512. offsets I32 [B+1] (device, not
  * decreasing; values are clamped into [0, T]): sequence b owns rows
  * offsets[b] .. offsets[b+1] - 1, none if they are equal, and its row t sees
- * rows offsets[b] .. t. scale <= 0 selects 1/sqrt(D). out [T,Hq,D] F32|BF16:
- * rows outside every sequence are 0 in a new buffer and left as they were by
- * _into. */
+ * rows offsets[b] .. t. scale as above. out [T,Hq,D] F32|BF16: rows outside
+ * every sequence are 0 in a new buffer and left as they were by _into. */
 int rxw8_gqa_prefill_packed(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k,
                             rxw8_buffer *v, rxw8_buffer *offsets, float scale,
                             int out_dtype, rxw8_buffer **out);

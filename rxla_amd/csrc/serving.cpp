@@ -107,6 +107,18 @@ static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, con
   return RXW8_OK;
 }
 
+constexpr float kScaleLog2e = 1.4426950408889634f;
+static float softmax_scale(float scale, int64_t D) {
+  // (above 0 for every scale, so that -inf times it stays -inf)
+  return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * kScaleLog2e;
+}
+static int check_scale(float scale) {
+  if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
+  if (scale > 0.f && !std::isfinite(scale * kScaleLog2e))
+    return fail(RXW8_INVALID_ARGUMENT, "attention scale %g times log2(e) must be finite", (double)scale);
+  return RXW8_OK;
+}
+
 static int check_paged_decode(const Buffer *q, const Buffer *kp, const Buffer *vp, const Buffer *table,
                               const Buffer *lens, float scale) {
   if (!q || !kp || !vp || !table || !lens) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: NULL buffer");
@@ -119,7 +131,7 @@ static int check_paged_decode(const Buffer *q, const Buffer *kp, const Buffer *v
   if (Hq <= 0 || Hq % kp->dims[1] != 0)
     return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
   if (!is_vec(lens, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: lens must be I32 [B]");
-  if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
+  if (int rc = check_scale(scale)) return rc;
   if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: head dim %lld > 512", (long long)D);
   if (Hq > INT32_MAX || B > grid_max(256) / Hq)
     return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: %lld x %lld rows exceed the kernel's grid", (long long)B,
@@ -138,17 +150,12 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
     return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
   if (offsets->dtype != RXW8_I32 || offsets->rank != 1 || offsets->dims[0] < 1)
     return fail(RXW8_INVALID_ARGUMENT, "packed GQA prefill: offsets must be I32 [sequences + 1]");
-  if (!std::isfinite(scale)) return fail(RXW8_INVALID_ARGUMENT, "attention scale must be finite");
+  if (int rc = check_scale(scale)) return rc;
   if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: head dim %lld > 512", (long long)D);
   if (T > INT32_MAX || Hq > INT32_MAX || T > 4 * grid_max(256) / Hq || offsets->dims[0] > INT32_MAX)
     return fail(RXW8_UNIMPLEMENTED, "packed GQA prefill: %lld x %lld rows exceed the kernel's grid", (long long)T,
                 (long long)Hq);
   return RXW8_OK;
-}
-
-static float softmax_scale(float scale, int64_t D) {
-  // (above 0 for every scale, so that -inf times it stays -inf)
-  return (scale <= 0.f ? 1.0f / std::sqrt((float)D) : scale) * 1.4426950408889634f;
 }
 
 // The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row
