@@ -118,6 +118,9 @@ __device__ __forceinline__ void unrolled(F f) {
 }
 
 constexpr int kStep = 32;  // keys
+// The fragments' LDS addresses are formed by XOR within a row: dynamic LDS begins at a multiple of
+// the longest, whatever static LDS comes before it
+constexpr int kLdsAlign = 512;
 // A row's least sum of weights: those 2^-42 of its largest and the three bf16 parts of these
 // are normal numbers
 constexpr float kLeastSum = 0x1p-60f;
@@ -181,8 +184,9 @@ __device__ __forceinline__ void rows_again(const PackedArgs &a, int D, float *qs
 // the rings have three places: V is then copied a step later.
 template <int D, int QT, int PQ, int P, bool QL = PQ == 3 && D == 256>
 __device__ void packed_prefill(const PackedArgs &a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [RING][32][D] K, the same V; q's third parts
+  extern __shared__ __attribute__((aligned(kLdsAlign))) uint16_t lds[];  // [RING][32][D] K, the same V; q's third parts
   constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 4096;  // copies of a wave per tile
+  static_assert(ROWB <= kLdsAlign, "rows begin at multiples of their size");
   constexpr int RING = QL ? 3 : 4, QR = QL ? PQ - 1 : PQ;                         // parts of q in registers
   constexpr int NK = D / 16, ND = D / 32, WR = 32 * QT;                            // WR: rows of a wave
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -595,8 +599,9 @@ RXW8_PACKED_PREFILL(256, 1, 3, 3, 1, f32)
 // the registers do not hold them (at D = 256 O takes 128, two parts of q as many).
 template <int D, int PQ, int P, bool QL = PQ == 3 && D == 256>
 __device__ void packed_quarters(const PackedArgs &a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t lds[];  // [4][K, V of 32 rows], then [4][32] (m, l), a flag, q's third parts
+  extern __shared__ __attribute__((aligned(kLdsAlign))) uint16_t lds[];  // [4][K, V of 32 rows], then [4][32] (m, l), a flag, q's third parts
   constexpr int ROWB = 2 * D, CH = D / 8, TILE = kStep * ROWB, NI = TILE / 1024, NK = D / 16, ND = D / 32;
+  static_assert(ROWB <= kLdsAlign, "rows begin at multiples of their size");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 31, hf = lane >> 5;
   const int hq = blockIdx.x % a.Hq, kvh = hq / (a.Hq / a.Hkv);
