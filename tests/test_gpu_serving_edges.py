@@ -193,3 +193,59 @@ def test_the_least_scale(rt, d, pk):
         q, k, v, offsets = prompts(rng, [40, 100], 2, 1, d, "f32")
         y = packed(rt, q, "f32", k, v, offsets, scale=scale, copies=copies)
         check(y, *ref.packed_prefill(q, k, v, offsets, scale=scale))
+
+
+# ---- what f32 keeps -----------------------------------------------------------------
+
+def cut(x, parts):
+    """x >= 0 as the kernels' bf16 parts: cut ones and a rounded last one."""
+    rest, total = np.asarray(x, np.float32), np.zeros(np.shape(x))
+    for _ in range(parts - 1):
+        high = ((np.maximum(rest.view(np.uint32), 1) - 1) & 0xffff0000).astype(np.uint32).view(np.float32)
+        rest, total = rest - high, total + high
+    return total + ref.bf16_value(ref.bf16_bits(rest))
+
+
+def attend_exact(q, k, v, scale, weights=lambda w: w):
+    """A row [D] with one element that is not 0: its scores are one product each, of three parts (two sums
+    round). Scores within S of 0 and c cost a difference of two 4 2^-24 S for the sums, 2 2^-24 S for c and as
+    much for its own rounding; a quotient takes twice that. Then n weights in a sum, their exponentials and
+    the division."""
+    s = (k.astype(np.float64) @ q.astype(np.float64)) * scale
+    w = np.exp(s - s.max())
+    y = weights(w) @ v / w.sum()
+    rel = np.expm1(16 * ref.F32 * np.abs(s).max()) + (s.size + 8) * ref.F32
+    return y, rel * (w @ np.abs(v)) / w.sum() + ref.F32 * np.abs(y)
+
+
+@pytest.mark.parametrize("copies", [1, 60])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_f32_rows_keep_24_bits(rt, d, copies):
+    """An f32 q enters whole and an f32 output takes whole weights, on the matrix cores too: two bf16 parts
+    of either would pass the bound (which the same test shows)."""
+    rng = np.random.default_rng(d)
+    counts, scale = [8] * 12, 0.5
+    q, k, v, offsets = prompts(rng, counts, 2, 1, d, "f32")
+    at = rng.integers(0, d, q.shape[:2])
+    one = np.zeros_like(q)
+    np.put_along_axis(one, at[..., None], rng.uniform(4, 16, at.shape + (1,)).astype(np.float32), 2)
+    packed_y = packed(rt, one, "f32", k, v, offsets, scale=scale, copies=copies)
+    # the last rows' queries over the same keys, one page a sequence
+    last, kp, vp = offsets[1:] - 1, np.zeros((12, 1, 16, d), np.float32), np.zeros((12, 1, 16, d), np.float32)
+    for b, a in enumerate(offsets[:-1]):
+        kp[b, 0, :8], vp[b, 0, :8] = k[a:a + 8, 0], v[a:a + 8, 0]
+    table = np.arange(12, dtype=np.int32)[:, None]
+    paged_y = [decode(rt, one[last], "f32", kp, vp, pk, table, [8] * 12, scale=scale) for pk in ("bf16", "f32")]
+    over = {"q": 0, "weights": 0}
+    for b, a in enumerate(offsets[:-1]):
+        for row in range(a, a + 8):
+            for h in range(2):
+                keys, vals = k[a:row + 1, 0], v[a:row + 1, 0].astype(np.float64)
+                want, bound = attend_exact(one[row, h], keys, vals, scale)
+                check(packed_y[row, h], want, bound)
+                if row == last[b]:
+                    for y in paged_y:
+                        check(y[b, h], want, bound)
+                    over["q"] += (np.abs(attend_exact(cut(one[row, h], 2), keys, vals, scale)[0] - want) > bound).any()
+                    over["weights"] += (np.abs(attend_exact(one[row, h], keys, vals, scale, lambda w: cut(w, 2))[0] - want) > bound).any()
+    assert over["q"] > 0 and over["weights"] > 0, over
