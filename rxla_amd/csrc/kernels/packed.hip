@@ -68,19 +68,23 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_packed_fill(PackedArgs a)
 // products, and these by a share of the softmax, in that order (a barrier to the
 // scheduler keeps it). bf16 q and outputs of 128 run QT = 1 with two workgroups to a CU,
 // whose prologues and stores pass under the other's products: 12 prompts of 64 to 2000 rows, 32 / 8
-// heads, take 124 us so and 136 with QT = 2 on a CU alone, though there the LDS reads take half
+// heads, take 114 us so and 126 with QT = 2 on a CU alone, though there the LDS reads take half
 // the time of the products (one fragment of K or V serves 32 QT rows); of 5000 and 7000 rows, 64 /
-// 8 heads, 1113 (1.09 PFLOP/s) and 1129. At 64 QT = 2 leaves registers for two workgroups all the
+// 8 heads, 1137 (1.07 PFLOP/s) and 1166. At 64 QT = 2 leaves registers for two workgroups all the
 // same (78 us for 4 of 2048 rows, 82 with QT = 1 and four). At 256 O alone is 128 registers: QT = 1
 // and one workgroup. f32 ones split q and P in their three bf16 parts (exact products, f32 sums)
 // and run QT = 1, from 128 on a CU alone (two spill: 480 us for 4 of 2048 rows, 32 / 8 heads of
-// 128, 382 so: 0.36 PFLOP/s, each product counted once).
+// 128, 382 so: 0.36 PFLOP/s, each product counted once). Behind a bf16 output the weights are one
+// bf16 part, rounded by 2^-8 at most, as the output itself is, their sum taken before that: a second
+// part would add half of all products again. The outputs of the two sets of prompts above are 2.0e-3
+// and 2.1e-3 of their norm off the 64-bit ones, 1.6e-3 where the output alone is rounded.
 //
 // m is the maximum of the row's first 32 keys (0 where these are at -inf) and does not move:
 // weights may grow past 1 as far as f32 and bf16 go (2^127), and O / l is the same. Rows whose l
 // or O leaves that range, whose l shows that weights were lost below it, or that meet values that
 // are no numbers (a key that a row does not see has weight 0, and 0 times an infinity is none),
-// are done again, key by key, by the wave alone.
+// are done again, key by key, by the wave alone: right, but slow (the 12 prompts above with an
+// infinite value in the 41st row of one, which all its rows after that see: 2.2 ms).
 // (the lambdas below hold the wave's registers: they have to be part of the kernel)
 #define RXW8_INLINE __attribute__((always_inline))
 

@@ -26,9 +26,10 @@
 // there is no list), one where each has its own. What bounds a batch is reading the
 // logits, once from memory and once or twice more from the caches; a row without a list
 // takes an exponential in f64 and an LDS atomic or two for each word besides. 64 rows of
-// 248320 f32 words: 47 us with top_k 200 (1.35 TB/s of logits read once: 22 us the maxima,
-// 14 the list, 11 the joins and launches), 70 without. A single row of 151936 is bound by
-// the length of the chain: 27 us, a third of it the words.
+// 248320 f32 words: 46 to 49 us with top_k 200 (1.3 TB/s of logits read once; by themselves 17 us
+// the maxima, 30 the list and what follows, 4 the last launch, which finds nothing to do), 76 to 92
+// without a filter, 99 to 109 with top_p alone. A single row of 151936 is bound by the length of
+// the chain: 26 us, of it 9, 17 and 4 by themselves.
 #include <stddef.h>
 
 #include "common.h"

@@ -210,8 +210,8 @@ static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Bu
   // Few rows: the kernel whose waves share a row's keys, 32 rows of one head to a workgroup, two
   // of them on a CU (one at D = 256). It needs no more rounds of workgroups than pay for steps
   // done a quarter at a time, by the sequences' mean length: 3/4 and one more for each 512 rows,
-  // at most 2; or, where bf16 tiles run two workgroups to a CU or D = 256, 2/5 and one more for
-  // each 800, at most 1.05. In us, the tiles above and that one. 16 heads of 128, bf16: 8 x 100
+  // at most 2; or, for bf16 rows of 128 (whose tiles run two workgroups to a CU) and of 256, 2/5 and
+  // one more for each 800, at most 1.05. In us, the tiles above and that one. 16 heads of 128, bf16: 8 x 100
   // rows 8.1, 8.6; 1 x 300 10.6, 9.4; 4 x 300 11.4, 16.6; 1 x 1000 21.9, 16.2; 2 x 1000 23.7, 27.8;
   // f32: 1 x 2000 78.3, 69.5; 4 x 500 27.9, 32.5. 16 of 256, f32: 1 x 1000 68.3, 59.9;
   // 1 x 1100 73.7, 78.3; 3 x 100 18.1, 16.7; 4 x 150 21.6, 29.3; bf16: 1 x 500 21.8, 19.1;
