@@ -125,8 +125,8 @@ constexpr int kStep = 32;  // keys
 // The fragments' LDS addresses are formed by XOR within a row: dynamic LDS begins at a multiple of
 // the longest, whatever static LDS comes before it
 constexpr int kLdsAlign = 512;
-// A row's least sum of weights: those 2^-42 of its largest and the three bf16 parts of these
-// are normal numbers
+// A row's least sum of weights: with 2^20 keys, weights down to 2^-24 of the largest and the
+// third bf16 parts of these (2^-16 below) are normal numbers
 constexpr float kLeastSum = 0x1p-60f;
 
 // The row tile of the given rank, those that see the most keys first: its index in its
