@@ -319,6 +319,69 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q,
                                rxw8_buffer *table, rxw8_buffer *lens,
                                float scale, rxw8_buffer *out);
 
+/* ---- 8-bit pages ------------------------------------------------------------
+ * k_pages/v_pages U8 [P,Hkv,ps,D] with k_scales/v_scales F32 [P,Hkv,ps]: a row x
+ * [D] of a kv head is held by the W8 encoder's rule (rxw8_quantize_w8 with groups
+ * of D), s = max(amax |x|, 1e-12) / 127 and codes clamp(rne(x / s), -127, 127) +
+ * 128, and stands for (code - 128) s. A row that holds a NaN or an infinity gets
+ * the scale NaN and the codes 128: all of it stands for NaN. (127 s may round past
+ * f32's end where amax is its last value.) */
+
+/* rxw8_paged_kv_append into 8-bit pages (all four buffers are written). */
+int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages,
+                            rxw8_buffer *v_pages, rxw8_buffer *k_scales,
+                            rxw8_buffer *v_scales, rxw8_buffer *k,
+                            rxw8_buffer *v, rxw8_buffer *table,
+                            rxw8_buffer *starts, rxw8_buffer *offsets);
+
+/* The append's inverse, over pages of every type (BF16|F32 with NULL scales, U8
+ * with both): position starts[b] + i of sequence b goes to row offsets[b] + i of
+ * k, v [T,Hkv,D] BF16|F32 (new rows for rxw8_gqa_prefill_packed, say). Values of
+ * 8-bit rows are formed in f32; what k, v cannot hold is rounded to nearest even.
+ * Rows at positions without a page, negative ones and ones behind the table are
+ * 0; rows outside every sequence are left as they were. */
+int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages,
+                       rxw8_buffer *v_pages, rxw8_buffer *k_scales,
+                       rxw8_buffer *v_scales, rxw8_buffer *table,
+                       rxw8_buffer *starts, rxw8_buffer *offsets,
+                       rxw8_buffer *k, rxw8_buffer *v);
+
+/* rxw8_gqa_decode_paged over 8-bit pages: the attention over the values that the
+ * rows stand for, products and sums to f32 accuracy. */
+int rxw8_gqa_decode_paged_q8(rxw8_runtime *rt, rxw8_buffer *q,
+                             rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                             rxw8_buffer *k_scales, rxw8_buffer *v_scales,
+                             rxw8_buffer *table, rxw8_buffer *lens, float scale,
+                             int out_dtype, rxw8_buffer **out);
+int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q,
+                                  rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                                  rxw8_buffer *k_scales, rxw8_buffer *v_scales,
+                                  rxw8_buffer *table, rxw8_buffer *lens,
+                                  float scale, rxw8_buffer *out);
+
+/* rxw8_gqa_decode_paged where sequences share a prefix (a system prompt, a
+ * document, the prompt of several samples), whose keys and values are read once
+ * for all of them: sequences groups[n] .. groups[n+1] - 1 (groups I32 [N+1], not
+ * decreasing) see the first prefix_lens[n] (I32 [N]) positions of the page table
+ * prefixes[n] (I32 [N,MP]) and then their own: the first lens[b] of table[b].
+ * Sequences outside every group have no prefix. Pages of every type, in one
+ * pool: BF16|F32 with NULL scales, U8 with both. Lengths, missing pages, heads,
+ * scale and out as in rxw8_gqa_decode_paged. */
+int rxw8_gqa_decode_shared(rxw8_runtime *rt, rxw8_buffer *q,
+                           rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                           rxw8_buffer *k_scales, rxw8_buffer *v_scales,
+                           rxw8_buffer *prefixes, rxw8_buffer *prefix_lens,
+                           rxw8_buffer *groups, rxw8_buffer *table,
+                           rxw8_buffer *lens, float scale, int out_dtype,
+                           rxw8_buffer **out);
+int rxw8_gqa_decode_shared_into(rxw8_runtime *rt, rxw8_buffer *q,
+                                rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                                rxw8_buffer *k_scales, rxw8_buffer *v_scales,
+                                rxw8_buffer *prefixes, rxw8_buffer *prefix_lens,
+                                rxw8_buffer *groups, rxw8_buffer *table,
+                                rxw8_buffer *lens, float scale,
+                                rxw8_buffer *out);
+
 /* rxw8_gqa_prefill for whole prompts of different lengths packed one after
  * another, keys and values beside their queries: q [T,Hq,D] F32|BF16, k/v
  * [T,Hkv,D] BF16, Hq % Hkv == 0, D <= 512. offsets I32 [B+1] (device, not
@@ -342,6 +405,36 @@ int rxw8_gqa_prefill_packed_into(rxw8_runtime *rt, rxw8_buffer *q,
  * empty result. The same two kernels end every decoder step (greedy ids). */
 int rxw8_argmax(rxw8_runtime *rt, rxw8_buffer *x, int axis, int keep_dims,
                 rxw8_buffer **out);
+
+/* What is done to the logits ahead of sampling; a NULL buffer: off. */
+typedef struct rxw8_logits_options {
+  /* a row's history: tokens offsets[b] .. offsets[b+1] - 1 of I32 [T] (offsets I32
+   * [B+1], clamped into [0, T]; tokens outside [0, V) count for nothing), of which
+   * the first prompts[b] (I32 [B]) count for the repetition alone */
+  rxw8_buffer *tokens, *offsets, *prompts;
+  /* F32 [B]: the repetition's factor (one that is not above 0: off), what each
+   * occurrence takes, and what the first one takes */
+  rxw8_buffer *repetition, *frequency, *presence;
+  /* entries bias_offsets[b] .. bias_offsets[b+1] - 1 of I32 [E], F32 [E] (offsets
+   * I32 [B+1], clamped into [0, E]): bias[e] is added to the logit of bias_words[e],
+   * the last entry's where a word has several; words outside [0, V) are left out */
+  rxw8_buffer *bias_words, *bias, *bias_offsets;
+  /* I32 [R, (V+31)/32], bit v % 32 of element v / 32: word v is allowed; row b goes
+   * by mask mask_rows[b] (I32 [B]; none if outside [0, R)), or by mask b (NULL, R = B) */
+  rxw8_buffer *mask, *mask_rows;
+} rxw8_logits_options;
+
+/* Logits [B,V] F32|BF16 (V <= 2^24) adjusted in f32, row by row: a word of the
+ * history has z = z / repetition where z > 0, else z repetition; one that occurs n
+ * times behind the prompt z - frequency n - presence; then z + bias; and words that
+ * the mask lacks -inf, whatever they held. out [B,V] F32|BF16; _into may be given
+ * the logits themselves. */
+int rxw8_adjust_logits(rxw8_runtime *rt, rxw8_buffer *logits,
+                       const rxw8_logits_options *options, int out_dtype,
+                       rxw8_buffer **out);
+int rxw8_adjust_logits_into(rxw8_runtime *rt, rxw8_buffer *logits,
+                            const rxw8_logits_options *options,
+                            rxw8_buffer *out);
 
 /* The next token of each row of logits [B,V] F32|BF16 (V <= 2^24) from a random
  * number in [0, 1), uniform F32 [B] (clamped into [0, 1 - 2^-24]; NaN counts as

@@ -10,7 +10,10 @@ names follow the reference's operator surface:
   in its decode form over a contiguous per-sequence cache
 * ``paged_kv_append``, ``grouped_query_attention_paged``,
   ``grouped_query_attention_packed``, ``sample`` -- serving over many sequences: a
-  paged cache, packed prompts, the next token (no counterpart in the reference)
+  paged cache, packed prompts, the next token (no counterpart in the reference);
+  ``paged_kv_append_q8``, ``paged_kv_read``, ``grouped_query_attention_paged_q8``
+  -- the cache in 8 bits; ``grouped_query_attention_shared`` -- over a prefix that
+  sequences share; ``adjust_logits`` -- penalties, biases and grammar masks
 * ``KvCache.update_at / update_at_checked`` -- crates/rxla-core/src/kv_cache.rs:53-111
 * ``DecoderModel.compile().bind_parameters(...).run(...)`` --
   ``AppliedModel::compile`` / ``CompiledModel::bind_parameters`` / ``BoundModel::run``
@@ -450,6 +453,66 @@ def grouped_query_attention_paged(rt: Runtime, q: Buffer, k_pages: Buffer, v_pag
     return Buffer(h)
 
 
+def paged_kv_append_q8(rt: Runtime, k_pages: Buffer, v_pages: Buffer, k_scales: Buffer,
+                       v_scales: Buffer, k: Buffer, v: Buffer, table: Buffer, starts: Buffer,
+                       offsets: Buffer | None = None):
+    """``paged_kv_append`` into pages of 8-bit codes U8 [P, Hkv, ps, D] with a scale for
+    each row, F32 [P, Hkv, ps] (``quantize_w8`` with groups of D). Returns all four."""
+    o = offsets.handle if offsets is not None else None
+    _check(_lib.rxw8_paged_kv_append_q8(rt.handle, k_pages.handle, v_pages.handle, k_scales.handle,
+                                        v_scales.handle, k.handle, v.handle, table.handle,
+                                        starts.handle, o))
+    return k_pages, v_pages, k_scales, v_scales
+
+
+def paged_kv_read(rt: Runtime, k_pages: Buffer, v_pages: Buffer, table: Buffer, starts: Buffer,
+                  offsets: Buffer | None, k: Buffer, v: Buffer, k_scales: Buffer | None = None,
+                  v_scales: Buffer | None = None):
+    """Rows back out of their pages (of 8-bit codes with both scales): position
+    starts[b] + i of sequence b to row offsets[b] + i of k, v [T, Hkv, D], 0 where it
+    has no page. Returns k, v."""
+    o = offsets.handle if offsets is not None else None
+    ks, vs = (s.handle if s is not None else None for s in (k_scales, v_scales))
+    _check(_lib.rxw8_paged_kv_read(rt.handle, k_pages.handle, v_pages.handle, ks, vs, table.handle,
+                                   starts.handle, o, k.handle, v.handle))
+    return k, v
+
+
+def grouped_query_attention_paged_q8(rt: Runtime, q: Buffer, k_pages: Buffer, v_pages: Buffer,
+                                     k_scales: Buffer, v_scales: Buffer, table: Buffer,
+                                     lens: Buffer, scale: float | None = None,
+                                     out_dtype=DType.F32, out: Buffer | None = None) -> Buffer:
+    """``grouped_query_attention_paged`` over 8-bit pages and their rows' scales."""
+    s = 0.0 if scale is None else float(scale)
+    bufs = [b.handle for b in (q, k_pages, v_pages, k_scales, v_scales, table, lens)]
+    if out is not None:
+        _check(_lib.rxw8_gqa_decode_paged_q8_into(rt.handle, *bufs, s, out.handle))
+        return out
+    h = c_void_p()
+    _check(_lib.rxw8_gqa_decode_paged_q8(rt.handle, *bufs, s, int(out_dtype), byref(h)))
+    return Buffer(h)
+
+
+def grouped_query_attention_shared(rt: Runtime, q: Buffer, k_pages: Buffer, v_pages: Buffer,
+                                   prefixes: Buffer, prefix_lens: Buffer, groups: Buffer,
+                                   table: Buffer, lens: Buffer, k_scales: Buffer | None = None,
+                                   v_scales: Buffer | None = None, scale: float | None = None,
+                                   out_dtype=DType.F32, out: Buffer | None = None) -> Buffer:
+    """``grouped_query_attention_paged`` where sequences groups[n] .. groups[n + 1] - 1
+    see the first prefix_lens[n] positions of the page table prefixes[n] before their own:
+    the prefix's keys and values are read once for all of them."""
+    s = 0.0 if scale is None else float(scale)
+    bufs = [b.handle if b is not None else None
+            for b in (q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups,
+                      table, lens)]
+    if out is not None:
+        _check(_lib.rxw8_gqa_decode_shared_into(rt.handle, *bufs, s, out.handle))
+        return out
+    h = c_void_p()
+    _check(_lib.rxw8_gqa_decode_shared(rt.handle, *bufs, s, int(out_dtype), byref(h)))
+    return Buffer(h)
+
+
 def grouped_query_attention_packed(rt: Runtime, q: Buffer, k: Buffer, v: Buffer, offsets: Buffer,
                                    scale: float | None = None, out_dtype=DType.F32,
                                    out: Buffer | None = None) -> Buffer:
@@ -464,6 +527,28 @@ def grouped_query_attention_packed(rt: Runtime, q: Buffer, k: Buffer, v: Buffer,
     h = c_void_p()
     _check(_lib.rxw8_gqa_prefill_packed(rt.handle, q.handle, k.handle, v.handle, offsets.handle,
                                         s, int(out_dtype), byref(h)))
+    return Buffer(h)
+
+
+def adjust_logits(rt: Runtime, logits: Buffer, tokens: Buffer | None = None,
+                  offsets: Buffer | None = None, prompts: Buffer | None = None,
+                  repetition: Buffer | None = None, frequency: Buffer | None = None,
+                  presence: Buffer | None = None, bias_words: Buffer | None = None,
+                  bias: Buffer | None = None, bias_offsets: Buffer | None = None,
+                  mask: Buffer | None = None, mask_rows: Buffer | None = None,
+                  out_dtype=None, out: Buffer | None = None) -> Buffer:
+    """Logits [B, V] with the penalties of each row's history, its biases and its grammar's
+    mask applied (None: off; see ``rxw8_logits_options``), for ``sample``. ``out`` may be
+    ``logits``; a new buffer has their dtype unless ``out_dtype`` says otherwise."""
+    given = (tokens, offsets, prompts, repetition, frequency, presence, bias_words, bias,
+             bias_offsets, mask, mask_rows)
+    options = _ffi.LogitsOptions(*[b.handle if b is not None else None for b in given])
+    if out is not None:
+        _check(_lib.rxw8_adjust_logits_into(rt.handle, logits.handle, byref(options), out.handle))
+        return out
+    h = c_void_p()
+    dtype = logits.dtype if out_dtype is None else out_dtype
+    _check(_lib.rxw8_adjust_logits(rt.handle, logits.handle, byref(options), int(dtype), byref(h)))
     return Buffer(h)
 
 
@@ -591,6 +676,7 @@ __all__ = ["Runtime", "Buffer", "DType", "Status", "Error", "quantize_w8", "dequ
            "grouped_query_attention_prefill", "grouped_query_attention_noalloc", "gqa_attention",
            "scaled_dot_product_attention", "causal_attention_mask", "causal_attention_mask_static",
            "argmax", "KvCache", "paged_kv_append", "grouped_query_attention_paged",
-           "grouped_query_attention_packed", "sample",
+           "grouped_query_attention_packed", "sample", "paged_kv_append_q8", "paged_kv_read",
+           "grouped_query_attention_paged_q8", "grouped_query_attention_shared", "adjust_logits",
            "SafeTensors",
            "DecoderConfig", "DecoderModel", "Qwen35Config", "Qwen35Model", "bf16_to_f32"]

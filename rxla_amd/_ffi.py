@@ -29,6 +29,9 @@ EXPORTS = [
     "rxw8_gqa_prefill", "rxw8_gqa_prefill_into", "rxw8_kv_update_at", "rxw8_argmax",
     "rxw8_paged_kv_append", "rxw8_gqa_decode_paged", "rxw8_gqa_decode_paged_into",
     "rxw8_gqa_prefill_packed", "rxw8_gqa_prefill_packed_into", "rxw8_sample", "rxw8_sample_into",
+    "rxw8_paged_kv_append_q8", "rxw8_paged_kv_read", "rxw8_gqa_decode_paged_q8",
+    "rxw8_gqa_decode_paged_q8_into", "rxw8_gqa_decode_shared", "rxw8_gqa_decode_shared_into",
+    "rxw8_adjust_logits", "rxw8_adjust_logits_into",
     "rxw8_safetensors_open", "rxw8_safetensors_close", "rxw8_safetensors_num_tensors",
     "rxw8_safetensors_tensor_info", "rxw8_safetensors_find", "rxw8_safetensors_metadata",
     "rxw8_safetensors_upload",
@@ -49,6 +52,12 @@ class DecoderConfig(Structure):
                 ("vocab", c_int64), ("max_batch", c_int64), ("max_seq", c_int64),
                 ("group", c_int64), ("eps", c_float), ("theta", c_float),
                 ("qk_norm", c_int32)]
+
+
+class LogitsOptions(Structure):
+    _fields_ = [(name, c_void_p) for name in
+                ("tokens", "offsets", "prompts", "repetition", "frequency", "presence",
+                 "bias_words", "bias", "bias_offsets", "mask", "mask_rows")]
 
 
 class Qwen35Config(Structure):
@@ -110,6 +119,14 @@ def _declare(L):
         "rxw8_gqa_prefill_packed_into": (c_int, [vp, vp, vp, vp, vp, c_float, vp]),
         "rxw8_sample": (c_int, [vp, vp, vp, vp, vp, vp, vp, POINTER(vp)]),
         "rxw8_sample_into": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp]),
+        "rxw8_paged_kv_append_q8": (c_int, [vp] * 10),
+        "rxw8_paged_kv_read": (c_int, [vp] * 10),
+        "rxw8_gqa_decode_paged_q8": (c_int, [vp] * 8 + [c_float, c_int, POINTER(vp)]),
+        "rxw8_gqa_decode_paged_q8_into": (c_int, [vp] * 8 + [c_float, vp]),
+        "rxw8_gqa_decode_shared": (c_int, [vp] * 11 + [c_float, c_int, POINTER(vp)]),
+        "rxw8_gqa_decode_shared_into": (c_int, [vp] * 11 + [c_float, vp]),
+        "rxw8_adjust_logits": (c_int, [vp, vp, POINTER(LogitsOptions), c_int, POINTER(vp)]),
+        "rxw8_adjust_logits_into": (c_int, [vp, vp, POINTER(LogitsOptions), vp]),
         "rxw8_safetensors_open": (c_int, [c_char_p, POINTER(vp)]),
         "rxw8_safetensors_close": (c_int, [vp]),
         "rxw8_safetensors_num_tensors": (c_int, [vp, i64p]),

@@ -47,14 +47,24 @@ __device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t (&part)[
   part[N - 1] = pack_bf16x2(a, b);
 }
 
+// Keys and values as they stand in memory: element i of the row at element offset `off`
+struct AnyPlain {
+  const void *k, *v;
+  bool f32;
+  __device__ __forceinline__ float key(int64_t off, int i) const { return any_load(k, off + i, f32); }
+  __device__ __forceinline__ float value(int64_t off, int i) const { return any_load(v, off + i, f32); }
+  __device__ __forceinline__ float key_scale(int64_t) const { return 1.f; }
+  __device__ __forceinline__ float value_scale(int64_t) const { return 1.f; }
+};
+
 // One wave over keys first, first + 1, .. in chunks of 64 (lane = key), the next
 // chunk `step` chunks on: s_j = c q.k_j (c = scale log2 e), online softmax,
 // acc += p v. row(j) is the element offset of key j's row (K and V alike), or
 // negative where the key is not seen; a key whose weight is zero adds nothing,
 // whatever its value holds. q: D floats in LDS.
-template <typename Row>
-__device__ void any_walk(AnyState &st, const float *q, const void *k, const void *v, bool kv_f32,
-                         int d, int64_t first, int64_t end, int step, float c, Row row) {
+template <typename KV, typename Row>
+__device__ void any_walk(AnyState &st, const float *q, KV kv, int d, int64_t first, int64_t end,
+                         int step, float c, Row row) {
   const int lane = threadIdx.x & 63;
   for (int64_t j0 = first; j0 < end; j0 += (int64_t)64 * step) {
     const int64_t j = j0 + lane;
@@ -62,8 +72,8 @@ __device__ void any_walk(AnyState &st, const float *q, const void *k, const void
     float s = kMinusInf;
     if (off >= 0) {
       float dot = 0.f;
-      for (int i = 0; i < d; ++i) dot = fmaf(q[i], any_load(k, off + i, kv_f32), dot);
-      s = dot * c;
+      for (int i = 0; i < d; ++i) dot = fmaf(q[i], kv.key(off, i), dot);
+      s = dot * kv.key_scale(off) * c;
     }
     // (fmaxf passes over a NaN; its weight below is NaN all the same)
     const float m_new = fmaxf(st.m, wave_max64(s));
@@ -73,16 +83,43 @@ __device__ void any_walk(AnyState &st, const float *q, const void *k, const void
     st.l = st.l * f + wave_sum64(p);
 #pragma unroll
     for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i) st.acc[i] *= f;
+    const float ps = p == 0.f ? 0.f : p * kv.value_scale(off);
     const int n = (int)(end - j0 < 64 ? end - j0 : 64);
     for (int t = 0; t < n; ++t) {
-      const float pt = __shfl(p, t);
+      const float pt = __shfl(ps, t);
       if (pt == 0.f) continue;
       const int64_t ot = __shfl(off, t);
 #pragma unroll
       for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i)
-        if (lane + 64 * i < d) st.acc[i] = fmaf(pt, any_load(v, ot + lane + 64 * i, kv_f32), st.acc[i]);
+        if (lane + 64 * i < d) st.acc[i] = fmaf(pt, kv.value(ot, lane + 64 * i), st.acc[i]);
     }
   }
+}
+template <typename Row>
+__device__ void any_walk(AnyState &st, const float *q, const void *k, const void *v, bool kv_f32,
+                         int d, int64_t first, int64_t end, int step, float c, Row row) {
+  any_walk(st, q, AnyPlain{k, v, kv_f32}, d, first, end, step, c, row);
+}
+
+// The states of a workgroup's 4 waves joined by the first one (true there) through
+// `part`, and `mw`, `lw`
+__device__ __forceinline__ bool any_join(AnyState &all, const AnyState &st, float (*part)[RXW8_ATTN_ANY_MAX_D],
+                                         float *mw, float *lw) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) mw[wave] = st.m, lw[wave] = st.l;
+#pragma unroll
+  for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i) part[wave][lane + 64 * i] = st.acc[i];
+  __syncthreads();
+  if (wave) return false;
+  float m = kMinusInf;
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, mw[w]);
+  for (int w = 0; w < 4; ++w) {
+    const float f = mw[w] == kMinusInf ? (lw[w] != lw[w] ? lw[w] : 0.f) : exp2f(mw[w] - m);
+    all.l += f * lw[w];
+#pragma unroll
+    for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i) all.acc[i] += f * part[w][lane + 64 * i];
+  }
+  return true;
 }
 
 // out[i] = acc / l; a row that saw no key (or only weights of zero) is 0

@@ -1,11 +1,8 @@
 // The paged key/value cache: the append that fills its pages and the attention of
-// one new token per sequence that reads them. Pages are [P, Hkv, ps, D] (a kv
-// head's ps rows of a page in one piece); table [B, M] I32 gives sequence b the
-// page of its positions ps i .. ps i + ps - 1 in entry i, anything outside [0, P)
-// where it has none. An entry is checked before its page is touched.
+// one new token per sequence that reads them.
 #include <type_traits>
 
-#include "attn_any.h"
+#include "paged.h"
 
 struct PagedAppendArgs {
   const void *k, *v;         // [T, Hkv, D] f32 | bf16
@@ -17,27 +14,6 @@ struct PagedAppendArgs {
   int B, M, Hkv, D, ps;
   int k_f32, p_f32;
 };
-
-// Row t of k and v: the page and the place in it (below 0: none) of the position
-// starts[b] + i, for row i of sequence b; rows outside every sequence and positions
-// without a page have none. By a whole wave, t uniform.
-struct PagedPlace {
-  int64_t page;
-  int at;
-};
-__device__ __forceinline__ PagedPlace paged_place(const PagedAppendArgs &a, int64_t t) {
-  int64_t b = t, i = 0;
-  if (a.offsets) {
-    b = any_sequence(a.offsets, a.B, t);
-    if (b < 0 || t >= a.offsets[b + 1]) return PagedPlace{-1, 0};
-    i = t - a.offsets[b];
-  }
-  const int64_t pos = a.starts[b] + i;
-  if (pos < 0 || pos >= (int64_t)a.M * a.ps) return PagedPlace{-1, 0};
-  const int slot = (int)(pos / a.ps);
-  const int64_t page = a.table[b * a.M + slot];
-  return PagedPlace{page < a.P ? page : -1, (int)(pos - (int64_t)slot * a.ps)};
-}
 
 // Any width and alignment: a wave for each (row, kv head), an element a lane (9000 bf16 rows of 8
 // heads of 100: 30 us, 1.9 TB/s).
@@ -127,29 +103,6 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_paged_append(PagedAppendA
     paged_append<uint16_t, uint16_t>(a);
 }
 
-struct PagedDecodeArgs {
-  const void *q;          // [B, Hq, D] f32 | bf16
-  const void *kp, *vp;    // [P, Hkv, ps, D] f32 | bf16
-  const int32_t *table;   // [B, M]
-  const int32_t *lens;    // [B]
-  void *out;              // [B, Hq, D] f32 | bf16
-  int64_t P;
-  int B, M, Hq, Hkv, D, ps;
-  float c;                // scale log2 e
-  int q_f32, p_f32, out_f32;
-  // the matrix-core kernels: `units` workgroups for each kv head and 16 of its
-  // query heads; counters [Hkv HT units], zero between launches, and two
-  // records of min(G, 16) (D + 4) floats each, padded to whole KiB
-  int units, waves;       // waves that walk keys (a workgroup has 8; the others help to join)
-  int *counters;
-  float *part;
-};
-
-__device__ __forceinline__ int64_t paged_len(const PagedDecodeArgs &a, int b) {
-  const int64_t n = a.lens[b], most = (int64_t)a.M * a.ps;
-  return n < 0 ? 0 : n > most ? most : n;
-}
-
 // Any head width up to 512, any page size: one workgroup of 4 waves per (sequence,
 // query head), the waves' chunks of 64 keys in turn, merged in LDS. Bound by its reads of a key a
 // lane, element by element (8 sequences of 512 to 8192 keys, 32 / 8 heads: 1.9 ms at a width of 96).
@@ -165,20 +118,8 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_paged_decode_any(PagedDec
     const int64_t page = a.table[(int64_t)b * a.M + j / a.ps];
     return page < 0 || page >= a.P ? -1 : ((page * a.Hkv + h) * a.ps + j % a.ps) * a.D;
   });
-  if (lane == 0) mw[wave] = st.m, lw[wave] = st.l;
-#pragma unroll
-  for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i) part[wave][lane + 64 * i] = st.acc[i];
-  __syncthreads();
-  if (wave) return;
-  float m = kMinusInf;
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, mw[w]);
   AnyState all;
-  for (int w = 0; w < 4; ++w) {
-    const float f = mw[w] == kMinusInf ? (lw[w] != lw[w] ? lw[w] : 0.f) : exp2f(mw[w] - m);
-    all.l += f * lw[w];
-#pragma unroll
-    for (int i = 0; i < RXW8_ATTN_ANY_MAX_D / 64; ++i) all.acc[i] += f * part[w][lane + 64 * i];
-  }
+  if (!any_join(all, st, part, mw, lw)) return;
   any_store(all, a.out, at, a.D, a.out_f32);
 }
 

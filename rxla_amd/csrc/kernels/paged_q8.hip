@@ -1,0 +1,113 @@
+// The paged cache in 8 bits: a row x [D] of a kv head is held as codes (int8 + 128) and
+// one f32 scale,
+//   s = max(amax |x|, 1e-12) / 127,  code = clamp(rne(x / s), -127, 127) + 128,
+// and stands for (code - 128) s: at most s / 2 off (1/254 of the row's largest), and the
+// same codes as rxw8_quantize_w8 with groups of D. A row that holds a NaN or an infinity
+// has the scale NaN and the codes 128: all of it stands for NaN. Here are the append that
+// writes such rows, the reading back of pages of any type, and the attention of one new
+// token per sequence over 8-bit pages.
+#include "paged.h"
+
+struct PagedQ8Args {
+  const void *k, *v;         // [T, Hkv, D] f32 | bf16
+  uint8_t *kp, *vp;          // [P, Hkv, ps, D]
+  float *ks, *vs;            // [P, Hkv, ps]
+  const int32_t *table;      // [B, M]
+  const int32_t *starts;     // [B]
+  const int32_t *offsets;    // [B + 1], or null: row b of sequence b
+  int64_t T, P;
+  int B, M, Hkv, D, ps;
+  int k_f32;
+};
+
+// The scale of a row from its largest magnitude (NaN: the row holds a NaN or an infinity)
+__device__ __forceinline__ float q8_scale(float amax) { return (amax >= 1e-12f ? amax : amax != amax ? amax : 1e-12f) / 127.0f; }
+__device__ __forceinline__ uint32_t q8_code(float x, float s) {
+  return s != s ? 128u : (uint32_t)(fminf(fmaxf(rintf(x / s), -127.0f), 127.0f) + 128.0f);
+}
+// |x| for a maximum by bits: NaN for what is no finite number, above every other
+__device__ __forceinline__ uint32_t q8_size(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return u >= 0x7f800000u ? 0x7fc00000u : u;
+}
+
+// Any width and alignment: a wave for each (row, kv head), an element a lane
+extern "C" __global__ void __launch_bounds__(256) rxw8_q8_append_any(PagedQ8Args a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= a.T * a.Hkv) return;  // whole waves only; no barriers below
+  const int64_t t = unit / a.Hkv;
+  const int h = (int)(unit - t * a.Hkv);
+  const PagedPlace to = paged_place(a, t);
+  if (to.page < 0) return;
+  const int64_t src = unit * a.D, row = (to.page * a.Hkv + h) * a.ps + to.at;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const void *x = kv ? a.v : a.k;
+    uint8_t *codes = (kv ? a.vp : a.kp) + row * a.D;
+    uint32_t top = 0;
+    for (int e = lane; e < a.D; e += 64) top = max(top, q8_size(any_load(x, src + e, a.k_f32)));
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+    const float s = q8_scale(__uint_as_float(top));
+    for (int e = lane; e < a.D; e += 64) codes[e] = (uint8_t)q8_code(any_load(x, src + e, a.k_f32), s);
+    if (lane == 0) (kv ? a.vs : a.ks)[row] = s;
+  }
+}
+
+struct PagedReadArgs {
+  const void *kp, *vp;       // [P, Hkv, ps, D] bf16 | f32 | u8
+  const float *ks, *vs;      // [P, Hkv, ps] (u8)
+  void *k, *v;               // [T, Hkv, D] f32 | bf16
+  const int32_t *table;      // [B, M]
+  const int32_t *starts;     // [B]
+  const int32_t *offsets;    // [B + 1], or null: row b of sequence b
+  int64_t T, P;
+  int B, M, Hkv, D, ps;
+  int kind;                  // 0 bf16, 1 f32, 2 u8 pages
+  int k_f32;
+};
+
+// Any width and alignment: a wave for each (row, kv head), an element a lane
+extern "C" __global__ void __launch_bounds__(256) rxw8_q8_read_any(PagedReadArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= a.T * a.Hkv) return;
+  const int64_t t = unit / a.Hkv;
+  const int h = (int)(unit - t * a.Hkv);
+  const PagedPlace of = paged_place(a, t);
+  if (of.at < 0) return;
+  const int64_t dst = unit * a.D, row = (of.page * a.Hkv + h) * a.ps + of.at;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const void *pages = kv ? a.vp : a.kp;
+    void *to = kv ? a.v : a.k;
+    const float s = of.page >= 0 && a.kind == 2 ? (kv ? a.vs : a.ks)[row] : 1.f;
+    for (int e = lane; e < a.D; e += 64) {
+      float y = 0.f;
+      if (of.page >= 0)
+        y = a.kind == 2 ? ((float)((const uint8_t *)pages)[row * a.D + e] - 128.f) * s : any_load(pages, row * a.D + e, a.kind);
+      if (a.k_f32) ((float *)to)[dst + e] = y;
+      else ((uint16_t *)to)[dst + e] = f32_to_bf16_bits(y);
+    }
+  }
+}
+
+// Any head width up to 512, any page size: one workgroup of 4 waves per (sequence, query
+// head), the waves' chunks of 64 keys in turn, merged in LDS
+extern "C" __global__ void __launch_bounds__(256) rxw8_q8_decode_any(PagedDecodeArgs a) {
+  __shared__ float q[RXW8_ATTN_ANY_MAX_D], part[4][RXW8_ATTN_ANY_MAX_D], mw[4], lw[4];
+  const int wave = threadIdx.x >> 6;
+  const int b = blockIdx.x / a.Hq, hq = blockIdx.x - b * a.Hq, h = hq / (a.Hq / a.Hkv);
+  const int64_t at = (int64_t)blockIdx.x * a.D;
+  for (int i = threadIdx.x; i < a.D; i += 256) q[i] = any_load(a.q, at + i, a.q_f32);
+  __syncthreads();
+  AnyState st;
+  any_walk(st, q, AnyCodes{(const uint8_t *)a.kp, (const uint8_t *)a.vp, a.ks, a.vs, a.D}, a.D, 64 * wave, paged_len(a, b), 4, a.c,
+           [&](int64_t j) -> int64_t {
+             const int64_t page = a.table[(int64_t)b * a.M + j / a.ps];
+             return page < 0 || page >= a.P ? -1 : ((page * a.Hkv + h) * a.ps + j % a.ps) * a.D;
+           });
+  AnyState all;
+  if (!any_join(all, st, part, mw, lw)) return;
+  any_store(all, a.out, at, a.D, a.out_f32);
+}

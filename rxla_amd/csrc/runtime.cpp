@@ -27,6 +27,9 @@ extern const unsigned char rxw8_co_qwen35[], rxw8_co_qwen35_end[];
 extern const unsigned char rxw8_co_paged[], rxw8_co_paged_end[];
 extern const unsigned char rxw8_co_packed[], rxw8_co_packed_end[];
 extern const unsigned char rxw8_co_sample[], rxw8_co_sample_end[];
+extern const unsigned char rxw8_co_paged_q8[], rxw8_co_paged_q8_end[];
+extern const unsigned char rxw8_co_shared[], rxw8_co_shared_end[];
+extern const unsigned char rxw8_co_logits[], rxw8_co_logits_end[];
 }
 
 namespace rxw8 {
@@ -99,7 +102,8 @@ static int module_of(const char *kname) {
                 {"rxw8_quantize_w8", 1},
                 {"rxw8_gqa_tile_", 7}, {"rxw8_gqa_quad_", 7}, {"rxw8_gqa_", 2},
                 {"rxw8_w8a16_gemm", 3}, {"rxw8_gemm_mid_", 8}, {"rxw8_gemm_", 3},   {"rxw8_dec_", 4},
-                {"rxw8_q35_", 5},          {"rxw8_paged_", 9},     {"rxw8_packed_", 10},    {"rxw8_sample_", 11}};
+                {"rxw8_q35_", 5},          {"rxw8_paged_", 9},     {"rxw8_packed_", 10},    {"rxw8_sample_", 11},
+                {"rxw8_q8_", 12},          {"rxw8_shared_", 13},   {"rxw8_logits_", 14}};
   for (const auto &r : routes)
     if (std::strncmp(kname, r.prefix, std::strlen(r.prefix)) == 0) return r.module;
   return -1;
@@ -353,7 +357,10 @@ int rxw8_runtime_create(int device, rxw8_runtime **out) {
                {"gemm_mid", rxw8_co_gemm_mid, rxw8_co_gemm_mid_end},
                {"paged", rxw8_co_paged, rxw8_co_paged_end},
                {"packed", rxw8_co_packed, rxw8_co_packed_end},
-               {"sample", rxw8_co_sample, rxw8_co_sample_end}};
+               {"sample", rxw8_co_sample, rxw8_co_sample_end},
+               {"paged_q8", rxw8_co_paged_q8, rxw8_co_paged_q8_end},
+               {"shared", rxw8_co_shared, rxw8_co_shared_end},
+               {"logits", rxw8_co_logits, rxw8_co_logits_end}};
   for (auto &blob : blobs) {  // order = module indices of module_of()
     if (blob.end - blob.begin <= 0) {
       for (hipModule_t mm : rt->modules) (void)hipModuleUnload(mm);

@@ -1,5 +1,6 @@
-// The serving operators: the paged key/value cache (append, decode attention),
-// causal attention of packed prompts, and sampling of the next token.
+// The serving operators: the paged key/value cache (append, reading back, decode
+// attention, over a shared prefix too; in 8 bits too), causal attention of packed
+// prompts, the logits' adjustments and sampling of the next token.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
@@ -9,7 +10,8 @@
 
 namespace rxw8 {
 
-// (the kernels' argument structs: kernels/paged.hip, packed.hip, sample.hip)
+// (the kernels' argument structs: kernels/paged.h, paged.hip, paged_q8.hip, shared.hip,
+// packed.hip, logits.hip, sample.hip)
 struct PagedAppendArgs {
   const void *k, *v;
   void *kp, *vp;
@@ -29,6 +31,50 @@ struct PagedDecodeArgs {
   int units, waves;
   int *counters;
   float *part;
+  const float *ks, *vs;
+};
+struct PagedQ8Args {
+  const void *k, *v;
+  uint8_t *kp, *vp;
+  float *ks, *vs;
+  const int32_t *table, *starts, *offsets;
+  int64_t T, P;
+  int B, M, Hkv, D, ps;
+  int k_f32;
+};
+struct PagedReadArgs {
+  const void *kp, *vp;
+  const float *ks, *vs;
+  void *k, *v;
+  const int32_t *table, *starts, *offsets;
+  int64_t T, P;
+  int B, M, Hkv, D, ps;
+  int kind;
+  int k_f32;
+};
+struct SharedArgs {
+  const void *q, *kp, *vp;
+  const float *ks, *vs;
+  const int32_t *prefixes, *prefix_lens, *groups, *table, *lens;
+  void *out;
+  int64_t P;
+  int B, N, MP, M, Hq, Hkv, D, ps;
+  float c;
+  int q_f32, kind, out_f32;
+};
+struct LogitsArgs {
+  const void *logits;
+  void *out;
+  const int32_t *tokens, *offsets, *prompts;
+  const float *repetition, *frequency, *presence;
+  const int32_t *bias_words;
+  const float *bias;
+  const int32_t *bias_offsets;
+  const uint32_t *mask;
+  const int32_t *mask_rows;
+  int64_t T, E, R, V;
+  int in_f32, out_f32;
+  int chunk, chunks;
 };
 struct PackedArgs {
   const void *q;
@@ -72,6 +118,8 @@ static bool same_shape(const Buffer *a, const Buffer *b) {
 // Workgroups of `threads` that one launch takes: 2^32 - 1 threads
 constexpr int64_t grid_max(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 constexpr int64_t kAnyMaxD = 512;  // RXW8_ATTN_ANY_MAX_D
+constexpr int64_t kLogitsChunk = 8192;
+static int page_kind(const Buffer *pages) { return pages->dtype == RXW8_U8 ? 2 : pages->dtype == RXW8_F32 ? 1 : 0; }
 
 // Whether the buffers (NULL ones aside) are the runtime's, and none of the first `written`
 // shares memory with another
@@ -90,20 +138,49 @@ static int check_buffers(const char *what, const Runtime *rt, std::initializer_l
   return RXW8_OK;
 }
 
-// Pages [P, Hkv, ps, D] F32|BF16 and the table I32 [B, M]
-static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, const Buffer *table) {
-  if (kp->rank != 4 || !is_f(kp->dtype) || !same_shape(kp, vp))
-    return fail(RXW8_INVALID_ARGUMENT, "%s: pages must be two F32/BF16 [P,Hkv,ps,D] of one shape and type", what);
-  if (kp->dims[1] <= 0 || kp->dims[2] <= 0 || kp->dims[3] <= 0)
-    return fail(RXW8_INVALID_ARGUMENT, "%s: pages %s need positive heads, rows and width", what, dims_str(kp).c_str());
+// A page table I32 [B, M] over pages of `ps` positions
+static int check_table(const char *what, const Buffer *table, int64_t ps) {
   if (table->dtype != RXW8_I32 || table->rank != 2)
     return fail(RXW8_INVALID_ARGUMENT, "%s: the page table must be I32 [B,M]", what);
+  // positions are I32
+  if (table->dims[0] > INT32_MAX || (table->dims[1] > 0 && ps > INT32_MAX / table->dims[1]))
+    return fail(RXW8_UNIMPLEMENTED, "%s: %lld pages of %lld positions exceed 32-bit positions", what,
+                (long long)table->dims[1], (long long)ps);
+  return RXW8_OK;
+}
+
+// Pages [P, Hkv, ps, D] F32|BF16, or U8 with scales F32 [P, Hkv, ps], and the table I32 [B, M]
+static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, const Buffer *table,
+                       const Buffer *ks = nullptr, const Buffer *vs = nullptr) {
+  const bool codes = ks || vs;
+  if (kp->rank != 4 || !(codes ? kp->dtype == RXW8_U8 : is_f(kp->dtype)) || !same_shape(kp, vp))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: pages must be two %s [P,Hkv,ps,D] of one shape and type", what,
+                codes ? "U8" : "F32/BF16");
+  if (kp->dims[1] <= 0 || kp->dims[2] <= 0 || kp->dims[3] <= 0)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: pages %s need positive heads, rows and width", what, dims_str(kp).c_str());
+  if (codes) {
+    bool ok = ks && vs && ks->dtype == RXW8_F32 && ks->rank == 3 && same_shape(ks, vs);
+    for (int i = 0; ok && i < 3; ++i) ok = ks->dims[i] == kp->dims[i];
+    if (!ok) return fail(RXW8_INVALID_ARGUMENT, "%s: 8-bit pages need two F32 [P,Hkv,ps] of scales", what);
+  }
   for (int i = 1; i < 4; ++i)
     if (kp->dims[i] > INT32_MAX) return fail(RXW8_UNIMPLEMENTED, "%s: pages %s", what, dims_str(kp).c_str());
-  // positions are I32
-  if (table->dims[0] > INT32_MAX || (table->dims[1] > 0 && kp->dims[2] > INT32_MAX / table->dims[1]))
-    return fail(RXW8_UNIMPLEMENTED, "%s: %lld pages of %lld positions exceed 32-bit positions", what,
-                (long long)table->dims[1], (long long)kp->dims[2]);
+  return check_table(what, table, kp->dims[2]);
+}
+
+// Rows k, v F32|BF16 [T, Hkv, D] of the pages' heads and width, their sequences' first
+// positions I32 [B] and the rows of each I32 [B + 1] (NULL: one each). A wave takes 128
+// pieces of 8 elements of a row, or a row of one head.
+static int check_rows(const char *what, const Buffer *kp, const Buffer *k, const Buffer *v, const Buffer *table,
+                      const Buffer *starts, const Buffer *offsets) {
+  if (k->rank != 3 || !is_f(k->dtype) || !same_shape(k, v) || k->dims[1] != kp->dims[1] || k->dims[2] != kp->dims[3])
+    return fail(RXW8_INVALID_ARGUMENT, "%s requires F32/BF16 k, v [T,Hkv,D] of the pages' heads and width", what);
+  const int64_t T = k->dims[0], B = table->dims[0], parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
+  if (!is_vec(starts, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "%s: starts must be I32 [B]", what);
+  if (offsets ? !is_vec(offsets, RXW8_I32, B + 1) : T != B)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: offsets must be I32 [B+1] (without them k, v hold one row a sequence)", what);
+  if (T > 4 * grid_max(256) / std::max(k->dims[1], parts))
+    return fail(RXW8_UNIMPLEMENTED, "%s: %lld rows exceed the kernel's grid", what, (long long)T);
   return RXW8_OK;
 }
 
@@ -119,24 +196,51 @@ static int check_scale(float scale) {
   return RXW8_OK;
 }
 
+static int check_decode(const char *what, const Buffer *q, const Buffer *kp, const Buffer *table, const Buffer *lens,
+                        float scale) {
+  if (q->rank != 3 || !is_f(q->dtype)) return fail(RXW8_INVALID_ARGUMENT, "%s requires F32/BF16 q [B,Hq,D]", what);
+  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (table->dims[0] != B || D != kp->dims[3])
+    return fail(RXW8_INVALID_ARGUMENT, "%s: q, page table and pages differ in batch or head width", what);
+  if (Hq <= 0 || Hq % kp->dims[1] != 0)
+    return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
+  if (!is_vec(lens, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "%s: lens must be I32 [B]", what);
+  if (int rc = check_scale(scale)) return rc;
+  if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "%s: head dim %lld > 512", what, (long long)D);
+  if (Hq > INT32_MAX || B > grid_max(256) / Hq)
+    return fail(RXW8_UNIMPLEMENTED, "%s: %lld x %lld rows exceed the kernel's grid", what, (long long)B, (long long)Hq);
+  return RXW8_OK;
+}
 static int check_paged_decode(const Buffer *q, const Buffer *kp, const Buffer *vp, const Buffer *table,
                               const Buffer *lens, float scale) {
   if (!q || !kp || !vp || !table || !lens) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: NULL buffer");
   if (int rc = check_pages("paged GQA decode", kp, vp, table)) return rc;
-  if (q->rank != 3 || !is_f(q->dtype))
-    return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode requires F32/BF16 q [B,Hq,D]");
-  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
-  if (table->dims[0] != B || D != kp->dims[3])
-    return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: q, page table and pages differ in batch or head width");
-  if (Hq <= 0 || Hq % kp->dims[1] != 0)
-    return fail(RXW8_INVALID_ARGUMENT, "GQA requires equal batch prefixes and divisible positive head counts");
-  if (!is_vec(lens, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged GQA decode: lens must be I32 [B]");
-  if (int rc = check_scale(scale)) return rc;
-  if (D > kAnyMaxD) return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: head dim %lld > 512", (long long)D);
-  if (Hq > INT32_MAX || B > grid_max(256) / Hq)
-    return fail(RXW8_UNIMPLEMENTED, "paged GQA decode: %lld x %lld rows exceed the kernel's grid", (long long)B,
-                (long long)Hq);
-  return RXW8_OK;
+  return check_decode("paged GQA decode", q, kp, table, lens, scale);
+}
+static int check_paged_decode_q8(const Buffer *q, const Buffer *kp, const Buffer *vp, const Buffer *ks, const Buffer *vs,
+                                 const Buffer *table, const Buffer *lens, float scale) {
+  const char *what = "8-bit paged GQA decode";
+  if (!q || !kp || !vp || !ks || !vs || !table || !lens) return fail(RXW8_INVALID_ARGUMENT, "%s: NULL buffer", what);
+  if (int rc = check_pages(what, kp, vp, table, ks, vs)) return rc;
+  return check_decode(what, q, kp, table, lens, scale);
+}
+static int check_shared(const Buffer *q, const Buffer *kp, const Buffer *vp, const Buffer *ks, const Buffer *vs,
+                        const Buffer *prefixes, const Buffer *prefix_lens, const Buffer *groups, const Buffer *table,
+                        const Buffer *lens, float scale) {
+  const char *what = "GQA decode over shared prefixes";
+  if (!q || !kp || !vp || !prefixes || !prefix_lens || !groups || !table || !lens)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: NULL buffer", what);
+  if (int rc = check_pages(what, kp, vp, table, ks, vs)) return rc;
+  if (int rc = check_table(what, prefixes, kp->dims[2])) return rc;
+  const int64_t N = prefixes->dims[0];
+  if (!is_vec(prefix_lens, RXW8_I32, N) || !is_vec(groups, RXW8_I32, N + 1))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: prefix_lens must be I32 [N] and groups I32 [N+1] for prefixes I32 [N,M]", what);
+  return check_decode(what, q, kp, table, lens, scale);
+}
+static bool is_output(const Buffer *out, const Buffer *q) {  // F32|BF16 of q's shape
+  bool ok = is_f(out->dtype) && out->rank == q->rank;
+  for (int i = 0; ok && i < q->rank; ++i) ok = out->dims[i] == q->dims[i];
+  return ok;
 }
 
 static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets, float scale) {
@@ -241,17 +345,8 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
     return fail(RXW8_INVALID_ARGUMENT, "paged KV append: NULL argument");
   if (int rc = check_pages("paged KV append", k_pages, v_pages, table)) return rc;
   if (k_pages == v_pages) return fail(RXW8_INVALID_ARGUMENT, "K and V pages must be distinct buffers");
-  if (k->rank != 3 || !is_f(k->dtype) || !same_shape(k, v) || k->dims[1] != k_pages->dims[1] ||
-      k->dims[2] != k_pages->dims[3])
-    return fail(RXW8_INVALID_ARGUMENT, "paged KV append requires F32/BF16 k, v [T,Hkv,D] of the pages' heads and width");
-  const int64_t T = k->dims[0], B = table->dims[0];
-  if (!is_vec(starts, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "paged KV append: starts must be I32 [B]");
-  if (offsets ? !is_vec(offsets, RXW8_I32, B + 1) : T != B)
-    return fail(RXW8_INVALID_ARGUMENT, "paged KV append: offsets must be I32 [B+1] (without them k, v hold one row a sequence)");
-  // a wave takes 128 pieces of 8 elements of a row, or a row of one head
-  const int64_t parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
-  if (T > 4 * grid_max(256) / std::max(k->dims[1], parts))
-    return fail(RXW8_UNIMPLEMENTED, "paged KV append: %lld rows exceed the kernel's grid", (long long)T);
+  if (int rc = check_rows("paged KV append", k_pages, k, v, table, starts, offsets)) return rc;
+  const int64_t T = k->dims[0], B = table->dims[0], parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
   if (int rc = check_buffers("paged KV append", rt, {k_pages, v_pages, k, v, table, starts, offsets}, 2)) return rc;
   if (T == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
@@ -278,7 +373,7 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_
   PagedDecodeArgs a{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
                     out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
                     (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32,
-                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32, 0, 0, nullptr, nullptr};
+                    k_pages->dtype == RXW8_F32, out->dtype == RXW8_F32, 0, 0, nullptr, nullptr, nullptr, nullptr};
   return paged_decode_launch(rt, a);
 }
 
@@ -329,6 +424,211 @@ int rxw8_gqa_prefill_packed(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k, rx
     return rc;
   }
   *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pages, rxw8_buffer *k_scales,
+                            rxw8_buffer *v_scales, rxw8_buffer *k, rxw8_buffer *v, rxw8_buffer *table,
+                            rxw8_buffer *starts, rxw8_buffer *offsets) {
+  const char *what = "8-bit paged KV append";
+  if (!rt || !k_pages || !v_pages || !k_scales || !v_scales || !k || !v || !table || !starts)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: NULL argument", what);
+  if (int rc = check_pages(what, k_pages, v_pages, table, k_scales, v_scales)) return rc;
+  if (k_pages == v_pages || k_scales == v_scales)
+    return fail(RXW8_INVALID_ARGUMENT, "K and V pages and scales must be distinct buffers");
+  if (int rc = check_rows(what, k_pages, k, v, table, starts, offsets)) return rc;
+  if (int rc = check_buffers(what, rt, {k_pages, v_pages, k_scales, v_scales, k, v, table, starts, offsets}, 4)) return rc;
+  const int64_t T = k->dims[0];
+  if (T == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  PagedQ8Args a{k->ptr, v->ptr, (uint8_t *)k_pages->ptr, (uint8_t *)v_pages->ptr, (float *)k_scales->ptr,
+                (float *)v_scales->ptr, (const int32_t *)table->ptr, (const int32_t *)starts->ptr,
+                offsets ? (const int32_t *)offsets->ptr : nullptr, T, k_pages->dims[0], (int)table->dims[0],
+                (int)table->dims[1], (int)k->dims[1], (int)k->dims[2], (int)k_pages->dims[2], k->dtype == RXW8_F32};
+  return launch(rt, "rxw8_q8_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+}
+
+int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pages, rxw8_buffer *k_scales,
+                       rxw8_buffer *v_scales, rxw8_buffer *table, rxw8_buffer *starts, rxw8_buffer *offsets,
+                       rxw8_buffer *k, rxw8_buffer *v) {
+  const char *what = "paged KV read";
+  if (!rt || !k_pages || !v_pages || !k || !v || !table || !starts)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: NULL argument", what);
+  if (int rc = check_pages(what, k_pages, v_pages, table, k_scales, v_scales)) return rc;
+  if (k == v) return fail(RXW8_INVALID_ARGUMENT, "%s: k and v must be distinct buffers", what);
+  if (int rc = check_rows(what, k_pages, k, v, table, starts, offsets)) return rc;
+  if (int rc = check_buffers(what, rt, {k, v, k_pages, v_pages, k_scales, v_scales, table, starts, offsets}, 2)) return rc;
+  const int64_t T = k->dims[0];
+  if (T == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  PagedReadArgs a{k_pages->ptr, v_pages->ptr, k_scales ? (const float *)k_scales->ptr : nullptr,
+                  v_scales ? (const float *)v_scales->ptr : nullptr, k->ptr, v->ptr, (const int32_t *)table->ptr,
+                  (const int32_t *)starts->ptr, offsets ? (const int32_t *)offsets->ptr : nullptr, T,
+                  k_pages->dims[0], (int)table->dims[0], (int)table->dims[1], (int)k->dims[1], (int)k->dims[2],
+                  (int)k_pages->dims[2], page_kind(k_pages), k->dtype == RXW8_F32};
+  return launch(rt, "rxw8_q8_read_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+}
+
+int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                                  rxw8_buffer *k_scales, rxw8_buffer *v_scales, rxw8_buffer *table, rxw8_buffer *lens,
+                                  float scale, rxw8_buffer *out) {
+  const char *what = "8-bit paged GQA decode";
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_paged_decode_q8(q, k_pages, v_pages, k_scales, v_scales, table, lens, scale)) return rc;
+  if (!is_output(out, q)) return fail(RXW8_INVALID_ARGUMENT, "%s output: shape or dtype mismatch", what);
+  if (int rc = check_buffers(what, rt, {out, q, k_pages, v_pages, k_scales, v_scales, table, lens}, 1)) return rc;
+  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (B == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  PagedDecodeArgs a{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
+                    out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
+                    (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32, 0, out->dtype == RXW8_F32,
+                    0, 0, nullptr, nullptr, (const float *)k_scales->ptr, (const float *)v_scales->ptr};
+  return launch(rt, "rxw8_q8_decode_any", dim3((unsigned)B * (unsigned)Hq), dim3(256), a);
+}
+
+int rxw8_gqa_decode_paged_q8(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                             rxw8_buffer *k_scales, rxw8_buffer *v_scales, rxw8_buffer *table, rxw8_buffer *lens,
+                             float scale, int out_dtype, rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_paged_decode_q8(q, k_pages, v_pages, k_scales, v_scales, table, lens, scale)) return rc;
+  if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA: out dtype must be F32 or BF16");
+  if (int rc = check_buffers("8-bit paged GQA decode", rt, {q, k_pages, v_pages, k_scales, v_scales, table, lens}, 0)) return rc;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *o = nullptr;
+  int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
+  if (rc) return rc;
+  rc = rxw8_gqa_decode_paged_q8_into(rt, q, k_pages, v_pages, k_scales, v_scales, table, lens, scale,
+                                     static_cast<rxw8_buffer *>(o));
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(o));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+int rxw8_gqa_decode_shared_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                                rxw8_buffer *k_scales, rxw8_buffer *v_scales, rxw8_buffer *prefixes,
+                                rxw8_buffer *prefix_lens, rxw8_buffer *groups, rxw8_buffer *table, rxw8_buffer *lens,
+                                float scale, rxw8_buffer *out) {
+  const char *what = "GQA decode over shared prefixes";
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_shared(q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups, table, lens, scale)) return rc;
+  if (!is_output(out, q)) return fail(RXW8_INVALID_ARGUMENT, "%s output: shape or dtype mismatch", what);
+  if (int rc = check_buffers(what, rt, {out, q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups, table, lens}, 1))
+    return rc;
+  const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
+  if (B == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  SharedArgs a{q->ptr, k_pages->ptr, v_pages->ptr, k_scales ? (const float *)k_scales->ptr : nullptr,
+               v_scales ? (const float *)v_scales->ptr : nullptr, (const int32_t *)prefixes->ptr,
+               (const int32_t *)prefix_lens->ptr, (const int32_t *)groups->ptr, (const int32_t *)table->ptr,
+               (const int32_t *)lens->ptr, out->ptr, k_pages->dims[0], (int)B, (int)prefixes->dims[0],
+               (int)prefixes->dims[1], (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
+               (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32, page_kind(k_pages),
+               out->dtype == RXW8_F32};
+  return launch(rt, "rxw8_shared_any", dim3((unsigned)B * (unsigned)Hq), dim3(256), a);
+}
+
+int rxw8_gqa_decode_shared(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
+                           rxw8_buffer *k_scales, rxw8_buffer *v_scales, rxw8_buffer *prefixes,
+                           rxw8_buffer *prefix_lens, rxw8_buffer *groups, rxw8_buffer *table, rxw8_buffer *lens,
+                           float scale, int out_dtype, rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_shared(q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups, table, lens, scale)) return rc;
+  if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "GQA: out dtype must be F32 or BF16");
+  if (int rc = check_buffers("GQA decode over shared prefixes", rt,
+                             {q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups, table, lens}, 0))
+    return rc;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *o = nullptr;
+  int rc = new_buffer(rt, out_dtype, q->dims, 3, false, &o);
+  if (rc) return rc;
+  rc = rxw8_gqa_decode_shared_into(rt, q, k_pages, v_pages, k_scales, v_scales, prefixes, prefix_lens, groups, table,
+                                   lens, scale, static_cast<rxw8_buffer *>(o));
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(o));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(o);
+  return RXW8_OK;
+}
+
+static int check_logits(const rxw8_logits_options *o, const Buffer *logits) {
+  const char *what = "logits adjustment";
+  if (!logits || !o) return fail(RXW8_INVALID_ARGUMENT, "%s: NULL argument", what);
+  if (logits->rank != 2 || !is_f(logits->dtype) || logits->dims[1] <= 0)
+    return fail(RXW8_INVALID_ARGUMENT, "%s requires F32/BF16 logits [B,V] with V > 0", what);
+  const int64_t B = logits->dims[0], V = logits->dims[1];
+  if (!o->tokens != !o->offsets || (!o->tokens && (o->prompts || o->repetition || o->frequency || o->presence)))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: prompts and penalties need tokens and their offsets", what);
+  if (o->tokens && (o->tokens->dtype != RXW8_I32 || o->tokens->rank != 1 || !is_vec(o->offsets, RXW8_I32, B + 1) ||
+                    (o->prompts && !is_vec(o->prompts, RXW8_I32, B))))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: tokens must be I32 [T], offsets I32 [B+1], prompts I32 [B]", what);
+  for (const rxw8_buffer *x : {o->repetition, o->frequency, o->presence})
+    if (x && !is_vec(x, RXW8_F32, B))
+      return fail(RXW8_INVALID_ARGUMENT, "%s: repetition, frequency and presence must be F32 [B]", what);
+  if (!o->bias != !o->bias_words || !o->bias != !o->bias_offsets)
+    return fail(RXW8_INVALID_ARGUMENT, "%s: biases need bias_words, bias and bias_offsets", what);
+  if (o->bias && (o->bias->rank != 1 || !is_vec(o->bias, RXW8_F32, o->bias->dims[0]) ||
+                  !is_vec(o->bias_words, RXW8_I32, o->bias->dims[0]) || !is_vec(o->bias_offsets, RXW8_I32, B + 1)))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: bias_words must be I32 [E], bias F32 [E], bias_offsets I32 [B+1]", what);
+  if (o->mask_rows && !o->mask) return fail(RXW8_INVALID_ARGUMENT, "%s: mask_rows need a mask", what);
+  if (o->mask && (o->mask->dtype != RXW8_I32 || o->mask->rank != 2 || o->mask->dims[1] != (V + 31) / 32 ||
+                  (o->mask_rows ? !is_vec(o->mask_rows, RXW8_I32, B) : o->mask->dims[0] != B)))
+    return fail(RXW8_INVALID_ARGUMENT, "%s: mask must be I32 [R,(V+31)/32] and mask_rows I32 [B] (without them R = B)", what);
+  if (V > ((int64_t)1 << 24)) return fail(RXW8_UNIMPLEMENTED, "%s: %lld words > 2^24", what, (long long)V);
+  for (const rxw8_buffer *x : {o->tokens, o->bias})
+    if (x && x->dims[0] > INT32_MAX)
+      return fail(RXW8_UNIMPLEMENTED, "%s: %lld entries exceed 32-bit offsets", what, (long long)x->dims[0]);
+  if (B > grid_max(512) / ((V + kLogitsChunk - 1) / kLogitsChunk))
+    return fail(RXW8_UNIMPLEMENTED, "%s: %lld rows exceed the kernel's grid", what, (long long)B);
+  return RXW8_OK;
+}
+
+int rxw8_adjust_logits_into(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_logits_options *o, rxw8_buffer *out) {
+  const char *what = "logits adjustment";
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_logits(o, logits)) return rc;
+  if (!is_output(out, logits)) return fail(RXW8_INVALID_ARGUMENT, "%s output: shape or dtype mismatch", what);
+  // (in place: each logit is read by the thread that writes it)
+  const bool in_place = out->ptr == logits->ptr && out->dtype == logits->dtype && out->rt == logits->rt;
+  if (int rc = check_buffers(what, rt, {out, in_place ? nullptr : logits, o->tokens, o->offsets, o->prompts, o->repetition,
+                                        o->frequency, o->presence, o->bias_words, o->bias, o->bias_offsets, o->mask, o->mask_rows}, 1))
+    return rc;
+  const int64_t B = logits->dims[0], V = logits->dims[1];
+  if (B == 0) return RXW8_OK;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  auto i32 = [](const rxw8_buffer *b) { return b ? (const int32_t *)b->ptr : nullptr; };
+  auto f32 = [](const rxw8_buffer *b) { return b ? (const float *)b->ptr : nullptr; };
+  LogitsArgs a{logits->ptr, out->ptr, i32(o->tokens), i32(o->offsets), i32(o->prompts), f32(o->repetition),
+               f32(o->frequency), f32(o->presence), i32(o->bias_words), f32(o->bias), i32(o->bias_offsets),
+               (const uint32_t *)i32(o->mask), i32(o->mask_rows), o->tokens ? o->tokens->dims[0] : 0,
+               o->bias ? o->bias->dims[0] : 0, o->mask ? o->mask->dims[0] : 0, V, logits->dtype == RXW8_F32,
+               out->dtype == RXW8_F32, (int)kLogitsChunk, (int)((V + kLogitsChunk - 1) / kLogitsChunk)};
+  return launch(rt, "rxw8_logits_adjust", dim3((unsigned)(B * a.chunks)), dim3(512), a,
+                sizeof(int) * (size_t)a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr)));
+}
+
+int rxw8_adjust_logits(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_logits_options *o, int out_dtype,
+                       rxw8_buffer **out) {
+  if (!rt || !out) return fail(RXW8_INVALID_ARGUMENT, "NULL argument");
+  if (int rc = check_logits(o, logits)) return rc;
+  if (!is_f(out_dtype)) return fail(RXW8_INVALID_ARGUMENT, "logits adjustment: out dtype must be F32 or BF16");
+  if (int rc = check_buffers("logits adjustment", rt, {logits, o->tokens, o->offsets, o->prompts, o->repetition, o->frequency, o->presence,
+                                                       o->bias_words, o->bias, o->bias_offsets, o->mask, o->mask_rows}, 0))
+    return rc;
+  std::lock_guard<std::recursive_mutex> g(rt->mu);
+  Buffer *y = nullptr;
+  int rc = new_buffer(rt, out_dtype, logits->dims, 2, false, &y);
+  if (rc) return rc;
+  rc = rxw8_adjust_logits_into(rt, logits, o, static_cast<rxw8_buffer *>(y));
+  if (rc) {
+    rxw8_buffer_release(static_cast<rxw8_buffer *>(y));
+    return rc;
+  }
+  *out = static_cast<rxw8_buffer *>(y);
   return RXW8_OK;
 }
 

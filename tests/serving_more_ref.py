@@ -1,0 +1,99 @@
+"""Plain 64-bit forms of the 8-bit cache, of attention behind shared prefixes and of
+the logits' adjustments. Attention's bounds are serving_ref's: an 8-bit value is
+(code - 128) s exactly, its score c s_k (q . codes) and its weight p s_v each take
+two roundings more, and joining the records of a row a few, which 8 half steps of
+f32 cover (`MORE`)."""
+import math
+
+import numpy as np
+
+import serving_ref as ref
+
+MORE = 8 * ref.F32
+
+
+def encode(x):
+    """Rows [..., D] f32 as (codes, scales), the encoder's rule in f32."""
+    x = np.asarray(x, np.float32)
+    with np.errstate(invalid="ignore", over="ignore"):
+        amax = np.abs(x).max(axis=-1)
+        s = np.maximum(amax, np.float32(1e-12)) / np.float32(127)
+        s = np.where(np.isfinite(amax), s, np.float32(np.nan)).astype(np.float32)
+        code = np.clip(np.rint(x / s[..., None]), -127, 127) + 128
+    return np.where(np.isnan(s)[..., None], 128, code).astype(np.uint8), s
+
+
+def value(codes, scales):
+    """What codes [..., D] and scales [...] stand for, in 64 bits."""
+    return (codes.astype(np.float64) - 128) * np.asarray(scales, np.float64)[..., None]
+
+
+def read(pages, table, starts, offsets, total):
+    """Rows [total, Hkv, D] of pages [P, Hkv, ps, D]; NaN outside every sequence."""
+    _, hkv, ps, d = pages.shape
+    out = np.full((total, hkv, d), np.nan)
+    for b, start in enumerate(starts):
+        for i, row in enumerate(range(max(offsets[b], 0), min(offsets[b + 1], total))):
+            pos, out[row] = int(start) + i + max(-offsets[b], 0), 0
+            if 0 <= pos and pos // ps < table.shape[1] and 0 <= table[b][pos // ps] < pages.shape[0]:
+                out[row] = pages[table[b][pos // ps], :, pos % ps]
+    return out
+
+
+def shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale=None, p_step=ref.SPLIT,
+           out_step=ref.F32):
+    """(y, bound) over pages of values."""
+    b, hq, d = q.shape
+    g = hq // kp.shape[1]
+    y, bound = np.zeros((b, hq, d)), np.zeros((b, hq, d))
+    for i in range(b):
+        for h in range(kp.shape[1]):
+            parts = [(table[i], lens[i])]
+            for n in range(len(prefixes)):
+                if groups[n] <= i < groups[n + 1]:
+                    parts.insert(0, (prefixes[n], prefix_lens[n]))
+            k, v = (np.concatenate([ref.paged_keys(x, t, max(0, int(n)), h) for t, n in parts])
+                    for x in (kp, vp))
+            for r in range(h * g, h * g + g):
+                y[i, r], bound[i, r] = ref.attend(q[i, r], k, v, scale or 1 / math.sqrt(d),
+                                                  p_step + MORE, out_step)
+    return y, bound
+
+
+def adjust(z, step, tokens=None, offsets=None, prompts=None, repetition=None, frequency=None,
+           presence=None, bias_words=None, bias=None, bias_offsets=None, mask=None, mask_rows=None):
+    """(y, bound): four roundings of f32 at most, each half a step of the largest value on the
+    way (the quotient, n frequency + presence, the difference, the sum), and the output's."""
+    y = np.asarray(z, np.float64).copy()
+    size = np.abs(np.where(np.isfinite(y), y, 0))
+    rows, vocab = y.shape
+    for b in range(rows):
+        if tokens is not None:
+            words = np.asarray(tokens[max(0, offsets[b]):max(0, offsets[b + 1])])
+            skip = max(0, int(prompts[b])) if prompts is not None else 0
+            good = (words >= 0) & (words < vocab)
+            count = np.bincount(words[skip:][good[skip:]], minlength=vocab)
+            seen = np.bincount(words[good], minlength=vocab) > 0
+            r = float(repetition[b]) if repetition is not None else 1.0
+            if r > 0:
+                with np.errstate(invalid="ignore"):
+                    y[b] = np.where(seen, np.where(y[b] > 0, y[b] / r, y[b] * r), y[b])
+            size[b] = np.maximum(size[b], np.abs(np.where(np.isfinite(y[b]), y[b], 0)))
+            off = (count * (float(frequency[b]) if frequency is not None else 0.0)
+                   + (count > 0) * (float(presence[b]) if presence is not None else 0.0))
+            y[b] -= off
+            size[b] += np.abs(off)
+        if bias is not None:
+            for e in range(max(0, bias_offsets[b]), min(max(0, bias_offsets[b + 1]), bias.size)):
+                w = int(bias_words[e])
+                later = [x for x in bias_words[e + 1:bias_offsets[b + 1]] if x == w]
+                if 0 <= w < vocab and not later:
+                    y[b, w] += float(bias[e])
+                    if np.isfinite(bias[e]):
+                        size[b, w] += abs(float(bias[e]))
+        m = -1 if mask is None else b if mask_rows is None else int(mask_rows[b])
+        if mask is not None and 0 <= m < mask.shape[0]:
+            bits = np.unpackbits(np.ascontiguousarray(mask[m]).view(np.uint8), bitorder="little")
+            y[b, bits[:vocab] == 0] = -np.inf
+    with np.errstate(invalid="ignore"):
+        return y, 4 * ref.F32 * size + step * np.where(np.isfinite(y), np.abs(y), 0) * 1.01 + 1e-30
