@@ -6,7 +6,7 @@
 // has the scale NaN and the codes 128: all of it stands for NaN. Here are the append that
 // writes such rows, the reading back of pages of any type, and the attention of one new
 // token per sequence over 8-bit pages.
-#include "paged.h"
+#include "paged_decode.h"
 
 struct PagedQ8Args {
   const void *k, *v;         // [T, Hkv, D] f32 | bf16
@@ -111,3 +111,11 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_q8_decode_any(PagedDecode
   if (!any_join(all, st, part, mw, lw)) return;
   any_store(all, a.out, at, a.D, a.out_f32);
 }
+
+#define RXW8_Q8_DECODE(D)                                                                     \
+  extern "C" __global__ void __launch_bounds__(64 * kPagedWaves) rxw8_q8_decode_d##D(PagedDecodeArgs a) { \
+    paged_decode<D, kCodes>(a, paged_place_of(a));                                            \
+  }
+RXW8_Q8_DECODE(64)
+RXW8_Q8_DECODE(128)
+RXW8_Q8_DECODE(256)

@@ -262,6 +262,16 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
   return RXW8_OK;
 }
 
+// PagedTile (kernels/paged_decode.h): a tile's keys, and the bytes of a wave's K, V and scales
+struct PagedTiles {
+  int keys, ring;
+  PagedTiles(int kind, int64_t D) {  // kind: page_kind
+    const int row = (int)D * (kind == 2 ? 1 : kind == 1 ? 4 : 2);
+    keys = kind == 2 ? (D == 64 ? 64 : 32) : row < 256 ? 32 : 16;
+    ring = 2 * keys * row + (kind == 2 ? 8 * keys : 0);
+  }
+};
+
 // The matrix-core kernels take head widths 64, 128 and 256, pages of whole 16-row
 // pieces, 16-byte aligned operands and tile counts within 32 bits; else the plain
 // kernel. As many waves walk keys, up to 8, as tiles and records of the group's heads
@@ -269,12 +279,12 @@ static int check_packed(const Buffer *q, const Buffer *k, const Buffer *v, const
 // leaves the fewest CUs idle in the last round.
 static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   const int64_t G = a.Hq / a.Hkv, heads = a.Hkv * ((G + 15) / 16), gcap = G < 16 ? G : 16;
-  const int es = a.p_f32 ? 4 : 2, row = a.D * es, tile = row < 256 ? 32 : 16;
+  const PagedTiles t(a.ks ? 2 : a.p_f32, a.D);
   if ((a.D != 64 && a.D != 128 && a.D != 256) || a.ps % 16 || a.P == 0 || heads > 4096 ||
       ((uintptr_t)a.q | (uintptr_t)a.kp | (uintptr_t)a.vp | (uintptr_t)a.out) % 16 ||
-      (int64_t)a.B * (((int64_t)a.M * a.ps + tile - 1) / tile) >= ((int64_t)1 << 30))
-    return launch(rt, "rxw8_paged_decode_any", dim3((unsigned)a.B * (unsigned)a.Hq), dim3(256), a);
-  const size_t record = (size_t)gcap * (size_t)(a.D + 4) * sizeof(float), wave = std::max((size_t)(2 * tile * row), record) + record;
+      (int64_t)a.B * (((int64_t)a.M * a.ps + t.keys - 1) / t.keys) >= ((int64_t)1 << 30))
+    return launch(rt, a.ks ? "rxw8_q8_decode_any" : "rxw8_paged_decode_any", dim3((unsigned)a.B * (unsigned)a.Hq), dim3(256), a);
+  const size_t record = (size_t)gcap * (size_t)(a.D + 4) * sizeof(float), wave = std::max((size_t)t.ring, record) + record;
   a.waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>({256, (int64_t)(RXW8_NOALLOC_COUNTER_BYTES / sizeof(int)) / heads,
                                                                (int64_t)(RXW8_NOALLOC_PARTIAL_BYTES / (2 * ((record + 1023) & ~(size_t)1023))) / heads}));
@@ -287,7 +297,8 @@ static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   a.counters = (int *)block;
   a.part = (float *)(block + RXW8_NOALLOC_COUNTER_BYTES);
   char kname[40];
-  std::snprintf(kname, sizeof kname, "rxw8_paged_decode_%s_d%d", a.p_f32 ? "f32" : "bf16", a.D);
+  if (a.ks) std::snprintf(kname, sizeof kname, "rxw8_q8_decode_d%d", a.D);
+  else std::snprintf(kname, sizeof kname, "rxw8_paged_decode_%s_d%d", a.p_f32 ? "f32" : "bf16", a.D);
   return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(512), a, wave * (size_t)a.waves);
 }
 
@@ -484,7 +495,7 @@ int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer 
                     out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
                     (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32, 0, out->dtype == RXW8_F32,
                     0, 0, nullptr, nullptr, (const float *)k_scales->ptr, (const float *)v_scales->ptr};
-  return launch(rt, "rxw8_q8_decode_any", dim3((unsigned)B * (unsigned)Hq), dim3(256), a);
+  return paged_decode_launch(rt, a);
 }
 
 int rxw8_gqa_decode_paged_q8(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
