@@ -85,6 +85,8 @@ struct Deal {
 constexpr int kPagedWaves = 8;
 
 enum { kBf16, kF32, kCodes };  // what pages hold
+// q's type: as the arguments say, or one that a kernel is made for (beside f32 pages: all one)
+enum { kQAny, kQBf16, kQF32 };
 
 template <int D, int KIND>
 struct PagedTile {
@@ -136,6 +138,12 @@ __device__ __forceinline__ void store_pair(float *p, float x, float y) {
   const unsigned long long v = (unsigned long long)__float_as_uint(y) << 32 | __float_as_uint(x);
   __hip_atomic_store((unsigned long long *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// A wave-uniform address, in scalar registers
+__device__ __forceinline__ const void *uniform(const void *p) {
+  const uint64_t x = (uint64_t)(uintptr_t)p;
+  return (const void *)(uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32 |
+                                   (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
 // dma16 (common.h) of what others wrote so: past this die's caches
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -175,11 +183,12 @@ __device__ __forceinline__ void dma4(const void *from, uint32_t lds) {
 
 // What a wave holds for CT x 16 query rows (columns of the products) of one kv head: q, O
 // and the softmax, and the steps over a tile in its memory `mem` (K, V, scales).
-template <int D, int KIND, int CT>
+template <int D, int KIND, int CT, int Q>
 struct PagedWave {
   using T = PagedTile<D, KIND>;
   static constexpr bool F32 = T::F32, CODES = T::CODES;
   static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row's q per lane
+  static constexpr int NL = F32 || Q == kQBf16 ? 1 : NQ;  // (f32 q over bf16 and 8-bit rows: three parts)
   typedef const __attribute__((address_space(3))) char *Lds;
 
   struct Tile {
@@ -190,7 +199,7 @@ struct PagedWave {
   const PagedDecodeArgs &a;
   const int lane, col, g4, h;
   char *const mem;
-  u32x4 q[CT][NQ], ql[CT][F32 ? 1 : NQ], qe[CT][F32 ? 1 : NQ];  // (f32 q over bf16 and 8-bit rows: three parts)
+  u32x4 q[CT][NQ], ql[CT][NL], qe[CT][NL];
   f32x4 o[CT][D / 16], s[CT][T::SUB];
   f32x4 vs[CODES ? T::SUB : 1];     // V's scales
   float m[CT], l[CT];
@@ -241,6 +250,7 @@ struct PagedWave {
   }
   __device__ RXW8_INLINE void copy_v(const Tile &x) const { copy(a.vp, x, 1); }
 
+  __device__ RXW8_INLINE bool q_f32() const { return Q == kQAny ? a.q_f32 : Q == kQF32; }
   // q of the lane's row of column tile c, at element qo
   __device__ RXW8_INLINE void load_q(int c, int64_t qo) {
 #pragma unroll
@@ -255,13 +265,13 @@ struct PagedWave {
         }
       } else {
         const int64_t at8 = qo + (CODES ? 64 * (i >> 1) + 16 * g4 + 8 * (i & 1) : 32 * i + 8 * g4);
-        if (a.q_f32) {
+        if (q_f32()) {
           const f32x4 r[2] = {*(const f32x4 *)((const float *)a.q + at8), *(const f32x4 *)((const float *)a.q + at8 + 4)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t x[3];
             split_bf16x2(r[e >> 1][2 * (e & 1)], r[e >> 1][2 * (e & 1) + 1], x);
-            q[c][i][e] = x[0], ql[c][i][e] = x[1], qe[c][i][e] = x[2];
+            q[c][i][e] = x[0], ql[c][NL > 1 ? i : 0][e] = x[1], qe[c][NL > 1 ? i : 0][e] = x[2];
           }
         } else {
           q[c][i] = *(const u32x4 *)((const uint16_t *)a.q + at8);
@@ -297,9 +307,9 @@ struct PagedWave {
         for (int c = 0; c < CT; ++c) {
           if (c && c >= ct) break;
           acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[c][n]), acc[c][n & 1]);
-          if (a.q_f32) {
-            acc[c][~n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[c][n]), acc[c][~n & 1]);
-            acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][n]), acc[c][n & 1]);
+          if (q_f32()) {
+            acc[c][~n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[c][NL > 1 ? n : 0]), acc[c][~n & 1]);
+            acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][NL > 1 ? n : 0]), acc[c][n & 1]);
           }
         }
       };
@@ -407,28 +417,22 @@ struct PagedWave {
           }
       return;
     }
-    uint2 p[CT][T::SUB][3];  // weights in parts: three behind an f32 output, two behind a bf16 one
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      if (c && c >= ct) break;
-#pragma unroll
-      for (int u = 0; u < T::SUB; ++u) {
-        const f32x4 w = s[c][u];
-        if (a.out_f32) {
-          uint32_t x[3], y[3];
-          split_bf16x2<true>(w[0], w[1], x);
-          split_bf16x2<true>(w[2], w[3], y);
-#pragma unroll
-          for (int k = 0; k < 3; ++k) p[c][u][k] = uint2{x[k], y[k]};
-        } else {
-          uint32_t x[2], y[2];
-          split_bf16x2<true>(w[0], w[1], x);
-          split_bf16x2<true>(w[2], w[3], y);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) p[c][u][k] = uint2{x[k], y[k]};
-        }
+    // weights in parts: three behind an f32 output, two behind a bf16 one
+    struct Parts {
+      uint2 k0, k1, k2;
+    };
+    auto parts = [&](f32x4 w) RXW8_INLINE {
+      if (a.out_f32) {
+        uint32_t x[3], y[3];
+        split_bf16x2<true>(w[0], w[1], x);
+        split_bf16x2<true>(w[2], w[3], y);
+        return Parts{uint2{x[0], y[0]}, uint2{x[1], y[1]}, uint2{x[2], y[2]}};
       }
-    }
+      uint32_t x[2], y[2];
+      split_bf16x2<true>(w[0], w[1], x);
+      split_bf16x2<true>(w[2], w[3], y);
+      return Parts{uint2{x[0], y[0]}, uint2{x[1], y[1]}, uint2{0, 0}};
+    };
     if constexpr (CODES) {
       constexpr int W = D / 64;  // dwords of a lane's dims of a key
 #pragma unroll
@@ -451,6 +455,13 @@ struct PagedWave {
               for (int i = 0; i < 4; ++i) w[k][j][i] = x[i];
             }
           }
+        Parts p[CT][2];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (c && c >= ct) break;
+          p[c][0] = parts(s[c][u]);
+          p[c][1] = parts(s[c][u + 1]);
+        }
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
           u32x4 f;
@@ -464,12 +475,10 @@ struct PagedWave {
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             if (c && c >= ct) break;
-            auto add = [&](int k) RXW8_INLINE {
-              o[c][n] = mfma16x16x32(as_bf16x8(f), as_bf16x8(u32x4{p[c][u][k].x, p[c][u][k].y, p[c][u + 1][k].x, p[c][u + 1][k].y}), o[c][n]);
-            };
-            add(0);
-            add(1);
-            if (a.out_f32) add(2);
+            auto add = [&](uint2 x, uint2 y) RXW8_INLINE { o[c][n] = mfma16x16x32(as_bf16x8(f), as_bf16x8(u32x4{x.x, x.y, y.x, y.y}), o[c][n]); };
+            add(p[c][0].k0, p[c][1].k0);
+            add(p[c][0].k1, p[c][1].k1);
+            if (a.out_f32) add(p[c][0].k2, p[c][1].k2);
           }
         }
       }
@@ -477,7 +486,13 @@ struct PagedWave {
       const int tr_j = col >> 2, tr_q = col & 3;
       const uint32_t vf = v0 + (4 * g4 + tr_j) * T::ROW + 8 * (tr_q & 1);
 #pragma unroll
-      for (int u = 0; u < T::SUB; ++u)
+      for (int u = 0; u < T::SUB; ++u) {
+        Parts p[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (c && c >= ct) break;
+          p[c] = parts(s[c][u]);
+        }
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
           const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
@@ -485,14 +500,15 @@ struct PagedWave {
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             if (c && c >= ct) break;
-            auto add = [&](int k) RXW8_INLINE {
-              o[c][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, p[c][u][k]), o[c][n], 0, 0, 0);
+            auto add = [&](uint2 x) RXW8_INLINE {
+              o[c][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, x), o[c][n], 0, 0, 0);
             };
-            add(0);
-            add(1);
-            if (a.out_f32) add(2);
+            add(p[c].k0);
+            add(p[c].k1);
+            if (a.out_f32) add(p[c].k2);
           }
         }
+      }
     }
   }
 
@@ -530,10 +546,10 @@ __device__ __forceinline__ PagedPlaceOf paged_place_of(const PagedDecodeArgs &a)
   return PagedPlaceOf{(int)(blockIdx.x % heads), (int)(blockIdx.x / heads), a.units, nullptr};
 }
 
-template <int D, int KIND, bool RECORDS = false>
+template <int D, int KIND, bool RECORDS = false, int Q = kQAny>
 __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf place) {
   using T = PagedTile<D, KIND>;
-  using Wave = PagedWave<D, KIND, 1>;
+  using Wave = PagedWave<D, KIND, 1, Q>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Piece piece[kPagedWaves][2];
   __shared__ int last_one[2];
@@ -793,7 +809,7 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
 #pragma unroll 1
           for (int y = wave; y < n * pieces; y += kPagedWaves) {
             const int c = y / pieces;
-            dma16_coherent(a.part + (c0 + c == 0 ? on : past + c0 + c) * rec_size + 256 * (y - c * pieces), 16 * lane,
+            dma16_coherent(uniform(a.part + (c0 + c == 0 ? on : past + c0 + c) * rec_size + 256 * (y - c * pieces)), 16 * lane,
                            lds_addr(lds) + 1024 * y);
           }
           wait_vm<0>();

@@ -53,14 +53,14 @@ struct PagedReadArgs {
   int k_f32;
 };
 struct SharedArgs {
-  const void *q, *kp, *vp;
-  const float *ks, *vs;
-  const int32_t *prefixes, *prefix_lens, *groups, *table, *lens;
-  void *out;
-  int64_t P;
-  int B, N, MP, M, Hq, Hkv, D, ps;
-  float c;
-  int q_f32, kind, out_f32;
+  PagedDecodeArgs d;
+  const int32_t *prefixes, *prefix_lens, *groups;
+  int N, MP;
+  int b0;
+  int kind;
+  float *own, *whole, *parts;
+  int *plan;
+  int columns, keys;
 };
 struct LogitsArgs {
   const void *logits;
@@ -302,6 +302,61 @@ static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(512), a, wave * (size_t)a.waves);
 }
 
+// The matrix-core kernels on paged decode's terms. Records of parts take at most 12 MiB of the
+// runtime's block (all of it where a single one is larger), those of rows the rest: a
+// batch with more rows than fit goes in several launches of the two.
+static int shared_launch(Runtime *rt, SharedArgs a) {
+  PagedDecodeArgs &d = a.d;
+  const int64_t G = d.Hq / d.Hkv, HT = (G + 15) / 16, heads = d.Hkv * HT, rec = (int64_t)(d.D + 4) * sizeof(float);
+  const PagedTiles t(a.kind, d.D);
+  // block_tiles (kernels/shared.hip)
+  const bool split = d.q_f32 && a.kind != 1;
+  const int ct = d.D == 256 ? 1 : d.D == 128 ? (split ? 1 : 2) : split || a.kind == 2 ? 2 : 4;
+  a.columns = 16 * ct, a.keys = t.keys;
+  auto tiles = [&](int64_t m) { return (m * d.ps + t.keys - 1) / t.keys; };
+  const int64_t blocks = (int64_t)d.B * G / a.columns + a.N;
+  bool any = (d.D != 64 && d.D != 128 && d.D != 256) || d.ps % 16 || d.P == 0 || heads > 4096 || a.N == 0 || a.MP == 0 ||
+             ((uintptr_t)d.q | (uintptr_t)d.kp | (uintptr_t)d.vp | (uintptr_t)d.out) % 16 ||
+             tiles(d.M) >= ((int64_t)1 << 30) / d.B || tiles(a.MP) >= ((int64_t)1 << 30) / blocks;
+  const size_t record = (size_t)std::min<int64_t>(G, 16) * (size_t)rec;
+  const size_t wave = std::max({(size_t)t.ring, record, (size_t)(16 * rec)}) + record;
+  d.waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
+  const int64_t block = (int64_t)RXW8_NOALLOC_PARTIAL_BYTES - 1024;
+  auto round = [](int64_t x) { return (x + 1023) & ~(int64_t)1023; };
+  const int64_t own_part = round((int64_t)record), prefix_part = a.columns * rec;
+  auto parts = [&](int64_t units) { return round(2 * heads * units * own_part) + round(2 * heads * units * prefix_part); };
+  d.units = 1;
+  for (int64_t u = 2; u <= std::min<int64_t>(256, (int64_t)(RXW8_NOALLOC_COUNTER_BYTES / sizeof(int)) / heads) && parts(u) <= 12 << 20; ++u) {
+    const int64_t r0 = (heads * d.units + rt->cus - 1) / rt->cus, r1 = (heads * u + rt->cus - 1) / rt->cus;
+    if (r1 * d.units < r0 * u) d.units = (int)u;
+  }
+  const int64_t most = (block - parts(d.units)) / (2 * rec * d.Hq);
+  if (any || most < 1) return launch(rt, "rxw8_shared_any", dim3((unsigned)d.B * (unsigned)d.Hq), dim3(256), a);
+  const int64_t launches = (d.B + most - 1) / most, each = (d.B + launches - 1) / launches;
+  char *const at = rt->f32_attn[stream_capturing(rt) ? 1 : 0], *const recs = at + RXW8_NOALLOC_COUNTER_BYTES + 1024;
+  d.counters = (int *)at;
+  a.plan = (int *)(at + RXW8_NOALLOC_COUNTER_BYTES);
+  d.part = (float *)recs;
+  a.parts = (float *)(recs + round(2 * heads * d.units * own_part));
+  a.own = (float *)(recs + parts(d.units));
+  a.whole = a.own + each * d.Hq * (d.D + 4);
+  char kname[40];
+  std::snprintf(kname, sizeof kname, "rxw8_shared_%s%s_d%d", a.kind == 2 ? "q8" : a.kind == 1 ? "f32" : "bf16", split ? "_qf32" : "", d.D);
+  const int64_t B = d.B, q_size = d.q_f32 ? 4 : 2, out_size = d.out_f32 ? 4 : 2;
+  for (int64_t b0 = 0; b0 < B; b0 += each) {
+    SharedArgs c = a;
+    c.b0 = (int)b0;
+    c.d.B = (int)std::min(each, B - b0);
+    c.d.q = (const char *)d.q + b0 * d.Hq * d.D * q_size;
+    c.d.out = (char *)d.out + b0 * d.Hq * d.D * out_size;
+    c.d.table = d.table + b0 * d.M;
+    c.d.lens = d.lens + b0;
+    if (int rc = launch(rt, kname, dim3((unsigned)(heads * d.units)), dim3(512), c, wave * (size_t)d.waves)) return rc;
+    if (int rc = launch(rt, "rxw8_shared_join", dim3((unsigned)(((int64_t)c.d.B * d.Hq + 3) / 4)), dim3(256), c)) return rc;
+  }
+  return RXW8_OK;
+}
+
 static int packed_launch(Runtime *rt, const Buffer *q, const Buffer *k, const Buffer *v, const Buffer *offsets,
                          float scale, const Buffer *out, bool fill) {
   const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2];
@@ -532,14 +587,14 @@ int rxw8_gqa_decode_shared_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k
   const int64_t B = q->dims[0], Hq = q->dims[1], D = q->dims[2];
   if (B == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
-  SharedArgs a{q->ptr, k_pages->ptr, v_pages->ptr, k_scales ? (const float *)k_scales->ptr : nullptr,
-               v_scales ? (const float *)v_scales->ptr : nullptr, (const int32_t *)prefixes->ptr,
-               (const int32_t *)prefix_lens->ptr, (const int32_t *)groups->ptr, (const int32_t *)table->ptr,
-               (const int32_t *)lens->ptr, out->ptr, k_pages->dims[0], (int)B, (int)prefixes->dims[0],
-               (int)prefixes->dims[1], (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
-               (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32, page_kind(k_pages),
-               out->dtype == RXW8_F32};
-  return launch(rt, "rxw8_shared_any", dim3((unsigned)B * (unsigned)Hq), dim3(256), a);
+  PagedDecodeArgs d{q->ptr, k_pages->ptr, v_pages->ptr, (const int32_t *)table->ptr, (const int32_t *)lens->ptr,
+                    out->ptr, k_pages->dims[0], (int)B, (int)table->dims[1], (int)Hq, (int)k_pages->dims[1], (int)D,
+                    (int)k_pages->dims[2], softmax_scale(scale, D), q->dtype == RXW8_F32, k_pages->dtype == RXW8_F32,
+                    out->dtype == RXW8_F32, 0, 0, nullptr, nullptr, k_scales ? (const float *)k_scales->ptr : nullptr,
+                    v_scales ? (const float *)v_scales->ptr : nullptr};
+  return shared_launch(rt, SharedArgs{d, (const int32_t *)prefixes->ptr, (const int32_t *)prefix_lens->ptr,
+                                      (const int32_t *)groups->ptr, (int)prefixes->dims[0], (int)prefixes->dims[1], 0,
+                                      page_kind(k_pages), nullptr, nullptr, nullptr, nullptr, 0, 0});
 }
 
 int rxw8_gqa_decode_shared(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
