@@ -54,6 +54,78 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_q8_append_any(PagedQ8Args
   }
 }
 
+// Head widths of 64, 128, 256 and 512 at 16-byte boundaries: a wave for each row and
+// `kRows` x 64 of its pieces of 8 elements, D / 8 lanes to a head, K's and V's pieces
+// under way before the wave looks for its sequence and page. A quotient is taken by the
+// scale's inverse: both are off by at most 2^-24 of it, so the two products of 127 at most
+// differ from the true quotient by less than 127 2^-23 < 2e-5, and a value that is further
+// than 1e-4 from the middle between two codes rounds to the same one. The few others are
+// divided.
+constexpr int kRows = 2;
+
+template <typename S>
+__device__ __forceinline__ void q8_append(const PagedQ8Args &a) {
+  constexpr int NS = sizeof(S) / 2;  // 16-byte words of 8 elements
+  const int lane = threadIdx.x & 63, per_head = a.D / 8, pieces = a.Hkv * per_head;
+  const int parts = (pieces + 64 * kRows - 1) / (64 * kRows);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = unit / parts;
+  const int p0 = (int)(unit - t * parts) * 64 * kRows + lane;
+  if (t >= a.T) return;  // whole waves only; no barriers below
+  u32x4 x[kRows][2][NS];
+#pragma unroll
+  for (int n = 0; n < kRows; ++n)
+    if (p0 + 64 * n < pieces) {
+      const int64_t at = (t * pieces + p0 + 64 * n) * NS;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) x[n][0][i] = ((const u32x4 *)a.k)[at + i], x[n][1][i] = ((const u32x4 *)a.v)[at + i];
+    }
+  const PagedPlace to = paged_place(a, t);
+  if (to.page < 0) return;
+#pragma unroll
+  for (int n = 0; n < kRows; ++n) {
+    const int p = p0 + 64 * n;
+    const bool mine = p < pieces;  // (whole heads: the lanes of one are all in or all out)
+    const int h = p / per_head;
+    const int64_t row = (to.page * a.Hkv + h) * a.ps + to.at;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w = x[n][kv][i / (8 / NS)][NS == 2 ? i & 3 : i >> 1];
+        v[i] = __uint_as_float(NS == 2 ? w : i & 1 ? w & 0xffff0000u : w << 16);
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, q8_size(v[i]));
+      for (int o = per_head >> 1; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+      const float s = q8_scale(__uint_as_float(top)), inv = 1.0f / s;
+      uint32_t code[2] = {0, 0};
+      bool middle = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = v[i] * inv, r = rintf(y);
+        middle |= fabsf(y - r) > 0.4999f;
+        code[i >> 2] |= (uint32_t)(int)(r + 128.f) << 8 * (i & 3);
+      }
+      if (middle) {
+        code[0] = code[1] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) code[i >> 2] |= q8_code(v[i], s) << 8 * (i & 3);
+      }
+      if (s != s) code[0] = code[1] = 0x80808080u;
+      if (mine) {
+        *(uint2 *)((kv ? a.vp : a.kp) + row * a.D + 8 * (p - h * per_head)) = uint2{code[0], code[1]};
+        if (p == h * per_head) (kv ? a.vs : a.ks)[row] = s;
+      }
+    }
+  }
+}
+extern "C" __global__ void __launch_bounds__(256) rxw8_q8_append(PagedQ8Args a) {
+  if (a.k_f32) q8_append<float>(a);
+  else q8_append<uint16_t>(a);
+}
+
 struct PagedReadArgs {
   const void *kp, *vp;       // [P, Hkv, ps, D] bf16 | f32 | u8
   const float *ks, *vs;      // [P, Hkv, ps] (u8)
@@ -89,6 +161,77 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_q8_read_any(PagedReadArgs
       if (a.k_f32) ((float *)to)[dst + e] = y;
       else ((uint16_t *)to)[dst + e] = f32_to_bf16_bits(y);
     }
+  }
+}
+
+// Widths of whole 8 elements at 16-byte boundaries: a wave for each row and `kRows` x 64
+// of its pieces of 8 elements
+template <int KIND, typename S>
+__device__ __forceinline__ void paged_read(const PagedReadArgs &a) {
+  constexpr int NP = KIND == 1 ? 2 : 1, NS = sizeof(S) / 2;  // 16-byte words of 8 elements (codes: half a one)
+  const int lane = threadIdx.x & 63, per_head = a.D / 8, pieces = a.Hkv * per_head;
+  const int parts = (pieces + 64 * kRows - 1) / (64 * kRows);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), t = unit / parts;
+  const int p0 = (int)(unit - t * parts) * 64 * kRows + lane;
+  if (t >= a.T) return;
+  const PagedPlace of = paged_place(a, t);
+  if (of.at < 0) return;
+  u32x4 x[kRows][2][NP];
+  float s[kRows][2];
+#pragma unroll
+  for (int n = 0; n < kRows; ++n) {
+    const int p = p0 + 64 * n, h = p / per_head;
+    const int64_t row = (of.page * a.Hkv + h) * a.ps + of.at, at = row * per_head + (p - h * per_head);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      const void *pages = kv ? a.vp : a.kp;
+      s[n][kv] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) x[n][kv][i] = KIND == 2 ? u32x4{0x80808080u, 0x80808080u, 0, 0} : u32x4{0, 0, 0, 0};
+      if (p >= pieces || of.page < 0) continue;
+      if constexpr (KIND == 2) {
+        const uint2 c = ((const uint2 *)pages)[at];
+        x[n][kv][0][0] = c.x, x[n][kv][0][1] = c.y;
+        s[n][kv] = (kv ? a.vs : a.ks)[row];
+      } else {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) x[n][kv][i] = ((const u32x4 *)pages)[at * NP + i];
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kRows; ++n) {
+    const int p = p0 + 64 * n;
+    if (p >= pieces) return;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (KIND == 2) v[i] = ((float)(x[n][kv][0][i >> 2] >> 8 * (i & 3) & 0xffu) - 128.f) * s[n][kv];
+        else if constexpr (KIND == 1) v[i] = __uint_as_float(x[n][kv][i >> 2][i & 3]);
+        else v[i] = __uint_as_float(i & 1 ? x[n][kv][0][i >> 1] & 0xffff0000u : x[n][kv][0][i >> 1] << 16);
+      }
+      u32x4 *const to = (u32x4 *)(kv ? a.v : a.k) + (t * pieces + p) * NS;
+      if constexpr (NS == 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          to[i] = u32x4{__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3])};
+      } else {
+        to[0] = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+      }
+    }
+  }
+}
+extern "C" __global__ void __launch_bounds__(256) rxw8_q8_read(PagedReadArgs a) {
+  if (a.k_f32) {
+    if (a.kind == 2) paged_read<2, float>(a);
+    else if (a.kind == 1) paged_read<1, float>(a);
+    else paged_read<0, float>(a);
+  } else {
+    if (a.kind == 2) paged_read<2, uint16_t>(a);
+    else if (a.kind == 1) paged_read<1, uint16_t>(a);
+    else paged_read<0, uint16_t>(a);
   }
 }
 

@@ -118,7 +118,7 @@ static bool same_shape(const Buffer *a, const Buffer *b) {
 // Workgroups of `threads` that one launch takes: 2^32 - 1 threads
 constexpr int64_t grid_max(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 constexpr int64_t kAnyMaxD = 512;  // RXW8_ATTN_ANY_MAX_D
-constexpr int64_t kLogitsChunk = 8192;
+constexpr int64_t kLogitsChunk = 2048;  // words of a workgroup, at least
 static int page_kind(const Buffer *pages) { return pages->dtype == RXW8_U8 ? 2 : pages->dtype == RXW8_F32 ? 1 : 0; }
 
 // Whether the buffers (NULL ones aside) are the runtime's, and none of the first `written`
@@ -168,18 +168,21 @@ static int check_pages(const char *what, const Buffer *kp, const Buffer *vp, con
   return check_table(what, table, kp->dims[2]);
 }
 
+// Waves of a row [Hkv, D]: 128 pieces of 8 elements each
+static int64_t row_parts(const Buffer *k) { return (k->dims[1] * k->dims[2] / 8 + 127) / 128; }
+
 // Rows k, v F32|BF16 [T, Hkv, D] of the pages' heads and width, their sequences' first
-// positions I32 [B] and the rows of each I32 [B + 1] (NULL: one each). A wave takes 128
-// pieces of 8 elements of a row, or a row of one head.
+// positions I32 [B] and the rows of each I32 [B + 1] (NULL: one each). A wave takes a part
+// of a row, or a row of one head.
 static int check_rows(const char *what, const Buffer *kp, const Buffer *k, const Buffer *v, const Buffer *table,
                       const Buffer *starts, const Buffer *offsets) {
   if (k->rank != 3 || !is_f(k->dtype) || !same_shape(k, v) || k->dims[1] != kp->dims[1] || k->dims[2] != kp->dims[3])
     return fail(RXW8_INVALID_ARGUMENT, "%s requires F32/BF16 k, v [T,Hkv,D] of the pages' heads and width", what);
-  const int64_t T = k->dims[0], B = table->dims[0], parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
+  const int64_t T = k->dims[0], B = table->dims[0];
   if (!is_vec(starts, RXW8_I32, B)) return fail(RXW8_INVALID_ARGUMENT, "%s: starts must be I32 [B]", what);
   if (offsets ? !is_vec(offsets, RXW8_I32, B + 1) : T != B)
     return fail(RXW8_INVALID_ARGUMENT, "%s: offsets must be I32 [B+1] (without them k, v hold one row a sequence)", what);
-  if (T > 4 * grid_max(256) / std::max(k->dims[1], parts))
+  if (T > 4 * grid_max(256) / std::max(k->dims[1], row_parts(k)))
     return fail(RXW8_UNIMPLEMENTED, "%s: %lld rows exceed the kernel's grid", what, (long long)T);
   return RXW8_OK;
 }
@@ -412,7 +415,7 @@ int rxw8_paged_kv_append(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_
   if (int rc = check_pages("paged KV append", k_pages, v_pages, table)) return rc;
   if (k_pages == v_pages) return fail(RXW8_INVALID_ARGUMENT, "K and V pages must be distinct buffers");
   if (int rc = check_rows("paged KV append", k_pages, k, v, table, starts, offsets)) return rc;
-  const int64_t T = k->dims[0], B = table->dims[0], parts = (k->dims[1] * k->dims[2] / 8 + 127) / 128;
+  const int64_t T = k->dims[0], B = table->dims[0], parts = row_parts(k);
   if (int rc = check_buffers("paged KV append", rt, {k_pages, v_pages, k, v, table, starts, offsets}, 2)) return rc;
   if (T == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
@@ -511,7 +514,10 @@ int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer 
                 (float *)v_scales->ptr, (const int32_t *)table->ptr, (const int32_t *)starts->ptr,
                 offsets ? (const int32_t *)offsets->ptr : nullptr, T, k_pages->dims[0], (int)table->dims[0],
                 (int)table->dims[1], (int)k->dims[1], (int)k->dims[2], (int)k_pages->dims[2], k->dtype == RXW8_F32};
-  return launch(rt, "rxw8_q8_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  if ((a.D != 64 && a.D != 128 && a.D != 256 && a.D != 512) ||
+      ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
+    return launch(rt, "rxw8_q8_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  return launch(rt, "rxw8_q8_append", dim3((unsigned)((T * row_parts(k) + 3) / 4)), dim3(256), a);
 }
 
 int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pages, rxw8_buffer *k_scales,
@@ -532,7 +538,9 @@ int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pa
                   (const int32_t *)starts->ptr, offsets ? (const int32_t *)offsets->ptr : nullptr, T,
                   k_pages->dims[0], (int)table->dims[0], (int)table->dims[1], (int)k->dims[1], (int)k->dims[2],
                   (int)k_pages->dims[2], page_kind(k_pages), k->dtype == RXW8_F32};
-  return launch(rt, "rxw8_q8_read_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  if (a.D % 8 || ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
+    return launch(rt, "rxw8_q8_read_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
+  return launch(rt, "rxw8_q8_read", dim3((unsigned)((T * row_parts(k) + 3) / 4)), dim3(256), a);
 }
 
 int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
@@ -648,7 +656,7 @@ static int check_logits(const rxw8_logits_options *o, const Buffer *logits) {
   for (const rxw8_buffer *x : {o->tokens, o->bias})
     if (x && x->dims[0] > INT32_MAX)
       return fail(RXW8_UNIMPLEMENTED, "%s: %lld entries exceed 32-bit offsets", what, (long long)x->dims[0]);
-  if (B > grid_max(512) / ((V + kLogitsChunk - 1) / kLogitsChunk))
+  if (B > grid_max(256) / ((V + kLogitsChunk - 1) / kLogitsChunk))
     return fail(RXW8_UNIMPLEMENTED, "%s: %lld rows exceed the kernel's grid", what, (long long)B);
   return RXW8_OK;
 }
@@ -672,8 +680,13 @@ int rxw8_adjust_logits_into(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_lo
                f32(o->frequency), f32(o->presence), i32(o->bias_words), f32(o->bias), i32(o->bias_offsets),
                (const uint32_t *)i32(o->mask), i32(o->mask_rows), o->tokens ? o->tokens->dims[0] : 0,
                o->bias ? o->bias->dims[0] : 0, o->mask ? o->mask->dims[0] : 0, V, logits->dtype == RXW8_F32,
-               out->dtype == RXW8_F32, (int)kLogitsChunk, (int)((V + kLogitsChunk - 1) / kLogitsChunk)};
-  return launch(rt, "rxw8_logits_adjust", dim3((unsigned)(B * a.chunks)), dim3(512), a,
+               out->dtype == RXW8_F32, 0, 0};
+  const bool pieces = V % 8 == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15);
+  const int times = B * V <= 2 * kLogitsChunk * rt->cus ? 1 : 2;
+  a.chunk = (int)(kLogitsChunk * times), a.chunks = (int)((V + a.chunk - 1) / a.chunk);
+  char kname[40];
+  std::snprintf(kname, sizeof kname, pieces ? "rxw8_logits_adjust%d" : "rxw8_logits_any", times);
+  return launch(rt, kname, dim3((unsigned)(B * a.chunks)), dim3(256), a,
                 sizeof(int) * (size_t)a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr)));
 }
 
