@@ -28,140 +28,152 @@ struct LogitsArgs {
 // A workgroup takes `chunk` words of a row. It counts those of the row's history that
 // fall on them in LDS (bit 31: seen in the prompt; the rest: n; additions of whole numbers,
 // whose order changes nothing) and finds the last bias entry of each, then goes over the
-// words once.
-constexpr int kLogitsThreads = 256;
+// words once. Under a full memory system every load that waits for another one costs
+// microseconds, so there are two rounds of them: the row's settings, then the logits, the
+// mask's bits, the first tokens and the biases together. 64 rows of 248320 f32 logits with
+// histories of 1 to 8000, up to 300 biases and masks: 33.7 us (46 with the loads one after
+// another), 3.8 TB/s; 25 us with no setting at all, a copy. Chunks of 1024, 2048, 4096 and
+// 8192 words, 8 a thread: 43.6, 34.9, 33.7 and 39.5 us (every workgroup of a row goes over
+// the row's history). One row of 151936 and 800 tokens: 5 us, the two rounds and the launch.
+constexpr int kTokens = 8, kValues = 512;  // tokens of a thread under way; biases kept in LDS
+
+// Device memory that the launch does not write, at a wave-uniform address (scalar loads)
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T *p, int64_t i) {
+  return ((const __attribute__((address_space(4))) T *)(uintptr_t)p)[i];
+}
 
 struct LogitsRow {
-  int64_t b, w0, e0;        // row, its workgroup's first word, its first bias entry
-  int n;                    // words
+  int64_t b, w0, t0, t1, mine, e0, e1;  // row, first word; its tokens, and those behind the prompt; its bias entries
+  int n;                                // words of the workgroup
   float r, f, p;
   const uint32_t *mask;
   uint32_t *counts, *entries;
-};
+  float *values;
+  int tokens[kTokens], word;            // the thread's first ones
+  float value;
 
-__device__ __forceinline__ LogitsRow logits_row(const LogitsArgs &a, uint32_t *lds) {
-  LogitsRow x;
-  x.b = blockIdx.x / a.chunks, x.w0 = (int64_t)(blockIdx.x - x.b * a.chunks) * a.chunk;
-  x.n = (int)min((int64_t)a.chunk, a.V - x.w0);
-  x.counts = lds, x.entries = lds + (a.tokens ? a.chunk : 0);
-  x.r = a.repetition ? a.repetition[x.b] : 1.f;
-  x.f = a.frequency ? a.frequency[x.b] : 0.f;
-  x.p = a.presence ? a.presence[x.b] : 0.f;
-  const int64_t m = a.mask ? a.mask_rows ? a.mask_rows[x.b] : x.b : -1;
-  x.mask = m >= 0 && m < a.R ? a.mask + m * ((a.V + 31) / 32) : nullptr;
-  return x;
-}
-
-// Counts and entries of the workgroup's words
-__device__ __forceinline__ void logits_count(const LogitsArgs &a, LogitsRow &x) {
-  typedef uint32_t u32x4a __attribute__((ext_vector_type(4)));
-  const int64_t b = x.b, w0 = x.w0;
-  const int total = a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr));  // (multiples of 4)
-  for (int i = 4 * threadIdx.x; i < total; i += 4 * kLogitsThreads) *(u32x4a *)(x.counts + i) = u32x4a{0, 0, 0, 0};
-  __syncthreads();
-  auto bounded = [](int64_t i, int64_t most) { return i < 0 ? 0 : i < most ? i : most; };
-  if (a.tokens) {
-    const int64_t t0 = bounded(a.offsets[b], a.T), t1 = bounded(a.offsets[b + 1], a.T);
-    const int64_t mine = t0 + (a.prompts ? max(a.prompts[b], 0) : 0);
-    constexpr int U = 8;  // loads under way
-    for (int64_t t = t0 + threadIdx.x; t < t1; t += U * kLogitsThreads) {
-      int w[U];
+  __device__ __forceinline__ LogitsRow(const LogitsArgs &a, uint32_t *lds) {
+    b = blockIdx.x / a.chunks, w0 = (int64_t)(blockIdx.x - b * a.chunks) * a.chunk;
+    n = (int)min((int64_t)a.chunk, a.V - w0);
+    counts = lds, entries = lds + (a.tokens ? a.chunk : 0), values = (float *)(entries + a.chunk);
+    auto bounded = [](int64_t i, int64_t most) { return i < 0 ? 0 : i < most ? i : most; };
+    t0 = a.tokens ? uniform_load(a.offsets, b) : 0, t1 = a.tokens ? uniform_load(a.offsets, b + 1) : 0;
+    mine = a.prompts ? uniform_load(a.prompts, b) : 0;
+    e0 = a.bias ? uniform_load(a.bias_offsets, b) : 0, e1 = a.bias ? uniform_load(a.bias_offsets, b + 1) : 0;
+    r = a.repetition ? uniform_load(a.repetition, b) : 1.f;
+    f = a.frequency ? uniform_load(a.frequency, b) : 0.f;
+    p = a.presence ? uniform_load(a.presence, b) : 0.f;
+    const int64_t m = a.mask ? a.mask_rows ? uniform_load(a.mask_rows, b) : b : -1;
+    t0 = bounded(t0, a.T), t1 = bounded(t1, a.T), e0 = bounded(e0, a.E), e1 = bounded(e1, a.E);
+    mine = t0 + max(mine, (int64_t)0);
+    mask = m >= 0 && m < a.R ? a.mask + m * ((a.V + 31) / 32) : nullptr;
+  }
+  __device__ __forceinline__ void load_tokens(const LogitsArgs &a, int64_t t) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = t + u * kLogitsThreads < t1 ? a.tokens[t + u * kLogitsThreads] : -1;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t at = (int64_t)w[u] - w0;
-        if (at < 0 || at >= x.n) continue;
-        if (t + u * kLogitsThreads < mine) atomicOr(x.counts + at, 0x80000000u);
-        else atomicAdd(x.counts + at, 1u);
-      }
+    for (int u = 0; u < kTokens; ++u) {
+      const int64_t i = t + u * (int)blockDim.x;
+      tokens[u] = i < t1 ? a.tokens[i] : -1;
     }
   }
-  x.e0 = a.bias ? bounded(a.bias_offsets[b], a.E) : 0;
-  const int64_t e1 = a.bias ? bounded(a.bias_offsets[b + 1], a.E) : 0;
-  for (int64_t e = x.e0 + threadIdx.x; e < e1; e += kLogitsThreads) {
-    const int64_t at = (int64_t)a.bias_words[e] - w0;
-    if (at >= 0 && at < x.n) atomicMax(x.entries + at, (uint32_t)(e - x.e0 + 1));
+  __device__ __forceinline__ void load(const LogitsArgs &a) {
+    load_tokens(a, t0 + threadIdx.x);
+    const int64_t e = e0 + threadIdx.x;
+    word = e < e1 ? a.bias_words[e] : -1;
+    value = e < e1 ? a.bias[e] : 0.f;
   }
-  __syncthreads();
-}
-
-// One word's logit: c its count, e its bias entry, allowed by the mask
-__device__ __forceinline__ float logits_word(const LogitsArgs &a, const LogitsRow &x, float z, uint32_t c, uint32_t e, bool allowed) {
-  if (c) {
-    if (x.r > 0.f) z = z > 0.f ? z / x.r : z * x.r;
-    if (const uint32_t m = c & 0x7fffffffu) z -= x.f * (float)m + x.p;
+  // Counts and entries of the workgroup's words
+  __device__ __forceinline__ void count(const LogitsArgs &a) {
+    const int total = a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr));  // (a multiple of 4)
+    for (int i = 4 * threadIdx.x; i < total; i += 4 * blockDim.x) *(u32x4 *)(counts + i) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += kTokens * (int)blockDim.x) {
+      if (t >= t0 + kTokens * (int)blockDim.x) load_tokens(a, t);
+#pragma unroll
+      for (int u = 0; u < kTokens; ++u) {
+        const int64_t at = (int64_t)tokens[u] - w0;
+        if (at < 0 || at >= n) continue;
+        if (t + u * (int)blockDim.x < mine) atomicOr(counts + at, 0x80000000u);
+        else atomicAdd(counts + at, 1u);
+      }
+    }
+    for (int64_t e = e0 + threadIdx.x; e < e1; e += (int)blockDim.x) {
+      const bool first = e < e0 + (int)blockDim.x;
+      const int64_t at = (int64_t)(first ? word : a.bias_words[e]) - w0;
+      if (at < 0 || at >= n) continue;
+      atomicMax(entries + at, (uint32_t)(e - e0 + 1));
+      if (e - e0 < kValues) values[e - e0] = first ? value : a.bias[e];
+    }
+    __syncthreads();
   }
-  if (e) z += a.bias[x.e0 + e - 1];
-  return allowed ? z : kMinusInf;
-}
+  // One word's logit: c its count, e its bias entry, allowed by the mask
+  __device__ __forceinline__ float adjust(const LogitsArgs &a, float z, uint32_t c, uint32_t e, bool allowed) const {
+    if (c) {
+      if (r > 0.f) z = z > 0.f ? z / r : z * r;
+      if (const uint32_t m = c & 0x7fffffffu) z -= f * (float)m + p;
+    }
+    if (e) z += e <= kValues ? values[e - 1] : a.bias[e0 + e - 1];
+    return allowed ? z : kMinusInf;
+  }
+};
 
-// Rows of any length and alignment: a word a thread
-extern "C" __global__ void __launch_bounds__(kLogitsThreads) rxw8_logits_any(LogitsArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];  // counts [chunk], entries [chunk]
-  LogitsRow x = logits_row(a, lds);
-  logits_count(a, x);
-  for (int i = threadIdx.x; i < x.n; i += kLogitsThreads) {
+// Rows of any length and alignment: a word a thread at a time
+extern "C" __global__ void __launch_bounds__(512) rxw8_logits_any(LogitsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];  // counts [chunk], entries [chunk], values
+  LogitsRow x(a, lds);
+  x.load(a);
+  x.count(a);
+  for (int i = threadIdx.x; i < x.n; i += blockDim.x) {
     const int64_t w = x.w0 + i, at = x.b * a.V + w;
-    const float z = logits_word(a, x, any_load(a.logits, at, a.in_f32), a.tokens ? x.counts[i] : 0, a.bias ? x.entries[i] : 0,
-                                !x.mask || x.mask[w >> 5] >> (w & 31) & 1);
+    const float z = x.adjust(a, any_load(a.logits, at, a.in_f32), a.tokens ? x.counts[i] : 0, a.bias ? x.entries[i] : 0,
+                             !x.mask || x.mask[w >> 5] >> (w & 31) & 1);
     if (a.out_f32) ((float *)a.out)[at] = z;
     else ((uint16_t *)a.out)[at] = f32_to_bf16_bits(z);
   }
 }
 
-// Rows of whole 8 words at 16-byte boundaries: 8 words a thread, I times, whose logits and
-// mask bits are on their way while the history is counted
-template <typename S, typename P, int I>
+// Rows of whole 8 words at 16-byte boundaries: 8 words a thread (chunk = 8 threads)
+template <typename S, typename P>
 __device__ __forceinline__ void logits_adjust(const LogitsArgs &a, uint32_t *lds) {
   constexpr int NS = sizeof(S) / 2;  // 16-byte words of 8 logits
-  LogitsRow x = logits_row(a, lds);
-  u32x4 in[I][NS];
-  uint32_t bits[I];
-  const u32x4 *const from = (const u32x4 *)((const S *)a.logits + x.b * a.V + x.w0);
+  LogitsRow x(a, lds);
+  u32x4 in[NS];
+  uint32_t bits = 0xff;
+  const int64_t at = x.b * a.V + x.w0 + 8 * threadIdx.x;
+  const bool mine = 8 * (int)threadIdx.x < x.n;
+  if (mine) {
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int p = threadIdx.x + i * kLogitsThreads;  // of the workgroup's pieces of 8 words
-    bits[i] = 0xff;
-    if (8 * p < x.n) {
-#pragma unroll
-      for (int k = 0; k < NS; ++k) in[i][k] = from[p * NS + k];
-      if (x.mask) bits[i] = ((const uint8_t *)x.mask)[(x.w0 >> 3) + p];
-    }
+    for (int k = 0; k < NS; ++k) in[k] = ((const u32x4 *)((const S *)a.logits + at))[k];
+    if (x.mask) bits = ((const uint8_t *)x.mask)[(x.w0 >> 3) + threadIdx.x];
   }
-  logits_count(a, x);
+  u32x4 c[2] = {}, e[2] = {};
+  if (a.tokens || a.bias) {
+    x.load(a);
+    x.count(a);
+    if (a.tokens) c[0] = *(const u32x4 *)(x.counts + 8 * threadIdx.x), c[1] = *(const u32x4 *)(x.counts + 8 * threadIdx.x + 4);
+    if (a.bias) e[0] = *(const u32x4 *)(x.entries + 8 * threadIdx.x), e[1] = *(const u32x4 *)(x.entries + 8 * threadIdx.x + 4);
+  }
+  if (!mine) return;
+  float z[8];
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const int p = threadIdx.x + i * kLogitsThreads;
-    if (8 * p >= x.n) return;
-    u32x4 c[2] = {}, e[2] = {};
-    if (a.tokens) c[0] = *(const u32x4 *)(x.counts + 8 * p), c[1] = *(const u32x4 *)(x.counts + 8 * p + 4);
-    if (a.bias) e[0] = *(const u32x4 *)(x.entries + 8 * p), e[1] = *(const u32x4 *)(x.entries + 8 * p + 4);
-    float z[8];
+  for (int k = 0; k < 8; ++k) {
+    const uint32_t w = in[k / (8 / NS)][NS == 2 ? k & 3 : k >> 1];
+    z[k] = __uint_as_float(NS == 2 ? w : k & 1 ? w & 0xffff0000u : w << 16);
+    z[k] = x.adjust(a, z[k], c[k >> 2][k & 3], e[k >> 2][k & 3], bits >> k & 1);
+  }
+  u32x4 *const to = (u32x4 *)((P *)a.out + at);
+  if constexpr (sizeof(P) == 4) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t w = in[i][k / (8 / NS)][NS == 2 ? k & 3 : k >> 1];
-      z[k] = __uint_as_float(NS == 2 ? w : k & 1 ? w & 0xffff0000u : w << 16);
-      z[k] = logits_word(a, x, z[k], c[k >> 2][k & 3], e[k >> 2][k & 3], bits[i] >> k & 1);
-    }
-    u32x4 *const to = (u32x4 *)((P *)a.out + x.b * a.V + x.w0) + p * (sizeof(P) / 2);
-    if constexpr (sizeof(P) == 4) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        to[k] = u32x4{__float_as_uint(z[4 * k]), __float_as_uint(z[4 * k + 1]), __float_as_uint(z[4 * k + 2]), __float_as_uint(z[4 * k + 3])};
-    } else {
-      to[0] = u32x4{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]), pack_bf16x2(z[6], z[7])};
-    }
+    for (int k = 0; k < 2; ++k)
+      to[k] = u32x4{__float_as_uint(z[4 * k]), __float_as_uint(z[4 * k + 1]), __float_as_uint(z[4 * k + 2]), __float_as_uint(z[4 * k + 3])};
+  } else {
+    to[0] = u32x4{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]), pack_bf16x2(z[6], z[7])};
   }
 }
-#define RXW8_LOGITS(I)                                                                              \
-  extern "C" __global__ void __launch_bounds__(kLogitsThreads) rxw8_logits_adjust##I(LogitsArgs a) { \
-    extern __shared__ __attribute__((aligned(16))) uint32_t lds[];                                  \
-    if (a.in_f32 && a.out_f32) logits_adjust<float, float, I>(a, lds);                              \
-    else if (a.in_f32) logits_adjust<float, uint16_t, I>(a, lds);                                   \
-    else if (a.out_f32) logits_adjust<uint16_t, float, I>(a, lds);                                  \
-    else logits_adjust<uint16_t, uint16_t, I>(a, lds);                                              \
-  }
-RXW8_LOGITS(1)
-RXW8_LOGITS(2)
-RXW8_LOGITS(4)
+extern "C" __global__ void __launch_bounds__(512) rxw8_logits_adjust(LogitsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
+  if (a.in_f32 && a.out_f32) logits_adjust<float, float>(a, lds);
+  else if (a.in_f32) logits_adjust<float, uint16_t>(a, lds);
+  else if (a.out_f32) logits_adjust<uint16_t, float>(a, lds);
+  else logits_adjust<uint16_t, uint16_t>(a, lds);
+}

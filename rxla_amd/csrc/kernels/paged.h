@@ -13,19 +13,38 @@ struct PagedPlace {
   int64_t page;
   int at;
 };
+// (As any_sequence, the starts beside the offsets: what the row's position needs is in the
+// lanes when its sequence is known, and the page table is the next thing that is waited for.)
 template <typename Args>
 __device__ __forceinline__ PagedPlace paged_place(const Args &a, int64_t t) {
-  int64_t b = t, i = 0;
+  int64_t b = t, pos;
   if (a.offsets) {
-    b = any_sequence(a.offsets, a.B, t);
-    if (b < 0 || t >= a.offsets[b + 1]) return PagedPlace{-1, -1};
-    i = t - a.offsets[b];
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = a.B;
+    while (n > 64) {
+      const int step = (n + 63) / 64, i = lo + lane * step;
+      const unsigned long long le = __ballot(lane * step < n && a.offsets[i < a.B ? i : a.B] <= t);
+      const int c = __popcll(le);
+      if (c == 0) return PagedPlace{-1, -1};
+      const int skip = (c - 1) * step;
+      lo += skip;
+      n = n - skip < step ? n - skip : step;
+    }
+    const int i = lo + lane < a.B ? lo + lane : a.B;
+    const int first = a.offsets[i], start = i < a.B ? a.starts[i] : 0;
+    const int c = __popcll(__ballot(lane < n && first <= t));
+    if (c == 0) return PagedPlace{-1, -1};
+    b = lo + c - 1;
+    const int64_t end = c < 64 ? __builtin_amdgcn_readlane(first, c) : a.offsets[b + 1];
+    if (t >= end) return PagedPlace{-1, -1};
+    pos = (int64_t)__builtin_amdgcn_readlane(start, c - 1) + (t - __builtin_amdgcn_readlane(first, c - 1));
+  } else {
+    pos = a.starts[b];
   }
-  const int64_t pos = a.starts[b] + i;
   if (pos < 0 || pos >= (int64_t)a.M * a.ps) return PagedPlace{-1, 0};
-  const int slot = (int)(pos / a.ps);
+  const int slot = (int)((uint32_t)pos / (uint32_t)a.ps);  // (positions of a table are 31 bits)
   const int64_t page = a.table[b * a.M + slot];
-  return PagedPlace{page < a.P ? page : -1, (int)(pos - (int64_t)slot * a.ps)};
+  return PagedPlace{page < a.P ? page : -1, (int)pos - slot * a.ps};
 }
 
 struct PagedDecodeArgs {

@@ -118,7 +118,8 @@ static bool same_shape(const Buffer *a, const Buffer *b) {
 // Workgroups of `threads` that one launch takes: 2^32 - 1 threads
 constexpr int64_t grid_max(int threads) { return (((int64_t)1 << 32) - 1) / threads; }
 constexpr int64_t kAnyMaxD = 512;  // RXW8_ATTN_ANY_MAX_D
-constexpr int64_t kLogitsChunk = 2048;  // words of a workgroup, at least
+constexpr int64_t kLogitsChunk = 4096;   // words of a workgroup, 8 a thread
+constexpr size_t kLogitsValues = 512;    // biases that it keeps in LDS
 static int page_kind(const Buffer *pages) { return pages->dtype == RXW8_U8 ? 2 : pages->dtype == RXW8_F32 ? 1 : 0; }
 
 // Whether the buffers (NULL ones aside) are the runtime's, and none of the first `written`
@@ -514,10 +515,10 @@ int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer 
                 (float *)v_scales->ptr, (const int32_t *)table->ptr, (const int32_t *)starts->ptr,
                 offsets ? (const int32_t *)offsets->ptr : nullptr, T, k_pages->dims[0], (int)table->dims[0],
                 (int)table->dims[1], (int)k->dims[1], (int)k->dims[2], (int)k_pages->dims[2], k->dtype == RXW8_F32};
-  if ((a.D != 64 && a.D != 128 && a.D != 256 && a.D != 512) ||
+  if ((a.D != 64 && a.D != 128 && a.D != 256 && a.D != 512) || row_parts(k) > 65535 ||
       ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
     return launch(rt, "rxw8_q8_append_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
-  return launch(rt, "rxw8_q8_append", dim3((unsigned)((T * row_parts(k) + 3) / 4)), dim3(256), a);
+  return launch(rt, "rxw8_q8_append", dim3((unsigned)((T + 3) / 4), (unsigned)row_parts(k)), dim3(256), a);
 }
 
 int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pages, rxw8_buffer *k_scales,
@@ -538,9 +539,9 @@ int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages, rxw8_buffer *v_pa
                   (const int32_t *)starts->ptr, offsets ? (const int32_t *)offsets->ptr : nullptr, T,
                   k_pages->dims[0], (int)table->dims[0], (int)table->dims[1], (int)k->dims[1], (int)k->dims[2],
                   (int)k_pages->dims[2], page_kind(k_pages), k->dtype == RXW8_F32};
-  if (a.D % 8 || ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
+  if (a.D % 8 || row_parts(k) > 65535 || ((uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.kp | (uintptr_t)a.vp) & 15)
     return launch(rt, "rxw8_q8_read_any", dim3((unsigned)((T * a.Hkv + 3) / 4)), dim3(256), a);
-  return launch(rt, "rxw8_q8_read", dim3((unsigned)((T * row_parts(k) + 3) / 4)), dim3(256), a);
+  return launch(rt, "rxw8_q8_read", dim3((unsigned)((T + 3) / 4), (unsigned)row_parts(k)), dim3(256), a);
 }
 
 int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q, rxw8_buffer *k_pages, rxw8_buffer *v_pages,
@@ -656,7 +657,7 @@ static int check_logits(const rxw8_logits_options *o, const Buffer *logits) {
   for (const rxw8_buffer *x : {o->tokens, o->bias})
     if (x && x->dims[0] > INT32_MAX)
       return fail(RXW8_UNIMPLEMENTED, "%s: %lld entries exceed 32-bit offsets", what, (long long)x->dims[0]);
-  if (B > grid_max(256) / ((V + kLogitsChunk - 1) / kLogitsChunk))
+  if (B > grid_max(kLogitsChunk / 8) / ((V + kLogitsChunk - 1) / kLogitsChunk))
     return fail(RXW8_UNIMPLEMENTED, "%s: %lld rows exceed the kernel's grid", what, (long long)B);
   return RXW8_OK;
 }
@@ -680,14 +681,10 @@ int rxw8_adjust_logits_into(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_lo
                f32(o->frequency), f32(o->presence), i32(o->bias_words), f32(o->bias), i32(o->bias_offsets),
                (const uint32_t *)i32(o->mask), i32(o->mask_rows), o->tokens ? o->tokens->dims[0] : 0,
                o->bias ? o->bias->dims[0] : 0, o->mask ? o->mask->dims[0] : 0, V, logits->dtype == RXW8_F32,
-               out->dtype == RXW8_F32, 0, 0};
+               out->dtype == RXW8_F32, (int)kLogitsChunk, (int)((V + kLogitsChunk - 1) / kLogitsChunk)};
   const bool pieces = V % 8 == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15);
-  const int times = B * V <= 2 * kLogitsChunk * rt->cus ? 1 : 2;
-  a.chunk = (int)(kLogitsChunk * times), a.chunks = (int)((V + a.chunk - 1) / a.chunk);
-  char kname[40];
-  std::snprintf(kname, sizeof kname, pieces ? "rxw8_logits_adjust%d" : "rxw8_logits_any", times);
-  return launch(rt, kname, dim3((unsigned)(B * a.chunks)), dim3(256), a,
-                sizeof(int) * (size_t)a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr)));
+  return launch(rt, pieces ? "rxw8_logits_adjust" : "rxw8_logits_any", dim3((unsigned)(B * a.chunks)), dim3(kLogitsChunk / 8), a,
+                sizeof(int) * (size_t)a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr)) + (a.bias ? kLogitsValues * sizeof(float) : 0));
 }
 
 int rxw8_adjust_logits(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_logits_options *o, int out_dtype,

@@ -238,3 +238,32 @@ def test_decode8_scales_far_apart(rt, d):
     vs *= np.float32(10) ** rng.integers(-12, 13, vs.shape).astype(np.float32)
     ks *= np.float32(10) ** rng.integers(-3, 3, ks.shape).astype(np.float32)
     check(decode8(rt, q, "f32", kc, vc, ks, vs, table, lens), *want8(q, kc, vc, ks, vs, table, lens))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_append_codes_at_the_middle(rt, kind):
+    """Every quotient near the middle between two codes: values (k + 1/2) s and the ones beside them, for
+    scales of every mantissa length (all ones among them) and rows whose largest is an odd multiple."""
+    r, rng = rx(), np.random.default_rng(9)
+    t, hkv, d = 400, 2, 128
+    amax = (1 + rng.random((t, hkv, 1))).astype(np.float32) * np.float32(2) ** rng.integers(-30, 100, (t, hkv, 1)).astype(np.float32)
+    amax[:8] = np.nextafter(np.float32(2), np.float32(0)) * np.float32(127) * np.float32(2) ** np.arange(8, dtype=np.float32)[:, None, None]
+    if kind == "bf16":
+        amax = ref.bf16_value(ref.bf16_bits(amax))
+    s = more.encode(amax)[1][..., None]
+    half = (rng.integers(-126, 126, (t, hkv, d)) + 0.5) * s.astype(np.float64)
+    x = half.astype(np.float32)
+    if kind == "bf16":
+        x = ref.bf16_value(ref.bf16_bits(x))
+    else:
+        for _ in range(2):
+            x = np.where(rng.random(x.shape) < 0.3, np.nextafter(x, np.float32(np.inf)), x)
+            x = np.where(rng.random(x.shape) < 0.3, np.nextafter(x, np.float32(-np.inf)), x)
+    x[..., :1] = amax
+    x = np.clip(x, -amax, amax)
+    pages, scales = [rt.zeros((t, hkv, 16, d), r.DType.U8) for _ in range(2)], [rt.zeros((t, hkv, 16), r.DType.F32) for _ in range(2)]
+    r.paged_kv_append_q8(rt, *pages, *scales, up(rt, x, kind), up(rt, -x, kind), i32(rt, np.arange(t)[:, None]), i32(rt, np.zeros(t)))
+    for sign, p, q in ((1, *[pages[0], scales[0]]), (-1, *[pages[1], scales[1]])):
+        c, want = more.encode(sign * x)
+        np.testing.assert_array_equal(q.to_numpy()[:, :, 0], want)
+        np.testing.assert_array_equal(p.to_numpy()[:, :, 0], c)
