@@ -33,21 +33,24 @@
 // V rows that a tile's last key or a missing page leaves unseen are cleared in LDS
 // (their weights are zero, what they hold may be NaN); K's scores there are -inf.
 //
-// 8-bit rows come as codes, half the bytes, and their scales beside them by 4-byte
-// copies: a tile's K and V scales are under way with its K rows. A code less 128 is a
-// bf16 number exactly (8 bits), so the products are the bf16 rows' with the scales
-// outside: scores are times s_k, weights times s_v ahead of their split. V needs no
-// transposing reads: a lane takes D / 16 dims of its own of each of its keys, one read a
-// key, and converts byte n of four keys into the operand of product n; 32 keys at a
+// 8-bit rows come as codes, half the bytes, and their scales beside them by 4-byte copies: a
+// tile's K and V scales are under way with its K rows. What bounds them is the arithmetic
+// (a vector instruction takes four cycles of its SIMD), so everything there is in f16, which
+// has 8-bit numbers for two instructions a pair: a byte pair spread by a permute is a pair of
+// subnormals u 2^-24, and one packed fma gives (u - 128) 2^-9, exactly. Scores and weights
+// take the scales outside the products:
+//   q      times the power of two that brings its row's largest magnitude to 2^14: one part
+//          for bf16 (exact to 2^-39 of the largest), two for f32 (2^-24);
+//   p s_v  are held between 2^-24 and 2^15 by the row's reference, which need not be the
+//          scores' maximum: p = exp2(s - ref), and where a tile's largest weight passes 2^15,
+//          ref moves so that it is 2^10. No maximum is taken otherwise, of lanes or
+//          tiles. One f16 part behind a bf16 output (2^-12 of a weight, the output's rounding
+//          is 2^-9 of it), two behind an f32 one; what is below 2^-24 / 2^10 of the largest
+//          weight so far rounds to multiples of that.
+// V needs no transposing reads: a lane takes D / 16 dims of its own of each of its keys, one
+// read a key, and converts byte n of four keys into the operand of product n; 32 keys at a
 // time (16x16x32). What is not seen is masked at the scores and the weights: codes are
 // numbers whatever they hold.
-//
-// A sequence inside one wave's piece is written at once. Pieces of a sequence are
-// joined in the order of its keys: the waves' in LDS, then, if it passes a
-// workgroup's piece, by the last of its workgroups to arrive, over (max, sum, acc)
-// records in device memory (at most two a workgroup). Those are stored and copied
-// past the dies' own caches, around an arrival counter that the last one sets back to
-// zero.
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -85,8 +88,9 @@ struct Deal {
 constexpr int kPagedWaves = 8;
 
 enum { kBf16, kF32, kCodes };  // what pages hold
-// q's type: as the arguments say, or one that a kernel is made for (beside f32 pages: all one)
-enum { kQAny, kQBf16, kQF32 };
+// What q and the output are, for the parts that bf16 products take: as the arguments say;
+// both bf16; or anything, in the three parts of f32 (beside f32 pages all are one)
+enum { kAny, kLow, kHigh };
 
 template <int D, int KIND>
 struct PagedTile {
@@ -164,6 +168,36 @@ __device__ __forceinline__ int scan64(int v) {
   return v;
 }
 
+// f(0), f(1), .., f(N - 1) with constants for arguments
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    unrolled<N, I + 1>(f);
+  }
+}
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+// Codes as f16 pairs of (u - 128) 2^-9: byte i of x and byte j of y
+template <int I, int J>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t x, uint32_t y) {
+  const f16x2 u = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(y, x, 0x0c000c00u | (4 + J) << 16 | I));
+  const f16x2 up = {(_Float16)32768.f, (_Float16)32768.f}, less = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, up, less));
+}
+constexpr float kCodeUnit = 0x1p9f;
+// Two f32 as an f16 pair, round to nearest even, and what that leaves
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2));
+}
+__device__ __forceinline__ uint32_t rest_f16x2(float a, float b, uint32_t part) {
+  const f16x2 h = __builtin_bit_cast(f16x2, part);
+  return pack_f16x2(a - (float)h[0], b - (float)h[1]);
+}
+__device__ __forceinline__ f32x4 mfma_f16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
 struct Piece {  // of a sequence, that one wave or workgroup went over
   int b, first, n;  // sequence; its first tile in the head's run; its tiles
 };
@@ -183,48 +217,74 @@ __device__ __forceinline__ void dma4(const void *from, uint32_t lds) {
 
 // What a wave holds for CT x 16 query rows (columns of the products) of one kv head: q, O
 // and the softmax, and the steps over a tile in its memory `mem` (K, V, scales).
-template <int D, int KIND, int CT, int Q>
+template <int D, int KIND, int CT, int PREC>
 struct PagedWave {
   using T = PagedTile<D, KIND>;
   static constexpr bool F32 = T::F32, CODES = T::CODES;
   static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row's q per lane
-  static constexpr int NL = F32 || Q == kQBf16 ? 1 : NQ;  // (f32 q over bf16 and 8-bit rows: three parts)
+  // an f32 q's further parts: two over bf16 rows, one over codes
+  static constexpr int NL = F32 || PREC == kLow ? 1 : NQ, NE = CODES ? 1 : NL;
   typedef const __attribute__((address_space(3))) char *Lds;
 
   struct Tile {
     int t, seen, holes;             // its number, keys in it; bit s: its 16-key piece s has no page
-    int64_t off[T::SUB];            // bytes from the pool's start
   };
 
   const PagedDecodeArgs &a;
   const int lane, col, g4, h;
-  char *const mem;
-  u32x4 q[CT][NQ], ql[CT][NL], qe[CT][NL];
+  // the walk over a page table: its entries and positions, the next tile, the entry and the
+  // 16-key piece within its page that it begins at, its pieces' pages (on their way while
+  // the tile before is worked on); of the tile last begun, bytes from the pool's start
+  const int32_t *table;
+  int entries, len, t, e, r, page[T::SUB];
+  int64_t off[T::SUB];
+  const uint32_t mem;               // LDS address of the wave's K, V and scales
+  u32x4 q[CT][NQ], ql[CT][NL], qe[CT][NE];
   f32x4 o[CT][D / 16], s[CT][T::SUB];
   f32x4 vs[CODES ? T::SUB : 1];     // V's scales
-  float m[CT], l[CT];
+  float m[CT], l[CT];               // (codes: m is the reference)
+  float unit[CODES ? CT : 1];       // codes: what a product of q and codes counts in a score, but for s_k
 
   __device__ RXW8_INLINE PagedWave(const PagedDecodeArgs &a, int h, char *mem)
-      : a(a), lane(threadIdx.x & 63), col(lane & 15), g4(lane >> 4), h(h), mem(mem) {}
+      : a(a), lane(threadIdx.x & 63), col(lane & 15), g4(lane >> 4), h(h), mem(lds_addr(mem)) {}
 
-  // Tile t of the `len` positions that `table` has the pages of
-  __device__ RXW8_INLINE Tile tile(const int32_t *table, int len, int t) const {
+  // Walks on at tile t0 of the `n` positions that `pages` [m] has the pages of
+  __device__ RXW8_INLINE void begin(const int32_t *pages, int m, int n, int t0) {
+    const unsigned sub = (unsigned)(t0 * T::SUB), ps16 = (unsigned)a.ps >> 4;
+    table = pages, entries = m, len = n, t = t0;
+    e = (int)(sub / ps16), r = (int)(sub - e * ps16);
+    look();
+  }
+  __device__ RXW8_INLINE void look() {
+    int e1 = e, r1 = r;
+#pragma unroll
+    for (int u = 0; u < T::SUB; ++u) {
+      page[u] = uniform_load(table, min(e1, entries - 1));
+      if (++r1 == a.ps >> 4) r1 = 0, ++e1;
+    }
+  }
+  // The next tile
+  __device__ RXW8_INLINE Tile tile() {
     Tile x;
-    const int ps16 = a.ps >> 4;
     x.t = t, x.holes = 0;
     x.seen = min(len - t * T::KT, T::KT);
 #pragma unroll
     for (int u = 0; u < T::SUB; ++u) {
-      const unsigned sub = (unsigned)(t * T::SUB + (16 * u < x.seen ? u : 0));
-      const unsigned e = sub / (unsigned)ps16;
-      int page = uniform_load(table, e);
-      if (page < 0 || page >= a.P) page = 0, x.holes |= 1 << u;
-      x.off[u] = (((int64_t)page * a.Hkv + h) * a.ps + 16 * (int)(sub - e * ps16)) * T::ROW;
+      if (16 * u >= x.seen) {
+        off[u] = off[0];
+        continue;
+      }
+      int id = page[u];
+      if (id < 0 || id >= a.P) id = 0, x.holes |= 1 << u;
+      off[u] = (((int64_t)id * a.Hkv + h) * a.ps + 16 * r) * T::ROW;
+      if (++r == a.ps >> 4) r = 0, ++e;
     }
+    ++t;
+    look();
     return x;
   }
-  __device__ RXW8_INLINE void copy(const void *pool, const Tile &x, int half) const {
-    const uint32_t dst = lds_addr(mem) + half * T::HALF;
+  __device__ RXW8_INLINE void copy(const void *pool, int half) const {
+    const uint32_t dst = mem + half * T::HALF;
     const int lrow = lane / T::CH, lch = lane % T::CH;
 #pragma unroll
     for (int i = 0; i < T::N; ++i) {
@@ -232,29 +292,68 @@ struct PagedWave {
       int from = row & 15;
       // (V's codes: keys j, 4 + j, 8 + j, 12 + j beside one another, which a read takes)
       if (CODES && half) from = 4 * (from & 3) + (from >> 2);
-      dma16((const char *)pool + x.off[i * T::RPI / 16], (uint32_t)from * T::ROW + ((lch ^ sx) << 4), dst + 1024 * i);
+      dma16((const char *)pool + off[i * T::RPI / 16], (uint32_t)from * T::ROW + ((lch ^ sx) << 4), dst + 1024 * i);
     }
   }
-  __device__ RXW8_INLINE void copy_k(const Tile &x) const {
-    copy(a.kp, x, 0);
+  // The copies of the tile last begun
+  __device__ RXW8_INLINE void copy_k() const {
+    copy(a.kp, 0);
     if constexpr (CODES) {
 #pragma unroll
       for (int i = 0; i < T::NS; ++i) {
         const int at = 64 * i + lane, key = at & (T::KT - 1);  // K's KT scales, then V's
-        int64_t off = x.off[0];
+        int64_t from = off[0];
 #pragma unroll
-        for (int u = 1; u < T::SUB; ++u) off = key >> 4 == u ? x.off[u] : off;
-        dma4((const char *)(at < T::KT ? a.ks : a.vs) + off / T::ROW * 4 + 4 * (key & 15), lds_addr(mem) + 2 * T::HALF + 256 * i);
+        for (int u = 1; u < T::SUB; ++u) from = key >> 4 == u ? off[u] : from;
+        dma4((const char *)(at < T::KT ? a.ks : a.vs) + from / T::ROW * 4 + 4 * (key & 15), mem + 2 * T::HALF + 256 * i);
       }
     }
   }
-  __device__ RXW8_INLINE void copy_v(const Tile &x) const { copy(a.vp, x, 1); }
+  __device__ RXW8_INLINE void copy_v() const { copy(a.vp, 1); }
 
-  __device__ RXW8_INLINE bool q_f32() const { return Q == kQAny ? a.q_f32 : Q == kQF32; }
-  // q of the lane's row of column tile c, at element qo
-  __device__ RXW8_INLINE void load_q(int c, int64_t qo) {
+  __device__ RXW8_INLINE bool q_parts() const { return PREC == kAny ? a.q_f32 : PREC == kHigh; }
+  __device__ RXW8_INLINE bool p_parts() const { return PREC == kAny ? a.out_f32 : PREC == kHigh; }
+  __device__ RXW8_INLINE void load_q_f16(int c, int64_t qo) {
+    float x[NQ][8];
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
+      const int64_t at = qo + 64 * (i >> 1) + 16 * g4 + 8 * (i & 1);
+      if (PREC != kLow && a.q_f32) {
+        const f32x4 r[2] = {*(const f32x4 *)((const float *)a.q + at), *(const f32x4 *)((const float *)a.q + at + 4)};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[i][k] = r[k >> 2][k & 3];
+      } else {
+        const u32x4 r = *(const u32x4 *)((const uint16_t *)a.q + at);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[i][k] = __uint_as_float(k & 1 ? r[k >> 1] & 0xffff0000u : r[k >> 1] << 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
+    uint2 two = pair_xor16(__uint_as_float(top));
+    two = pair_xor32(__uint_as_float(max(two.x, two.y)));
+    // 2^14 / 2^e, e the exponent of the largest
+    const int scale = min(127 + 14 + 127 - (int)(max(two.x, two.y) >> 23), 254);
+    const float up = __uint_as_float((uint32_t)scale << 23);
+    unit[c] = a.c * kCodeUnit * __uint_as_float((uint32_t)(254 - scale) << 23);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float y = x[i][2 * k] * up, z = x[i][2 * k + 1] * up;
+        q[c][i][k] = pack_f16x2(y, z);
+        if constexpr (PREC != kLow) ql[c][NL > 1 ? i : 0][k] = rest_f16x2(y, z, q[c][i][k]);
+      }
+  }
+  // q of the lane's row of column tile c, at element qo
+  __device__ RXW8_INLINE void load_q(int c, int64_t qo) {
+    if constexpr (CODES) load_q_f16(c, qo);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      if constexpr (CODES) break;
       if constexpr (F32) {
         const int64_t at4 = qo + 16 * i + 4 * g4;
         if (a.q_f32) {
@@ -264,17 +363,18 @@ struct PagedWave {
           q[c][i] = u32x4{r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
         }
       } else {
-        const int64_t at8 = qo + (CODES ? 64 * (i >> 1) + 16 * g4 + 8 * (i & 1) : 32 * i + 8 * g4);
-        if (q_f32()) {
+        const int64_t at8 = qo + 32 * i + 8 * g4;
+        if (PREC != kLow && a.q_f32) {
           const f32x4 r[2] = {*(const f32x4 *)((const float *)a.q + at8), *(const f32x4 *)((const float *)a.q + at8 + 4)};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             uint32_t x[3];
             split_bf16x2(r[e >> 1][2 * (e & 1)], r[e >> 1][2 * (e & 1) + 1], x);
-            q[c][i][e] = x[0], ql[c][NL > 1 ? i : 0][e] = x[1], qe[c][NL > 1 ? i : 0][e] = x[2];
+            q[c][i][e] = x[0], ql[c][NL > 1 ? i : 0][e] = x[1], qe[c][NE > 1 ? i : 0][e] = x[2];
           }
         } else {
           q[c][i] = *(const u32x4 *)((const uint16_t *)a.q + at8);
+          if constexpr (PREC == kHigh) ql[c][NL > 1 ? i : 0] = qe[c][NE > 1 ? i : 0] = u32x4{0, 0, 0, 0};
         }
       }
     }
@@ -293,7 +393,7 @@ struct PagedWave {
 
   // S^T = K q^T of the tile whose K is there, for the first `ct` column tiles
   __device__ RXW8_INLINE void scores(int ct) {
-    const uint32_t kf = lds_addr(mem) + col * T::ROW;
+    const uint32_t kf = mem + col * T::ROW;
     constexpr int NA = F32 ? 4 : 2;  // sums in turn: no product waits for the one before
 #pragma unroll
     for (int u = 0; u < T::SUB; ++u) {
@@ -306,10 +406,15 @@ struct PagedWave {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           if (c && c >= ct) break;
+          if constexpr (CODES) {
+            acc[c][n & 1] = mfma_f16(f, q[c][n], acc[c][n & 1]);
+            if constexpr (PREC != kLow) acc[c][~n & 1] = mfma_f16(f, ql[c][NL > 1 ? n : 0], acc[c][~n & 1]);
+            continue;
+          }
           acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[c][n]), acc[c][n & 1]);
-          if (q_f32()) {
+          if (q_parts()) {
             acc[c][~n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[c][NL > 1 ? n : 0]), acc[c][~n & 1]);
-            acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][NL > 1 ? n : 0]), acc[c][n & 1]);
+            acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][NE > 1 ? n : 0]), acc[c][n & 1]);
           }
         }
       };
@@ -328,8 +433,8 @@ struct PagedWave {
         } else if constexpr (CODES) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const uint2 x = u8x4_to_signed_bf16x4(f[2 * k]), y = u8x4_to_signed_bf16x4(f[2 * k + 1]);
-            add(2 * n + k, u32x4{x.x, x.y, y.x, y.y});
+            const uint32_t x = f[2 * k], y = f[2 * k + 1];
+            add(2 * n + k, u32x4{codes_f16<0, 1>(x, x), codes_f16<2, 3>(x, x), codes_f16<0, 1>(y, y), codes_f16<2, 3>(y, y)});
           }
         } else {
           add(n, f);
@@ -337,15 +442,15 @@ struct PagedWave {
       }
       f32x4 scale = f32x4{a.c, a.c, a.c, a.c};
       if constexpr (CODES) {
-        const uint32_t at = lds_addr(mem) + 2 * T::HALF + 4 * (16 * u + 4 * g4);
-        scale = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)at * a.c;
+        const uint32_t at = mem + 2 * T::HALF + 4 * (16 * u + 4 * g4);
+        scale = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)at;
         vs[u] = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(at + 4 * T::KT);
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         s[c][u] = acc[c][0] + acc[c][1];
         if constexpr (F32) s[c][u] += acc[c][2] + acc[c][3];
-        s[c][u] *= scale;
+        s[c][u] *= CODES ? scale * unit[CODES ? c : 0] : scale;
       }
     }
   }
@@ -355,6 +460,10 @@ struct PagedWave {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       if (c && c >= ct) break;
+      if constexpr (CODES) {
+        softmax_codes(c, x, part);
+        continue;
+      }
       float mt = kMinusInf;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u)
@@ -378,9 +487,57 @@ struct PagedWave {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(s[c][u][r] - ref);
           l[c] += p;
-          s[c][u][r] = !CODES ? p : part && (16 * u + 4 * g4 + r >= x.seen || (x.holes >> u & 1)) ? 0.f : p * vs[CODES ? u : 0][r];
+          s[c][u][r] = p;
         }
     }
+  }
+
+  __device__ RXW8_INLINE void softmax_codes(int c, const Tile &x, bool part) {
+    f32x4 w[T::SUB];
+    float sum, top;
+    if (part) {
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * u + 4 * g4 + r >= x.seen || (x.holes >> u & 1)) s[c][u][r] = kMinusInf, vs[u][r] = 0.f;
+    }
+    auto weigh = [&]() RXW8_INLINE {
+      const float ref = m[c] == kMinusInf ? 0.f : m[c];
+      sum = top = 0.f;
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(s[c][u][r] - ref);
+          sum += p;
+          w[u][r] = p * vs[u][r];
+          top = fmaxf(top, fabsf(w[u][r]));
+        }
+    };
+    weigh();
+    if (__ballot(top > 0x1p15f || m[c] == kMinusInf)) {
+      // the largest weight becomes 2^10; a key that it leaves far behind the largest score
+      // (a scale of 0) not more than 2^100
+      float largest = kMinusInf, highest = kMinusInf;
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          largest = fmaxf(largest, s[c][u][r] + fminf(__builtin_amdgcn_logf(fabsf(vs[u][r])), 128.f));
+          highest = fmaxf(highest, s[c][u][r]);
+        }
+      const float to = fmaxf(m[c], fmaxf(max4(largest) - 10.f, max4(highest) - 100.f));
+      const float f = to == kMinusInf ? 1.f : exp2f(m[c] - to);
+      m[c] = to;
+      l[c] *= f;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) o[c][n] *= f;
+      weigh();
+    }
+    l[c] += sum;
+#pragma unroll
+    for (int u = 0; u < T::SUB; ++u) s[c][u] = w[u];
   }
 
   // V rows that are not seen, cleared
@@ -390,14 +547,14 @@ struct PagedWave {
     for (int n = 0; n < T::N; ++n) {
       const int row = n * T::RPI + lrow;
       if (row >= x.seen || (x.holes >> (row >> 4) & 1))
-        *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(lds_addr(mem) + T::HALF + 1024 * n + 16 * lane) = u32x4{0, 0, 0, 0};
+        *(__attribute__((address_space(3))) u32x4 *)(uintptr_t)(mem + T::HALF + 1024 * n + 16 * lane) = u32x4{0, 0, 0, 0};
     }
     wait_lds();
   }
 
   // O^T += V^T P^T of the tile whose V is there
   __device__ RXW8_INLINE void values(int ct) {
-    const uint32_t v0 = lds_addr(mem) + T::HALF;
+    const uint32_t v0 = mem + T::HALF;
     if constexpr (F32) {
       const uint32_t vf = v0 + 4 * g4 * T::ROW + 16 * col;
 #pragma unroll
@@ -417,12 +574,16 @@ struct PagedWave {
           }
       return;
     }
+    if constexpr (CODES) {
+      values_codes(ct, v0);
+      return;
+    }
     // weights in parts: three behind an f32 output, two behind a bf16 one
     struct Parts {
       uint2 k0, k1, k2;
     };
     auto parts = [&](f32x4 w) RXW8_INLINE {
-      if (a.out_f32) {
+      if (p_parts()) {
         uint32_t x[3], y[3];
         split_bf16x2<true>(w[0], w[1], x);
         split_bf16x2<true>(w[2], w[3], y);
@@ -433,56 +594,7 @@ struct PagedWave {
       split_bf16x2<true>(w[2], w[3], y);
       return Parts{uint2{x[0], y[0]}, uint2{x[1], y[1]}, uint2{0, 0}};
     };
-    if constexpr (CODES) {
-      constexpr int W = D / 64;  // dwords of a lane's dims of a key
-#pragma unroll
-      for (int u = 0; u < T::SUB; u += 2) {
-        uint32_t w[2][4][W];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t at = v0 + ((u + k) * 16 + 4 * j + g4) * T::ROW + 4 * W * col;
-            if constexpr (W == 1) {
-              w[k][j][0] = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)at;
-            } else if constexpr (W == 2) {
-              typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-              const u32x2 x = *(const __attribute__((address_space(3))) u32x2 *)(uintptr_t)at;
-              w[k][j][0] = x[0], w[k][j][1] = x[1];
-            } else {
-              const u32x4 x = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)at;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[k][j][i] = x[i];
-            }
-          }
-        Parts p[CT][2];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          if (c && c >= ct) break;
-          p[c][0] = parts(s[c][u]);
-          p[c][1] = parts(s[c][u + 1]);
-        }
-#pragma unroll
-        for (int n = 0; n < D / 16; ++n) {
-          u32x4 f;
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              auto code = [&](int key) RXW8_INLINE { return (float)(w[k][key][n >> 2] >> (8 * (n & 3)) & 0xffu) - 128.f; };
-              f[2 * k + j] = pack_bf16x2(code(2 * j), code(2 * j + 1));
-            }
-#pragma unroll
-          for (int c = 0; c < CT; ++c) {
-            if (c && c >= ct) break;
-            auto add = [&](uint2 x, uint2 y) RXW8_INLINE { o[c][n] = mfma16x16x32(as_bf16x8(f), as_bf16x8(u32x4{x.x, x.y, y.x, y.y}), o[c][n]); };
-            add(p[c][0].k0, p[c][1].k0);
-            add(p[c][0].k1, p[c][1].k1);
-            if (a.out_f32) add(p[c][0].k2, p[c][1].k2);
-          }
-        }
-      }
-    } else {
+    {
       const int tr_j = col >> 2, tr_q = col & 3;
       const uint32_t vf = v0 + (4 * g4 + tr_j) * T::ROW + 8 * (tr_q & 1);
 #pragma unroll
@@ -505,10 +617,58 @@ struct PagedWave {
             };
             add(p[c].k0);
             add(p[c].k1);
-            if (a.out_f32) add(p[c].k2);
+            if (p_parts()) add(p[c].k2);
           }
         }
       }
+    }
+  }
+
+  __device__ RXW8_INLINE void values_codes(int ct, uint32_t v0) {
+    constexpr int W = D / 64;  // dwords of a lane's dims of a key
+#pragma unroll
+    for (int u = 0; u < T::SUB; u += 2) {
+      uint32_t w[2][4][W];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t at = v0 + ((u + k) * 16 + 4 * j + g4) * T::ROW + 4 * W * col;
+          if constexpr (W == 1) {
+            w[k][j][0] = *(const __attribute__((address_space(3))) uint32_t *)(uintptr_t)at;
+          } else if constexpr (W == 2) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 x = *(const __attribute__((address_space(3))) u32x2 *)(uintptr_t)at;
+            w[k][j][0] = x[0], w[k][j][1] = x[1];
+          } else {
+            const u32x4 x = *(const __attribute__((address_space(3))) u32x4 *)(uintptr_t)at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[k][j][i] = x[i];
+          }
+        }
+      u32x4 p[CT], rest[PREC == kLow ? 1 : CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        if (c && c >= ct) break;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = s[c][u + (i >> 1)][2 * (i & 1)], y = s[c][u + (i >> 1)][2 * (i & 1) + 1];
+          p[c][i] = pack_f16x2(x, y);
+          if constexpr (PREC != kLow) rest[c][i] = rest_f16x2(x, y, p[c][i]);
+        }
+      }
+      auto dim = [&](auto n) RXW8_INLINE {  // byte n % 4 of dword n / 4 of eight keys
+        constexpr int N = decltype(n)::value, I = N & 3, i = N >> 2;
+        const u32x4 f = {codes_f16<I, I>(w[0][0][i], w[0][1][i]), codes_f16<I, I>(w[0][2][i], w[0][3][i]),
+                         codes_f16<I, I>(w[1][0][i], w[1][1][i]), codes_f16<I, I>(w[1][2][i], w[1][3][i])};
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (c && c >= ct) break;
+          o[c][N] = mfma_f16(f, p[c], o[c][N]);
+          if constexpr (PREC != kLow) o[c][N] = mfma_f16(f, rest[PREC == kLow ? 0 : c], o[c][N]);
+        }
+      };
+      unrolled<D / 16>(dim);
     }
   }
 
@@ -520,6 +680,7 @@ struct PagedWave {
     f32x4 y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = o[c][(i & ~3) + r][i & 3];
+    if (CODES) y *= kCodeUnit;
     return y;
   }
   __device__ RXW8_INLINE int quad_dim(int i) const {
@@ -546,10 +707,10 @@ __device__ __forceinline__ PagedPlaceOf paged_place_of(const PagedDecodeArgs &a)
   return PagedPlaceOf{(int)(blockIdx.x % heads), (int)(blockIdx.x / heads), a.units, nullptr};
 }
 
-template <int D, int KIND, bool RECORDS = false, int Q = kQAny>
+template <int D, int KIND, bool RECORDS = false, int PREC = kAny>
 __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf place) {
   using T = PagedTile<D, KIND>;
-  using Wave = PagedWave<D, KIND, 1, Q>;
+  using Wave = PagedWave<D, KIND, 1, PREC>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Piece piece[kPagedWaves][2];
   __shared__ int last_one[2];
@@ -609,9 +770,10 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       int b, n;
     };
     Wave w(a, h, mem);
+    w.begin(a.table + (int64_t)b * a.M, a.M, ah.len, t);
     auto next = [&](bool more) {  // the tile that `ah` stands at; `more`: another one follows
       Tile x;
-      (typename Wave::Tile &)x = w.tile(a.table + (int64_t)ah.b * a.M, ah.len, ah.t);
+      (typename Wave::Tile &)x = w.tile();
       x.b = ah.b, x.n = ah.n;
       if (more && ++ah.t == ah.n) {
         do {
@@ -620,6 +782,7 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
         } while (ah.len == 0);
         ah.n = tiles_of(ah.len);
         ah.t = 0;
+        w.begin(a.table + (int64_t)ah.b * a.M, a.M, ah.len, 0);
       }
       return x;
     };
@@ -669,8 +832,8 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
     start(b);
     cur = next(left > 1);
     w.wait_q();
-    w.copy_k(cur);
-    w.copy_v(cur);
+    w.copy_k();
+    w.copy_v();
 
     int begun = cur.t;  // the tile at which this wave began the sequence
     for (;;) {
@@ -680,7 +843,7 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       const Tile done = cur;
       if (left > 1) {
         cur = next(left > 2);
-        w.copy_k(cur);
+        w.copy_k();
       }
       const bool part = done.seen < T::KT || done.holes;
       w.softmax(done, part, 1);
@@ -689,7 +852,7 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       if (part && KIND != kCodes) w.clear_v(done);
       w.values(1);
       wait_lds();
-      if (left > 1) w.copy_v(cur);
+      if (left > 1) w.copy_v();
       // ---- the sequence's end, or the wave's
       const bool ends = done.t == done.n - 1;
       if (ends || left == 1) {

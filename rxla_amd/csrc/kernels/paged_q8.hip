@@ -289,10 +289,13 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_q8_decode_any(PagedDecode
   any_store(all, a.out, at, a.D, a.out_f32);
 }
 
-#define RXW8_Q8_DECODE(D)                                                                     \
-  extern "C" __global__ void __launch_bounds__(64 * kPagedWaves) rxw8_q8_decode_d##D(PagedDecodeArgs a) { \
-    paged_decode<D, kCodes>(a, paged_place_of(a));                                            \
+#define RXW8_Q8_DECODE(D, NAME, PREC)                                                          \
+  extern "C" __global__ void __launch_bounds__(64 * kPagedWaves) rxw8_q8_decode##NAME##_d##D(PagedDecodeArgs a) { \
+    paged_decode<D, kCodes, false, PREC>(a, paged_place_of(a));                                \
   }
-RXW8_Q8_DECODE(64)
-RXW8_Q8_DECODE(128)
-RXW8_Q8_DECODE(256)
+RXW8_Q8_DECODE(64, , kLow)
+RXW8_Q8_DECODE(128, , kLow)
+RXW8_Q8_DECODE(256, , kLow)
+RXW8_Q8_DECODE(64, _high, kHigh)
+RXW8_Q8_DECODE(128, _high, kHigh)
+RXW8_Q8_DECODE(256, _high, kHigh)

@@ -67,9 +67,9 @@ namespace {
 constexpr float kPrefixTile = 0.5f;
 
 // Column tiles of a block: as many as leave no register spilled
-template <int D, int KIND, int Q>
+template <int D, int KIND, int PREC>
 constexpr int block_tiles() {
-  return D == 256 ? 1 : D == 128 ? (Q == kQF32 && KIND != kF32 ? 1 : 2) : Q == kQF32 || KIND == kCodes ? 2 : 4;
+  return D == 256 ? 1 : D == 128 ? (PREC == kHigh ? 1 : 2) : PREC == kHigh || KIND == kCodes ? 2 : 4;
 }
 
 // Group n's sequences within this launch's (relative to b0), blocks and tiles
@@ -105,11 +105,11 @@ __device__ __forceinline__ int tiles_before(const SharedArgs &a, int n, int &tot
 }  // namespace
 
 // Workgroup `unit` of `units` for the prefixes of kv head h, whose run has `total` tiles
-template <int D, int KIND, int Q>
+template <int D, int KIND, int PREC>
 __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int units, int total) {
   using T = PagedTile<D, KIND>;
-  constexpr int CT = block_tiles<D, KIND, Q>(), CB = 16 * CT, DP = D / 2;
-  using Wave = PagedWave<D, KIND, CT, Q>;
+  constexpr int CT = block_tiles<D, KIND, PREC>(), CB = 16 * CT, DP = D / 2;
+  using Wave = PagedWave<D, KIND, CT, PREC>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nw = a.d.waves, G = a.d.Hq / a.d.Hkv;
@@ -141,19 +141,19 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         const int i = min(block * CB + 16 * c + w.col, x.rows - 1), r = i / G;
         w.load_q(c, ((int64_t)(x.g0 + r) * a.d.Hq + h * G + (i - r * G)) * D);
       }
-      const int32_t *const table = a.prefixes + (int64_t)n * a.MP;
-      typename Wave::Tile cur = w.tile(table, x.len, first);
+      w.begin(a.prefixes + (int64_t)n * a.MP, a.MP, x.len, first);
+      typename Wave::Tile cur = w.tile();
       w.wait_q();
-      w.copy_k(cur);
-      w.copy_v(cur);
+      w.copy_k();
+      w.copy_v();
       for (;;) {
         wait_vm<T::N>();
         w.scores(ct);
         wait_lds();
         const typename Wave::Tile done = cur;
         if (left > 1) {
-          cur = w.tile(table, x.len, done.t + 1);
-          w.copy_k(cur);
+          cur = w.tile();
+          w.copy_k();
         }
         const bool part = done.seen < T::KT || done.holes;
         w.softmax(done, part, ct);
@@ -162,7 +162,7 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         if (part && KIND != kCodes) w.clear_v(done);
         w.values(ct);
         wait_lds();
-        if (left > 1) w.copy_v(cur);
+        if (left > 1) w.copy_v();
         if (--left == 0) break;
       }
     }
@@ -208,7 +208,7 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
   }
 }
 
-template <int D, int KIND, int Q>
+template <int D, int KIND, int PREC>
 __device__ RXW8_INLINE void shared_walk(const SharedArgs &a) {
   using T = PagedTile<D, KIND>;
   const int lane = threadIdx.x & 63, G = a.d.Hq / a.d.Hkv, HT = (G + 15) / 16, heads = a.d.Hkv * HT;
@@ -225,23 +225,23 @@ __device__ RXW8_INLINE void shared_walk(const SharedArgs &a) {
   up = prefix == 0 ? 0 : own == 0 ? units : min(max(up, 1), max(units - 1, 1));
   const int uo = own == 0 ? 0 : max(units - up, 1);
   if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = up * HT;
-  if (unit < up) prefix_walk<D, KIND, Q>(a, hk / HT, unit * HT + hk % HT, up * HT, prefix);
+  if (unit < up) prefix_walk<D, KIND, PREC>(a, hk / HT, unit * HT + hk % HT, up * HT, prefix);
   if (unit >= units - uo) {
     if (unit < up) __syncthreads();  // (one workgroup to a head does both)
-    paged_decode<D, KIND, true, Q>(a.d, PagedPlaceOf{hk, unit - (units - uo), uo, a.own});
+    paged_decode<D, KIND, true, PREC>(a.d, PagedPlaceOf{hk, unit - (units - uo), uo, a.own});
   }
 }
 
-#define RXW8_SHARED(D, NAME, KIND, Q)                                                              \
+#define RXW8_SHARED(D, NAME, KIND, PREC)                                                           \
   extern "C" __global__ void __launch_bounds__(64 * kPagedWaves) rxw8_shared_##NAME##_d##D(SharedArgs a) { \
-    shared_walk<D, KIND, Q>(a);                                                                    \
+    shared_walk<D, KIND, PREC>(a);                                                                 \
   }
-#define RXW8_SHARED_D(D)                 \
-  RXW8_SHARED(D, bf16, kBf16, kQBf16)    \
-  RXW8_SHARED(D, bf16_qf32, kBf16, kQF32) \
-  RXW8_SHARED(D, q8, kCodes, kQBf16)     \
-  RXW8_SHARED(D, q8_qf32, kCodes, kQF32) \
-  RXW8_SHARED(D, f32, kF32, kQAny)
+#define RXW8_SHARED_D(D)                   \
+  RXW8_SHARED(D, bf16, kBf16, kLow)        \
+  RXW8_SHARED(D, bf16_high, kBf16, kHigh)  \
+  RXW8_SHARED(D, q8, kCodes, kLow)         \
+  RXW8_SHARED(D, q8_high, kCodes, kHigh)   \
+  RXW8_SHARED(D, f32, kF32, kAny)
 RXW8_SHARED_D(64)
 RXW8_SHARED_D(128)
 RXW8_SHARED_D(256)

@@ -301,7 +301,7 @@ static int paged_decode_launch(Runtime *rt, PagedDecodeArgs a) {
   a.counters = (int *)block;
   a.part = (float *)(block + RXW8_NOALLOC_COUNTER_BYTES);
   char kname[40];
-  if (a.ks) std::snprintf(kname, sizeof kname, "rxw8_q8_decode_d%d", a.D);
+  if (a.ks) std::snprintf(kname, sizeof kname, "rxw8_q8_decode%s_d%d", a.q_f32 || a.out_f32 ? "_high" : "", a.D);
   else std::snprintf(kname, sizeof kname, "rxw8_paged_decode_%s_d%d", a.p_f32 ? "f32" : "bf16", a.D);
   return launch(rt, kname, dim3((unsigned)(heads * a.units)), dim3(512), a, wave * (size_t)a.waves);
 }
@@ -314,8 +314,8 @@ static int shared_launch(Runtime *rt, SharedArgs a) {
   const int64_t G = d.Hq / d.Hkv, HT = (G + 15) / 16, heads = d.Hkv * HT, rec = (int64_t)(d.D + 4) * sizeof(float);
   const PagedTiles t(a.kind, d.D);
   // block_tiles (kernels/shared.hip)
-  const bool split = d.q_f32 && a.kind != 1;
-  const int ct = d.D == 256 ? 1 : d.D == 128 ? (split ? 1 : 2) : split || a.kind == 2 ? 2 : 4;
+  const bool high = (d.q_f32 || d.out_f32) && a.kind != 1;
+  const int ct = d.D == 256 ? 1 : d.D == 128 ? (high ? 1 : 2) : high || a.kind == 2 ? 2 : 4;
   a.columns = 16 * ct, a.keys = t.keys;
   auto tiles = [&](int64_t m) { return (m * d.ps + t.keys - 1) / t.keys; };
   const int64_t blocks = (int64_t)d.B * G / a.columns + a.N;
@@ -345,7 +345,7 @@ static int shared_launch(Runtime *rt, SharedArgs a) {
   a.own = (float *)(recs + parts(d.units));
   a.whole = a.own + each * d.Hq * (d.D + 4);
   char kname[40];
-  std::snprintf(kname, sizeof kname, "rxw8_shared_%s%s_d%d", a.kind == 2 ? "q8" : a.kind == 1 ? "f32" : "bf16", split ? "_qf32" : "", d.D);
+  std::snprintf(kname, sizeof kname, "rxw8_shared_%s%s_d%d", a.kind == 2 ? "q8" : a.kind == 1 ? "f32" : "bf16", high ? "_high" : "", d.D);
   const int64_t B = d.B, q_size = d.q_f32 ? 4 : 2, out_size = d.out_f32 ? 4 : 2;
   for (int64_t b0 = 0; b0 < B; b0 += each) {
     SharedArgs c = a;

@@ -2,7 +2,12 @@
 the logits' adjustments. Attention's bounds are serving_ref's: an 8-bit value is
 (code - 128) s exactly, its score c s_k (q . codes) and its weight p s_v each take
 two roundings more, and joining the records of a row a few, which 8 half steps of
-f32 cover (`MORE`)."""
+f32 cover (`MORE`). Over 8-bit rows q and the weights go into the products in f16, whose
+half step is 2^-11: q in parts that leave 2^-22 of an element and 2^-39 of the row's
+largest, less than SPLIT of the sums of |q k|; weights in one part behind a bf16 output
+(`F16`), in two, 2^-22 and so less than SPLIT, behind an f32 one. A weight p s_v is a
+multiple of 2^-24 where the largest so far is 2^10 at least: half of that, 2^-35 of the
+largest, for each key and at most 127 units of its code (`grain`)."""
 import math
 
 import numpy as np
@@ -10,6 +15,34 @@ import numpy as np
 import serving_ref as ref
 
 MORE = 8 * ref.F32
+F16 = 2.0 ** -11
+
+
+def p_step(kind, out):
+    """What weights are rounded by, beside f32's own roundings."""
+    return (F16 if kind == "q8" and out == "bf16" else ref.SPLIT) + MORE
+
+
+def grain(q, k, vs, scale):
+    """Of one query row over keys k [n, D] whose values have the scales vs [n]."""
+    if k.shape[0] == 0:
+        return 0.0
+    s = (np.asarray(k, np.float64) @ np.asarray(q, np.float64)) * scale
+    w = np.exp(s - s.max())
+    return k.shape[0] * 2.0 ** -35 * 127 * float((w * np.abs(vs)).max() / w.sum())
+
+
+def decode8(q, kc, vc, ks, vs, table, lens, scale=None, out="f32"):
+    """(y, bound) of decode attention over codes and scales."""
+    step = ref.BF16 if out == "bf16" else ref.F32
+    y, bound = ref.paged_decode(q, value(kc, ks), value(vc, vs), table, lens, scale, p_step("q8", out), step)
+    g, c = q.shape[1] // kc.shape[1], scale or 1 / math.sqrt(q.shape[2])
+    for i in range(q.shape[0]):
+        for h in range(q.shape[1]):
+            n = max(0, int(lens[i]))
+            k = ref.paged_keys(value(kc, ks), table[i], n, h // g)
+            bound[i, h] += grain(q[i, h], k, ref.paged_keys(vs[..., None], table[i], n, h // g)[:, 0], c)
+    return y, bound
 
 
 def encode(x):
@@ -40,9 +73,9 @@ def read(pages, table, starts, offsets, total):
     return out
 
 
-def shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale=None, p_step=ref.SPLIT,
-           out_step=ref.F32):
-    """(y, bound) over pages of values."""
+def shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale=None, out="f32", vs=None):
+    """(y, bound) over pages of values; vs: the scales of V's codes."""
+    step, weights = ref.BF16 if out == "bf16" else ref.F32, p_step("bf16" if vs is None else "q8", out)
     b, hq, d = q.shape
     g = hq // kp.shape[1]
     y, bound = np.zeros((b, hq, d)), np.zeros((b, hq, d))
@@ -54,9 +87,12 @@ def shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale=None, p_
                     parts.insert(0, (prefixes[n], prefix_lens[n]))
             k, v = (np.concatenate([ref.paged_keys(x, t, max(0, int(n)), h) for t, n in parts])
                     for x in (kp, vp))
+            if vs is not None:
+                scales = np.concatenate([ref.paged_keys(vs[..., None], t, max(0, int(n)), h) for t, n in parts])[:, 0]
             for r in range(h * g, h * g + g):
-                y[i, r], bound[i, r] = ref.attend(q[i, r], k, v, scale or 1 / math.sqrt(d),
-                                                  p_step + MORE, out_step)
+                c = scale or 1 / math.sqrt(d)
+                y[i, r], bound[i, r] = ref.attend(q[i, r], k, v, c, weights, step)
+                bound[i, r] += 0 if vs is None else grain(q[i, r], k, scales, c)
     return y, bound
 
 

@@ -5,7 +5,7 @@ import pytest
 
 import serving_more_ref as more
 import serving_ref as ref
-from test_gpu_serving import STEP, check, down, dt, floats, make_pages, rx, up
+from test_gpu_serving import check, down, dt, floats, make_pages, rx, up
 
 pytestmark = pytest.mark.gpu
 
@@ -35,8 +35,7 @@ def decode8(rt, q, qk, kc, vc, ks, vs, table, lens, out="f32", scale=None, into=
 
 
 def want8(q, kc, vc, ks, vs, table, lens, scale=None, out="f32"):
-    return ref.paged_decode(q, more.value(kc, ks), more.value(vc, vs), table, lens, scale,
-                            ref.SPLIT + more.MORE, STEP[out])
+    return more.decode8(q, kc, vc, ks, vs, table, lens, scale, out)
 
 
 # ---- the append ------------------------------------------------------------------------

@@ -4,7 +4,7 @@ import pytest
 
 import serving_more_ref as more
 import serving_ref as ref
-from test_gpu_serving import STEP, check, down, dt, floats, make_pages, rx, up
+from test_gpu_serving import check, down, dt, floats, make_pages, rx, up
 
 pytestmark = pytest.mark.gpu
 
@@ -44,7 +44,7 @@ def run(rt, rng, prefix_lens, groups, lens, hq, hkv, d, kind, qk="f32", out="f32
     kp, vp, codes, prefixes, table = make(rng, prefix_lens, lens, hkv, ps, d, kind)
     q = floats(rng, (len(lens), hq, d), qk)
     y = call(rt, q, qk, kp, vp, codes, kind, prefixes, prefix_lens, groups, table, lens, out, scale, into)
-    check(y, *more.shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale, out_step=STEP[out]))
+    check(y, *more.shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, scale, out, codes and codes[3]))
     return y
 
 
@@ -119,7 +119,7 @@ def test_shared_what_is_not_seen(rt, d, kind, ps):
         x[np.broadcast_to(~seen[:, None, :, None], x.shape)] = fill
     q = floats(rng, (6, 8, d), "f32")
     y = call(rt, q, "f32", kp, vp, codes, kind, prefixes, prefix_lens, groups, table, lens)
-    check(y, *more.shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens))
+    check(y, *more.shared(q, kp, vp, prefixes, prefix_lens, groups, table, lens, vs=codes and codes[3]))
     assert not y[5].any()
 
 
@@ -130,7 +130,7 @@ def test_shared_large_scores(rt, kind):
     kp, vp, codes, prefixes, table = make(rng, [200], [30, 30, 1], 2, 16, 128, kind)
     q = floats(rng, (3, 8, 128), "f32") * 20
     y = call(rt, q, "f32", kp, vp, codes, kind, prefixes, [200], [0, 3], table, [30, 30, 1])
-    check(y, *more.shared(q, kp, vp, prefixes, [200], [0, 3], table, [30, 30, 1]))
+    check(y, *more.shared(q, kp, vp, prefixes, [200], [0, 3], table, [30, 30, 1], vs=codes and codes[3]))
 
 
 def test_infinite_values_of_a_prefix(rt):
