@@ -93,10 +93,14 @@ enum { kBf16, kF32, kCodes };  // what pages hold
 enum { kAny, kLow, kHigh };
 
 template <int D, int KIND>
+constexpr int paged_keys() {
+  return KIND == kCodes ? (D == 64 ? 64 : 32) : D * (KIND == kF32 ? 4 : 2) < 256 ? 32 : 16;
+}
+template <int D, int KIND, int KEYS = paged_keys<D, KIND>()>
 struct PagedTile {
   static constexpr bool F32 = KIND == kF32, CODES = KIND == kCodes;
   static constexpr int ES = F32 ? 4 : CODES ? 1 : 2, ROW = D * ES, CH = ROW / 16;
-  static constexpr int KT = CODES ? (D == 64 ? 64 : 32) : ROW < 256 ? 32 : 16;  // keys of a tile
+  static constexpr int KT = KEYS;                // keys of a tile
   static constexpr int SUB = KT / 16, HALF = KT * ROW, N = HALF / 1024, RPI = 1024 / ROW;
   static constexpr int NS = CODES ? KT / 32 : 0;  // copies of 64 scales: the tile's K's, its V's
   static constexpr int NK = N + NS;               // copies that K's products wait for
@@ -217,11 +221,12 @@ __device__ __forceinline__ void dma4(const void *from, uint32_t lds) {
 
 // What a wave holds for CT x 16 query rows (columns of the products) of one kv head: q, O
 // and the softmax, and the steps over a tile in its memory `mem` (K, V, scales).
-template <int D, int KIND, int CT, int PREC>
+template <int D, int KIND, int CT, int PREC, int KEYS = paged_keys<D, KIND>()>
 struct PagedWave {
-  using T = PagedTile<D, KIND>;
+  using T = PagedTile<D, KIND, KEYS>;
   static constexpr bool F32 = T::F32, CODES = T::CODES;
   static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row's q per lane
+  static constexpr bool LAZY = KIND == kBf16 && PREC != kAny;
   // an f32 q's further parts: two over bf16 rows, one over codes
   static constexpr int NL = F32 || PREC == kLow ? 1 : NQ, NE = CODES ? 1 : NL;
   typedef const __attribute__((address_space(3))) char *Lds;
@@ -363,6 +368,7 @@ struct PagedWave {
           q[c][i] = u32x4{r.x << 16, r.x & 0xffff0000u, r.y << 16, r.y & 0xffff0000u};
         }
       } else {
+        if (PREC == kHigh && D == 256 && i == NQ / 2) __builtin_amdgcn_sched_barrier(0);  // (registers for half of q at a time)
         const int64_t at8 = qo + 32 * i + 8 * g4;
         if (PREC != kLow && a.q_f32) {
           const f32x4 r[2] = {*(const f32x4 *)((const float *)a.q + at8), *(const f32x4 *)((const float *)a.q + at8 + 4)};
@@ -394,7 +400,7 @@ struct PagedWave {
   // S^T = K q^T of the tile whose K is there, for the first `ct` column tiles
   __device__ RXW8_INLINE void scores(int ct) {
     const uint32_t kf = mem + col * T::ROW;
-    constexpr int NA = F32 ? 4 : 2;  // sums in turn: no product waits for the one before
+    constexpr int NA = F32 ? 4 : CT > 1 ? 1 : 2;  // sums in turn: no product waits for the one before
 #pragma unroll
     for (int u = 0; u < T::SUB; ++u) {
       f32x4 acc[CT][NA];
@@ -407,14 +413,14 @@ struct PagedWave {
         for (int c = 0; c < CT; ++c) {
           if (c && c >= ct) break;
           if constexpr (CODES) {
-            acc[c][n & 1] = mfma_f16(f, q[c][n], acc[c][n & 1]);
-            if constexpr (PREC != kLow) acc[c][~n & 1] = mfma_f16(f, ql[c][NL > 1 ? n : 0], acc[c][~n & 1]);
+            acc[c][n & (NA - 1)] = mfma_f16(f, q[c][n], acc[c][n & (NA - 1)]);
+            if constexpr (PREC != kLow) acc[c][~n & (NA - 1)] = mfma_f16(f, ql[c][NL > 1 ? n : 0], acc[c][~n & (NA - 1)]);
             continue;
           }
-          acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[c][n]), acc[c][n & 1]);
+          acc[c][n & (NA - 1)] = mfma16x16x32(as_bf16x8(f), as_bf16x8(q[c][n]), acc[c][n & (NA - 1)]);
           if (q_parts()) {
-            acc[c][~n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[c][NL > 1 ? n : 0]), acc[c][~n & 1]);
-            acc[c][n & 1] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][NE > 1 ? n : 0]), acc[c][n & 1]);
+            acc[c][~n & (NA - 1)] = mfma16x16x32(as_bf16x8(f), as_bf16x8(ql[c][NL > 1 ? n : 0]), acc[c][~n & (NA - 1)]);
+            acc[c][n & (NA - 1)] = mfma16x16x32(as_bf16x8(f), as_bf16x8(qe[c][NE > 1 ? n : 0]), acc[c][n & (NA - 1)]);
           }
         }
       };
@@ -448,9 +454,10 @@ struct PagedWave {
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        s[c][u] = acc[c][0] + acc[c][1];
+        s[c][u] = acc[c][0];
+        if constexpr (NA > 1) s[c][u] += acc[c][1];
         if constexpr (F32) s[c][u] += acc[c][2] + acc[c][3];
-        s[c][u] *= CODES ? scale * unit[CODES ? c : 0] : scale;
+        if constexpr (!LAZY) s[c][u] *= CODES ? scale * unit[CODES ? c : 0] : scale;
       }
     }
   }
@@ -462,6 +469,10 @@ struct PagedWave {
       if (c && c >= ct) break;
       if constexpr (CODES) {
         softmax_codes(c, x, part);
+        continue;
+      }
+      if constexpr (LAZY) {
+        softmax_lazy(c, x, part);
         continue;
       }
       float mt = kMinusInf;
@@ -490,6 +501,49 @@ struct PagedWave {
           s[c][u][r] = p;
         }
     }
+  }
+
+  // The reference a score that need not be the largest: weights up to 2^8 (a score is q.k here)
+  __device__ RXW8_INLINE void softmax_lazy(int c, const Tile &x, bool part) {
+    f32x4 w[T::SUB];
+    float sum, top;
+    if (part) {
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * u + 4 * g4 + r >= x.seen || (x.holes >> u & 1)) s[c][u][r] = kMinusInf;
+    }
+    auto weigh = [&]() RXW8_INLINE {
+      const float ref = m[c] == kMinusInf ? 0.f : m[c];
+      sum = top = 0.f;
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          w[u][r] = __builtin_amdgcn_exp2f(fmaf(s[c][u][r], a.c, -ref));
+          sum += w[u][r];
+          top = fmaxf(top, w[u][r]);
+        }
+    };
+    weigh();
+    if (__ballot(top > 0x1p8f || m[c] == kMinusInf)) {
+      float highest = kMinusInf;
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) highest = fmaxf(highest, s[c][u][r]);
+      const float to = fmaxf(m[c], max4(highest) * a.c);
+      const float f = to == kMinusInf ? 1.f : exp2f(m[c] - to);
+      m[c] = to;
+      l[c] *= f;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) o[c][n] *= f;
+      weigh();
+    }
+    l[c] += sum;
+#pragma unroll
+    for (int u = 0; u < T::SUB; ++u) s[c][u] = w[u];
   }
 
   __device__ RXW8_INLINE void softmax_codes(int c, const Tile &x, bool part) {
@@ -578,11 +632,13 @@ struct PagedWave {
       values_codes(ct, v0);
       return;
     }
-    // weights in parts: three behind an f32 output, two behind a bf16 one
+    // weights in parts: three behind an f32 output, two behind a bf16 one; one, rounded by
+    // 2^-8 as the output is, where a kernel is made for bf16 outputs
     struct Parts {
       uint2 k0, k1, k2;
     };
     auto parts = [&](f32x4 w) RXW8_INLINE {
+      if constexpr (PREC == kLow) return Parts{uint2{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])}, uint2{0, 0}, uint2{0, 0}};
       if (p_parts()) {
         uint32_t x[3], y[3];
         split_bf16x2<true>(w[0], w[1], x);
@@ -594,31 +650,58 @@ struct PagedWave {
       split_bf16x2<true>(w[2], w[3], y);
       return Parts{uint2{x[0], y[0]}, uint2{x[1], y[1]}, uint2{0, 0}};
     };
-    {
-      const int tr_j = col >> 2, tr_q = col & 3;
-      const uint32_t vf = v0 + (4 * g4 + tr_j) * T::ROW + 8 * (tr_q & 1);
+    const int tr_j = col >> 2, tr_q = col & 3;
+    const uint32_t vf = v0 + (4 * g4 + tr_j) * T::ROW + 8 * (tr_q & 1);
+    auto read = [&](int u, int n) RXW8_INLINE {
+      return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
+          vf + u * 16 * T::ROW + (((2 * n + (tr_q >> 1)) ^ T::vx(4 * g4 + tr_j)) << 4)));
+    };
+    if constexpr (PREC != kAny && T::SUB % 2 == 0) {  // 32 keys at a time
 #pragma unroll
-      for (int u = 0; u < T::SUB; ++u) {
-        Parts p[CT];
+      for (int u = 0; u < T::SUB; u += 2) {
+        Parts p[CT][2];
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           if (c && c >= ct) break;
-          p[c] = parts(s[c][u]);
+          p[c][0] = parts(s[c][u]);
+          p[c][1] = parts(s[c][u + 1]);
         }
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
-          const s16x4 f = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(uintptr_t)(
-              vf + u * 16 * T::ROW + (((2 * n + (tr_q >> 1)) ^ T::vx(4 * g4 + tr_j)) << 4)));
+          const uint2 lo = __builtin_bit_cast(uint2, read(u, n)), hi = __builtin_bit_cast(uint2, read(u + 1, n));
+          const u32x4 f = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
             if (c && c >= ct) break;
-            auto add = [&](uint2 x) RXW8_INLINE {
-              o[c][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, x), o[c][n], 0, 0, 0);
-            };
-            add(p[c].k0);
-            add(p[c].k1);
-            if (p_parts()) add(p[c].k2);
+            auto add = [&](uint2 x, uint2 y) RXW8_INLINE { o[c][n] = mfma16x16x32(as_bf16x8(f), as_bf16x8(u32x4{x.x, x.y, y.x, y.y}), o[c][n]); };
+            add(p[c][0].k0, p[c][1].k0);
+            if constexpr (PREC != kLow) add(p[c][0].k1, p[c][1].k1);
+            if (p_parts()) add(p[c][0].k2, p[c][1].k2);
           }
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < T::SUB; ++u) {
+      Parts p[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        if (c && c >= ct) break;
+        p[c] = parts(s[c][u]);
+      }
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        const s16x4 f = read(u, n);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          if (c && c >= ct) break;
+          auto add = [&](uint2 x) RXW8_INLINE {
+            o[c][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, x), o[c][n], 0, 0, 0);
+          };
+          add(p[c].k0);
+          if constexpr (PREC != kLow) add(p[c].k1);
+          if (p_parts()) add(p[c].k2);
         }
       }
     }
@@ -827,13 +910,21 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       if (lane == 0) *p = Piece{seq, first, n};
     };
 
-    // (q is on its way while the first pages are looked up, and in before the copies
-    // go out)
-    start(b);
-    cur = next(left > 1);
-    w.wait_q();
-    w.copy_k();
-    w.copy_v();
+    if constexpr (PREC == kAny) {
+      // (q is on its way while the first pages are looked up, and in before the copies
+      // go out)
+      start(b);
+      cur = next(left > 1);
+      w.wait_q();
+      w.copy_k();
+      w.copy_v();
+    } else {  // (the wait for q is one for the first tile as well: it is needed next)
+      cur = next(left > 1);
+      w.copy_k();
+      w.copy_v();
+      start(b);
+      w.wait_q();
+    }
 
     int begun = cur.t;  // the tile at which this wave began the sequence
     for (;;) {

@@ -15,7 +15,7 @@ struct SharedArgs {
   // of parts of prefixes [2, Hkv, units], and how the workgroups were dealt
   float *own, *whole, *parts;
   int *plan;
-  int columns, keys;          // of a block; of a tile
+  int columns, keys;          // of a block; of a prefix's tile
 };
 
 // Any head width up to 512, any page size: one workgroup of 4 waves per (sequence, query
@@ -64,12 +64,19 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_any(SharedArgs a) 
 // How the prefixes' tiles were dealt follows from the same numbers there.
 namespace {
 
-constexpr float kPrefixTile = 0.5f;
+constexpr float kPrefixTile = 2.f;
 
 // Column tiles of a block: as many as leave no register spilled
 template <int D, int KIND, int PREC>
 constexpr int block_tiles() {
   return D == 256 ? 1 : D == 128 ? (PREC == kHigh ? 1 : 2) : PREC == kHigh || KIND == kCodes ? 2 : 4;
+}
+
+// Keys of a prefix's tile: as many as registers and the rings of 8 waves have room for, so
+// that a wave has more to do while the next ones come
+template <int D, int KIND>
+constexpr int prefix_keys() {
+  return KIND == kCodes ? (D == 256 ? 32 : 64) : KIND == kF32 || D == 256 ? 16 : 32;
 }
 
 // Group n's sequences within this launch's (relative to b0), blocks and tiles
@@ -107,9 +114,9 @@ __device__ __forceinline__ int tiles_before(const SharedArgs &a, int n, int &tot
 // Workgroup `unit` of `units` for the prefixes of kv head h, whose run has `total` tiles
 template <int D, int KIND, int PREC>
 __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int units, int total) {
-  using T = PagedTile<D, KIND>;
-  constexpr int CT = block_tiles<D, KIND, PREC>(), CB = 16 * CT, DP = D / 2;
-  using Wave = PagedWave<D, KIND, CT, PREC>;
+  using T = PagedTile<D, KIND, prefix_keys<D, KIND>()>;
+  constexpr int CT = block_tiles<D, KIND, PREC>(), CB = 16 * CT;
+  using Wave = PagedWave<D, KIND, CT, PREC, T::KT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nw = a.d.waves, G = a.d.Hq / a.d.Hkv;
@@ -136,16 +143,16 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
     const int first = t0 + waves.start(wave);
     int left = wave < nw ? t0 + waves.start(wave + 1) - first : 0;
     if (left > 0) {
+      w.begin(a.prefixes + (int64_t)n * a.MP, a.MP, x.len, first);
+      typename Wave::Tile cur = w.tile();
+      w.copy_k();
+      w.copy_v();
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const int i = min(block * CB + 16 * c + w.col, x.rows - 1), r = i / G;
         w.load_q(c, ((int64_t)(x.g0 + r) * a.d.Hq + h * G + (i - r * G)) * D);
       }
-      w.begin(a.prefixes + (int64_t)n * a.MP, a.MP, x.len, first);
-      typename Wave::Tile cur = w.tile();
-      w.wait_q();
-      w.copy_k();
-      w.copy_v();
+      w.wait_q();  // (and for the first tile)
       for (;;) {
         wait_vm<T::N>();
         w.scores(ct);
@@ -176,24 +183,32 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
       __syncthreads();
       if (wave < count) w.record(c, (float *)lds + (wave * 16 + w.col) * T::REC);
       __syncthreads();
-      for (int i = threadIdx.x; i < 16 * DP; i += blockDim.x) {
-        const int r = i / DP, d = 2 * (i - r * DP), at = 16 * c + r;
+      for (int i = threadIdx.x; i < 16 * (D / 4); i += blockDim.x) {  // (four dims of a row)
+        const int r = i / (D / 4), d = 4 * (i - r * (D / 4)), at = 16 * c + r;
         if (at >= cols) break;
-        Joined j;
-#pragma unroll 1
-        for (int k0 = 0; k0 < count; k0 += 4)
-          join<4>(j, k0, count, [&](int, int k, float &m, float &l, float2 &o) {
-            const float *const rec = (const float *)lds + (k * 16 + r) * T::REC;
-            const float2 ml = *(const float2 *)(rec + D);
-            m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
-          });
+        const float *const rec = (const float *)lds + r * T::REC;
+        float2 ml[kPagedWaves];
+        float M = kMinusInf, L = 0.f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kPagedWaves; ++k) {
+          ml[k] = k < count ? *(const float2 *)(rec + k * 16 * T::REC + D) : float2{kMinusInf, 0.f};
+          M = fmaxf(M, ml[k].x);
+        }
+#pragma unroll
+        for (int k = 0; k < kPagedWaves; ++k)
+          if (k < count) {
+            const float f = record_weight(ml[k].x, ml[k].y, M);
+            L += f * ml[k].y;
+            O += f * *(const f32x4 *)(rec + k * 16 * T::REC + d);
+          }
         float *to = part + at * T::REC;
         if (all) {
           const int row = block * CB + at, seq = row / G;
           to = a.whole + ((int64_t)(x.g0 + seq) * a.d.Hq + h * G + (row - seq * G)) * T::REC;
         }
-        *(float2 *)(to + d) = j.O;
-        if (d == 0) *(float2 *)(to + D) = float2{j.M, j.L};
+        *(f32x4 *)(to + d) = O;
+        if (d == 0) *(float2 *)(to + D) = float2{M, L};
       }
     }
     u0 += piece;
@@ -246,30 +261,44 @@ RXW8_SHARED_D(64)
 RXW8_SHARED_D(128)
 RXW8_SHARED_D(256)
 
-// The records of a row joined: a wave a row
+// The records of a row joined: a wave a row. Up to 64 groups, all that a row has to know is
+// loaded at once, its records next: the two round trips are what bounds it.
 extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a) {
   const int lane = threadIdx.x & 63, D = a.d.D, REC = D + 4, G = a.d.Hq / a.d.Hkv, nw = a.d.waves;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.d.B * a.d.Hq) return;  // whole waves only; no barriers below
   const int b = (int)(row / a.d.Hq), hq = (int)(row - (int64_t)b * a.d.Hq), h = hq / G;
-  const int n = any_sequence(a.groups, a.N, a.b0 + b), units = a.plan[0];
+  const int units = a.plan[0], len = a.d.lens[b];
+  Group x;
+  int start = 0, total = 0;
+  x.tiles = x.rows = 0;
+  for (int n0 = 0; n0 < a.N; n0 += 64) {
+    const int i = min(n0 + lane, a.N - 1);
+    const Group g = group_of(a, a.groups[i], a.groups[i + 1], a.prefix_lens[i]);
+    const int mine = n0 + lane < a.N ? g.blocks * g.tiles : 0, incl = scan64(mine);
+    // (the row's group, the last that begins at it or before and has rows: offsets do not decrease)
+    const unsigned long long in = __ballot(n0 + lane < a.N && g.g0 <= b && g.g0 + g.rows / G > b);
+    if (in) {
+      const int k = __builtin_ctzll(in);
+      x.g0 = __builtin_amdgcn_readlane(g.g0, k), x.rows = __builtin_amdgcn_readlane(g.rows, k);
+      x.tiles = __builtin_amdgcn_readlane(g.tiles, k);
+      start = total + __builtin_amdgcn_readlane(incl, k) - __builtin_amdgcn_readlane(mine, k);
+    }
+    total += __builtin_amdgcn_readlane(incl, 63);
+  }
   const float *first_rec = nullptr, *others = nullptr;  // of the prefix
   int prefix = 0;
-  if (n >= 0 && a.b0 + b < a.groups[n + 1]) {
-    const Group x = group_of(a, a.groups[n], a.groups[n + 1], a.prefix_lens[n]);
-    if (x.tiles) {
-      int total;
-      const int i = (b - x.g0) * G + (hq - h * G), block = i / a.columns, col = i - block * a.columns;
-      const int start = tiles_before(a, n, total) + block * x.tiles;
-      const Deal deal(total, min(units, (total + nw - 1) / nw));
-      const int first = deal.taker(start);
-      prefix = deal.taker(start + x.tiles - 1) - first + 1;
-      const int64_t size = (int64_t)a.columns * REC;
-      first_rec = prefix == 1 ? a.whole + row * REC : a.parts + (((int64_t)a.d.Hkv + h) * units + first) * size + col * REC;
-      others = a.parts + ((int64_t)h * units + first) * size + col * REC;
-    }
+  if (x.rows && x.tiles) {
+    const int i = (b - x.g0) * G + (hq - h * G), block = i / a.columns, col = i - block * a.columns;
+    start += block * x.tiles;
+    const Deal deal(total, min(units, (total + nw - 1) / nw));
+    const int first = deal.taker(start);
+    prefix = deal.taker(start + x.tiles - 1) - first + 1;
+    const int64_t size = (int64_t)a.columns * REC;
+    first_rec = prefix == 1 ? a.whole + row * REC : a.parts + (((int64_t)a.d.Hkv + h) * units + first) * size + col * REC;
+    others = a.parts + ((int64_t)h * units + first) * size + col * REC;
   }
-  const int count = prefix + (a.d.lens[b] > 0 && a.d.M > 0);
+  const int count = prefix + (len > 0 && a.d.M > 0);
   for (int d = 2 * lane; d < D; d += 128) {
     Joined j;
 #pragma unroll 1

@@ -316,14 +316,18 @@ static int shared_launch(Runtime *rt, SharedArgs a) {
   // block_tiles (kernels/shared.hip)
   const bool high = (d.q_f32 || d.out_f32) && a.kind != 1;
   const int ct = d.D == 256 ? 1 : d.D == 128 ? (high ? 1 : 2) : high || a.kind == 2 ? 2 : 4;
-  a.columns = 16 * ct, a.keys = t.keys;
-  auto tiles = [&](int64_t m) { return (m * d.ps + t.keys - 1) / t.keys; };
+  // prefix_keys (kernels/shared.hip)
+  a.keys = a.kind == 2 ? (d.D == 256 ? 32 : 64) : a.kind == 1 || d.D == 256 ? 16 : 32;
+  a.columns = 16 * ct;
+  const int row = d.D * (a.kind == 2 ? 1 : a.kind == 1 ? 4 : 2), ring = 2 * a.keys * row + (a.kind == 2 ? 8 * a.keys : 0);
+  auto tiles = [&](int64_t m) { return (m * d.ps + std::min(t.keys, a.keys) - 1) / std::min(t.keys, a.keys); };
   const int64_t blocks = (int64_t)d.B * G / a.columns + a.N;
   bool any = (d.D != 64 && d.D != 128 && d.D != 256) || d.ps % 16 || d.P == 0 || heads > 4096 || a.N == 0 || a.MP == 0 ||
              ((uintptr_t)d.q | (uintptr_t)d.kp | (uintptr_t)d.vp | (uintptr_t)d.out) % 16 ||
              tiles(d.M) >= ((int64_t)1 << 30) / d.B || tiles(a.MP) >= ((int64_t)1 << 30) / blocks;
   const size_t record = (size_t)std::min<int64_t>(G, 16) * (size_t)rec;
-  const size_t wave = std::max({(size_t)t.ring, record, (size_t)(16 * rec)}) + record;
+  // LDS of a wave: its own keys' ring and two records, or a prefix's ring and, over that, 16 of a block's records
+  const size_t wave = std::max(std::max((size_t)t.ring, record) + record, (size_t)std::max<int64_t>(ring, 16 * rec));
   d.waves = (int)std::min<size_t>(8, (rt->lds_max - 1024) / wave);
   const int64_t block = (int64_t)RXW8_NOALLOC_PARTIAL_BYTES - 1024;
   auto round = [](int64_t x) { return (x + 1023) & ~(int64_t)1023; };

@@ -7,7 +7,8 @@ half step is 2^-11: q in parts that leave 2^-22 of an element and 2^-39 of the r
 largest, less than SPLIT of the sums of |q k|; weights in one part behind a bf16 output
 (`F16`), in two, 2^-22 and so less than SPLIT, behind an f32 one. A weight p s_v is a
 multiple of 2^-24 where the largest so far is 2^10 at least: half of that, 2^-35 of the
-largest, for each key and at most 127 units of its code (`grain`)."""
+largest, for each key and at most 127 units of its code (`grain`). Behind a shared
+prefix the weights of bf16 rows are one bf16 part (2^-8) for a bf16 output."""
 import math
 
 import numpy as np
@@ -20,7 +21,7 @@ F16 = 2.0 ** -11
 
 def p_step(kind, out):
     """What weights are rounded by, beside f32's own roundings."""
-    return (F16 if kind == "q8" and out == "bf16" else ref.SPLIT) + MORE
+    return (ref.SPLIT if out == "f32" else F16 if kind == "q8" else ref.BF16) + MORE
 
 
 def grain(q, k, vs, scale):
