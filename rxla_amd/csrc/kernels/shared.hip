@@ -64,7 +64,7 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_any(SharedArgs a) 
 // How the prefixes' tiles were dealt follows from the same numbers there.
 namespace {
 
-constexpr float kPrefixTile = 2.f;
+constexpr float kPrefixTile = 1.4f, kPrefixCodes = 2.f, kPrefixBlock = 4.f;
 
 // Column tiles of a block: as many as leave no register spilled
 template <int D, int KIND, int PREC>
@@ -94,33 +94,34 @@ __device__ __forceinline__ Group group_of(const SharedArgs &a, int g_from, int g
   return x;
 }
 
-// Tiles that the groups before `n` have in a head's run; total: all groups'. By a whole wave.
-__device__ __forceinline__ int tiles_before(const SharedArgs &a, int n, int &total) {
+// Tiles and blocks of a head's run. By a whole wave.
+struct Run {
+  int tiles, blocks;
+};
+__device__ __forceinline__ Run run_of(const SharedArgs &a) {
   const int lane = threadIdx.x & 63;
-  int before = 0;
-  total = 0;
+  int tiles = 0, blocks = 0;
   for (int n0 = 0; n0 < a.N; n0 += 64) {
     const int i = min(n0 + lane, a.N - 1);
     const Group x = group_of(a, a.groups[i], a.groups[i + 1], a.prefix_lens[i]);
-    const int mine = n0 + lane < a.N ? x.blocks * x.tiles : 0, incl = scan64(mine);
-    if (n >= n0 && n < n0 + 64) before = total + __builtin_amdgcn_readlane(incl, n - n0) - __builtin_amdgcn_readlane(mine, n - n0);
-    total += __builtin_amdgcn_readlane(incl, 63);
+    const bool in = n0 + lane < a.N && x.tiles > 0;
+    tiles += __builtin_amdgcn_readlane(scan64(in ? x.blocks * x.tiles : 0), 63);
+    blocks += __builtin_amdgcn_readlane(scan64(in ? x.blocks : 0), 63);
   }
-  return before;
+  return Run{tiles, blocks};
 }
 
 }  // namespace
 
 // Workgroup `unit` of `units` for the prefixes of kv head h, whose run has `total` tiles
 template <int D, int KIND, int PREC>
-__device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int units, int total) {
+__device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int units, int used, int total) {
   using T = PagedTile<D, KIND, prefix_keys<D, KIND>()>;
   constexpr int CT = block_tiles<D, KIND, PREC>(), CB = 16 * CT;
   using Wave = PagedWave<D, KIND, CT, PREC, T::KT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nw = a.d.waves, G = a.d.Hq / a.d.Hkv;
-  const int used = min(units, (total + nw - 1) / nw);
   if (unit >= used) return;
   const Deal deal(total, used);
   int u0 = __builtin_amdgcn_readfirstlane(deal.start(unit));
@@ -228,19 +229,21 @@ __device__ RXW8_INLINE void shared_walk(const SharedArgs &a) {
   using T = PagedTile<D, KIND>;
   const int lane = threadIdx.x & 63, G = a.d.Hq / a.d.Hkv, HT = (G + 15) / 16, heads = a.d.Hkv * HT;
   const int hk = blockIdx.x % heads, unit = blockIdx.x / heads, units = a.d.units, most = a.d.M * a.d.ps;
-  int prefix = 0, own = 0;
-  tiles_before(a, 0, prefix);
+  const Run run = run_of(a);
+  int own = 0;
   for (int b0 = 0; b0 < a.d.B; b0 += 64) {
     const int len = b0 + lane < a.d.B ? a.d.lens[b0 + lane] : 0;
     own += __builtin_amdgcn_readlane(scan64((int)(((unsigned)min(max(len, 0), most) + T::KT - 1) / T::KT)), 63);
   }
   // a head's workgroups for its prefixes, and for the sequences' own keys
-  const float cost = kPrefixTile * (float)prefix / HT;
+  const float cost = (KIND == kCodes ? kPrefixCodes : kPrefixTile) * ((float)run.tiles + kPrefixBlock * (float)run.blocks) / HT;
   int up = __builtin_amdgcn_readfirstlane((int)rintf(units * cost / fmaxf(cost + (float)own, 1.f)));
-  up = prefix == 0 ? 0 : own == 0 ? units : min(max(up, 1), max(units - 1, 1));
+  up = run.tiles == 0 ? 0 : own == 0 ? units : min(max(up, 1), max(units - 1, 1));
   const int uo = own == 0 ? 0 : max(units - up, 1);
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = up * HT;
-  if (unit < up) prefix_walk<D, KIND, PREC>(a, hk / HT, unit * HT + hk % HT, up * HT, prefix);
+  // one to every wave's tile, or to every block of fewer
+  const int used = min(up * HT, max((run.tiles + a.d.waves - 1) / a.d.waves, run.blocks));
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = up * HT, a.plan[1] = used;
+  if (unit < up) prefix_walk<D, KIND, PREC>(a, hk / HT, unit * HT + hk % HT, up * HT, used, run.tiles);
   if (unit >= units - uo) {
     if (unit < up) __syncthreads();  // (one workgroup to a head does both)
     paged_decode<D, KIND, true, PREC>(a.d, PagedPlaceOf{hk, unit - (units - uo), uo, a.own});
@@ -264,11 +267,11 @@ RXW8_SHARED_D(256)
 // The records of a row joined: a wave a row. Up to 64 groups, all that a row has to know is
 // loaded at once, its records next: the two round trips are what bounds it.
 extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a) {
-  const int lane = threadIdx.x & 63, D = a.d.D, REC = D + 4, G = a.d.Hq / a.d.Hkv, nw = a.d.waves;
+  const int lane = threadIdx.x & 63, D = a.d.D, REC = D + 4, G = a.d.Hq / a.d.Hkv;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.d.B * a.d.Hq) return;  // whole waves only; no barriers below
   const int b = (int)(row / a.d.Hq), hq = (int)(row - (int64_t)b * a.d.Hq), h = hq / G;
-  const int units = a.plan[0], len = a.d.lens[b];
+  const int units = a.plan[0], used = a.plan[1], len = a.d.lens[b];
   Group x;
   int start = 0, total = 0;
   x.tiles = x.rows = 0;
@@ -291,7 +294,7 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a)
   if (x.rows && x.tiles) {
     const int i = (b - x.g0) * G + (hq - h * G), block = i / a.columns, col = i - block * a.columns;
     start += block * x.tiles;
-    const Deal deal(total, min(units, (total + nw - 1) / nw));
+    const Deal deal(total, used);
     const int first = deal.taker(start);
     prefix = deal.taker(start + x.tiles - 1) - first + 1;
     const int64_t size = (int64_t)a.columns * REC;
