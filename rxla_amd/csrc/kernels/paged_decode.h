@@ -226,7 +226,9 @@ struct PagedWave {
   using T = PagedTile<D, KIND, KEYS>;
   static constexpr bool F32 = T::F32, CODES = T::CODES;
   static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row's q per lane
-  static constexpr bool LAZY = KIND == kBf16 && PREC != kAny;
+  // (not where two tries at the weights and q's three parts want more registers than there are:
+  // 41 sequences of 87 keys behind 7, 64 / 8 heads of 256, f32 queries: 86 us with it, 60 without)
+  static constexpr bool LAZY = KIND == kBf16 && PREC != kAny && !(D == 256 && PREC == kHigh);
   // an f32 q's further parts: two over bf16 rows, one over codes
   static constexpr int NL = F32 || PREC == kLow ? 1 : NQ, NE = CODES ? 1 : NL;
   typedef const __attribute__((address_space(3))) char *Lds;
