@@ -52,19 +52,28 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_any(SharedArgs a) 
 // ---- head widths 64, 128, 256, pages of whole 16-row pieces: matrix cores --------
 //
 // The G query heads of a kv head of all of a prefix's sequences are rows of one product:
-// B_n G of them, in blocks of CT x 16 columns that a wave holds in registers. A workgroup walks a piece of a prefix for one block, its waves
-// equal pieces of that with a ring of their own each (paged_decode.h), so a block's keys
-// are read once by one workgroup, and by the blocks of a head out of its die's cache (the
-// workgroups of a head are 8 or more apart, on one die where there are 8 heads).
+// B_n G of them, in blocks of CT x 16 columns that a wave holds in registers. A workgroup walks
+// a piece of a prefix for one block, its waves equal pieces of that with a ring of their own each
+// (paged_decode.h), so a block's keys are read once by one workgroup, and by the blocks of
+// a head out of its die's cache (the workgroups of a head are 8 or more apart, on one die
+// where there are 8 heads).
 //
-// The launch has both kinds of work: of a head's `units` workgroups some walk prefixes,
-// the others the sequences' own keys (paged_decode), in proportion to the tiles that each
-// kind has, a prefix's counting kPrefixTile. Both leave records (acc, max, sum) of their
-// rows; a second launch joins those of a row in order: the parts of its prefix, its own.
-// How the prefixes' tiles were dealt follows from the same numbers there.
+// The launch has both kinds of work: of a head's `units` workgroups some walk prefixes, the
+// others the sequences' own keys (paged_decode). A prefix's blocks are cut into equal pieces, in
+// number by its share of all prefixes' tiles (plan_of), and a workgroup has one, or a few whole:
+// what a piece costs beside its tiles (q's way and the first tile's, the joins) is some tiles'
+// time, and pieces dealt by tiles alone, across the borders of blocks, made many workgroups
+// pay it twice (48 sequences behind 8192 positions in 8 bits, 32 / 4 heads of 128: 37.6 us, 34.0
+// so; 20 behind 4 prefixes of 6391, 32 / 8 heads, f32: 31.4, 25.6; 64 behind 6000, bf16,
+// 32 / 8 heads: 48.2, 47.0). Both kinds leave records (acc, max, sum) of their rows; a second
+// launch joins those of a row in order: the pieces of its prefix, its own.
 namespace {
 
-constexpr float kPrefixTile = 1.4f, kPrefixCodes = 2.f, kPrefixBlock = 4.f;
+// What a tile of a prefix costs of one of own keys, and a piece and a sequence of own keys of a
+// tile, beside their tiles. (3 prefixes of 700 to 4000 before 96 sequences of up to 300, f32, 16 / 8 heads
+// of 128: 41.1 us; with 4 for a sequence 50.6, own keys left to too few. 166 of up to 78 behind 1 to 4
+// positions, 8 heads: 23.0; with 8 for a piece 22.9, with 8 and 16 for a sequence 26.3.)
+constexpr float kPrefixTile = 2.f, kPrefixBlock = 24.f, kOwnSequence = 8.f;
 
 // Column tiles of a block: as many as leave no register spilled
 template <int D, int KIND, int PREC>
@@ -94,51 +103,130 @@ __device__ __forceinline__ Group group_of(const SharedArgs &a, int g_from, int g
   return x;
 }
 
-// Tiles and blocks of a head's run. By a whole wave.
-struct Run {
-  int tiles, blocks;
-};
-__device__ __forceinline__ Run run_of(const SharedArgs &a) {
-  const int lane = threadIdx.x & 63;
-  int tiles = 0, blocks = 0;
-  for (int n0 = 0; n0 < a.N; n0 += 64) {
-    const int i = min(n0 + lane, a.N - 1);
-    const Group x = group_of(a, a.groups[i], a.groups[i + 1], a.prefix_lens[i]);
-    const bool in = n0 + lane < a.N && x.tiles > 0;
-    tiles += __builtin_amdgcn_readlane(scan64(in ? x.blocks * x.tiles : 0), 63);
-    blocks += __builtin_amdgcn_readlane(scan64(in ? x.blocks : 0), 63);
+// Pieces of a prefix of `tiles`, `rate` of them to a tile: one at least, and a tile for every wave
+__device__ __forceinline__ int pieces_of(int tiles, float rate) {
+  return min(max((int)((float)tiles * rate + 0.5f), 1), (int)(((unsigned)tiles + kPagedWaves - 1) / kPagedWaves));
+}
+// Groups in lanes: those from n0 on
+__device__ __forceinline__ Group groups_from(const SharedArgs &a, int n0) {
+  const int lane = threadIdx.x & 63, i = min(n0 + lane, a.N - 1);
+  Group x = group_of(a, a.groups[i], a.groups[i + 1], a.prefix_lens[i]);
+  if (n0 + lane >= a.N) x.rows = x.blocks = 0;
+  return x;
+}
+struct Pieces {
+  int each, count, incl, parts, part_incl;  // of a block, of all; the sums; those that leave parts
+  __device__ __forceinline__ Pieces(const Group &x, float rate) {
+    each = pieces_of(x.tiles, rate);
+    count = x.blocks * each;
+    parts = each > 1 ? count : 0;
+    incl = scan64(count), part_incl = scan64(parts);
   }
-  return Run{tiles, blocks};
+};
+__device__ __forceinline__ int max64(int v) {  // over the 64 lanes, of numbers from 0 on
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+// Workgroups of a kv head (its HT heads of columns together) for its prefixes, and the pieces'
+// rate: those by which the longer of two takes least, the longest piece (times the pieces of a
+// workgroup) and a workgroup's share of the own keys, in tiles. Tried are rates around the one
+// that makes both the same, each with a workgroup to a piece and with as many as that one has.
+// By a whole wave.
+struct Plan {
+  int takers;
+  float rate;
+};
+__device__ __forceinline__ Plan plan_of(const SharedArgs &a, const Group &first, float own, int HT) {
+  constexpr int kRates = 4;
+  const float factor[kRates] = {0.7f, 0.85f, 1.f, 1.2f};
+  int tiles = 0, blocks = 0, finest = 0;
+  for (int n0 = 0; n0 < a.N; n0 += 64) {
+    const Group x = n0 ? groups_from(a, n0) : first;
+    finest += __builtin_amdgcn_readlane(scan64(x.blocks * pieces_of(x.tiles, 1.f)), 63);
+    tiles += __builtin_amdgcn_readlane(scan64(x.blocks * x.tiles), 63);
+    blocks += __builtin_amdgcn_readlane(scan64(x.tiles ? x.blocks : 0), 63);
+  }
+  if (tiles <= 0) return Plan{0, 0.f};
+  const int most = (own == 0.f ? a.d.units : max(a.d.units - 1, 1)) * HT;
+  const float cost = kPrefixTile * ((float)tiles + kPrefixBlock * (float)blocks) / HT;
+  const int even = min(max((int)rintf(a.d.units * HT * cost / (cost + own)), 1), most);
+  if (finest <= even) return Plan{finest, 1.f};
+  const float rate = (float)even / (float)tiles;
+  int items[kRates] = {0, 0, 0, 0}, longest[kRates] = {0, 0, 0, 0};
+  for (int n0 = 0; n0 < a.N; n0 += 64) {
+    const Group x = n0 ? groups_from(a, n0) : first;
+#pragma unroll
+    for (int j = 0; j < kRates; ++j) {
+      const int each = pieces_of(x.tiles, factor[j] * rate);
+      const int len = x.blocks && each ? (int)ceilf((float)x.tiles * __builtin_amdgcn_rcpf((float)each)) : 0;
+      items[j] += __builtin_amdgcn_readlane(scan64(x.blocks * each), 63);
+      longest[j] = max(longest[j], max64(len));
+    }
+  }
+  Plan best{1, 0.f};
+  float least = INFINITY;
+#pragma unroll
+  for (int j = 0; j < kRates; ++j)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int takers = max(min(k ? even : items[j], most), 1), up = (takers + HT - 1) / HT;
+      const float walk = kPrefixTile * ((float)longest[j] + kPrefixBlock) * ceilf((float)items[j] * __builtin_amdgcn_rcpf((float)takers) - 0.01f);
+      const float rest = own * __builtin_amdgcn_rcpf((float)max(a.d.units - up, 1)), t = fmaxf(walk, rest);
+      if (t < least) least = t, best = Plan{takers, factor[j] * rate};
+    }
+  best.takers = __builtin_amdgcn_readfirstlane(best.takers);
+  best.rate = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(best.rate)));
+  return best;
+}
+// The place of a part's record of kv head h: at most 2 d.units HT of them by plan_of
+__device__ __forceinline__ float *part_of(const SharedArgs &a, int HT, int h, int at) {
+  const int most = 2 * a.d.units * HT;
+  return a.parts + ((int64_t)h * most + min(max(at, 0), most - 1)) * ((int64_t)a.columns * (a.d.D + 4));
 }
 
 }  // namespace
 
-// Workgroup `unit` of `units` for the prefixes of kv head h, whose run has `total` tiles
+// Workgroup `unit` of plan.takers for the prefixes of kv head h
 template <int D, int KIND, int PREC>
-__device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int units, int used, int total) {
+__device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, int HT, const Plan &plan, const Group &in_lanes) {
   using T = PagedTile<D, KIND, prefix_keys<D, KIND>()>;
   constexpr int CT = block_tiles<D, KIND, PREC>(), CB = 16 * CT;
   using Wave = PagedWave<D, KIND, CT, PREC, T::KT>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nw = a.d.waves, G = a.d.Hq / a.d.Hkv;
-  if (unit >= used) return;
-  const Deal deal(total, used);
-  int u0 = __builtin_amdgcn_readfirstlane(deal.start(unit));
-  const int u1 = __builtin_amdgcn_readfirstlane(deal.start(unit + 1));
-
-  // the group, block and tile of the run's tile u0
-  auto uniform_group = [&](int n) RXW8_INLINE {
-    return group_of(a, uniform_load(a.groups, n), uniform_load(a.groups, n + 1), uniform_load(a.prefix_lens, n));
-  };
-  int n = 0, before = 0;
-  Group x = uniform_group(0);
-  while (before + x.blocks * x.tiles <= u0) before += x.blocks * x.tiles, x = uniform_group(++n);
-  int block = (u0 - before) / x.tiles, t0 = (u0 - before) - block * x.tiles;
-
+  int n0 = 0, before = 0, parts = 0;  // 64 groups, and what those before have
   Wave w(a.d, h, lds + wave * T::RING);
-  for (;;) {
-    const int piece = min(u1 - u0, x.tiles - t0);
+  for (int item = unit;; item += plan.takers) {
+    // ---- the group, block and piece of the item
+    Group x;
+    int n, at, pieces, part_at;
+    for (;; n0 += 64) {
+      if (n0 >= a.N) return;
+      const Group g = n0 || D == 256 || KIND == kF32 ? groups_from(a, n0) : in_lanes;  // (no registers to keep them in)
+      const Pieces p(g, plan.rate);
+      const int total = __builtin_amdgcn_readlane(p.incl, 63);
+      if (item - before >= total) {
+        before += total, parts += __builtin_amdgcn_readlane(p.part_incl, 63);
+        continue;
+      }
+      const int k = __popcll(__ballot(p.incl <= item - before));
+      auto of = [&](int v) RXW8_INLINE { return __builtin_amdgcn_readlane(v, k); };
+      n = n0 + k, at = item - before - of(p.incl - p.count), pieces = of(p.each);
+      part_at = parts + of(p.part_incl - p.parts) + at;
+      x.g0 = of(g.g0), x.rows = of(g.rows), x.len = of(g.len), x.tiles = of(g.tiles);
+      break;
+    }
+    const int block = __builtin_amdgcn_readfirstlane(at / pieces);
+    const Deal deal(x.tiles, pieces);
+    const int t0 = __builtin_amdgcn_readfirstlane(deal.start(at - block * pieces));
+    const int piece = __builtin_amdgcn_readfirstlane(deal.start(at - block * pieces + 1)) - t0;
+    if (item != unit) __syncthreads();  // (the records have been read: the rings may be written)
     const int cols = min(CB, x.rows - block * CB), ct = (cols + 15) / 16;
     const Deal waves(piece, nw);
     const int first = t0 + waves.start(wave);
@@ -176,8 +264,8 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
     }
     // ---- the waves' records joined, 16 columns at a time
     const int count = min(nw, piece);
-    const bool all = piece == x.tiles;
-    float *const part = a.parts + (((int64_t)(t0 == 0) * a.d.Hkv + h) * units + unit) * (CB * T::REC);
+    const bool all = pieces == 1;
+    float *const part = part_of(a, HT, h, part_at);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       if (c >= ct) break;
@@ -212,15 +300,6 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         if (d == 0) *(float2 *)(to + D) = float2{M, L};
       }
     }
-    u0 += piece;
-    if (u0 >= u1) return;
-    __syncthreads();  // (the records have been read: the rings may be written)
-    t0 = 0;
-    if (++block == x.blocks) {
-      block = 0;
-      do x = uniform_group(++n);
-      while (x.blocks * x.tiles == 0);
-    }
   }
 }
 
@@ -229,21 +308,19 @@ __device__ RXW8_INLINE void shared_walk(const SharedArgs &a) {
   using T = PagedTile<D, KIND>;
   const int lane = threadIdx.x & 63, G = a.d.Hq / a.d.Hkv, HT = (G + 15) / 16, heads = a.d.Hkv * HT;
   const int hk = blockIdx.x % heads, unit = blockIdx.x / heads, units = a.d.units, most = a.d.M * a.d.ps;
-  const Run run = run_of(a);
-  int own = 0;
+  const Group first = groups_from(a, 0);
+  int own = 0, some = 0;  // tiles, and sequences that have any
   for (int b0 = 0; b0 < a.d.B; b0 += 64) {
     const int len = b0 + lane < a.d.B ? a.d.lens[b0 + lane] : 0;
-    own += __builtin_amdgcn_readlane(scan64((int)(((unsigned)min(max(len, 0), most) + T::KT - 1) / T::KT)), 63);
+    const int tiles = (int)(((unsigned)min(max(len, 0), most) + T::KT - 1) / T::KT);
+    own += __builtin_amdgcn_readlane(scan64(tiles), 63);
+    some += __popcll(__ballot(tiles > 0));
   }
   // a head's workgroups for its prefixes, and for the sequences' own keys
-  const float cost = (KIND == kCodes ? kPrefixCodes : kPrefixTile) * ((float)run.tiles + kPrefixBlock * (float)run.blocks) / HT;
-  int up = __builtin_amdgcn_readfirstlane((int)rintf(units * cost / fmaxf(cost + (float)own, 1.f)));
-  up = run.tiles == 0 ? 0 : own == 0 ? units : min(max(up, 1), max(units - 1, 1));
-  const int uo = own == 0 ? 0 : max(units - up, 1);
-  // one to every wave's tile, or to every block of fewer
-  const int used = min(up * HT, max((run.tiles + a.d.waves - 1) / a.d.waves, run.blocks));
-  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = up * HT, a.plan[1] = used;
-  if (unit < up) prefix_walk<D, KIND, PREC>(a, hk / HT, unit * HT + hk % HT, up * HT, used, run.tiles);
+  const Plan plan = plan_of(a, first, (float)own + kOwnSequence * (float)some, HT);
+  const int up = (plan.takers + HT - 1) / HT, uo = own == 0 ? 0 : max(units - up, 1);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[0] = __float_as_int(plan.rate);
+  if (unit < up && unit * HT + hk % HT < plan.takers) prefix_walk<D, KIND, PREC>(a, hk / HT, unit * HT + hk % HT, HT, plan, first);
   if (unit >= units - uo) {
     if (unit < up) __syncthreads();  // (one workgroup to a head does both)
     paged_decode<D, KIND, true, PREC>(a.d, PagedPlaceOf{hk, unit - (units - uo), uo, a.own});
@@ -267,39 +344,27 @@ RXW8_SHARED_D(256)
 // The records of a row joined: a wave a row. Up to 64 groups, all that a row has to know is
 // loaded at once, its records next: the two round trips are what bounds it.
 extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a) {
-  const int lane = threadIdx.x & 63, D = a.d.D, REC = D + 4, G = a.d.Hq / a.d.Hkv;
+  const int lane = threadIdx.x & 63, D = a.d.D, REC = D + 4, G = a.d.Hq / a.d.Hkv, HT = (G + 15) / 16;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (int64_t)a.d.B * a.d.Hq) return;  // whole waves only; no barriers below
   const int b = (int)(row / a.d.Hq), hq = (int)(row - (int64_t)b * a.d.Hq), h = hq / G;
-  const int units = a.plan[0], used = a.plan[1], len = a.d.lens[b];
-  Group x;
-  int start = 0, total = 0;
-  x.tiles = x.rows = 0;
+  const int len = a.d.lens[b];
+  const float rate = __int_as_float(a.plan[0]);
+  const float *first = nullptr;  // of the prefix
+  int prefix = 0, parts = 0;
   for (int n0 = 0; n0 < a.N; n0 += 64) {
-    const int i = min(n0 + lane, a.N - 1);
-    const Group g = group_of(a, a.groups[i], a.groups[i + 1], a.prefix_lens[i]);
-    const int mine = n0 + lane < a.N ? g.blocks * g.tiles : 0, incl = scan64(mine);
-    // (the row's group, the last that begins at it or before and has rows: offsets do not decrease)
-    const unsigned long long in = __ballot(n0 + lane < a.N && g.g0 <= b && g.g0 + g.rows / G > b);
+    const Group g = groups_from(a, n0);
+    const Pieces p(g, rate);
+    const unsigned long long in = __ballot(g.g0 <= b && g.g0 + g.rows / G > b);
     if (in) {
       const int k = __builtin_ctzll(in);
-      x.g0 = __builtin_amdgcn_readlane(g.g0, k), x.rows = __builtin_amdgcn_readlane(g.rows, k);
-      x.tiles = __builtin_amdgcn_readlane(g.tiles, k);
-      start = total + __builtin_amdgcn_readlane(incl, k) - __builtin_amdgcn_readlane(mine, k);
+      const int i = (b - __builtin_amdgcn_readlane(g.g0, k)) * G + (hq - h * G), block = i / a.columns, col = i - block * a.columns;
+      prefix = __builtin_amdgcn_readlane(p.each, k);
+      const int at = parts + __builtin_amdgcn_readlane(p.part_incl - p.parts, k) + block * prefix;
+      first = prefix == 1 ? a.whole + row * REC : part_of(a, HT, h, at) + col * REC;
+      break;
     }
-    total += __builtin_amdgcn_readlane(incl, 63);
-  }
-  const float *first_rec = nullptr, *others = nullptr;  // of the prefix
-  int prefix = 0;
-  if (x.rows && x.tiles) {
-    const int i = (b - x.g0) * G + (hq - h * G), block = i / a.columns, col = i - block * a.columns;
-    start += block * x.tiles;
-    const Deal deal(total, used);
-    const int first = deal.taker(start);
-    prefix = deal.taker(start + x.tiles - 1) - first + 1;
-    const int64_t size = (int64_t)a.columns * REC;
-    first_rec = prefix == 1 ? a.whole + row * REC : a.parts + (((int64_t)a.d.Hkv + h) * units + first) * size + col * REC;
-    others = a.parts + ((int64_t)h * units + first) * size + col * REC;
+    parts += __builtin_amdgcn_readlane(p.part_incl, 63);
   }
   const int count = prefix + (len > 0 && a.d.M > 0);
   for (int d = 2 * lane; d < D; d += 128) {
@@ -307,7 +372,7 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a)
 #pragma unroll 1
     for (int k0 = 0; k0 < count; k0 += 8)
       join<8>(j, k0, count, [&](int, int k, float &m, float &l, float2 &o) {
-        const float *const rec = k >= prefix ? a.own + row * REC : k == 0 ? first_rec : others + (int64_t)k * a.columns * REC;
+        const float *const rec = k >= prefix ? a.own + row * REC : first + (int64_t)k * a.columns * REC;
         const float2 ml = *(const float2 *)(rec + D);
         m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
       });
