@@ -394,6 +394,19 @@ def test_short_prefixes_of_many_rows(rt, hq, hkv, d, kind):
     run(rt, rng, [2], [0, 90], np.zeros(90, int), hq, hkv, d, kind)
 
 
+@pytest.mark.parametrize("kind,hq,hkv,d", [("bf16", 40, 1, 64), ("q8", 8, 4, 128), ("f32", 4, 4, 64), ("bf16", 6, 2, 256)])
+def test_prefixes_of_very_different_lengths(rt, kind, hq, hkv, d):
+    """More than 64 groups, of which two have long prefixes, cut into pieces, one of them the last; and
+    two, one of them with a sequence less than there are workgroups."""
+    rng = np.random.default_rng(d + hq)
+    b = 75
+    prefix_lens = rng.integers(0, 70, b)
+    prefix_lens[[7, 74]] = 2500, 3001
+    run(rt, rng, prefix_lens, np.arange(b + 1), rng.integers(0, 30, b), hq, hkv, d, kind, "bf16", "f32")
+    run(rt, rng, [2500, 17], [0, 3, 45], np.zeros(45, int), hq, hkv, d, kind, "bf16", "f32")
+    run(rt, rng, [40, 1999], [0, 30, 60], rng.integers(0, 200, 60), hq, hkv, d, kind, "bf16", "f32")
+
+
 # ---- sizes past 32 bits --------------------------------------------------------------------
 
 def test_8_bit_pools_past_32_bits(rt):
