@@ -200,7 +200,8 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_q8_read_any(PagedReadArgs
 }
 
 // Widths of whole 8 elements at 16-byte boundaries: a wave for each row and `kRows` x 64
-// of its pieces of 8 elements
+// of its pieces of 8 elements, bound by HBM: 13800 positions of 8 heads of 128 in 8 bits to bf16
+// rows 18.5 us, 4.6 TB/s (pieces of 64 for a wave, one round of loads each: 20.3)
 template <int KIND, typename S>
 __device__ __forceinline__ void paged_read(const PagedReadArgs &a) {
   constexpr int NP = KIND == 1 ? 2 : 1, NS = sizeof(S) / 2;  // 16-byte words of 8 elements (codes: half a one)
