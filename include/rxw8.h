@@ -278,11 +278,12 @@ int rxw8_gqa_prefill_into(rxw8_runtime *rt, rxw8_buffer *q,
                           rxw8_buffer *k_cache, rxw8_buffer *v_cache,
                           rxw8_buffer *starts, float scale, rxw8_buffer *out);
 
-/* The serving calls (paged cache, packed prompts, rxw8_sample) take buffers of their
- * runtime only, and what they write must share no memory with another argument. Paged
- * decode and rxw8_sample work in the f32 attention's fixed blocks of their runtime, one
- * for the calls that run and one for those that a capture records: a graph may replay
- * beside the runtime's other calls, two graphs at the same time need a runtime each. */
+/* The serving calls (paged cache, packed prompts, logits, rxw8_sample) take buffers of
+ * their runtime only, and what they write must share no memory with another argument
+ * (rxw8_adjust_logits_into aside). Paged decode, over shared prefixes too, and rxw8_sample
+ * work in the f32 attention's fixed blocks of their runtime, one for the calls that run and
+ * one for those that a capture records: a graph may replay beside the runtime's other
+ * calls, two graphs at the same time need a runtime each. */
 
 /* ---- paged key/value cache (no counterpart in the reference, whose cache is one
  * plane per sequence, kv_cache.rs:7-111) --------------------------------------
@@ -327,7 +328,8 @@ int rxw8_gqa_decode_paged_into(rxw8_runtime *rt, rxw8_buffer *q,
  * the scale NaN and the codes 128: all of it stands for NaN. (127 s may round past
  * f32's end where amax is its last value.) */
 
-/* rxw8_paged_kv_append into 8-bit pages (all four buffers are written). */
+/* rxw8_paged_kv_append into 8-bit pages (all four buffers are written; rows that race
+ * for one position may leave the codes of one and the scale of another). */
 int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages,
                             rxw8_buffer *v_pages, rxw8_buffer *k_scales,
                             rxw8_buffer *v_scales, rxw8_buffer *k,
