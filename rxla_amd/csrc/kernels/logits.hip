@@ -23,19 +23,23 @@ struct LogitsArgs {
   int64_t T, E, R, V;
   int in_f32, out_f32;
   int chunk, chunks;             // words of a workgroup; workgroups of a row
+  int given;                     // bits kOffsets ..: what there is (else a readable word stands there)
 };
 
 // A workgroup takes `chunk` words of a row. It counts those of the row's history that
 // fall on them in LDS (bit 31: seen in the prompt; the rest: n; additions of whole numbers,
 // whose order changes nothing) and finds the last bias entry of each, then goes over the
 // words once. Under a full memory system every load that waits for another one costs
-// microseconds, so there are two rounds of them: the row's settings, then the logits, the
+// microseconds, so there are two rounds of them: the row's settings beside the logits, then the
 // mask's bits, the first tokens and the biases together. 64 rows of 248320 f32 logits with
-// histories of 1 to 8000, up to 300 biases and masks: 33.7 us (46 with the loads one after
-// another), 3.8 TB/s; 25 us with no setting at all, a copy. Chunks of 1024, 2048, 4096 and
-// 8192 words, 8 a thread: 43.6, 34.9, 33.7 and 39.5 us (every workgroup of a row goes over
-// the row's history). One row of 151936 and 800 tokens: 5 us, the two rounds and the launch.
-constexpr int kTokens = 8, kValues = 512;  // tokens of a thread under way; biases kept in LDS
+// histories of 1 to 8000, up to 300 biases and masks: 31.1 us, 4.1 TB/s (33.7 with a wait for
+// each setting, 46 with the other loads one after another too; 25 with no setting at all, a
+// copy). Chunks of 1024, 2048, 4096 and 8192 words, 8 a thread: 39.8, 32.4, 31.1 and 31.9 us,
+// and 16 rows of 151936 bf16 logits 7.2, 6.1, 6.2 and 7.0 (every workgroup of a row goes over
+// its history). Two, 4 and 8 tokens a thread at once, before that: 34.2, 33.4 and 33.6, and 7.2,
+// 6.9 and 7.7 us. One row of 151936 and 800 tokens: 5 us, the two rounds and the launch.
+enum { kOffsets, kPrompts, kRepetition, kFrequency, kPresence, kBiases, kRows };
+constexpr int kThreads = 512, kTokens = 4, kValues = 512;  // tokens of a thread under way; biases kept in LDS
 
 // Device memory that the launch does not write, at a wave-uniform address (scalar loads)
 template <typename T>
@@ -44,8 +48,9 @@ __device__ __forceinline__ T uniform_load(const T *p, int64_t i) {
 }
 
 struct LogitsRow {
-  int64_t b, w0, t0, t1, mine, e0, e1;  // row, first word; its tokens, and those behind the prompt; its bias entries
-  int n;                                // words of the workgroup
+  int64_t b, w0;                        // row, first word
+  uint32_t t0, t1, mine, e0, e1;        // its tokens, and those behind the prompt; its bias entries
+  uint32_t n;                           // words of the workgroup
   float r, f, p;
   const uint32_t *mask;
   uint32_t *counts, *entries;
@@ -55,53 +60,60 @@ struct LogitsRow {
 
   __device__ __forceinline__ LogitsRow(const LogitsArgs &a, uint32_t *lds) {
     b = blockIdx.x / a.chunks, w0 = (int64_t)(blockIdx.x - b * a.chunks) * a.chunk;
-    n = (int)min((int64_t)a.chunk, a.V - w0);
+    n = (uint32_t)min((int64_t)a.chunk, a.V - w0);
     counts = lds, entries = lds + (a.tokens ? a.chunk : 0), values = (float *)(entries + a.chunk);
-    auto bounded = [](int64_t i, int64_t most) { return i < 0 ? 0 : i < most ? i : most; };
-    t0 = a.tokens ? uniform_load(a.offsets, b) : 0, t1 = a.tokens ? uniform_load(a.offsets, b + 1) : 0;
-    mine = a.prompts ? uniform_load(a.prompts, b) : 0;
-    e0 = a.bias ? uniform_load(a.bias_offsets, b) : 0, e1 = a.bias ? uniform_load(a.bias_offsets, b + 1) : 0;
-    r = a.repetition ? uniform_load(a.repetition, b) : 1.f;
-    f = a.frequency ? uniform_load(a.frequency, b) : 0.f;
-    p = a.presence ? uniform_load(a.presence, b) : 0.f;
-    const int64_t m = a.mask ? a.mask_rows ? uniform_load(a.mask_rows, b) : b : -1;
-    t0 = bounded(t0, a.T), t1 = bounded(t1, a.T), e0 = bounded(e0, a.E), e1 = bounded(e1, a.E);
-    mine = t0 + max(mine, (int64_t)0);
+    // (loads without branches between them, one wait for all; T, E and R are 0 where there is none)
+    auto load = [&](int bit, auto *p, int i) {
+      const uint32_t at = (uint32_t)(b + i) * 4 & (uint32_t)__builtin_amdgcn_sbfe(a.given, bit, 1);
+      return *(const __attribute__((address_space(4))) uint32_t *)((uintptr_t)p + at);
+    };
+    auto or_zero = [&](int bit, uint32_t v) { return v & (uint32_t)__builtin_amdgcn_sbfe(a.given, bit, 1); };
+    uint32_t from = load(kOffsets, a.offsets, 0), to = load(kOffsets, a.offsets, 1), own = load(kPrompts, a.prompts, 0),
+             first = load(kBiases, a.bias_offsets, 0), end = load(kBiases, a.bias_offsets, 1), row = load(kRows, a.mask_rows, 0),
+             factor = load(kRepetition, a.repetition, 0), each = load(kFrequency, a.frequency, 0), once = load(kPresence, a.presence, 0);
+    asm volatile("" : "+s"(from), "+s"(to), "+s"(own), "+s"(first), "+s"(end), "+s"(row), "+s"(factor), "+s"(each), "+s"(once));
+    auto bounded = [](uint32_t i, int64_t most) { return min((uint32_t)max((int)i, 0), (uint32_t)most); };
+    t0 = bounded(from, a.T), t1 = bounded(to, a.T), e0 = bounded(first, a.E), e1 = bounded(end, a.E);
+    mine = t0 + (uint32_t)max((int)or_zero(kPrompts, own), 0);
+    r = a.given >> kRepetition & 1 ? __uint_as_float(factor) : 1.f;
+    f = __uint_as_float(or_zero(kFrequency, each)), p = __uint_as_float(or_zero(kPresence, once));
+    const int64_t m = a.given >> kRows & 1 ? (int)row : b;
     mask = m >= 0 && m < a.R ? a.mask + m * ((a.V + 31) / 32) : nullptr;
   }
-  __device__ __forceinline__ void load_tokens(const LogitsArgs &a, int64_t t) {
+  __device__ __forceinline__ void load_tokens(const LogitsArgs &a, uint32_t t) {
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      const int64_t i = t + u * (int)blockDim.x;
-      tokens[u] = i < t1 ? a.tokens[i] : -1;
+      const uint32_t i = t + u * kThreads;
+      const int token = a.tokens[min(i, (uint32_t)a.T - 1)];  // (no branch between the loads)
+      tokens[u] = i < t1 ? token : -1;
     }
   }
   __device__ __forceinline__ void load(const LogitsArgs &a) {
-    load_tokens(a, t0 + threadIdx.x);
-    const int64_t e = e0 + threadIdx.x;
-    word = e < e1 ? a.bias_words[e] : -1;
-    value = e < e1 ? a.bias[e] : 0.f;
+    if (a.tokens) load_tokens(a, t0 + threadIdx.x);
+    if (!a.bias) return;
+    const uint32_t e = min(e0 + threadIdx.x, (uint32_t)a.E - 1);
+    word = a.bias_words[e], value = a.bias[e];
   }
   // Counts and entries of the workgroup's words
   __device__ __forceinline__ void count(const LogitsArgs &a) {
     const int total = a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr));  // (a multiple of 4)
-    for (int i = 4 * threadIdx.x; i < total; i += 4 * blockDim.x) *(u32x4 *)(counts + i) = u32x4{0, 0, 0, 0};
+    for (int i = 4 * threadIdx.x; i < total; i += 4 * kThreads) *(u32x4 *)(counts + i) = u32x4{0, 0, 0, 0};
     __syncthreads();
-    for (int64_t t = t0 + threadIdx.x; t < t1; t += kTokens * (int)blockDim.x) {
-      if (t >= t0 + kTokens * (int)blockDim.x) load_tokens(a, t);
+    for (uint32_t t = t0 + threadIdx.x; t < t1; t += kTokens * kThreads) {
+      if (t >= t0 + kTokens * kThreads) load_tokens(a, t);
 #pragma unroll
       for (int u = 0; u < kTokens; ++u) {
-        const int64_t at = (int64_t)tokens[u] - w0;
-        if (at < 0 || at >= n) continue;
-        if (t + u * (int)blockDim.x < mine) atomicOr(counts + at, 0x80000000u);
+        const uint32_t at = (uint32_t)tokens[u] - (uint32_t)w0;  // (words before the first wrap past n)
+        if (at >= n) continue;
+        if (t + u * kThreads < mine) atomicOr(counts + at, 0x80000000u);
         else atomicAdd(counts + at, 1u);
       }
     }
-    for (int64_t e = e0 + threadIdx.x; e < e1; e += (int)blockDim.x) {
-      const bool first = e < e0 + (int)blockDim.x;
-      const int64_t at = (int64_t)(first ? word : a.bias_words[e]) - w0;
-      if (at < 0 || at >= n) continue;
-      atomicMax(entries + at, (uint32_t)(e - e0 + 1));
+    for (uint32_t e = e0 + threadIdx.x; e < e1; e += kThreads) {
+      const bool first = e < e0 + kThreads;
+      const uint32_t at = (uint32_t)(first ? word : a.bias_words[e]) - (uint32_t)w0;
+      if (at >= n) continue;
+      atomicMax(entries + at, e - e0 + 1);
       if (e - e0 < kValues) values[e - e0] = first ? value : a.bias[e];
     }
     __syncthreads();
@@ -118,12 +130,12 @@ struct LogitsRow {
 };
 
 // Rows of any length and alignment: a word a thread at a time
-extern "C" __global__ void __launch_bounds__(512) rxw8_logits_any(LogitsArgs a) {
+extern "C" __global__ void __launch_bounds__(kThreads) rxw8_logits_any(LogitsArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];  // counts [chunk], entries [chunk], values
   LogitsRow x(a, lds);
   x.load(a);
   x.count(a);
-  for (int i = threadIdx.x; i < x.n; i += blockDim.x) {
+  for (uint32_t i = threadIdx.x; i < x.n; i += kThreads) {
     const int64_t w = x.w0 + i, at = x.b * a.V + w;
     const float z = x.adjust(a, any_load(a.logits, at, a.in_f32), a.tokens ? x.counts[i] : 0, a.bias ? x.entries[i] : 0,
                              !x.mask || x.mask[w >> 5] >> (w & 31) & 1);
@@ -136,16 +148,16 @@ extern "C" __global__ void __launch_bounds__(512) rxw8_logits_any(LogitsArgs a) 
 template <typename S, typename P>
 __device__ __forceinline__ void logits_adjust(const LogitsArgs &a, uint32_t *lds) {
   constexpr int NS = sizeof(S) / 2;  // 16-byte words of 8 logits
-  LogitsRow x(a, lds);
+  const int64_t b = blockIdx.x / a.chunks, w = (int64_t)(blockIdx.x - b * a.chunks) * a.chunk + 8 * threadIdx.x, at = b * a.V + w;
+  const bool mine = w < a.V;
   u32x4 in[NS];
   uint32_t bits = 0xff;
-  const int64_t at = x.b * a.V + x.w0 + 8 * threadIdx.x;
-  const bool mine = 8 * (int)threadIdx.x < x.n;
   if (mine) {
 #pragma unroll
     for (int k = 0; k < NS; ++k) in[k] = ((const u32x4 *)((const S *)a.logits + at))[k];
-    if (x.mask) bits = ((const uint8_t *)x.mask)[(x.w0 >> 3) + threadIdx.x];
   }
+  LogitsRow x(a, lds);
+  if (mine && x.mask) bits = ((const uint8_t *)x.mask)[w >> 3];
   u32x4 c[2] = {}, e[2] = {};
   if (a.tokens || a.bias) {
     x.load(a);
@@ -170,7 +182,7 @@ __device__ __forceinline__ void logits_adjust(const LogitsArgs &a, uint32_t *lds
     to[0] = u32x4{pack_bf16x2(z[0], z[1]), pack_bf16x2(z[2], z[3]), pack_bf16x2(z[4], z[5]), pack_bf16x2(z[6], z[7])};
   }
 }
-extern "C" __global__ void __launch_bounds__(512) rxw8_logits_adjust(LogitsArgs a) {
+extern "C" __global__ void __launch_bounds__(kThreads) rxw8_logits_adjust(LogitsArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
   if (a.in_f32 && a.out_f32) logits_adjust<float, float>(a, lds);
   else if (a.in_f32) logits_adjust<float, uint16_t>(a, lds);

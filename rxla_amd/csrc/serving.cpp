@@ -75,6 +75,7 @@ struct LogitsArgs {
   int64_t T, E, R, V;
   int in_f32, out_f32;
   int chunk, chunks;
+  int given;
 };
 struct PackedArgs {
   const void *q;
@@ -679,13 +680,25 @@ int rxw8_adjust_logits_into(rxw8_runtime *rt, rxw8_buffer *logits, const rxw8_lo
   const int64_t B = logits->dims[0], V = logits->dims[1];
   if (B == 0) return RXW8_OK;
   std::lock_guard<std::recursive_mutex> g(rt->mu);
-  auto i32 = [](const rxw8_buffer *b) { return b ? (const int32_t *)b->ptr : nullptr; };
-  auto f32 = [](const rxw8_buffer *b) { return b ? (const float *)b->ptr : nullptr; };
-  LogitsArgs a{logits->ptr, out->ptr, i32(o->tokens), i32(o->offsets), i32(o->prompts), f32(o->repetition),
-               f32(o->frequency), f32(o->presence), i32(o->bias_words), f32(o->bias), i32(o->bias_offsets),
-               (const uint32_t *)i32(o->mask), i32(o->mask_rows), o->tokens ? o->tokens->dims[0] : 0,
-               o->bias ? o->bias->dims[0] : 0, o->mask ? o->mask->dims[0] : 0, V, logits->dtype == RXW8_F32,
-               out->dtype == RXW8_F32, (int)kLogitsChunk, (int)((V + kLogitsChunk - 1) / kLogitsChunk)};
+  // what a row loads of each setting that is off: a word of the runtime's own
+  const void *const none = rt->f32_attn[0];
+  int given = 0, bit = 0;
+  auto setting = [&](const rxw8_buffer *b) {
+    given |= (b != nullptr) << bit++;
+    return b ? b->ptr : none;
+  };
+  LogitsArgs a{};
+  a.logits = logits->ptr, a.out = out->ptr;
+  a.offsets = (const int32_t *)setting(o->offsets), a.prompts = (const int32_t *)setting(o->prompts);
+  a.repetition = (const float *)setting(o->repetition), a.frequency = (const float *)setting(o->frequency);
+  a.presence = (const float *)setting(o->presence), a.bias_offsets = (const int32_t *)setting(o->bias_offsets);
+  a.mask_rows = (const int32_t *)setting(o->mask_rows);
+  a.T = o->tokens ? o->tokens->dims[0] : 0, a.E = o->bias ? o->bias->dims[0] : 0, a.R = o->mask ? o->mask->dims[0] : 0, a.V = V;
+  if (a.T) a.tokens = (const int32_t *)o->tokens->ptr;
+  if (a.E) a.bias_words = (const int32_t *)o->bias_words->ptr, a.bias = (const float *)o->bias->ptr;
+  if (a.R) a.mask = (const uint32_t *)o->mask->ptr;
+  a.in_f32 = logits->dtype == RXW8_F32, a.out_f32 = out->dtype == RXW8_F32, a.given = given;
+  a.chunk = (int)kLogitsChunk, a.chunks = (int)((V + kLogitsChunk - 1) / kLogitsChunk);
   const bool pieces = V % 8 == 0 && !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15);
   return launch(rt, pieces ? "rxw8_logits_adjust" : "rxw8_logits_any", dim3((unsigned)(B * a.chunks)), dim3(kLogitsChunk / 8), a,
                 sizeof(int) * (size_t)a.chunk * ((a.tokens != nullptr) + (a.bias != nullptr)) + (a.bias ? kLogitsValues * sizeof(float) : 0));
