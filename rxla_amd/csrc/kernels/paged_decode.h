@@ -573,9 +573,9 @@ struct PagedWave {
         }
     };
     weigh();
-    if (__ballot(top > 0x1p15f || m[c] == kMinusInf)) {
+    if (__ballot(top > 0x1p15f || sum > 0x1p110f || m[c] == kMinusInf)) {
       // the largest weight becomes 2^10; a key that it leaves far behind the largest score
-      // (a scale of 0) not more than 2^100
+      // (a scale of 0, which the sum alone shows) not more than 2^100
       float largest = kMinusInf, highest = kMinusInf;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u)
