@@ -41,10 +41,13 @@
 // take the scales outside the products:
 //   q      times the power of two that brings its row's largest magnitude to 2^14: one part
 //          for bf16 (exact to 2^-39 of the largest), two for f32 (2^-24);
-//   p s_v  are held between 2^-24 and 2^15 by the row's reference, which need not be the
-//          scores' maximum: p = exp2(s - ref), and where a tile's largest weight passes 2^15,
-//          ref moves so that it is 2^10. No maximum is taken otherwise, of lanes or
-//          tiles. One f16 part behind a bf16 output (2^-12 of a weight, the output's rounding
+//   p s_v  are held between 2^-24 and 2^15 by a power of two of the row's: p = exp2(s - ref), ref a
+//          score that need not be the largest, and the products take p up s_v. Where a tile's largest of
+//          them passes 2^15 or its sum of p 2^10, ref becomes the largest score and `up` what
+//          brings the largest product to 2^10. No maximum is taken otherwise, of lanes or
+//          tiles. (One reference for both loses the sum where s_v are far apart: rows of 0
+//          and of 1e26 have products 2^126 from each other and weigh the same.) One f16 part
+//          behind a bf16 output (2^-12 of a weight, the output's rounding
 //          is 2^-9 of it), two behind an f32 one; what is below 2^-24 / 2^10 of the largest
 //          weight so far rounds to multiples of that.
 // V needs no transposing reads: a lane takes D / 16 dims of its own of each of its keys, one
@@ -106,33 +109,52 @@ struct PagedTile {
   static constexpr int NS = CODES ? KT / 32 : 0;  // copies of 64 scales: the tile's K's, its V's
   static constexpr int NK = N + NS;               // copies that K's products wait for
   static constexpr int RING = 2 * HALF + 256 * NS;  // a wave's K and V, scales behind them
-  static constexpr int REC = D + 4;               // floats of a record: acc [D], max, sum
+  static constexpr int REC = D + 4;               // floats of a record: acc [D], max, sum, codes: the power of acc
   static __device__ __forceinline__ int kx(int row) { return row & (CH < 16 ? CH - 1 : 15); }
   static __device__ __forceinline__ int vx(int row) { return KIND != kBf16 ? 0 : 2 * (row & (CH < 16 ? 3 : 7)); }
 };
 
 // (max, sum, acc) records joined in order: NB of them, number k0 + k with
-// get(k, min(k0 + k, count - 1), m, l, o); those from `count` on do not count. o is two
-// of a head's dims.
+// get(k, min(k0 + k, count - 1), m, l, up, o); those from `count` on do not count. o is two
+// of a head's dims. Over codes o is times 2^up, a power of each record's own.
 struct Joined {
-  float M = kMinusInf, L = 0.f;
+  float M = kMinusInf, L = 0.f, E = kMinusInf;  // (E: the power of O, for codes)
   float2 O = float2{0.f, 0.f};
 };
 __device__ __forceinline__ float record_weight(float m, float l, float M) {
   return m == kMinusInf ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M);  // (l NaN: scores were)
 }
-template <int NB, typename Get>
+// The power of two that o of a record is to be multiplied by next to others, and that times 2^-E
+__device__ __forceinline__ float record_power(float m, float up, float M) { return m == kMinusInf ? kMinusInf : (m - M) - up; }
+__device__ __forceinline__ float record_scale(float e, float E) { return e == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(e - E); }
+template <int NB, bool CODES, typename Get>
 __device__ __forceinline__ void join(Joined &j, int k0, int count, Get get) {
-  float m[NB], l[NB], M = j.M;
+  float m[NB], l[NB], up[NB], M = j.M;
   float2 o[NB];
 #pragma unroll
-  for (int k = 0; k < NB; ++k) get(k, min(k0 + k, count - 1), m[k], l[k], o[k]);
+  for (int k = 0; k < NB; ++k) get(k, min(k0 + k, count - 1), m[k], l[k], up[k], o[k]);
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
     if (k0 + k >= count) m[k] = kMinusInf, l[k] = 0.f, o[k] = float2{0.f, 0.f};
     M = fmaxf(M, m[k]);
   }
   const float f0 = record_weight(j.M, j.L, M);
+  if constexpr (CODES) {
+    const float e0 = record_power(j.M, -j.E, M);
+    float e[NB], E = e0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) e[k] = record_power(m[k], up[k], M), E = fmaxf(E, e[k]);
+    const float g0 = record_scale(e0, E);
+    j.M = M, j.E = E, j.L *= f0, j.O.x *= g0, j.O.y *= g0;
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const float g = record_scale(e[k], E);
+      j.L += record_weight(m[k], l[k], M) * l[k];
+      j.O.x += g * o[k].x;
+      j.O.y += g * o[k].y;
+    }
+    return;
+  }
   j.M = M, j.L *= f0, j.O.x *= f0, j.O.y *= f0;
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
@@ -191,6 +213,12 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x, uint32_t y) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, up, less));
 }
 constexpr float kCodeUnit = 0x1p9f;
+// V's scales are taken times 2^-24, so that what products and sums need beside them stays within
+// f32 for every scale from 2^-82 on (the append's begin at 2^-47)
+constexpr int kScaleShift = 24;
+constexpr float kMostUp = 116.f;
+// What a row of codes' products is to be multiplied by for its output: 2^e of them, e as in Joined
+__device__ __forceinline__ float codes_inverse(float e, float sum) { return __builtin_amdgcn_exp2f(e + (float)kScaleShift) * (1.0f / sum); }
 // Two f32 as an f16 pair, round to nearest even, and what that leaves
 __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2));
@@ -251,6 +279,7 @@ struct PagedWave {
   f32x4 o[CT][D / 16], s[CT][T::SUB];
   f32x4 vs[CODES ? T::SUB : 1];     // V's scales
   float m[CT], l[CT];               // (codes: m is the reference)
+  float up[CODES ? CT : 1];         // codes: what weights are multiplied by in the products, a power of two
   float unit[CODES ? CT : 1];       // codes: what a product of q and codes counts in a score, but for s_k
 
   __device__ RXW8_INLINE PagedWave(const PagedDecodeArgs &a, int h, char *mem)
@@ -389,6 +418,7 @@ struct PagedWave {
     }
     m[c] = kMinusInf;
     l[c] = 0.f;
+    if constexpr (CODES) up[c] = 1.f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -453,7 +483,7 @@ struct PagedWave {
       if constexpr (CODES) {
         const uint32_t at = mem + 2 * T::HALF + 4 * (16 * u + 4 * g4);
         scale = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)at;
-        vs[u] = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(at + 4 * T::KT);
+        vs[u] = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(at + 4 * T::KT) * (1.f / (1 << kScaleShift));
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
@@ -549,6 +579,8 @@ struct PagedWave {
     for (int u = 0; u < T::SUB; ++u) s[c][u] = w[u];
   }
 
+  // The power of up[c]
+  __device__ RXW8_INLINE float up_of(int c) const { return (float)((int)(__float_as_uint(up[CODES ? c : 0]) >> 23) - 127); }
   __device__ RXW8_INLINE void softmax_codes(int c, const Tile &x, bool part) {
     f32x4 w[T::SUB];
     float sum, top;
@@ -568,28 +600,32 @@ struct PagedWave {
         for (int r = 0; r < 4; ++r) {
           const float p = __builtin_amdgcn_exp2f(s[c][u][r] - ref);
           sum += p;
-          w[u][r] = p * vs[u][r];
+          w[u][r] = p * up[c] * vs[u][r];
           top = fmaxf(top, fabsf(w[u][r]));
         }
     };
     weigh();
-    if (__ballot(top > 0x1p15f || sum > 0x1p110f || m[c] == kMinusInf)) {
-      // the largest weight becomes 2^10; a key that it leaves far behind the largest score
-      // (a scale of 0, which the sum alone shows) not more than 2^100
-      float largest = kMinusInf, highest = kMinusInf;
+    if (__ballot(top > 0x1p15f || sum > 0x1p10f || m[c] == kMinusInf)) {
+      float highest = kMinusInf, largest = kMinusInf;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          largest = fmaxf(largest, s[c][u][r] + fminf(__builtin_amdgcn_logf(fabsf(vs[u][r])), 128.f));
-          highest = fmaxf(highest, s[c][u][r]);
-        }
-      const float to = fmaxf(m[c], fmaxf(max4(largest) - 10.f, max4(highest) - 100.f));
-      const float f = to == kMinusInf ? 1.f : exp2f(m[c] - to);
+        for (int r = 0; r < 4; ++r) highest = fmaxf(highest, s[c][u][r]);
+      const float to = fmaxf(m[c], max4(highest)), ref = to == kMinusInf ? 0.f : to;
+#pragma unroll
+      for (int u = 0; u < T::SUB; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          largest = fmaxf(largest, s[c][u][r] - ref + fminf(__builtin_amdgcn_logf(fabsf(vs[u][r])), 128.f));
+      // (no product so far grows: m / up does not fall; the first fminf passes over a NaN)
+      const float was = up_of(c), moved = to - m[c];
+      const float power = fminf(fminf(floorf(was + moved), 10.f - floorf(max4(largest))), kMostUp);
+      const float f = to == kMinusInf ? 1.f : exp2f(-moved), g = to == kMinusInf ? 1.f : exp2f(power - was - moved);
       m[c] = to;
+      up[c] = __uint_as_float((uint32_t)((int)power + 127) << 23);
       l[c] *= f;
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) o[c][n] *= f;
+      for (int n = 0; n < D / 16; ++n) o[c][n] *= g;
       weigh();
     }
     l[c] += sum;
@@ -777,7 +813,10 @@ struct PagedWave {
     const float sum = sum4(l[c]);
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) *(f32x4 *)(rec + quad_dim(i)) = quad(c, i);
-    if (g4 == 0) rec[D] = m[c], rec[D + 1] = sum;
+    if (g4 == 0) {
+      rec[D] = m[c], rec[D + 1] = sum;
+      if constexpr (CODES) rec[D + 2] = up_of(c);
+    }
   }
 };
 
@@ -885,11 +924,12 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = w.quad(0, i);
             if (w.g4 == 0) *(float2 *)(to + D) = float2{w.m[0], sum};
+            if (KIND == kCodes && w.g4 == 0) to[D + 2] = w.up_of(0);
           }
         } else {
           const float sum = sum4(w.l[0]);
           if (col < gt) {
-            const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+            const float inv = sum == 0.f ? 0.f : KIND == kCodes ? codes_inverse(-w.up_of(0), sum) : 1.0f / sum;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               const f32x4 y = w.quad(0, i) * inv;
@@ -909,6 +949,7 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = w.quad(0, i);
         if (w.g4 == 0) to[D] = w.m[0], to[D + 1] = sum;
+        if (KIND == kCodes && w.g4 == 0) to[D + 2] = w.up_of(0);
       }
       if (lane == 0) *p = Piece{seq, first, n};
     };
@@ -986,10 +1027,11 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       float *const rec = place.rows + ((int64_t)b * a.Hq + hq0 + r) * T::REC;
       *(float2 *)(rec + d) = j.O;
       if (d == 0) *(float2 *)(rec + D) = float2{j.M, j.L};
+      if (KIND == kCodes && d == 0) rec[D + 2] = -j.E;
       return;
     }
     const int64_t to = ((int64_t)b * a.Hq + hq0) * D + 2 * i;
-    const float inv = j.L == 0.f ? 0.f : 1.0f / j.L;
+    const float inv = j.L == 0.f ? 0.f : KIND == kCodes ? codes_inverse(j.E, j.L) : 1.0f / j.L;
     if (a.out_f32) *(float2 *)((float *)a.out + to) = float2{j.O.x * inv, j.O.y * inv};
     else *(uint32_t *)((uint16_t *)a.out + to) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
   };
@@ -1012,21 +1054,23 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       Joined j;
       uint32_t bits = same;
       int x = e;
-      auto get = [&](int, int, float &m, float &l, float2 &o) {
+      auto get = [&](int, int, float &m, float &l, float &up, float2 &o) {
         if (bits) x = __builtin_ctz(bits), bits &= bits - 1;
         const float *const rec = (const float *)(lds + (x >> 1) * (first_at + rec_bytes) + ((x & 1) ? 0 : first_at)) + r * T::REC;
         const float2 ml = *(const float2 *)(rec + D);
         m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
+        if constexpr (KIND == kCodes) up = rec[D + 2];
       };
       const int n = __builtin_popcount(same);
 #pragma unroll 1
-      for (int k0 = 0; k0 < n; k0 += 4) join<4>(j, k0, n, get);
+      for (int k0 = 0; k0 < n; k0 += 4) join<4, KIND == kCodes>(j, k0, n, get);
       if (whole) {
         write(p.b, i, j);
       } else {
         float *const tr = to + r * T::REC;
         store_pair(tr + d, j.O.x, j.O.y);
         if (d == 0) store_pair(tr + D, j.M, j.L);
+        if (KIND == kCodes && d == 0) store_pair(tr + D + 2, -j.E, 0.f);
       }
     }
   }
@@ -1074,10 +1118,11 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
         }
 #pragma unroll 1
         for (int k0 = 0; k0 < n; k0 += 4)
-          join<4>(j, k0, n, [&](int, int c, float &m, float &l, float2 &o) {
+          join<4, KIND == kCodes>(j, k0, n, [&](int, int c, float &m, float &l, float &up, float2 &o) {
             const float *const rec = (const float *)lds + c * rec_size + r * T::REC;
             const float2 ml = *(const float2 *)(rec + D);
             m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
+            if constexpr (KIND == kCodes) up = rec[D + 2];
           });
       }
       if (i0 + (int)threadIdx.x < pairs) write(p.b, i, j);

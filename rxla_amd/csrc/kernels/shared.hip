@@ -279,19 +279,26 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         if (at >= cols) break;
         const float *const rec = (const float *)lds + r * T::REC;
         float2 ml[kPagedWaves];
-        float M = kMinusInf, L = 0.f;
+        float M = kMinusInf, L = 0.f, E = kMinusInf, e[KIND == kCodes ? kPagedWaves : 1];
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kPagedWaves; ++k) {
           ml[k] = k < count ? *(const float2 *)(rec + k * 16 * T::REC + D) : float2{kMinusInf, 0.f};
           M = fmaxf(M, ml[k].x);
         }
+        if constexpr (KIND == kCodes) {
+#pragma unroll
+          for (int k = 0; k < kPagedWaves; ++k) {
+            e[k] = record_power(ml[k].x, k < count ? rec[k * 16 * T::REC + D + 2] : 0.f, M);
+            E = fmaxf(E, e[k]);
+          }
+        }
 #pragma unroll
         for (int k = 0; k < kPagedWaves; ++k)
           if (k < count) {
             const float f = record_weight(ml[k].x, ml[k].y, M);
             L += f * ml[k].y;
-            O += f * *(const f32x4 *)(rec + k * 16 * T::REC + d);
+            O += (KIND == kCodes ? record_scale(e[KIND == kCodes ? k : 0], E) : f) * *(const f32x4 *)(rec + k * 16 * T::REC + d);
           }
         float *to = part + at * T::REC;
         if (all) {
@@ -300,6 +307,7 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         }
         *(f32x4 *)(to + d) = O;
         if (d == 0) *(float2 *)(to + D) = float2{M, L};
+        if (KIND == kCodes && d == 0) to[D + 2] = -E;
       }
     }
   }
@@ -372,17 +380,23 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a)
     parts += __builtin_amdgcn_readlane(p.part_incl, 63);
   }
   const int count = prefix + (len > 0 && a.d.M > 0);
-  for (int d = 2 * lane; d < D; d += 128) {
-    Joined j;
+  auto out = [&](auto codes) {
+    constexpr bool CODES = decltype(codes)::value;
+    for (int d = 2 * lane; d < D; d += 128) {
+      Joined j;
 #pragma unroll 1
-    for (int k0 = 0; k0 < count; k0 += 8)
-      join<8>(j, k0, count, [&](int, int k, float &m, float &l, float2 &o) {
-        const float *const rec = k >= prefix ? a.own + row * REC : first + (int64_t)k * a.columns * REC;
-        const float2 ml = *(const float2 *)(rec + D);
-        m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
-      });
-    const float inv = j.L == 0.f ? 0.f : 1.0f / j.L;
-    if (a.d.out_f32) *(float2 *)((float *)a.d.out + row * D + d) = float2{j.O.x * inv, j.O.y * inv};
-    else *(uint32_t *)((uint16_t *)a.d.out + row * D + d) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
-  }
+      for (int k0 = 0; k0 < count; k0 += 8)
+        join<8, CODES>(j, k0, count, [&](int, int k, float &m, float &l, float &up, float2 &o) {
+          const float *const rec = k >= prefix ? a.own + row * REC : first + (int64_t)k * a.columns * REC;
+          const float2 ml = *(const float2 *)(rec + D);
+          m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
+          if constexpr (CODES) up = rec[D + 2];
+        });
+      const float inv = j.L == 0.f ? 0.f : CODES ? codes_inverse(j.E, j.L) : 1.0f / j.L;
+      if (a.d.out_f32) *(float2 *)((float *)a.d.out + row * D + d) = float2{j.O.x * inv, j.O.y * inv};
+      else *(uint32_t *)((uint16_t *)a.d.out + row * D + d) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
+    }
+  };
+  if (a.kind == 2) out(std::true_type{});
+  else out(std::false_type{});
 }

@@ -5,6 +5,7 @@ import pytest
 
 import serving_more_ref as more
 from test_gpu_cache8 import decode8
+from test_gpu_serving import STEP, check, floats
 from test_gpu_shared import call
 
 pytestmark = pytest.mark.gpu
@@ -33,6 +34,19 @@ def both8(rt, q, qk, k, v, out, scale=None, first=0, ps=16):
     return y, z
 
 
+def want8(q, k, v, out, scale=None):
+    """What both have to be, with its bound."""
+    kc, vc, ks, vs = (lay(x) for x in (k[0], v[0], k[1], v[1]))
+    table = np.tile(np.arange(kc.shape[0], dtype=np.int32), (q.shape[0], 1))
+    return more.decode8(q, kc, vc, ks, vs, table, [k[0].shape[0]] * q.shape[0], scale, out)
+
+
+def check8(rt, q, qk, k, v, out, scale=None, first=0):
+    want = want8(q, k, v, out, scale)
+    for y in both8(rt, q, qk, k, v, out, scale, first):
+        check(y, *want)
+
+
 def rows8(x):
     return more.encode(np.asarray(x, np.float32))
 
@@ -55,3 +69,72 @@ def test_a_value_scale_of_zero_under_the_largest_score(rt, d, ps, qk, out):
     for first in (0, 64, 208):
         for y in both8(rt, q, qk, rows8(k), v, out, 1.0, first, ps):
             assert np.isfinite(y).all() and np.abs(y).max() <= 1e-20
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("qk,out", TYPES)
+@pytest.mark.parametrize("large", [1e24, 1e26, 1e38])
+def test_values_of_zero_beside_very_large_ones(rt, d, qk, out, large):
+    """Rows of zeros (the least scale there is) weigh as much as rows of 1e38: in one tile and in tiles of several waves,
+    before and behind the large ones."""
+    rng = np.random.default_rng(d)
+    n = 1500
+    for where in (np.arange(8), n - 1 - np.arange(8), rng.permutation(n)[:8]):
+        v = np.zeros((n, 1, d), np.float32)
+        v[where] = large * rng.uniform(0.5, 1, (8, 1, d))
+        k, q = floats(rng, (n, 1, d), "f32"), floats(rng, (1, 2, d), qk)
+        check8(rt, q, qk, rows8(k), rows8(v), out, first=n // 2)
+
+
+@pytest.mark.parametrize("qk,out", TYPES)
+def test_values_of_zero_beside_very_large_ones_in_a_waves_tiles(rt, qk, out):
+    """The same over so many keys that every wave has several tiles."""
+    rng = np.random.default_rng(1)
+    n, d = 150000, 128
+    k, q = rows8(floats(rng, (n, 1, d), "f32")), floats(rng, (1, 1, d), qk)
+    for where in (np.arange(900), n - 1 - np.arange(900), rng.permutation(n)[:900]):
+        v = np.zeros((n, 1, d), np.float32)
+        v[where] = 1e26 * rng.uniform(0.5, 1, (900, 1, d))
+        check8(rt, q, qk, k, rows8(v), out, first=n // 2)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("qk,out", TYPES)
+def test_the_sum_keeps_light_keys_beside_very_large_values(rt, d, qk, out):
+    """1500 keys of weight exp(-12), with values of 0, beside one of weight 1 and 1e38."""
+    n = 1500
+    for at in (0, 700, n - 1):
+        k, v = np.zeros((n, 1, d), np.float32), np.zeros((n, 1, d), np.float32)
+        k[at, :, 0], v[at] = 12, 1e38
+        q = np.zeros((1, 4, d), np.float32)
+        q[:, :, 0] = 1
+        check8(rt, q, qk, rows8(k), rows8(v), out, 1.0, first=800)
+
+
+# ---- scores ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("qk,out", TYPES)
+@pytest.mark.parametrize("size", [1e8, 3e9, 1e12, 1e30])
+def test_8bit_scores_far_past_their_steps(rt, d, qk, out, size):
+    """Scores whose steps in f32 are larger than what a scale adds to them: the largest ones, equal to each
+    other, share the row. (Their weights are then the same number p, so that the row is the mean of their values but
+    for what weights are rounded by, MORE, the output's step and the grain.)"""
+    rng = np.random.default_rng(d)
+    n = 100
+    tops = [3, 40, 41, 77]
+    k = np.zeros((n, 1, d), np.float32)
+    k[:, :, 0] = -size * rng.uniform(0.1, 1, (n, 1))
+    k[tops, :, 0] = size
+    v = rng.standard_normal((n, 1, d)) * 10.0 ** rng.integers(-6, 7, (n, 1, 1))
+    v[tops] = rng.standard_normal((4, 1, d)) * 10.0 ** np.array([5, 4, 5, 3])[:, None, None]
+    v = rows8(v)
+    q = np.zeros((1, 2, d), np.float32)
+    q[:, :, 0] = 1
+    value = more.value(*v)[tops, 0]
+    want = value.mean(axis=0)
+    bound = (more.p_step("q8", out) * np.abs(value).mean(axis=0) + STEP[out] * np.abs(want)
+             + n * 2.0 ** -35 * 127 * v[1][tops].max())
+    for first in (0, 32, 64):
+        for y in both8(rt, q, qk, rows8(k), v, out, 1.0, first):
+            check(y, np.broadcast_to(want, y.shape), np.broadcast_to(bound, y.shape))
