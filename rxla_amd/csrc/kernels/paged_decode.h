@@ -109,50 +109,47 @@ struct PagedTile {
   static constexpr int NS = CODES ? KT / 32 : 0;  // copies of 64 scales: the tile's K's, its V's
   static constexpr int NK = N + NS;               // copies that K's products wait for
   static constexpr int RING = 2 * HALF + 256 * NS;  // a wave's K and V, scales behind them
-  static constexpr int REC = D + 4;               // floats of a record: acc [D], max, sum, codes: the power of acc
+  static constexpr int REC = D + 4;               // floats of a record: acc [D], max, sum
   static __device__ __forceinline__ int kx(int row) { return row & (CH < 16 ? CH - 1 : 15); }
   static __device__ __forceinline__ int vx(int row) { return KIND != kBf16 ? 0 : 2 * (row & (CH < 16 ? 3 : 7)); }
 };
 
 // (max, sum, acc) records joined in order: NB of them, number k0 + k with
-// get(k, min(k0 + k, count - 1), m, l, up, o); those from `count` on do not count. o is two
-// of a head's dims. Over codes o is times 2^up, a power of each record's own.
+// get(k, min(k0 + k, count - 1), m, l, o); those from `count` on do not count. o is two
+// of a head's dims. Over codes acc is divided by its sum already (NORMAL): acc by itself has a
+// power of two beside it that would have to be joined too.
 struct Joined {
-  float M = kMinusInf, L = 0.f, E = kMinusInf;  // (E: the power of O, for codes)
+  float M = kMinusInf, L = 0.f;
   float2 O = float2{0.f, 0.f};
 };
 __device__ __forceinline__ float record_weight(float m, float l, float M) {
   return m == kMinusInf ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - M);  // (l NaN: scores were)
 }
-// The power of two that o of a record is to be multiplied by next to others, and that times 2^-E
-__device__ __forceinline__ float record_power(float m, float up, float M) { return m == kMinusInf ? kMinusInf : (m - M) - up; }
-__device__ __forceinline__ float record_scale(float e, float E) { return e == kMinusInf ? 0.f : __builtin_amdgcn_exp2f(e - E); }
-template <int NB, bool CODES, typename Get>
+template <int NB, bool NORMAL, typename Get>
 __device__ __forceinline__ void join(Joined &j, int k0, int count, Get get) {
-  float m[NB], l[NB], up[NB], M = j.M;
+  float m[NB], l[NB], M = j.M;
   float2 o[NB];
 #pragma unroll
-  for (int k = 0; k < NB; ++k) get(k, min(k0 + k, count - 1), m[k], l[k], up[k], o[k]);
+  for (int k = 0; k < NB; ++k) get(k, min(k0 + k, count - 1), m[k], l[k], o[k]);
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
     if (k0 + k >= count) m[k] = kMinusInf, l[k] = 0.f, o[k] = float2{0.f, 0.f};
     M = fmaxf(M, m[k]);
   }
   const float f0 = record_weight(j.M, j.L, M);
-  if constexpr (CODES) {
-    const float e0 = record_power(j.M, -j.E, M);
-    float e[NB], E = e0;
+  if constexpr (NORMAL) {
+    j.M = M, j.L *= f0;
+    float L = j.L;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) e[k] = record_power(m[k], up[k], M), E = fmaxf(E, e[k]);
-    const float g0 = record_scale(e0, E);
-    j.M = M, j.E = E, j.L *= f0, j.O.x *= g0, j.O.y *= g0;
+    for (int k = 0; k < NB; ++k) l[k] *= record_weight(m[k], l[k], M), L += l[k];
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    j.O.x *= j.L * inv, j.O.y *= j.L * inv;
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
-      const float g = record_scale(e[k], E);
-      j.L += record_weight(m[k], l[k], M) * l[k];
-      j.O.x += g * o[k].x;
-      j.O.y += g * o[k].y;
+      j.O.x += l[k] * inv * o[k].x;
+      j.O.y += l[k] * inv * o[k].y;
     }
+    j.L = L;
     return;
   }
   j.M = M, j.L *= f0, j.O.x *= f0, j.O.y *= f0;
@@ -213,12 +210,9 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t x, uint32_t y) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, up, less));
 }
 constexpr float kCodeUnit = 0x1p9f;
-// V's scales are taken times 2^-24, so that what products and sums need beside them stays within
-// f32 for every scale from 2^-82 on (the append's begin at 2^-47)
-constexpr int kScaleShift = 24;
+// The largest power that p (up to 2^10) is taken times ahead of s_v: finite in f32, and enough for every
+// scale from 2^-106 on (the append's begin at 2^-47)
 constexpr float kMostUp = 116.f;
-// What a row of codes' products is to be multiplied by for its output: 2^e of them, e as in Joined
-__device__ __forceinline__ float codes_inverse(float e, float sum) { return __builtin_amdgcn_exp2f(e + (float)kScaleShift) * (1.0f / sum); }
 // Two f32 as an f16 pair, round to nearest even, and what that leaves
 __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2));
@@ -483,7 +477,7 @@ struct PagedWave {
       if constexpr (CODES) {
         const uint32_t at = mem + 2 * T::HALF + 4 * (16 * u + 4 * g4);
         scale = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)at;
-        vs[u] = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(at + 4 * T::KT) * (1.f / (1 << kScaleShift));
+        vs[u] = *(const __attribute__((address_space(3))) f32x4 *)(uintptr_t)(at + 4 * T::KT);
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
@@ -604,8 +598,12 @@ struct PagedWave {
           top = fmaxf(top, fabsf(w[u][r]));
         }
     };
-    weigh();
-    if (__ballot(top > 0x1p15f || sum > 0x1p10f || m[c] == kMinusInf)) {
+    bool move = __ballot(m[c] == kMinusInf);
+    if (CT > 1 || !move) {  // (not before the first reference, where registers allow that)
+      weigh();
+      move = __ballot(top > 0x1p15f || sum > 0x1p10f || m[c] == kMinusInf);
+    }
+    if (move) {
       float highest = kMinusInf, largest = kMinusInf;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u)
@@ -802,21 +800,24 @@ struct PagedWave {
     f32x4 y;
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] = o[c][(i & ~3) + r][i & 3];
-    if (CODES) y *= kCodeUnit;
     return y;
   }
   __device__ RXW8_INLINE int quad_dim(int i) const {
     return KIND == kBf16 ? 16 * i + 4 * g4 : F32 ? 64 * (i >> 2) + 16 * g4 + 4 * (i & 3) : D / 16 * (4 * g4 + (i & 3)) + 4 * (i >> 2);
   }
+  // What quads are to be multiplied by for an output (sum: of all lanes)
+  __device__ RXW8_INLINE float inverse(int c, float sum) const {
+    if (sum == 0.f) return 0.f;
+    const float inv = 1.0f / sum;
+    if constexpr (CODES) return inv * (kCodeUnit * __uint_as_float((254u << 23) - __float_as_uint(up[c])));
+    return inv;
+  }
   // The lane's row of column tile c as a record
   __device__ RXW8_INLINE void record(int c, float *rec) const {
     const float sum = sum4(l[c]);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) *(f32x4 *)(rec + quad_dim(i)) = quad(c, i);
-    if (g4 == 0) {
-      rec[D] = m[c], rec[D + 1] = sum;
-      if constexpr (CODES) rec[D + 2] = up_of(c);
-    }
+    for (int i = 0; i < D / 16; ++i) *(f32x4 *)(rec + quad_dim(i)) = CODES ? quad(c, i) * inverse(c, sum) : quad(c, i);
+    if (g4 == 0) rec[D] = m[c], rec[D + 1] = sum;
   }
 };
 
@@ -836,6 +837,7 @@ template <int D, int KIND, bool RECORDS = false, int PREC = kAny>
 __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf place) {
   using T = PagedTile<D, KIND>;
   using Wave = PagedWave<D, KIND, 1, PREC>;
+  constexpr bool NORMAL = KIND == kCodes;  // (as join)
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ Piece piece[kPagedWaves][2];
   __shared__ int last_one[2];
@@ -917,19 +919,18 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
     auto finish = [&](int seq, int first, int n, bool whole, float *rec, Piece *p) {
       if (whole) {
         const int64_t row = (int64_t)seq * a.Hq + hq0 + col;
+        const float sum = sum4(w.l[0]);  // (by all lanes)
         if constexpr (RECORDS) {
-          const float sum = sum4(w.l[0]);  // (by all lanes)
           if (col < gt) {
+            const float inv = w.inverse(0, sum);
             float *const to = place.rows + row * T::REC;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = w.quad(0, i);
+            for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = NORMAL ? w.quad(0, i) * inv : w.quad(0, i);
             if (w.g4 == 0) *(float2 *)(to + D) = float2{w.m[0], sum};
-            if (KIND == kCodes && w.g4 == 0) to[D + 2] = w.up_of(0);
           }
         } else {
-          const float sum = sum4(w.l[0]);
           if (col < gt) {
-            const float inv = sum == 0.f ? 0.f : KIND == kCodes ? codes_inverse(-w.up_of(0), sum) : 1.0f / sum;
+            const float inv = w.inverse(0, sum);
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
               const f32x4 y = w.quad(0, i) * inv;
@@ -945,11 +946,11 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       }
       const float sum = sum4(w.l[0]);
       if (col < gt) {
+        const float inv = w.inverse(0, sum);
         float *const to = rec + col * T::REC;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = w.quad(0, i);
+        for (int i = 0; i < D / 16; ++i) *(f32x4 *)(to + w.quad_dim(i)) = NORMAL ? w.quad(0, i) * inv : w.quad(0, i);
         if (w.g4 == 0) to[D] = w.m[0], to[D + 1] = sum;
-        if (KIND == kCodes && w.g4 == 0) to[D + 2] = w.up_of(0);
       }
       if (lane == 0) *p = Piece{seq, first, n};
     };
@@ -1027,11 +1028,10 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       float *const rec = place.rows + ((int64_t)b * a.Hq + hq0 + r) * T::REC;
       *(float2 *)(rec + d) = j.O;
       if (d == 0) *(float2 *)(rec + D) = float2{j.M, j.L};
-      if (KIND == kCodes && d == 0) rec[D + 2] = -j.E;
       return;
     }
     const int64_t to = ((int64_t)b * a.Hq + hq0) * D + 2 * i;
-    const float inv = j.L == 0.f ? 0.f : KIND == kCodes ? codes_inverse(j.E, j.L) : 1.0f / j.L;
+    const float inv = NORMAL ? 1.f : j.L == 0.f ? 0.f : 1.0f / j.L;
     if (a.out_f32) *(float2 *)((float *)a.out + to) = float2{j.O.x * inv, j.O.y * inv};
     else *(uint32_t *)((uint16_t *)a.out + to) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
   };
@@ -1054,23 +1054,21 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
       Joined j;
       uint32_t bits = same;
       int x = e;
-      auto get = [&](int, int, float &m, float &l, float &up, float2 &o) {
+      auto get = [&](int, int, float &m, float &l, float2 &o) {
         if (bits) x = __builtin_ctz(bits), bits &= bits - 1;
         const float *const rec = (const float *)(lds + (x >> 1) * (first_at + rec_bytes) + ((x & 1) ? 0 : first_at)) + r * T::REC;
         const float2 ml = *(const float2 *)(rec + D);
         m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
-        if constexpr (KIND == kCodes) up = rec[D + 2];
       };
       const int n = __builtin_popcount(same);
 #pragma unroll 1
-      for (int k0 = 0; k0 < n; k0 += 4) join<4, KIND == kCodes>(j, k0, n, get);
+      for (int k0 = 0; k0 < n; k0 += 4) join<4, NORMAL>(j, k0, n, get);
       if (whole) {
         write(p.b, i, j);
       } else {
         float *const tr = to + r * T::REC;
         store_pair(tr + d, j.O.x, j.O.y);
         if (d == 0) store_pair(tr + D, j.M, j.L);
-        if (KIND == kCodes && d == 0) store_pair(tr + D + 2, -j.E, 0.f);
       }
     }
   }
@@ -1118,11 +1116,10 @@ __device__ RXW8_INLINE void paged_decode(const PagedDecodeArgs &a, PagedPlaceOf 
         }
 #pragma unroll 1
         for (int k0 = 0; k0 < n; k0 += 4)
-          join<4, KIND == kCodes>(j, k0, n, [&](int, int c, float &m, float &l, float &up, float2 &o) {
+          join<4, NORMAL>(j, k0, n, [&](int, int c, float &m, float &l, float2 &o) {
             const float *const rec = (const float *)lds + c * rec_size + r * T::REC;
             const float2 ml = *(const float2 *)(rec + D);
             m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
-            if constexpr (KIND == kCodes) up = rec[D + 2];
           });
       }
       if (i0 + (int)threadIdx.x < pairs) write(p.b, i, j);

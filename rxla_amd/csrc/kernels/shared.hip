@@ -279,27 +279,23 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         if (at >= cols) break;
         const float *const rec = (const float *)lds + r * T::REC;
         float2 ml[kPagedWaves];
-        float M = kMinusInf, L = 0.f, E = kMinusInf, e[KIND == kCodes ? kPagedWaves : 1];
+        float M = kMinusInf, L = 0.f;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < kPagedWaves; ++k) {
           ml[k] = k < count ? *(const float2 *)(rec + k * 16 * T::REC + D) : float2{kMinusInf, 0.f};
           M = fmaxf(M, ml[k].x);
         }
-        if constexpr (KIND == kCodes) {
-#pragma unroll
-          for (int k = 0; k < kPagedWaves; ++k) {
-            e[k] = record_power(ml[k].x, k < count ? rec[k * 16 * T::REC + D + 2] : 0.f, M);
-            E = fmaxf(E, e[k]);
-          }
-        }
 #pragma unroll
         for (int k = 0; k < kPagedWaves; ++k)
           if (k < count) {
-            const float f = record_weight(ml[k].x, ml[k].y, M);
-            L += f * ml[k].y;
-            O += (KIND == kCodes ? record_scale(e[KIND == kCodes ? k : 0], E) : f) * *(const f32x4 *)(rec + k * 16 * T::REC + d);
+            ml[k].x = record_weight(ml[k].x, ml[k].y, M);
+            L += ml[k].x * ml[k].y;
           }
+        const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+        for (int k = 0; k < kPagedWaves; ++k)  // (over codes as join's records)
+          if (k < count) O += (KIND == kCodes ? ml[k].x * ml[k].y * inv : ml[k].x) * *(const f32x4 *)(rec + k * 16 * T::REC + d);
         float *to = part + at * T::REC;
         if (all) {
           const int row = block * CB + at, seq = row / G;
@@ -307,7 +303,6 @@ __device__ RXW8_INLINE void prefix_walk(const SharedArgs &a, int h, int unit, in
         }
         *(f32x4 *)(to + d) = O;
         if (d == 0) *(float2 *)(to + D) = float2{M, L};
-        if (KIND == kCodes && d == 0) to[D + 2] = -E;
       }
     }
   }
@@ -380,19 +375,18 @@ extern "C" __global__ void __launch_bounds__(256) rxw8_shared_join(SharedArgs a)
     parts += __builtin_amdgcn_readlane(p.part_incl, 63);
   }
   const int count = prefix + (len > 0 && a.d.M > 0);
-  auto out = [&](auto codes) {
-    constexpr bool CODES = decltype(codes)::value;
+  auto out = [&](auto normal) {
+    constexpr bool NORMAL = decltype(normal)::value;  // (as join)
     for (int d = 2 * lane; d < D; d += 128) {
       Joined j;
 #pragma unroll 1
       for (int k0 = 0; k0 < count; k0 += 8)
-        join<8, CODES>(j, k0, count, [&](int, int k, float &m, float &l, float &up, float2 &o) {
+        join<8, NORMAL>(j, k0, count, [&](int, int k, float &m, float &l, float2 &o) {
           const float *const rec = k >= prefix ? a.own + row * REC : first + (int64_t)k * a.columns * REC;
           const float2 ml = *(const float2 *)(rec + D);
           m = ml.x, l = ml.y, o = *(const float2 *)(rec + d);
-          if constexpr (CODES) up = rec[D + 2];
         });
-      const float inv = j.L == 0.f ? 0.f : CODES ? codes_inverse(j.E, j.L) : 1.0f / j.L;
+      const float inv = NORMAL ? 1.f : j.L == 0.f ? 0.f : 1.0f / j.L;
       if (a.d.out_f32) *(float2 *)((float *)a.d.out + row * D + d) = float2{j.O.x * inv, j.O.y * inv};
       else *(uint32_t *)((uint16_t *)a.d.out + row * D + d) = pack_bf16x2(j.O.x * inv, j.O.y * inv);
     }
