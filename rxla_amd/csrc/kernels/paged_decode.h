@@ -366,8 +366,8 @@ struct PagedWave {
       for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
     uint2 two = pair_xor16(__uint_as_float(top));
     two = pair_xor32(__uint_as_float(max(two.x, two.y)));
-    // 2^14 / 2^e, e the exponent of the largest
-    const int scale = min(127 + 14 + 127 - (int)(max(two.x, two.y) >> 23), 254);
+    // 2^14 / 2^e, e the exponent of the largest (2^126 at most: its inverse is no subnormal)
+    const int scale = min(127 + 14 + 127 - (int)(max(two.x, two.y) >> 23), 253);
     const float up = __uint_as_float((uint32_t)scale << 23);
     unit[c] = a.c * kCodeUnit * __uint_as_float((uint32_t)(254 - scale) << 23);
 #pragma unroll

@@ -138,3 +138,15 @@ def test_8bit_scores_far_past_their_steps(rt, d, qk, out, size):
     for first in (0, 32, 64):
         for y in both8(rt, q, qk, rows8(k), v, out, 1.0, first):
             check(y, np.broadcast_to(want, y.shape), np.broadcast_to(bound, y.shape))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("qk,out", TYPES)
+@pytest.mark.parametrize("size", [1e-34, 1e-36, 2e-38])
+def test_8bit_queries_near_0(rt, d, qk, out, size):
+    """Queries of 1e-36 over keys of 1e36: scores as of any other ones."""
+    rng = np.random.default_rng(d)
+    n, hkv = 150, 2
+    k, v = rows8(rng.standard_normal((n, hkv, d)) / (size * 10)), rows8(rng.standard_normal((n, hkv, d)))
+    q = floats(rng, (2, 4, d), qk, std=size * 10)
+    check8(rt, q, qk, k, v, out, first=64)
