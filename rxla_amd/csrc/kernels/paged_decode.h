@@ -369,7 +369,7 @@ struct PagedWave {
     // 2^14 / 2^e, e the exponent of the largest (2^126 at most: its inverse is no subnormal)
     const int scale = min(127 + 14 + 127 - (int)(max(two.x, two.y) >> 23), 253);
     const float up = __uint_as_float((uint32_t)scale << 23);
-    unit[c] = a.c * kCodeUnit * __uint_as_float((uint32_t)(254 - scale) << 23);
+    unit[c] = a.c * (kCodeUnit * __uint_as_float((uint32_t)(254 - scale) << 23));  // (a.c may be near f32's end)
 #pragma unroll
     for (int i = 0; i < NQ; ++i)
 #pragma unroll

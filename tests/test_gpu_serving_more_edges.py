@@ -150,3 +150,15 @@ def test_8bit_queries_near_0(rt, d, qk, out, size):
     k, v = rows8(rng.standard_normal((n, hkv, d)) / (size * 10)), rows8(rng.standard_normal((n, hkv, d)))
     q = floats(rng, (2, 4, d), qk, std=size * 10)
     check8(rt, q, qk, k, v, out, first=64)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("qk,out", TYPES)
+@pytest.mark.parametrize("scale", [1e34, 1e36, 1e38])
+def test_8bit_scales_of_the_scores_near_the_largest(rt, d, qk, out, scale):
+    """A softmax scale near f32's end, over queries as small as it is large."""
+    rng = np.random.default_rng(d)
+    n, hkv = 150, 2
+    k, v = rows8(rng.standard_normal((n, hkv, d))), rows8(rng.standard_normal((n, hkv, d)))
+    q = floats(rng, (2, 4, d), qk, std=0.2 / scale)
+    check8(rt, q, qk, k, v, out, scale, first=64)
