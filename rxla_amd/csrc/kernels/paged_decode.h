@@ -484,7 +484,7 @@ struct PagedWave {
         s[c][u] = acc[c][0];
         if constexpr (NA > 1) s[c][u] += acc[c][1];
         if constexpr (F32) s[c][u] += acc[c][2] + acc[c][3];
-        if constexpr (!LAZY) s[c][u] *= CODES ? scale * unit[CODES ? c : 0] : scale;
+        s[c][u] *= CODES ? scale * unit[CODES ? c : 0] : scale;
       }
     }
   }
@@ -530,7 +530,7 @@ struct PagedWave {
     }
   }
 
-  // The reference a score that need not be the largest: weights up to 2^8 (a score is q.k here)
+  // The reference a score that need not be the largest: weights up to 2^8
   __device__ RXW8_INLINE void softmax_lazy(int c, const Tile &x, bool part) {
     f32x4 w[T::SUB];
     float sum, top;
@@ -548,7 +548,7 @@ struct PagedWave {
       for (int u = 0; u < T::SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          w[u][r] = __builtin_amdgcn_exp2f(fmaf(s[c][u][r], a.c, -ref));
+          w[u][r] = __builtin_amdgcn_exp2f(s[c][u][r] - ref);
           sum += w[u][r];
           top = fmaxf(top, w[u][r]);
         }
@@ -560,7 +560,7 @@ struct PagedWave {
       for (int u = 0; u < T::SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) highest = fmaxf(highest, s[c][u][r]);
-      const float to = fmaxf(m[c], max4(highest) * a.c);
+      const float to = fmaxf(m[c], max4(highest));
       const float f = to == kMinusInf ? 1.f : exp2f(m[c] - to);
       m[c] = to;
       l[c] *= f;

@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 
 import serving_more_ref as more
+import serving_ref as ref
 from test_gpu_cache8 import decode8
-from test_gpu_serving import STEP, check, floats
+from test_gpu_serving import STEP, check, decode, floats
 from test_gpu_shared import call
 
 pytestmark = pytest.mark.gpu
@@ -162,3 +163,35 @@ def test_8bit_scales_of_the_scores_near_the_largest(rt, d, qk, out, scale):
     k, v = rows8(rng.standard_normal((n, hkv, d))), rows8(rng.standard_normal((n, hkv, d)))
     q = floats(rng, (2, 4, d), qk, std=0.2 / scale)
     check8(rt, q, qk, k, v, out, scale, first=64)
+
+
+def shared_and_paged(rt, q, qk, k, v, kind, out, scale, first):
+    """Rows k, v [n, hkv, d] of all sequences: the shared call's result, the first `first` (whole pages) as a prefix, and
+    the paged call's."""
+    n, b = k.shape[0], q.shape[0]
+    kp, vp = lay(k), lay(v)
+    table = np.tile(np.arange(kp.shape[0], dtype=np.int32), (b, 1))
+    cut = first // 16
+    y = call(rt, q, qk, kp, vp, None, kind, table[:1], [cut * 16], [0, b], table[:, cut:], [n - cut * 16] * b, out, scale)
+    return y, decode(rt, q, qk, kp, vp, kind, table, [n] * b, out, scale)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256, 96])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("qk,out", TYPES)
+@pytest.mark.parametrize("power", [24, 31, 34, 60, 100])
+def test_shared_scores_far_past_their_steps(rt, d, kind, qk, out, power):
+    """Scores of 2^24 to 2^100, whose steps pass 2^7 from 2^31 on: the largest one alone weighs, and the row is
+    its value, but for an f32 output's two roundings (the weight is a power of two, its inverse one too)."""
+    rng = np.random.default_rng(power)
+    n = 90
+    for first in (0, 48):
+        k = floats(rng, (n, 1, d), "bf16")
+        k[:, :, 0] = rng.permutation(n)[:, None] + 1 - n // 2
+        k[:, :, 0] = ref.bf16_value(ref.bf16_bits(k[:, :, 0] * np.float32(2.0 ** (power // 2))))
+        v = floats(rng, (n, 1, d), "bf16")
+        q = np.zeros((3, 4, d), np.float32)
+        q[:, :, 0] = np.float32(2.0 ** (power - power // 2)) * 1.25
+        want = v[k[:, 0, 0].argmax(), 0].astype(np.float64)
+        for y in shared_and_paged(rt, q, qk, k, v, kind, out, 1.0, first):
+            check(y, np.broadcast_to(want, y.shape), np.broadcast_to(4 * STEP["f32"] * np.abs(want), y.shape))
