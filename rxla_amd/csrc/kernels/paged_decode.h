@@ -530,7 +530,8 @@ struct PagedWave {
     }
   }
 
-  // The reference a score that need not be the largest: weights up to 2^8
+  // The reference up to 8 above the largest score, so that weights are at most 1 (as large values need: acc
+  // is theirs times the weights) and it need not move with every new maximum
   __device__ RXW8_INLINE void softmax_lazy(int c, const Tile &x, bool part) {
     f32x4 w[T::SUB];
     float sum, top;
@@ -554,13 +555,13 @@ struct PagedWave {
         }
     };
     weigh();
-    if (__ballot(top > 0x1p8f || m[c] == kMinusInf)) {
+    if (__ballot(top > 1.f || m[c] == kMinusInf)) {
       float highest = kMinusInf;
 #pragma unroll
       for (int u = 0; u < T::SUB; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) highest = fmaxf(highest, s[c][u][r]);
-      const float to = fmaxf(m[c], max4(highest));
+      const float to = fmaxf(m[c], max4(highest) + 8.f);
       const float f = to == kMinusInf ? 1.f : exp2f(m[c] - to);
       m[c] = to;
       l[c] *= f;

@@ -195,3 +195,26 @@ def test_shared_scores_far_past_their_steps(rt, d, kind, qk, out, power):
         want = v[k[:, 0, 0].argmax(), 0].astype(np.float64)
         for y in shared_and_paged(rt, q, qk, k, v, kind, out, 1.0, first):
             check(y, np.broadcast_to(want, y.shape), np.broadcast_to(4 * STEP["f32"] * np.abs(want), y.shape))
+
+
+# ---- values --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("qk,out", TYPES)
+def test_shared_values_near_the_largest(rt, d, qk, out):
+    """bf16 values of 3e36 at most, under scores that rise and fall by 2^7.8 from tile to tile, in many heads (so that a
+    wave has several tiles): finite where the paged call's are, and right."""
+    rng = np.random.default_rng(d)
+    n, hkv, b = 768, 64, 4
+    for first in (0, 384, 768):
+        k, v = np.zeros((n, hkv, d), np.float32), 3e36 * (0.5 + 0.5 * rng.random((n, hkv, d)))
+        k[:, :, 0] = (5.4 * (np.arange(n) // 32 % 2) - 8 * ((rng.random(n) < 0.85) & (np.arange(n) % 16 > 0)))[:, None]
+        k = ref.bf16_value(ref.bf16_bits(k))
+        v = ref.bf16_value(ref.bf16_bits(v.astype(np.float32)))
+        q = np.zeros((b, hkv, d), np.float32)
+        q[:, :, 0] = 1
+        y, z = shared_and_paged(rt, q, qk, k, v, "bf16", out, 1.0, first)
+        table = np.tile(np.arange(n // 16, dtype=np.int32), (1, 1))
+        want, bound = ref.paged_decode(q[:1], lay(k), lay(v), table, [n], 1.0, out_step=STEP[out])
+        check(z, *(np.broadcast_to(x, z.shape) for x in (want, bound)))
+        check(y, *(np.broadcast_to(x, y.shape) for x in (want, bound + more.p_step("bf16", out) * np.abs(want))))
