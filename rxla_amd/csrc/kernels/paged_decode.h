@@ -670,13 +670,11 @@ struct PagedWave {
       values_codes(ct, v0);
       return;
     }
-    // weights in parts: three behind an f32 output, two behind a bf16 one; one, rounded by
-    // 2^-8 as the output is, where a kernel is made for bf16 outputs
+    // weights in parts: three behind an f32 output, two behind a bf16 one
     struct Parts {
       uint2 k0, k1, k2;
     };
     auto parts = [&](f32x4 w) RXW8_INLINE {
-      if constexpr (PREC == kLow) return Parts{uint2{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])}, uint2{0, 0}, uint2{0, 0}};
       if (p_parts()) {
         uint32_t x[3], y[3];
         split_bf16x2<true>(w[0], w[1], x);
@@ -713,7 +711,7 @@ struct PagedWave {
             if (c && c >= ct) break;
             auto add = [&](uint2 x, uint2 y) RXW8_INLINE { o[c][n] = mfma16x16x32(as_bf16x8(f), as_bf16x8(u32x4{x.x, x.y, y.x, y.y}), o[c][n]); };
             add(p[c][0].k0, p[c][1].k0);
-            if constexpr (PREC != kLow) add(p[c][0].k1, p[c][1].k1);
+            add(p[c][0].k1, p[c][1].k1);
             if (p_parts()) add(p[c][0].k2, p[c][1].k2);
           }
         }
@@ -738,7 +736,7 @@ struct PagedWave {
             o[c][n] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(f, __builtin_bit_cast(s16x4, x), o[c][n], 0, 0, 0);
           };
           add(p[c].k0);
-          if constexpr (PREC != kLow) add(p[c].k1);
+          add(p[c].k1);
           if (p_parts()) add(p[c].k2);
         }
       }

@@ -218,3 +218,19 @@ def test_shared_values_near_the_largest(rt, d, qk, out):
         want, bound = ref.paged_decode(q[:1], lay(k), lay(v), table, [n], 1.0, out_step=STEP[out])
         check(z, *(np.broadcast_to(x, z.shape) for x in (want, bound)))
         check(y, *(np.broadcast_to(x, y.shape) for x in (want, bound + more.p_step("bf16", out) * np.abs(want))))
+
+
+# ---- the weights behind a bf16 output ------------------------------------------------------
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", [(8, 8), (16, 2), (64, 2)])
+@pytest.mark.parametrize("first", [0, 96, 320])
+def test_shared_weights_keep_16_bits(rt, d, hq, hkv, first):
+    """Behind a bf16 output too the weights over bf16 rows are held to 2^-16, as the paged call holds them: rows that few
+    keys decide are off by the output's rounding alone."""
+    rng = np.random.default_rng(d + first)
+    n, b = 320 + 40, 6
+    q, k, v = floats(rng, (b, hq, d), "bf16", std=4), floats(rng, (n, hkv, d), "bf16"), floats(rng, (n, hkv, d), "bf16")
+    y, _ = shared_and_paged(rt, q, "bf16", k, v, "bf16", "bf16", None, first)
+    table = np.tile(np.arange(-(-n // 16), dtype=np.int32), (b, 1))
+    check(y, *ref.paged_decode(q, lay(k), lay(v), table, [n] * b, p_step=ref.SPLIT + more.MORE, out_step=ref.BF16))
