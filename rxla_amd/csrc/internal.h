@@ -178,6 +178,15 @@ void rt_free(Runtime *rt, void *ptr, size_t bytes);
 // Replaying a caller's graph writes to the blocks that its capture recorded:
 // they are kept until the runtime ends.
 int ensure_workspace(Runtime *rt, Workspace &ws, size_t bytes, bool zero);
+// While it lives, this thread's HIP calls may do what a capture that this or another
+// thread has in progress would refuse, and end for: waits, memory and code objects
+// that do not touch the captured stream.
+struct BesideCaptures {
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+  ~BesideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+  BesideCaptures(const BesideCaptures &) = delete;
+};
 // Whether the runtime's stream is being captured into a graph
 bool stream_capturing(const Runtime *rt);
 // Validates a buffer shape (known dtype, rank <= RXW8_MAX_RANK, dims >= 0,
