@@ -218,6 +218,7 @@ static void add_param(Decoder *d, const std::string &path, int kind, int layer, 
 
 static void free_decoder_memory(Decoder *d) {
   Runtime *rt = d->rt;
+  const BesideCaptures relaxed;
   if (d->gexec) (void)hipGraphExecDestroy(d->gexec);
   if (d->graph) (void)hipGraphDestroy(d->graph);
   d->gexec = nullptr;

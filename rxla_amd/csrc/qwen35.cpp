@@ -922,6 +922,7 @@ int run_forward(Qwen35 *m, const int32_t *ids, float *logits, int64_t B, int64_t
 }
 
 void free_model(Qwen35 *m) {
+  const BesideCaptures relaxed;
   drop_graph(m);
   if (m->block || m->fused) (void)hipStreamSynchronize(m->rt->stream);
   if (m->block) (void)hipFree(m->block);

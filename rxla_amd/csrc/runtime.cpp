@@ -266,7 +266,9 @@ int new_buffer(Runtime *rt, int dtype, const int64_t *dims, int rank, bool zero,
   return RXW8_OK;
 }
 
+// (a collector may come to this at any time, beside any capture)
 static void runtime_free(Runtime *rt) {
+  const BesideCaptures relaxed;
   if (rt->stream) (void)hipStreamSynchronize(rt->stream);
   for (auto &kv : rt->free_blocks) (void)hipFree(kv.second);
   for (Workspace *w : {&rt->partials, &rt->scratch, &rt->xcast, &rt->wdeq, &rt->attn_counters})

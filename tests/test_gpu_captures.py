@@ -81,3 +81,53 @@ def test_the_first_runtime_of_a_process_is_created(mode, same_thread):
     code = FIRST.format(root=ROOT, tests=os.path.join(ROOT, "tests"), mode=mode, same=same_thread)
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert got.returncode == 0 and "right" in got.stdout, got.stderr[-2000:]
+
+
+@pytest.mark.parametrize("mode,same_thread", MODES)
+@pytest.mark.parametrize("last", ["runtime", "buffer"])
+def test_a_runtime_is_released(rt, mode, same_thread, last):
+    """By its owner, or with the last of its buffers: as the collector may, at any time."""
+    import rxla_amd as rx
+
+    own = rx.Runtime(0)
+    bufs = used(own)
+    if last == "buffer":
+        own.close()
+
+    def release():
+        for b in bufs:
+            b.release()
+        own.close()
+
+    beside(mode, same_thread, release)
+
+
+def decoder(rt):
+    import numpy as np
+    from decoder_fixtures import tiny_params
+    from test_gpu_decoder import build, small_cfg
+
+    cfg = small_cfg()
+    model = build(rt, cfg, tiny_params(cfg), 2)
+    model.generate(rt.buffer(np.zeros((2, 3), np.int32)), 5)  # (a graph of its step)
+    rt.synchronize()
+    return model
+
+
+def hybrid(rt):
+    import numpy as np
+    from oracle import qwen35
+    from test_gpu_qwen35 import CONFIGS, build
+
+    cfg = CONFIGS["tiny"]
+    model = build(rt, cfg, qwen35.random_params(cfg, seed=1, std=0.05))
+    for _ in range(3):
+        model.forward(rt.buffer(np.zeros((1, 4), np.int32)))
+    rt.synchronize()
+    return model
+
+
+@pytest.mark.parametrize("mode,same_thread", MODES)
+@pytest.mark.parametrize("make", [decoder, hybrid])
+def test_a_model_is_released(rt, mode, same_thread, make):
+    beside(mode, same_thread, make(rt).close)
