@@ -51,3 +51,15 @@ def rt():
     r = rxla_amd.Runtime(0)
     yield r
     r.synchronize()
+
+
+@pytest.fixture(autouse=True)
+def same_stream():
+    """After a test torch's current stream is the one from before: a capture that ended with an error
+    inside torch.cuda.graph leaves its own behind, which takes no more work."""
+    torch = sys.modules.get("torch")
+    before = torch.cuda.current_stream() if torch and torch.cuda.is_initialized() else None
+    yield
+    torch = sys.modules.get("torch")
+    if torch and torch.cuda.is_initialized():
+        torch.cuda.set_stream(before or torch.cuda.default_stream())
