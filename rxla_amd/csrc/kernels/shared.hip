@@ -105,9 +105,10 @@ __device__ __forceinline__ Group group_of(const SharedArgs &a, int g_from, int g
   return x;
 }
 
-// Pieces of a prefix of `tiles`, `rate` of them to a tile: one at least, and a tile for every wave
+// Pieces of a prefix of `tiles`, `rate` of them to a tile: one at least, and a tile for every wave.
+// (fmaf: the walk and the join's launch, which read each other's records, round alike)
 __device__ __forceinline__ int pieces_of(int tiles, float rate) {
-  return min(max((int)((float)tiles * rate + 0.5f), 1), (int)(((unsigned)tiles + kPagedWaves - 1) / kPagedWaves));
+  return min(max((int)fmaf((float)tiles, rate, 0.5f), 1), (int)(((unsigned)tiles + kPagedWaves - 1) / kPagedWaves));
 }
 // Groups in lanes: those from n0 on
 __device__ __forceinline__ Group groups_from(const SharedArgs &a, int n0) {
