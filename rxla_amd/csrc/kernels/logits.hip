@@ -37,15 +37,11 @@ struct LogitsArgs {
 // copy). Chunks of 1024, 2048, 4096 and 8192 words, 8 a thread: 39.8, 32.4, 31.1 and 31.9 us,
 // and 16 rows of 151936 bf16 logits 7.2, 6.1, 6.2 and 7.0 (every workgroup of a row goes over
 // its history). Two, 4 and 8 tokens a thread at once, before that: 34.2, 33.4 and 33.6, and 7.2,
-// 6.9 and 7.7 us. One row of 151936 and 800 tokens: 5 us, the two rounds and the launch.
+// 6.9 and 7.7 us. One row of 151936 and 800 tokens: 5 us, the two rounds and the launch. What a history
+// costs grows with the workgroups of its row: 64 rows of 248320 with 800, 8000, 32000 and 128000 tokens each 22, 29,
+// 52 and 153 us; one of 151936 4, 5, 9 and 26.
 enum { kOffsets, kPrompts, kRepetition, kFrequency, kPresence, kBiases, kRows };
 constexpr int kThreads = 512, kTokens = 4, kValues = 512;  // tokens of a thread under way; biases kept in LDS
-
-// Device memory that the launch does not write, at a wave-uniform address (scalar loads)
-template <typename T>
-__device__ __forceinline__ T uniform_load(const T *p, int64_t i) {
-  return ((const __attribute__((address_space(4))) T *)(uintptr_t)p)[i];
-}
 
 struct LogitsRow {
   int64_t b, w0;                        // row, first word
@@ -62,7 +58,8 @@ struct LogitsRow {
     b = blockIdx.x / a.chunks, w0 = (int64_t)(blockIdx.x - b * a.chunks) * a.chunk;
     n = (uint32_t)min((int64_t)a.chunk, a.V - w0);
     counts = lds, entries = lds + (a.tokens ? a.chunk : 0), values = (float *)(entries + a.chunk);
-    // (loads without branches between them, one wait for all; T, E and R are 0 where there is none)
+    // (scalar loads: the launch writes none of it, and the address is the wave's. No branches between them, one
+    // wait for all; T, E and R are 0 where there is none)
     auto load = [&](int bit, auto *p, int i) {
       const uint32_t at = (uint32_t)(b + i) * 4 & (uint32_t)__builtin_amdgcn_sbfe(a.given, bit, 1);
       return *(const __attribute__((address_space(4))) uint32_t *)((uintptr_t)p + at);

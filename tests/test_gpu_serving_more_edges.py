@@ -6,7 +6,8 @@ import pytest
 import serving_more_ref as more
 import serving_ref as ref
 from test_gpu_cache8 import decode8
-from test_gpu_serving import STEP, check, decode, floats
+from test_gpu_logits import I32, adjust, history
+from test_gpu_serving import STEP, check, decode, floats, make_pages
 from test_gpu_shared import call
 
 pytestmark = pytest.mark.gpu
@@ -234,3 +235,22 @@ def test_shared_weights_keep_16_bits(rt, d, hq, hkv, first):
     y, _ = shared_and_paged(rt, q, "bf16", k, v, "bf16", "bf16", None, first)
     table = np.tile(np.arange(-(-n // 16), dtype=np.int32), (b, 1))
     check(y, *ref.paged_decode(q, lay(k), lay(v), table, [n] * b, p_step=ref.SPLIT + more.MORE, out_step=ref.BF16))
+
+
+# ---- biases ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("vocab", [3001, 20000])
+def test_more_biases_than_a_workgroup_keeps(rt, vocab):
+    """511 to 2000 entries of a row, words with entries on both sides of the 512th: the last one counts."""
+    rng = np.random.default_rng(vocab)
+    counts = [511, 512, 513, 600, 1024, 2000]
+    offsets = np.concatenate([[0], np.cumsum(counts)]).astype(I32)
+    words = rng.integers(0, vocab, offsets[-1]).astype(I32)
+    for b, n in enumerate(counts):
+        words[offsets[b] + 3] = words[offsets[b] + n - 1] = 17          # first and last
+        words[offsets[b] + 510] = words[offsets[b] + min(512, n - 1)] = 18  # around the border
+    z = floats(rng, (len(counts), vocab), "f32", std=4.0)
+    o = dict(bias_words=words, bias=(5 * rng.standard_normal(offsets[-1])).astype(np.float32), bias_offsets=offsets)
+    check(adjust(rt, z, "f32", **o), *more.adjust(z, STEP["f32"], **o))
+    o.update(history(rng, len(counts), vocab, 0, 300))
+    check(adjust(rt, z, "f32", **o), *more.adjust(z, STEP["f32"], **o))
