@@ -73,7 +73,7 @@ __device__ void any_walk(AnyState &st, const float *q, KV kv, int d, int64_t fir
     if (off >= 0) {
       float dot = 0.f;
       for (int i = 0; i < d; ++i) dot = fmaf(q[i], kv.key(off, i), dot);
-      s = dot * kv.key_scale(off) * c;
+      s = dot * (kv.key_scale(off) * c);
     }
     // (fmaxf passes over a NaN; its weight below is NaN all the same)
     const float m_new = fmaxf(st.m, wave_max64(s));

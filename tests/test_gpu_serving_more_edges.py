@@ -166,6 +166,19 @@ def test_8bit_scales_of_the_scores_near_the_largest(rt, d, qk, out, scale):
     check8(rt, q, qk, k, v, out, scale, first=64)
 
 
+@pytest.mark.parametrize("d,ps", [(64, 16), (128, 16), (256, 16), (96, 16), (128, 7)])
+@pytest.mark.parametrize("qk,out", TYPES)
+def test_8bit_scales_of_the_scores_near_0(rt, d, ps, qk, out):
+    """A softmax scale of 2e-38 over queries and keys of 1e19: their products pass f32 before the scale."""
+    rng = np.random.default_rng(d)
+    n, hkv = 150, 2
+    k, v = rows8(1e19 * rng.standard_normal((n, hkv, d))), rows8(rng.standard_normal((n, hkv, d)))
+    q = floats(rng, (2, 4, d), qk, std=3e18)
+    want = want8(q, k, v, out, 2e-38)
+    for y in both8(rt, q, qk, k, v, out, 2e-38, 64, ps):
+        check(y, *want)
+
+
 def shared_and_paged(rt, q, qk, k, v, kind, out, scale, first):
     """Rows k, v [n, hkv, d] of all sequences: the shared call's result, the first `first` (whole pages) as a prefix, and
     the paged call's."""
