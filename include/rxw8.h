@@ -77,7 +77,9 @@ typedef struct rxw8_buffer rxw8_buffer;
 /* ---- runtime (replaces Client::load, runtime.rs:768) --------------------- */
 
 /* Select HIP device `device`, create its stream, load the gfx950 kernels.
- * FAILED_PRECONDITION when the device is not gfx950 or no device exists. */
+ * FAILED_PRECONDITION when the device is not gfx950 or no device exists. A stream
+ * capture that this or another thread has in progress meanwhile records on; so
+ * it does beside the release of runtimes and models on other streams. */
 int rxw8_runtime_create(int device, rxw8_runtime **out);
 /* Drops the caller's reference; the runtime lives until its last buffer is
  * released. */
@@ -338,7 +340,7 @@ int rxw8_paged_kv_append_q8(rxw8_runtime *rt, rxw8_buffer *k_pages,
 
 /* The append's inverse, over pages of every type (BF16|F32 with NULL scales, U8
  * with both): position starts[b] + i of sequence b goes to row offsets[b] + i of
- * k, v [T,Hkv,D] BF16|F32 (new rows for rxw8_gqa_prefill_packed, say). Values of
+ * k, v [T,Hkv,D] BF16|F32. Values of
  * 8-bit rows are formed in f32; what k, v cannot hold is rounded to nearest even.
  * Rows at positions without a page, negative ones and ones behind the table are
  * 0; rows outside every sequence are left as they were. */
@@ -349,7 +351,11 @@ int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages,
                        rxw8_buffer *k, rxw8_buffer *v);
 
 /* rxw8_gqa_decode_paged over 8-bit pages: the attention over the values that the
- * rows stand for, products and sums to f32 accuracy. */
+ * rows stand for. Codes, scales and sums are f32's; at head widths 64, 128 and 256
+ * an F32 q is held to 2^-22 of an element and 2^-39 of its row's largest, and a
+ * weight times its value's scale to 2^-22 of itself (2^-11 behind BF16 q and out,
+ * whose own rounding is 2^-8) and 2^-35 of the row's largest one. Scales may be any
+ * numbers; a row whose scale is NaN stands for NaN. */
 int rxw8_gqa_decode_paged_q8(rxw8_runtime *rt, rxw8_buffer *q,
                              rxw8_buffer *k_pages, rxw8_buffer *v_pages,
                              rxw8_buffer *k_scales, rxw8_buffer *v_scales,
@@ -368,7 +374,8 @@ int rxw8_gqa_decode_paged_q8_into(rxw8_runtime *rt, rxw8_buffer *q,
  * prefixes[n] (I32 [N,MP]) and then their own: the first lens[b] of table[b].
  * Sequences outside every group have no prefix. Pages of every type, in one
  * pool: BF16|F32 with NULL scales, U8 with both. Lengths, missing pages, heads,
- * scale and out as in rxw8_gqa_decode_paged. */
+ * scale, out and what weights are held to as in rxw8_gqa_decode_paged and its
+ * 8-bit form, which are the faster calls where there are no prefixes (N or MP 0). */
 int rxw8_gqa_decode_shared(rxw8_runtime *rt, rxw8_buffer *q,
                            rxw8_buffer *k_pages, rxw8_buffer *v_pages,
                            rxw8_buffer *k_scales, rxw8_buffer *v_scales,
@@ -430,7 +437,8 @@ typedef struct rxw8_logits_options {
  * history has z = z / repetition where z > 0, else z repetition; one that occurs n
  * times behind the prompt z - frequency n - presence; then z + bias; and words that
  * the mask lacks -inf, whatever they held. out [B,V] F32|BF16; _into may be given
- * the logits themselves. */
+ * the logits themselves. A history is gone over once for each 4096 words of its row:
+ * from some 30000 tokens on it takes longer than the logits. */
 int rxw8_adjust_logits(rxw8_runtime *rt, rxw8_buffer *logits,
                        const rxw8_logits_options *options, int out_dtype,
                        rxw8_buffer **out);

@@ -40,21 +40,21 @@
 // subnormals u 2^-24, and one packed fma gives (u - 128) 2^-9, exactly. Scores and weights
 // take the scales outside the products:
 //   q      times the power of two that brings its row's largest magnitude to 2^14: one part
-//          for bf16 (exact to 2^-39 of the largest), two for f32 (2^-24);
+//          for bf16 (exact to 2^-39 of the largest), two for f32 (2^-22);
 //   p s_v  are held between 2^-24 and 2^15 by a power of two of the row's: p = exp2(s - ref), ref a
 //          score that need not be the largest, and the products take p up s_v. Where a tile's largest of
 //          them passes 2^15 or its sum of p 2^10, ref becomes the largest score and `up` what
 //          brings the largest product to 2^10. No maximum is taken otherwise, of lanes or
 //          tiles. (One reference for both loses the sum where s_v are far apart: rows of 0
 //          and of 1e26 have products 2^126 from each other and weigh the same.) One f16 part
-//          behind a bf16 output (2^-12 of a weight, the output's rounding
-//          is 2^-9 of it), two behind an f32 one; what is below 2^-24 / 2^10 of the largest
-//          weight so far rounds to multiples of that.
+//          behind bf16 q and output (2^-11 of a weight, the output's rounding
+//          is 2^-8 of it; two parts take the batch of 8 from 19.1 to 19.6 us), two else; what is
+//          below 2^-24 / 2^10 of the largest weight so far rounds to multiples of that.
 // V needs no transposing reads: a lane takes D / 16 dims of its own of each of its keys, one
 // read a key, and converts byte n of four keys into the operand of product n; 32 keys at a
 // time (16x16x32). What is not seen is masked at the scores and the weights: codes are
-// numbers whatever they hold. (The two batches above over 8-bit pages: 18.5 us, 2.7 TB/s, and, with
-// f32 queries, 33.1, 3.3; some 8 us of each go by before the first product and after the last.)
+// numbers whatever they hold. (The two batches above over 8-bit pages: 19.1 us, 2.6 TB/s, and, with
+// f32 queries, 32.6, 3.3; some 8 us of each go by before the first product and after the last.)
 namespace {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -250,7 +250,7 @@ struct PagedWave {
   static constexpr bool F32 = T::F32, CODES = T::CODES;
   static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row's q per lane
   // (not where two tries at the weights and q's three parts want more registers than there are:
-  // 41 sequences of 87 keys behind 7, 64 / 8 heads of 256, f32 queries: 86 us with it, 60 without)
+  // 41 sequences of 87 keys behind 7, 64 / 8 heads of 256, f32 queries: 71 us with it, 50 without)
   static constexpr bool LAZY = KIND == kBf16 && PREC != kAny && !(D == 256 && PREC == kHigh);
   // an f32 q's further parts: two over bf16 rows, one over codes
   static constexpr int NL = F32 || PREC == kLow ? 1 : NQ, NE = CODES ? 1 : NL;
