@@ -354,8 +354,9 @@ int rxw8_paged_kv_read(rxw8_runtime *rt, rxw8_buffer *k_pages,
  * rows stand for. Codes, scales and sums are f32's; at head widths 64, 128 and 256
  * an F32 q is held to 2^-22 of an element and 2^-39 of its row's largest, and a
  * weight times its value's scale to 2^-22 of itself (2^-11 behind BF16 q and out,
- * whose own rounding is 2^-8) and 2^-35 of the row's largest one. Scales may be any
- * numbers; a row whose scale is NaN stands for NaN. */
+ * whose own rounding is 2^-8) and 2^-35 of the row's largest one. Weights below 2^-126
+ * of the largest may count as 0. Scales may be any numbers; a row whose scale is NaN
+ * stands for NaN. */
 int rxw8_gqa_decode_paged_q8(rxw8_runtime *rt, rxw8_buffer *q,
                              rxw8_buffer *k_pages, rxw8_buffer *v_pages,
                              rxw8_buffer *k_scales, rxw8_buffer *v_scales,
