@@ -6,7 +6,7 @@ import pytest
 import serving_more_ref as more
 import serving_ref as ref
 from test_gpu_cache8 import decode8
-from test_gpu_logits import I32, adjust, history
+from test_gpu_logits import I32, adjust, biases, history, masks
 from test_gpu_serving import STEP, check, decode, floats, make_pages
 from test_gpu_shared import call
 
@@ -267,3 +267,15 @@ def test_more_biases_than_a_workgroup_keeps(rt, vocab):
     check(adjust(rt, z, "f32", **o), *more.adjust(z, STEP["f32"], **o))
     o.update(history(rng, len(counts), vocab, 0, 300))
     check(adjust(rt, z, "f32", **o), *more.adjust(z, STEP["f32"], **o))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [8, 4096, 20000])
+def test_in_place_by_pieces(rt, kind, vocab):
+    """The logits as the output where rows are whole pieces of 16 bytes: the same bits as into another buffer."""
+    rng = np.random.default_rng(vocab)
+    z = floats(rng, (3, vocab), kind, std=4.0)
+    o = {**history(rng, 3, vocab, 0, 900), **biases(rng, 3, vocab, 50), "mask": masks(rng, 3, vocab, 0.9)}
+    y = adjust(rt, z, kind, into="logits", **o)
+    check(y, *more.adjust(z, STEP[kind], **o))
+    np.testing.assert_array_equal(y, adjust(rt, z, kind, **o))
